@@ -31,6 +31,8 @@ HIP_SOURCES = [
     "dh_conv.hip",
     "dh_elementwise.hip",
     "dh_f64.hip",
+    "dh_embedding.hip",
+    "dh_vocab.hip",
 ]
 RT_SOURCES = ["dream_rt.cpp"]
 

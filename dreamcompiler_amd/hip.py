@@ -83,6 +83,18 @@ _SIGS = {
     "dh_binary": (_i, [_i, _i, _vp, _sz, ctypes.POINTER(_i), _vp, _sz, ctypes.POINTER(_i), _vp,
                        ctypes.POINTER(_i), _vp]),
     "dh_unary": (_i, [_i, _i, _vp, _vp, _sz, ctypes.c_double, ctypes.c_double, _vp]),
+    "dh_embedding_fwd": (_i, [_i, _i, _i, _i, _f, _vp, _vp, _i, _vp, _i]),
+    "dh_embedding_bwd_workspace": (_sz, [_i, _i, _i]),
+    "dh_embedding_bwd": (_i, [_i, _i, _i, _i, _f, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _sz]),
+    "dh_linear_xent_workspace": (_sz, [_i, _i, _i, _i, _i]),
+    "dh_linear_xent_fwd": (_i, [_i, _i, _i, _i, _f, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _sz]),
+    "dh_linear_xent_bwd": (_i, [_i, _i, _i, _i, _f, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i,
+                                _vp, _i, _i, _i, _vp, _sz]),
+    "dh_linear_distill_workspace": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "dh_linear_distill_fwd": (_i, [_i, _i, _i, _i, _i, _f, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp,
+                                   _vp, _sz]),
+    "dh_linear_distill_bwd": (_i, [_i, _i, _i, _i, _i, _f, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp,
+                                   _vp, _i, _i, _vp, _i, _i, _i, _vp, _sz]),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -322,6 +334,61 @@ def unary(op, dtype, A, C, n, lo=0.0, hi=0.0, C32=None):
 def layer_norm_bwd(X, Y, DY, GX, R, C, accumulate=False):
     check(load().dh_layer_norm_bwd(_p(X), _p(Y), _p(DY), _p(GX), R, C, int(accumulate)),
           "dh_layer_norm_bwd")
+
+
+# Embedding and losses over a vocabulary (include/dream_hip.h): ws is device memory of at least
+# the _workspace query's bytes, ld* leading dimensions in elements.
+def embedding_fwd(dtype, N, V, D, scale, ids, W, ldw, Y, ldy):
+    check(load().dh_embedding_fwd(dtype, N, V, D, float(scale), _p(ids), _p(W), ldw, _p(Y), ldy),
+          "dh_embedding_fwd")
+
+
+def embedding_bwd_workspace(N, V, D):
+    return load().dh_embedding_bwd_workspace(N, V, D)
+
+
+def embedding_bwd(dtype, N, V, D, scale, ids, dY, lddy, dW, lddw, grad_type, accumulate, ws,
+                  ws_bytes):
+    check(load().dh_embedding_bwd(dtype, N, V, D, float(scale), _p(ids), _p(dY), lddy, _p(dW),
+                                  lddw, grad_type, int(accumulate), _p(ws), int(ws_bytes)),
+          "dh_embedding_bwd")
+
+
+def linear_xent_workspace(dtype, N, V, D, backward):
+    return load().dh_linear_xent_workspace(dtype, N, V, D, int(backward))
+
+
+def linear_xent_fwd(dtype, N, V, D, scale, H, ldh, W, ldw, target, loss, lse, ws, ws_bytes):
+    check(load().dh_linear_xent_fwd(dtype, N, V, D, float(scale), _p(H), ldh, _p(W), ldw,
+                                    _p(target), _p(loss), _p(lse), _p(ws), int(ws_bytes)),
+          "dh_linear_xent_fwd")
+
+
+def linear_xent_bwd(dtype, N, V, D, scale, H, ldh, W, ldw, target, lse, dloss, dH, lddh, acc_dH,
+                    dW, lddw, acc_dW, grad_type, ws, ws_bytes):
+    check(load().dh_linear_xent_bwd(dtype, N, V, D, float(scale), _p(H), ldh, _p(W), ldw,
+                                    _p(target), _p(lse), _p(dloss), _p(dH), lddh, int(acc_dH),
+                                    _p(dW), lddw, int(acc_dW), grad_type, _p(ws), int(ws_bytes)),
+          "dh_linear_xent_bwd")
+
+
+def linear_distill_workspace(dtype, N, V, D, K, backward):
+    return load().dh_linear_distill_workspace(dtype, N, V, D, K, int(backward))
+
+
+def linear_distill_fwd(dtype, N, V, D, K, T, H, ldh, W, ldw, top_id, top_logit, loss, lse, ws,
+                       ws_bytes):
+    check(load().dh_linear_distill_fwd(dtype, N, V, D, K, float(T), _p(H), ldh, _p(W), ldw,
+                                       _p(top_id), _p(top_logit), _p(loss), _p(lse), _p(ws),
+                                       int(ws_bytes)), "dh_linear_distill_fwd")
+
+
+def linear_distill_bwd(dtype, N, V, D, K, T, H, ldh, W, ldw, top_id, top_logit, lse, dloss, dH,
+                       lddh, acc_dH, dW, lddw, acc_dW, grad_type, ws, ws_bytes):
+    check(load().dh_linear_distill_bwd(dtype, N, V, D, K, float(T), _p(H), ldh, _p(W), ldw,
+                                       _p(top_id), _p(top_logit), _p(lse), _p(dloss), _p(dH), lddh,
+                                       int(acc_dH), _p(dW), lddw, int(acc_dW), grad_type, _p(ws),
+                                       int(ws_bytes)), "dh_linear_distill_bwd")
 
 
 class Timer:

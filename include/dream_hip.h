@@ -322,6 +322,61 @@ int dh_binary(int op, int dtype, const void* d_A, size_t a_len, const int* a_str
 int dh_unary(int op, int dtype, const void* d_A, void* d_C, size_t n, double lo, double hi,
              float* d_C32);
 
+/* ---- a language model's vocabulary: embedding, and losses over it ------------------------
+ * Additions to the reference, next to linear, log_softmax and their backward.  The table W is
+ * V x D in both; a model that shares it passes one dW to all of them with accumulate set.
+ * dtype DH_F32 or DH_BF16 for W, H, Y, dY.  Gradients are of grad_type: the inputs' type, or
+ * DH_F32.  Every sum is held in fp32; results are rounded once.
+ * Padding: a token, target or teacher entry outside 0 .. V-1 is none.  Its row of Y is zero; a
+ * row without a target has loss 0, lse 0 and no gradient (its dH is zero, or unchanged when
+ * accumulating), whatever its H holds, NaN included.
+ * Workspaces: the caller's device memory, 16-byte aligned, at least as large as the _workspace
+ * query says (the losses take larger pieces of the vocabulary out of more, which is faster); no
+ * call here allocates, so all of them can be captured.  Calls that may overlap in time, two
+ * captured graphs among them, need workspaces of their own; nothing is kept there between calls.
+ * The losses take an fp32 operand to 2^-24 of itself or 2^-134, whichever is more.
+ * Deterministic: no floating-point atomics.
+ *
+ * Y[n] = scale W[id[n]] for N tokens. */
+int dh_embedding_fwd(int dtype, int N, int V, int D, float scale, const int* d_ids,
+                     const void* d_W, int ldw, void* d_Y, int ldy);
+/* dW[v] = scale * sum of dY[n] over id[n] = v, every row of the table (zero without a token); with
+ * accumulate the rows that have tokens get it added, the others are not touched. */
+size_t dh_embedding_bwd_workspace(int N, int V, int D);   /* <= 18 N + N D / 2 + V + 8 D + 8192 */
+int dh_embedding_bwd(int dtype, int N, int V, int D, float scale, const int* d_ids,
+                     const void* d_dY, int lddy, void* d_dW, int lddw, int grad_type,
+                     int accumulate, void* d_ws, size_t ws_bytes);
+/* Softmax cross entropy of the logits z = scale H W^T (H is N x D) against one target a row, the
+ * logits never stored: loss[n] = lse[n] - z[n, target[n]], lse[n] = log sum_v exp z[n, v]
+ * (natural log, fp32; lse may be NULL).  scale finite and > 0. */
+size_t dh_linear_xent_workspace(int dtype, int N, int V, int D, int backward);
+int dh_linear_xent_fwd(int dtype, int N, int V, int D, float scale, const void* d_H, int ldh,
+                       const void* d_W, int ldw, const int* d_target, float* d_loss, float* d_lse,
+                       void* d_ws, size_t ws_bytes);
+/* Its gradient from the forward's lse: G = dloss[n] scale (softmax(z) - onehot(target)),
+ * dH = G W, dW = G^T H.  d_dloss (N, fp32) may be NULL: ones.  d_dH or d_dW may be NULL: not
+ * computed.  acc_dH / acc_dW add into them.  bf16: G is rounded to bf16 once before the products
+ * (as any bf16 training does), so bf16 inputs give gradients to bf16 precision also in DH_F32.
+ * dH must not overlap H, nor dW W. */
+int dh_linear_xent_bwd(int dtype, int N, int V, int D, float scale, const void* d_H, int ldh,
+                       const void* d_W, int ldw, const int* d_target, const float* d_lse,
+                       const float* d_dloss, void* d_dH, int lddh, int acc_dH, void* d_dW,
+                       int lddw, int acc_dW, int grad_type, void* d_ws, size_t ws_bytes);
+/* Distillation of the same logits at a temperature T > 0, z = H W^T / T, from a teacher's K best
+ * logits a row (top_id, top_logit: N x K, in any order; an entry of logit -inf is none):
+ * q = softmax(top_logit / T) over the row's entries, loss[n] = T^2 KL(q || softmax(z)) =
+ * T^2 sum_k q_k (log q_k - z_k + lse).  A token that occurs twice in a row counts with the sum of
+ * its probabilities.  A row without entries is padding. */
+size_t dh_linear_distill_workspace(int dtype, int N, int V, int D, int K, int backward);
+int dh_linear_distill_fwd(int dtype, int N, int V, int D, int K, float T, const void* d_H, int ldh,
+                          const void* d_W, int ldw, const int* d_top_id, const float* d_top_logit,
+                          float* d_loss, float* d_lse, void* d_ws, size_t ws_bytes);
+int dh_linear_distill_bwd(int dtype, int N, int V, int D, int K, float T, const void* d_H, int ldh,
+                          const void* d_W, int ldw, const int* d_top_id, const float* d_top_logit,
+                          const float* d_lse, const float* d_dloss, void* d_dH, int lddh,
+                          int acc_dH, void* d_dW, int lddw, int acc_dW, int grad_type, void* d_ws,
+                          size_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif
