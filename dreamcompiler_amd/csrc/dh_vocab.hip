@@ -15,11 +15,16 @@
 // products.  Rows without a target (padding) are taken out first: the rows that count are packed
 // side by side, so padding costs no product and nothing in it, NaN included, reaches a sum.
 //
-// All four products run on the bf16 matrix cores with fp32 accumulators.  An fp32 operand is
-// split into three bf16 parts, x = x1 + x2 + x3 (8 significant bits each, the last remainder is
-// exact), and a product takes the six pairs of parts that reach 2^-24 of it, smallest first:
-// x3 y1, x2 y2, x1 y3, x2 y1, x1 y2, x1 y1 -- six bf16 products at 16 times the rate of the fp32
-// ones.
+// All four products run on the 16-bit matrix cores with fp32 accumulators.  bf16 operands are taken
+// as they are.  An fp32 operand is scaled by a power of two and split into two fp16 parts of 11
+// significant bits, x = hi + 2^-11 lo; a product is 2^-11 (lo hi + hi lo) + hi hi: the two cross
+// products are added first, the accumulators scaled by 2^-11 (exactly), then the third is added.
+// Three 16-bit products at 16 times the rate of an fp32 one.  With the operand's largest value
+// scaled below 2^15, the others are taken to 2^-23 of themselves or 2^-51 of it, whichever is more,
+// and the product left out (lo lo) is below 2^-24 of a product.  What the scale is common to: a row
+// where k runs along the row (H, and W in the forward), else all of the operand (W in the
+// backward, where its rows are summed over; G, whose entries are p - q; and w_n H_n, the other
+// operand of dW).
 #include "dh_common.hpp"
 #include "dh_gemm_bf16.hpp"
 
@@ -56,118 +61,130 @@ __device__ inline void load8(const uint16_t* __restrict__ p, int c, int D, float
 }
 __device__ inline uint16_t rne_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
 
-// x = the sum of three bf16 values, to 24 bits.  Values whose nearest bf16 is infinite are
-// truncated instead; infinities and NaN are their own first part.
-__device__ inline void split3(float x, uint16_t (&b)[3]) {
-    b[0] = rne_bf16(x);
-    const bool finite = __builtin_fabsf(x) < INFINITY;
-    if (finite && (b[0] & 0x7FFF) == 0x7F80) b[0] = (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
-    const float r = finite ? x - bf16_bits_to_f32(b[0]) : 0.f;
-    b[1] = rne_bf16(r);
-    b[2] = rne_bf16(r - bf16_bits_to_f32(b[1]));
-}
-
 typedef uint16_t h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// 8 values as PLANES bf16 parts at dst, dst + plane, ...  One part: the values are bf16 already.
-template <int PLANES>
+// |x| < 2^16 as two fp16 parts, x = p[0] + 2^-11 p[1]; an infinity or NaN is its own first part.
+__device__ inline void split2(float x, uint16_t (&p)[2]) {
+    // Holds x to its fp32 value: a product that the compiler folds into the conversion is rounded
+    // once there and twice for the remainder, and near a tie hi and the remainder then belong to
+    // different neighbours.
+    asm("" : "+v"(x));
+    const _Float16 hi = (_Float16)x;
+    const float r = __builtin_fabsf(x) < INFINITY ? x - (float)hi : 0.f;
+    const _Float16 lo = (_Float16)(r * 2048.f);
+    p[0] = __builtin_bit_cast(uint16_t, hi);
+    p[1] = __builtin_bit_cast(uint16_t, lo);
+}
+// What the products take of a value: its nearest bf16, or its two fp16 parts.
+template <int PARTS>
+__device__ inline void to_parts(float x, uint16_t (&p)[PARTS]) {
+    if constexpr (PARTS == 1) p[0] = rne_bf16(x);
+    else split2(x, p);
+}
+template <int PARTS>
 __device__ inline void store_parts(uint16_t* __restrict__ dst, long long plane, const float (&v)[8]) {
-    h8 o[PLANES];
+    h8 o[PARTS];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        if constexpr (PLANES == 1) {
-            o[0][e] = rne_bf16(v[e]);
-        } else {
-            uint16_t b[3];
-            split3(v[e], b);
+        uint16_t x[PARTS];
+        to_parts<PARTS>(v[e], x);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) o[p][e] = b[p];
-        }
+        for (int p = 0; p < PARTS; ++p) o[p][e] = x[p];
     }
 #pragma unroll
-    for (int p = 0; p < PLANES; ++p) *reinterpret_cast<h8*>(dst + p * plane) = o[p];
+    for (int p = 0; p < PARTS; ++p) *reinterpret_cast<h8*>(dst + p * plane) = o[p];
+}
+
+// The scale of an operand whose largest finite value is mx: 2^-e puts it into [2^14, 2^15).  e is
+// at least -124, so that 2^-e is finite: what that loses lies below fp32's range.
+__device__ inline int scale_of(float mx) {
+    return mx > 0.f ? max(__builtin_amdgcn_frexp_expf(mx) - 15, -124) : 0;
+}
+__device__ inline float larger(float mx, const float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float a = __builtin_fabsf(x[e]);
+        mx = a < INFINITY ? fmaxf(mx, a) : mx;
+    }
+    return mx;
+}
+
+// One row of D values as parts with zeros up to Dp, by one wave.  Two parts: OWN, at the row's own
+// scale, which is returned; else v 2^-e f (f at most 1 in size, so nothing overflows on the way).
+template <typename T, int PARTS, bool OWN>
+__device__ inline int convert_row(const T* __restrict__ src, int D, uint16_t* __restrict__ dst, int Dp,
+                                  long long plane, int lane, int e = 0, float f = 1.f) {
+    if constexpr (PARTS == 1) {
+        for (int c = 8 * lane; c < Dp; c += 512) {
+            float v[8];
+            load8(src, c, D, v);
+            store_parts<1>(dst + c, plane, v);
+        }
+        return 0;
+    } else {
+        constexpr int KEEP = OWN ? 4 : 0;   // 2048 columns in registers, the rest is read again
+        float v[KEEP + 1][8];
+        if constexpr (OWN) {
+            float mx = 0.f;
+#pragma unroll
+            for (int t = 0; t < KEEP; ++t)
+                if (8 * lane + 512 * t < Dp) {
+                    load8(src, 8 * lane + 512 * t, D, v[t]);
+                    mx = larger(mx, v[t]);
+                }
+            for (int c = 8 * lane + 512 * KEEP; c < Dp; c += 512) {
+                float x[8];
+                load8(src, c, D, x);
+                mx = larger(mx, x);
+            }
+            e = scale_of(wave_reduce(mx, OpMax()));
+        }
+        const float scale = __builtin_ldexpf(1.f, -e);
+        auto put = [&](int c, float (&x)[8]) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[q] = OWN ? x[q] * scale : (x[q] * scale) * f;
+            store_parts<PARTS>(dst + c, plane, x);
+        };
+#pragma unroll
+        for (int t = 0; t < KEEP; ++t)
+            if (8 * lane + 512 * t < Dp) put(8 * lane + 512 * t, v[t]);
+        for (int c = 8 * lane + 512 * KEEP; c < Dp; c += 512) {
+            float x[8];
+            load8(src, c, D, x);
+            put(c, x);
+        }
+        return e;
+    }
 }
 
 // ---- packing ------------------------------------------------------------------------------------
-// What a packed row i is: its row n, target, loss weight and lse (backward).  Arrays are padded
-// to whole tiles of rows, so that a tile's epilogue may load past the last row.
+// What a packed row i is: its row n, target, loss weight and lse (backward), and its scale (two
+// parts).  Arrays are padded to whole tiles of rows, so that a tile's epilogue may load past the
+// last row.
 struct Rows {
     int* cnt;          // rows that count
     int* row;          // packed -> row
-    int* inv;          // row -> packed, or -1
     int* target;
+    int* hexp;
     float *w, *lse;    // backward only
 };
+// Two parts: the scales of the other operands.
+struct Exps {
+    int* e;            // forward: of the piece's table rows
+    int *X, *E;        // backward: of w_n H_n and of the table
+    int* group;        // per group of packed rows, the largest scale that w_n H_n asks for
+    float* wmax;       // per work-group of the scan, the table's largest value
+};
+constexpr int SCAN = 1024;   // most work-groups that look for it
+constexpr int NO_EXP = -(1 << 20);
+__device__ inline int exponent(float x) {   // of a finite value that is not zero
+    const float a = __builtin_fabsf(x);
+    return a > 0.f && a < INFINITY ? __builtin_amdgcn_frexp_expf(x) : NO_EXP;
+}
 
 __device__ inline bool counts(int target, int V) { return (unsigned)target < (unsigned)V; }
 
-// Work-group b packs rows 64 b .. 64 b + 63: it counts the rows that count before them (the
-// targets are few and stay in cache), then copies its own, a wave per row, as bf16 parts with
-// zeros up to Dp.  Forward (loss not null) also writes the padding's zeros.
-template <typename T, int PLANES>
-__global__ void __launch_bounds__(1024) pack_rows(const int* __restrict__ target, int N, int V, int D,
-                                                  const T* __restrict__ H, int ldh,
-                                                  uint16_t* __restrict__ Hp, int Dp, long long plane,
-                                                  Rows rows, float* __restrict__ loss,
-                                                  float* __restrict__ lse_out,
-                                                  const float* __restrict__ lse_in,
-                                                  const float* __restrict__ dloss, float wscale) {
-    __shared__ int red[16];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int n0 = blockIdx.x * 64;
-    int before = 0;
-    for (int n = threadIdx.x; n < n0; n += 1024) before += counts(target[n], V);
-    for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m, 64);
-    if (lane == 0) red[w] = before;
-    __syncthreads();
-    before = 0;
-    for (int x = 0; x < 16; ++x) before += red[x];
-    const bool mine = n0 + lane < N && counts(target[n0 + lane], V);
-    const uint64_t mask = __ballot(mine);
-    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *rows.cnt = before + __popcll(mask);
-    for (int r = w; r < 64 && n0 + r < N; r += 16) {
-        const int n = n0 + r;
-        const bool keep = (mask >> r) & 1;
-        const int i = before + __popcll(mask & ((1ull << r) - 1));
-        if (lane == 0) {
-            rows.inv[n] = keep ? i : -1;
-            if (keep) {
-                rows.row[i] = n;
-                rows.target[i] = target[n];
-                if (lse_in) {
-                    rows.lse[i] = lse_in[n];
-                    rows.w[i] = (dloss ? dloss[n] : 1.f) * wscale;
-                }
-            } else if (loss) {
-                loss[n] = 0.f;
-                if (lse_out) lse_out[n] = 0.f;
-            }
-        }
-        if (!keep) continue;
-        for (int c = 8 * lane; c < Dp; c += 512) {
-            float v[8];
-            load8(H + (size_t)n * ldh, c, D, v);
-            store_parts<PLANES>(Hp + (size_t)i * Dp + c, plane, v);
-        }
-    }
-}
-
-// Rows v0 .. v0 + R - 1 of the table as bf16 parts with zeros up to Dp, a wave per row.
-template <typename T, int PLANES>
-__global__ void __launch_bounds__(256) stage_table(const T* __restrict__ W, int ldw, int v0, int R, int D,
-                                                   uint16_t* __restrict__ dst, int Dp,
-                                                   long long plane) {
-    const int lane = threadIdx.x & 63;
-    const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= R) return;
-    for (int c = 8 * lane; c < Dp; c += 512) {
-        float v[8];
-        load8(W + (size_t)(v0 + r) * ldw, c, D, v);
-        store_parts<PLANES>(dst + (size_t)r * Dp + c, plane, v);
-    }
-}
-
-// ---- targets -------------------------------------------------------------------------------------
 // The K teacher entries of a row: token and logit.  An entry whose token lies outside the table
 // or whose logit is -inf is none.
 struct Teacher {
@@ -179,8 +196,21 @@ struct Teacher {
 __device__ inline bool entry_counts(const Teacher& t, size_t at, int V) {
     return counts(t.id[at], V) && !(t.logit[at] == -INFINITY);
 }
+// Whether row n counts: it has a target, or an entry.
+struct Targets {
+    const int* target;   // or null: the teacher's
+    Teacher t;
+    int V;
+    __device__ bool has(int n) const {
+        if (target) return counts(target[n], V);
+        for (int k = 0; k < t.K; ++k)
+            if (entry_counts(t, (size_t)n * t.K + k, V)) return true;
+        return false;
+    }
+};
 
-// flag[n] = 0 where row n has an entry, -1 where it has none (padding).  A wave per row.
+// flag[n] = 0 where row n has an entry, -1 where it has none: for so many entries that pack_rows
+// had better not look for them again and again.  A wave per row.
 __global__ void __launch_bounds__(256) teacher_flags(Teacher t, int N, int V, int* __restrict__ flag) {
     const int lane = threadIdx.x & 63;
     const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -204,18 +234,193 @@ __device__ inline float row_dot(const T* __restrict__ a, const T* __restrict__ b
     return wave_reduce(s, OpSum());
 }
 
-// base[i] = -z at the packed row's target: the row's loss is lse + base.  A wave per row.
-template <typename T>
-__global__ void __launch_bounds__(256) target_dot(Rows rows, const T* __restrict__ H, int ldh,
-                                                  const T* __restrict__ W, int ldw, int D, float c,
-                                                  float* __restrict__ base) {
-    const int lane = threadIdx.x & 63;
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= *rows.cnt) return;
-    const float d = row_dot(H + (size_t)rows.row[i] * ldh, W + (size_t)rows.target[i] * ldw, D, lane);
-    if (lane == 0) base[i] = -(c * d);
+template <typename OT>
+__device__ inline void zero_row(OT* p, int D, int lane) {
+    for (int c = lane; c < D; c += 64) p[c] = OT(0);
 }
 
+struct Pack {
+    Targets targets;
+    int N, D;
+    const void* H;
+    int ldh;
+    const void* W;
+    int ldw;
+    uint16_t* Hp;
+    int Dp;
+    long long plane;
+    Rows rows;
+    Exps exps;
+    int groups;              // of PACK rows
+    float c;
+    // forward
+    float *loss, *lse_out, *base;
+    // backward
+    const float *lse_in, *dloss;
+    float wscale;
+    void* dH;                // its padding rows are cleared here (or null)
+    int lddh, dh_f32;
+    // work-groups behind the groups
+    int tables;              // stage the table's first rows: R of them, 16 a work-group
+    int R;
+    uint16_t* staged;
+    long long wplane;
+};
+constexpr int PACK = 16;     // rows of a work-group, one per wave
+
+// Work-group b < groups packs rows 16 b .. 16 b + 15: it counts the rows that count before them (the
+// targets are few and stay in cache), then converts its own.  Forward: also the padding's zeros and,
+// for cross entropy, base = -z at the target (the loss is lse + base).  The work-groups behind
+// stage table rows, or (backward, two parts) look for the table's largest value.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(1024) pack_rows(Pack a) {
+    __shared__ int red[16];
+    __shared__ int own[PACK];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const T* H = (const T*)a.H;
+    const T* W = (const T*)a.W;
+    const int V = a.targets.V, D = a.D;
+    if ((int)blockIdx.x >= a.groups) {
+        const int b = blockIdx.x - a.groups;
+        if (b < a.tables) {
+            const int r = 16 * b + w;
+            if (r >= a.R) return;
+            const int e = convert_row<T, PARTS, true>(W + (size_t)r * a.ldw, D, a.staged + (size_t)r * a.Dp,
+                                                      a.Dp, a.wplane, lane);
+            if (PARTS == 2 && lane == 0) a.exps.e[r] = e;
+            return;
+        }
+        if constexpr (PARTS == 2) {
+            const int scan = gridDim.x - a.groups;
+            float mx = 0.f;
+            for (long long v = 16LL * b + w; v < V; v += 16LL * scan)
+                for (int c = 8 * lane; c < D; c += 512) {
+                    float x[8];
+                    load8(W + (size_t)v * a.ldw, c, D, x);
+                    mx = larger(mx, x);
+                }
+            mx = wave_reduce(mx, OpMax());
+            if (lane == 0) red[w] = __builtin_bit_cast(int, mx);
+            __syncthreads();
+            if (threadIdx.x != 0) return;
+            for (int x = 1; x < 16; ++x) mx = fmaxf(mx, __builtin_bit_cast(float, red[x]));
+            a.exps.wmax[b] = mx;
+        }
+        return;
+    }
+    const int n0 = blockIdx.x * PACK;
+    int before = 0;
+    for (int n = threadIdx.x; n < n0; n += 1024) before += a.targets.has(n);
+    for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m, 64);
+    if (lane == 0) red[w] = before;
+    if (threadIdx.x < PACK) own[threadIdx.x] = n0 + (int)threadIdx.x < a.N && a.targets.has(n0 + threadIdx.x);
+    __syncthreads();
+    before = 0;
+    for (int x = 0; x < 16; ++x) before += red[x];
+    int count = 0, i = before;
+    for (int x = 0; x < PACK; ++x) {
+        if (x < w) i += own[x];
+        count += own[x];
+    }
+    if ((int)blockIdx.x == a.groups - 1 && threadIdx.x == 0) *a.rows.cnt = before + count;
+    const int n = n0 + w;
+    const bool keep = own[w];
+    int most = NO_EXP;
+    if (keep) {
+        const int h = convert_row<T, PARTS, true>(H + (size_t)n * a.ldh, D, a.Hp + (size_t)i * a.Dp, a.Dp,
+                                                  a.plane, lane);
+        const int target = a.targets.target ? a.targets.target[n] : 0;
+        if (a.base) {
+            const float d = row_dot(H + (size_t)n * a.ldh, W + (size_t)target * a.ldw, D, lane);
+            if (lane == 0) a.base[i] = -(a.c * d);
+        }
+        if (lane == 0) {
+            a.rows.row[i] = n;
+            a.rows.target[i] = target;
+            a.rows.hexp[i] = h;
+            if (a.lse_in) {
+                const float wn = (a.dloss ? a.dloss[n] : 1.f) * a.wscale;
+                a.rows.lse[i] = a.lse_in[n];
+                a.rows.w[i] = wn;
+                most = exponent(wn) + h;   // |w_n H_n| < 2^(15 + this)
+            }
+        }
+    } else if (n < a.N) {
+        if (lane == 0 && a.loss) {
+            a.loss[n] = 0.f;
+            if (a.lse_out) a.lse_out[n] = 0.f;
+        }
+        if (a.dH) {
+            if (a.dh_f32) zero_row((float*)a.dH + (size_t)n * a.lddh, D, lane);
+            else zero_row((uint16_t*)a.dH + (size_t)n * a.lddh, D, lane);
+        }
+    }
+    if (PARTS == 2 && a.lse_in) {
+        __syncthreads();   // red[] has been read
+        if (lane == 0) red[w] = most;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int x = 1; x < 16; ++x) most = max(most, red[x]);
+            a.exps.group[blockIdx.x] = most;
+        }
+    }
+}
+
+// Forward, or one part: rows v0 .. v0 + R - 1 of the table as parts, a wave per row.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256) stage_table(const T* __restrict__ W, int ldw, int v0, int R, int D,
+                                                   uint16_t* __restrict__ dst, int Dp, long long plane,
+                                                   int* __restrict__ exps) {
+    const int lane = threadIdx.x & 63;
+    const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= R) return;
+    const int e = convert_row<T, PARTS, true>(W + (size_t)(v0 + r) * ldw, D, dst + (size_t)r * Dp, Dp, plane,
+                                              lane);
+    if (PARTS == 2 && lane == 0) exps[r] = e;
+}
+
+// Backward of two parts: the same at the table's scale, which each work-group finds from the scan's
+// results; the work-groups behind (first piece) convert the packed rows of w_n H_n at theirs.  The
+// first work-group writes both scales down for the products.
+__global__ void __launch_bounds__(256) stage_scaled(const float* __restrict__ W, int ldw, int v0, int R,
+                                                    int D, uint16_t* __restrict__ dst, int Dp,
+                                                    long long plane, Exps exps, int groups, int scan, int tables,
+                                                    Rows rows, const float* __restrict__ H, int ldh,
+                                                    uint16_t* __restrict__ Xp, long long xplane) {
+    __shared__ float redf[4];
+    __shared__ int redi[4];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    float mx = 0.f;
+    for (int g = threadIdx.x; g < scan; g += 256) mx = fmaxf(mx, exps.wmax[g]);
+    mx = wave_reduce(mx, OpMax());
+    int x = NO_EXP;
+    for (int g = threadIdx.x; g < groups; g += 256) x = max(x, exps.group[g]);
+    for (int m = 1; m < 64; m <<= 1) x = max(x, __shfl_xor(x, m, 64));
+    if (lane == 0) {
+        redf[w] = mx;
+        redi[w] = x;
+    }
+    __syncthreads();
+    const int E = scale_of(fmaxf(fmaxf(redf[0], redf[1]), fmaxf(redf[2], redf[3])));
+    const int X = max(max(redi[0], redi[1]), max(redi[2], redi[3]));
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *exps.E = E;
+        *exps.X = X;
+    }
+    if ((int)blockIdx.x < tables) {
+        const int r = blockIdx.x * 4 + w;
+        if (r < R)
+            convert_row<float, 2, false>(W + (size_t)(v0 + r) * ldw, D, dst + (size_t)r * Dp, Dp, plane, lane, E);
+        return;
+    }
+    const int i = (blockIdx.x - tables) * 4 + w;
+    if (i >= *rows.cnt) return;
+    const int h = rows.hexp[i];
+    convert_row<float, 2, false>(H + (size_t)rows.row[i] * ldh, D, Xp + (size_t)i * Dp, Dp, xplane, lane, h,
+                                 __builtin_ldexpf(rows.w[i], h - X));
+}
+
+// ---- teachers ------------------------------------------------------------------------------------
 // A work-group per packed row: the teacher's probabilities q (N x K, zero where there is no
 // entry), the student's logits z at its tokens, and base[i] = sum q (log q - z).
 template <typename T>
@@ -269,8 +474,9 @@ __global__ void __launch_bounds__(256) teacher_dots(Rows rows, Teacher t, int V,
 }
 
 // ---- products -------------------------------------------------------------------------------------
-// C (M x N) = sum over k of A and B, operands of bf16 parts.  AK: A is stored [m][k], else [k][m];
-// BK: B is stored [n][k], else [k][n].  One of M, N and K counts packed rows: its extent is *cnt.
+// C (M x N) = sum over k of A and B, operands of PARTS 16-bit parts.  AK: A is stored [m][k], else
+// [k][m]; BK: B is stored [n][k], else [k][n].  One of M, N and K counts packed rows: its extent
+// is *cnt.
 struct Prod {
     const uint16_t *A, *B;
     int lda, ldb;
@@ -281,78 +487,127 @@ struct Prod {
 };
 enum { TOK_M, TOK_N, TOK_K };
 
-// One operand's DMA for 32-k stages of a 256-wide tile: as FastOperand, with a resource per stage
-// whose base is the stage's first element and whose range ends with the operand's rows, so
-// operands of any size keep 32-bit offsets and what lies behind the rows reads as zero.
-template <bool KC>
-struct Stager {
-    FastOperand<KC, 8> f;
-    uint32_t last[FastOperand<KC, 8>::PER];   // offsets in the stage that K ends in
-    const uint16_t* base;    // the tile's first element
-    int ld, rows, K;         // rows: of the tile (KC)
+// One operand's tile of T rows (of m or n) and stages of BK k in LDS, by WAVES waves.  Filled by
+// direct DMA in blocks of 1 KB (lane l's 16 bytes land at 16 l), read as MFMA fragments of 32 rows
+// and 16 k.  16-byte chunks, swizzled so that neither kind of read meets bank conflicts:
+//   KC   [T rows][BK k]: chunk c of row r at c ^ (r / 4 % 4) (BK = 32) or c ^ (r / 2 % 8) (64);
+//        a fragment is one 16-byte read
+//   else [BK k][T]: chunk c of row k at c ^ 4 (k % 4), for T = 64 (two rows in the 64 banks)
+//        c ^ 4 (k / 2 % 2); a fragment is two transposing reads
+// A resource per stage whose base is the stage's first element and whose range ends with the
+// operand's rows: operands of any size keep 32-bit offsets, and what lies behind the rows reads as
+// zero.  PAIR (KC): tile row 32 b + i of each 64 is row 2 i + b, so that a lane's two blocks of 32
+// columns are neighbours.
+template <bool KC, int T, int BK, int WAVES, bool PAIR>
+struct Operand {
+    static constexpr int PER = T * BK / 512 / WAVES;   // blocks per wave
+    static constexpr int CPR = KC ? BK / 8 : T / 8;    // chunks in a row
+    static_assert(PER >= 1 && (!PAIR || KC), "tile shapes");
+    uint32_t off[PER];
+    uint32_t last[KC ? PER : 1];   // offsets in the stage that K ends in
+    const uint16_t* base;          // the tile's first element
+    int ld, rows, K;               // rows: of the tile (KC), or its first column
+
+    __device__ static int swizzle(int r) {
+        if (KC) return BK == 32 ? (r >> 2) & 3 : (r >> 1) & 7;
+        return T == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
+    }
     __device__ void init(const uint16_t* p, int ld_, int t0, int extent, int K_, int wave, int lane) {
         ld = ld_;
         K = K_;
-        f.init(ld, 0, 0, wave, lane);
         base = KC ? p + (size_t)t0 * ld : p + t0;
-        rows = KC ? min(extent - t0, 256) : t0;
-        if (KC) {
+        rows = KC ? min(extent - t0, T) : t0;
 #pragma unroll
-            for (int t = 0; t < f.PER; ++t) {
-                const int c = (lane & 3) ^ ((lane >> 4) & 3);
-                // chunks past K (a multiple of 8) lie outside the resource
-                last[t] = 8 * c < (K & 31) ? f.off[t] : 0xFFFFFFF0u;
-            }
+        for (int t = 0; t < PER; ++t) {
+            int r = 64 / CPR * (PER * wave + t) + lane / CPR;   // row of the LDS tile
+            const int c = (lane % CPR) ^ swizzle(r);
+            if (PAIR) r = (r & ~63) + 2 * (r & 31) + ((r >> 5) & 1);
+            off[t] = 2u * ((uint32_t)r * ld + 8 * c);
+            // chunks past K (a multiple of 8) lie outside the resource
+            if (KC) last[t] = 8 * c < K % BK ? off[t] : 0xFFFFFFF0u;
         }
     }
     __device__ void issue(long long plane, int kt, uint16_t* lds, int wave) const {
-        const uint16_t* p = base + plane + (KC ? (size_t)kt * 32 : (size_t)kt * 32 * ld);
-        const uint32_t bytes =
-            KC ? 2u * ((uint32_t)rows * ld - 32u * kt)
-               : 2u * ((uint32_t)min(K - 32 * kt, 32) * ld - (uint32_t)rows);
+        const uint16_t* p = base + plane + (KC ? (size_t)kt * BK : (size_t)kt * BK * ld);
+        const uint32_t bytes = KC ? 2u * ((uint32_t)rows * ld - (uint32_t)(BK * kt))
+                                  : 2u * ((uint32_t)min(K - BK * kt, BK) * ld - (uint32_t)rows);
         const u32x4 rs = make_rsrc(p, bytes);
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(lds) + 1024u * f.PER * wave);
-        const bool end = KC && 32 * kt + 32 > K;
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(lds) + 1024u * PER * wave);
+        const bool end = KC && BK * kt + BK > K;
 #pragma unroll
-        for (int t = 0; t < f.PER; ++t)
-            lds_dma16_buf_so(KC && end ? last[t] : f.off[t], rs, 0u, to + 1024u * t);
+        for (int t = 0; t < PER; ++t)
+            lds_dma16_buf_so(KC && end ? last[KC ? t : 0] : off[t], rs, 0u, to + 1024u * t);
+    }
+    // Tile rows o .. o + 31, 16-k step kk of the stage.
+    __device__ static bf16x8 frag(const uint16_t* lds, int o, int kk, int lane) {
+        const int h = lane >> 5;
+        if constexpr (KC) {
+            const int r = o + (lane & 31);
+            return *reinterpret_cast<const bf16x8*>(lds + r * BK + 8 * ((2 * kk + h) ^ swizzle(r)));
+        } else {
+            const int i = lane & 15, n = o + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+            s16x4 r[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int k = 16 * kk + 8 * h + 4 * q + (i >> 2);
+                r[q] = ds_read_tr(lds + k * T + 8 * ((n >> 3) ^ swizzle(k)) + 4 * ((n >> 2) & 1));
+            }
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
     }
 };
 
-// Pairs of parts in the order they are added (see the head of the file).
-template <int PLANES>
-__device__ inline void pair_of(int s, int& a, int& b) {
-    if (PLANES == 1) {
-        a = b = 0;
-        return;
-    }
-    constexpr uint32_t PA = 0x210100u, PB = 0x012010u;   // a digit per pair, the first on the left
-    a = (PA >> (4 * (5 - s))) & 0xF;
-    b = (PB >> (4 * (5 - s))) & 0xF;
+template <int PARTS, int FM, int FN>
+__device__ inline void mfma_parts(const bf16x8 (&fa)[FM], const bf16x8 (&fb)[FN], f32x16 (&acc)[FM][FN]) {
+#pragma unroll
+    for (int a = 0; a < FM; ++a)
+#pragma unroll
+        for (int b = 0; b < FN; ++b) {
+            if constexpr (PARTS == 1)
+                acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[a], fb[b], acc[a][b], 0, 0, 0);
+            else
+                acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    __builtin_bit_cast(f16x8, fa[a]), __builtin_bit_cast(f16x8, fb[b]), acc[a][b], 0, 0, 0);
+        }
 }
 
-// 256 x 256 tile, 8 waves of 128 x 64, 32-k stages through a ring of four in LDS filled by
-// direct DMA three stages ahead; each stage's two 16-k steps run while the next operands are
-// read (the schedule of the bf16 GEMM's 8-wave form).  Epi::run gets the tile's accumulators:
-// register r of block (a, b) is row m0 + wm + 32 a + 8 (r / 4) + 4 h + r % 4, column
-// n0 + wn + 32 b + l32 (lane = 32 h + l32).
-template <bool AK, bool BK, int TOK, int PLANES, class Epi>
-__global__ void __launch_bounds__(512) vocab_gemm(Prod g, Epi epi) {
-    constexpr int FM = 4, FN = 2, PAIRS = PLANES == 1 ? 1 : 6;
-    using OA = FastOperand<AK, 8>;
-    using OB = FastOperand<BK, 8>;
-    __shared__ __attribute__((aligned(16))) uint16_t ring[FAST_NSTAGE * 2 * FAST_TILE];
+// Tiles: 256 x 256 by 8 waves of 128 x 64 and 128 x 128 by 4 waves of 64 x 64, stages of 32 k; 64 x 64
+// by 4 waves of 32 x 32, stages of 64 k (few work-groups: half the barriers, and whole 128-byte
+// lines of a k-contiguous operand).
+template <int T_>
+struct Shape {
+    static constexpr int T = T_, BK = T == 64 ? 64 : 32, NS = 4;
+    static constexpr int WAVES = T == 256 ? 8 : 4;
+    static constexpr int WAVES_N = T == 256 ? 4 : 2;
+    static constexpr int WM = T * WAVES_N / WAVES, WN = T / WAVES_N;
+    static constexpr int FM = WM / 32, FN = WN / 32;
+    static constexpr int STAGE = 2 * T * BK;   // elements
+    static constexpr int THREADS = 64 * WAVES;
+};
+
+// One tile of one split: stages of BK k through a ring of four in LDS filled by direct DMA three
+// stages ahead; a stage's 16-k steps run while the next operands are read (the schedule of the
+// bf16 GEMM's 8-wave form).  Epi::run gets the tile's accumulators: register r of block (a, b) is
+// row m0 + wm + 32 a + 8 (r / 4) + 4 h + r % 4, column n0 + wn + 32 b + l32, or with Epi::PAIR and
+// two blocks n0 + wn + 2 l32 + b (lane = 32 h + l32).
+template <class S, bool AK, bool BK_, int TOK, int PARTS, class Epi>
+__device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, int tile, int tiles,
+                                 int split) {
+    constexpr int FM = S::FM, FN = S::FN, BK = S::BK, NS = S::NS, STEPS = BK / 16;
+    constexpr bool PAIR = BK_ && Epi::PAIR && FN == 2;
+    using OA = Operand<AK, S::T, BK, S::WAVES, false>;
+    using OB = Operand<BK_, S::T, BK, S::WAVES, PAIR>;
+    constexpr int BOFF = S::T * BK, LOADS = OA::PER + OB::PER;
     const int cnt = *g.cnt;
     const int M = TOK == TOK_M ? cnt : g.M, N = TOK == TOK_N ? cnt : g.N;
     const int Kall = TOK == TOK_K ? cnt : g.K;
-    const int tiles_m = (g.M + 255) / 256, tiles_n = (g.N + 255) / 256;
     int tm, tn;
-    xcd_tile_order(blockIdx.x, gridDim.x, tiles_m, tiles_n, 4, tm, tn);
-    const int m0 = tm * 256, n0 = tn * 256;
+    xcd_tile_order(tile, tiles, (g.M + S::T - 1) / S::T, (g.N + S::T - 1) / S::T, 4, tm, tn);
+    const int m0 = tm * S::T, n0 = tn * S::T;
     if (m0 >= M || n0 >= N) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = (wave / 4) * 128, wn = (wave % 4) * 64;
+    const int wm = (wave / S::WAVES_N) * S::WM, wn = (wave % S::WAVES_N) * S::WN;
 
     f32x16 acc[FM][FN];
 #pragma unroll
@@ -362,153 +617,228 @@ __global__ void __launch_bounds__(512) vocab_gemm(Prod g, Epi epi) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
 
-    const int kt0 = blockIdx.y * g.kstages;
-    const int nk = max(0, min((Kall + 31) / 32 - kt0, g.kstages));
-    const int total = nk * PAIRS;
+    const int kt0 = split * g.kstages;
+    const int nk = max(0, min((Kall + BK - 1) / BK - kt0, g.kstages));
+    // two parts: lo hi, hi lo, then (from stage `cross` on) hi hi
+    const int total = PARTS == 1 ? nk : 3 * nk, cross = 2 * nk;
     if (total > 0) {
-        Stager<AK> sa;
-        Stager<BK> sb;
+        OA sa;
+        OB sb;
         sa.init(g.A, g.lda, m0, M, Kall, wave, lane);
         sb.init(g.B, g.ldb, n0, N, Kall, wave, lane);
         int ikt = 0, ipair = 0, islot = 0;   // the next stage to fetch
         auto issue = [&]() {
-            int pa, pb;
-            pair_of<PLANES>(ipair, pa, pb);
-            uint16_t* st = ring + islot * 2 * FAST_TILE;
-            sa.issue(pa * g.pa, kt0 + ikt, st, wave);
-            sb.issue(pb * g.pb, kt0 + ikt, st + FAST_TILE, wave);
-            islot = (islot + 1) % FAST_NSTAGE;
+            uint16_t* st = ring + islot * S::STAGE;
+            sa.issue(PARTS == 2 && ipair == 0 ? g.pa : 0, kt0 + ikt, st, wave);
+            sb.issue(PARTS == 2 && ipair == 1 ? g.pb : 0, kt0 + ikt, st + BOFF, wave);
+            islot = (islot + 1) % NS;
             if (++ikt == nk) {
                 ikt = 0;
                 ++ipair;
             }
         };
-        auto stage = [&](int s) { return ring + (s % FAST_NSTAGE) * 2 * FAST_TILE; };
-        const int pre = min(total, FAST_NSTAGE - 1);
+        auto landed = [&](int ahead) {   // all but the youngest `ahead` stages
+            if (ahead >= 2) wait_vmcnt<2 * LOADS>();
+            else if (ahead == 1) wait_vmcnt<LOADS>();
+            else wait_vmcnt<0>();
+        };
+        auto scale_cross = [&](int s) {
+            if (PARTS == 2 && s == cross)
+#pragma unroll
+                for (int a = 0; a < FM; ++a)
+#pragma unroll
+                    for (int b = 0; b < FN; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[a][b][r] *= 0x1p-11f;
+        };
+        auto read = [&](int s, int kk, bf16x8 (&fa)[FM], bf16x8 (&fb)[FN]) {
+            const uint16_t* st = ring + (s % NS) * S::STAGE;
+#pragma unroll
+            for (int x = 0; x < FM; ++x) fa[x] = OA::frag(st, wm + 32 * x, kk, lane);
+#pragma unroll
+            for (int x = 0; x < FN; ++x) fb[x] = OB::frag(st + BOFF, wn + 32 * x, kk, lane);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        bf16x8 fa[2][FM], fb[2][FN];
+        auto mma = [&](int f) {
+            mfma_parts<PARTS, FM, FN>(fa[f], fb[f], acc);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto inner = [&](int s) {   // all steps but the last, whose operands it reads
+            scale_cross(s);
+#pragma unroll
+            for (int kk = 0; kk < STEPS - 1; ++kk) {
+                read(s, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
+                mma(kk & 1);
+            }
+        };
+        const int pre = min(total, NS - 1);
         for (int s = 0; s < pre; ++s) issue();
-        static_assert(OA::PER == 2 && OB::PER == 2, "wait_dma_stages<4>: 4 loads per stage");
-        wait_dma_stages<4>(pre - 1);
+        landed(pre - 1);
         __syncthreads();
-        bf16x8 f0a[FM], f0b[FN], f1a[FM], f1b[FN];
-        load_frags<OA, OB, FM, FN>(stage(0), 0, wm, wn, lane, f0a, f0b);
+        read(0, 0, fa[0], fb[0]);
         for (int s = 0; s < total - 1; ++s) {
-            if (s + FAST_NSTAGE - 1 < total) issue();
-            load_frags<OA, OB, FM, FN>(stage(s), 1, wm, wn, lane, f1a, f1b);
-            __builtin_amdgcn_sched_barrier(0);
-            mfma_block<FM, FN>(f0a, f0b, acc);
-            __builtin_amdgcn_sched_barrier(0);
-            const int ahead = min(total - 1, s + FAST_NSTAGE - 1) - (s + 1);
+            if (s + NS - 1 < total) issue();
+            inner(s);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            wait_dma_stages<4>(ahead);
+            landed(min(total - 1, s + NS - 1) - (s + 1));
             __syncthreads();
-            load_frags<OA, OB, FM, FN>(stage(s + 1), 0, wm, wn, lane, f0a, f0b);
-            __builtin_amdgcn_sched_barrier(0);
-            mfma_block<FM, FN>(f1a, f1b, acc);
-            __builtin_amdgcn_sched_barrier(0);
+            read(s + 1, 0, fa[0], fb[0]);
+            mma(1);
         }
-        load_frags<OA, OB, FM, FN>(stage(total - 1), 1, wm, wn, lane, f1a, f1b);
-        __builtin_amdgcn_sched_barrier(0);
-        mfma_block<FM, FN>(f0a, f0b, acc);
-        mfma_block<FM, FN>(f1a, f1b, acc);
+        inner(total - 1);
+        mma(1);
     }
-    epi.template run<FM, FN>(acc, M, N, m0 + wm, n0 + wn, lane);
+    epi.template run<FM, FN>(acc, M, N, m0 + wm, n0 + wn, lane, split);
+}
+
+template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
+__global__ void __launch_bounds__(S::THREADS) vocab_gemm(Prod g, Epi epi) {
+    __shared__ __attribute__((aligned(16))) uint16_t ring[S::NS * S::STAGE];
+    gemm_tile<S, AK, BK, TOK, PARTS>(ring, g, epi, blockIdx.x, gridDim.x, blockIdx.y);
+}
+
+// dH and dW of a piece in one launch: the first `first` work-groups are dH's, splits one after the
+// other.
+template <class S, int PARTS, class EpiH, class EpiW>
+__global__ void __launch_bounds__(S::THREADS) vocab_grads(Prod gh, EpiH eh, int tiles_h, int first, Prod gw,
+                                                          EpiW ew, int tiles_w) {
+    __shared__ __attribute__((aligned(16))) uint16_t ring[S::NS * S::STAGE];
+    const int b = blockIdx.x;
+    if (b < first)
+        gemm_tile<S, true, false, TOK_M, PARTS>(ring, gh, eh, b % tiles_h, tiles_h, b / tiles_h);
+    else
+        gemm_tile<S, false, false, TOK_K, PARTS>(ring, gw, ew, (b - first) % tiles_w, tiles_w,
+                                                 (b - first) / tiles_w);
 }
 
 // Row of register r of block a, relative to the wave's first row.
 __device__ inline int reg_row(int a, int r, int lane) { return 32 * a + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
 
-// Forward: rows are table rows, columns packed rows.  A lane holds 64 logits of each of its
-// columns, the other half's lane the wave's other 64: maximum and sum of exponentials of the
-// wave's 128 go to part[128-row block][column].
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Forward: rows are table rows, columns packed rows.  A lane holds half of the wave's logits of
+// each of its columns, lane + 32 the other half: their maximum and sum of exponentials go to
+// part[the wave's block of 32 FM rows][column].
+template <int PARTS>
 struct EpiLse {
+    static constexpr bool PAIR = false;
     float c;
+    const int *e, *h;      // exponents of the table's and the packed rows' scales (two parts)
     float2* part;
     int ldp;
     template <int FM, int FN>
-    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane) const {
+    __device__ void run(f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int) const {
         if (row0 >= M) return;   // the wave has no table row: its block is not joined either
+        const bool full = row0 + 32 * FM <= M;
+        float kc[FN];
+#pragma unroll
+        for (int b = 0; b < FN; ++b)
+            kc[b] = PARTS == 1 ? c : __builtin_ldexpf(c, h[col0 + 32 * b + (lane & 31)]);
+        // logits in place; -inf past the table's end
+#pragma unroll
+        for (int a = 0; a < FM; ++a)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int row = row0 + reg_row(a, 4 * r4, lane);
+                i32x4 e4;
+                if constexpr (PARTS == 2) e4 = *reinterpret_cast<const i32x4*>(e + row);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int b = 0; b < FN; ++b) {
+                        const float z =
+                            acc[a][b][4 * r4 + q] * (PARTS == 1 ? kc[b] : __builtin_ldexpf(kc[b], e4[q]));
+                        acc[a][b][4 * r4 + q] = full || row + q < M ? z : -INFINITY;
+                    }
+            }
 #pragma unroll
         for (int b = 0; b < FN; ++b) {
             float mx = -INFINITY;
-            bool full = row0 + 128 <= M;
 #pragma unroll
             for (int a = 0; a < FM; ++a)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (full || row0 + reg_row(a, r, lane) < M) mx = fmaxf(mx, c * acc[a][b][r]);
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[a][b][r]);
             mx = fmaxf(mx, xor32(mx));
             const float m = mx == -INFINITY ? 0.f : mx;   // all -inf: a sum of zeros, not of NaN
             float s = 0.f;
 #pragma unroll
             for (int a = 0; a < FM; ++a)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (full || row0 + reg_row(a, r, lane) < M) s += __expf(c * acc[a][b][r] - m);
+                for (int r = 0; r < 16; ++r) s += __expf(acc[a][b][r] - m);
             s += xor32(s);
             const int col = col0 + 32 * b + (lane & 31);
-            if (lane < 32 && col < N) part[(size_t)(row0 / 128) * ldp + col] = float2{mx, s};
+            if (lane < 32 && col < N) part[(size_t)(row0 / (32 * FM)) * ldp + col] = float2{mx, s};
         }
     }
 };
 
-// Backward: rows are packed rows, columns the piece's table rows.  G as bf16 (parts): one
-// rounding of each entry of G to the type that the products take (in three parts, to 24 bits).
-// Columns past the table's end up to the tile's are zero.
-template <int PLANES, bool HARD>
+// Backward: rows are packed rows, columns the piece's table rows.  One part: G = w (p - q), rounded
+// once to bf16, the type that the products take.  Two parts: 2^14 (p - q) to 22 bits.  Columns past
+// the table's end up to the tile's are zero.  Two blocks of columns are neighbours in a lane, so a
+// store instruction writes whole 128-byte lines of two rows.
+template <int PARTS, bool HARD>
 struct EpiG {
+    static constexpr bool PAIR = true;
     float c;
     const float *lse, *w;
-    const int* target;
+    const int *target, *h, *E;
     int v0;
     uint16_t* G;
     int ldg;
     long long plane;
     template <int FM, int FN>
-    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane) const {
+    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int) const {
+        int col[FN];
+#pragma unroll
+        for (int b = 0; b < FN; ++b) col[b] = col0 + (FN == 2 ? 2 * (lane & 31) + b : lane & 31);
+        const int table = PARTS == 1 ? 0 : *E;
 #pragma unroll
         for (int a = 0; a < FM; ++a)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int row = row0 + reg_row(a, 4 * r4, lane);
                 const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + row);
-                const f32x4 w4 = *reinterpret_cast<const f32x4*>(w + row);
-                int t4[4];
-                if constexpr (HARD)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) t4[e] = target[row + e] - v0;
+                f32x4 w4;
+                i32x4 t4, h4;
+                if constexpr (PARTS == 1) w4 = *reinterpret_cast<const f32x4*>(w + row);
+                if constexpr (PARTS == 2) h4 = *reinterpret_cast<const i32x4*>(h + row);
+                if constexpr (HARD) t4 = *reinterpret_cast<const i32x4*>(target + row);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (row + e >= M) continue;
+                    const float k = PARTS == 1 ? c : __builtin_ldexpf(c, h4[e] + table);
+                    const float f = PARTS == 1 ? w4[e] : 0x1p14f;
+                    uint16_t v[FN][PARTS];
 #pragma unroll
                     for (int b = 0; b < FN; ++b) {
-                        const int col = col0 + 32 * b + (lane & 31);
-                        float p = __expf(__builtin_fmaf(c, acc[a][b][4 * r4 + e], -l4[e]));
+                        float p = __expf(__builtin_fmaf(k, acc[a][b][4 * r4 + e], -l4[e]));
                         if constexpr (HARD)
-                            if (col == t4[e]) p -= 1.f;
-                        const float v = col < N ? w4[e] * p : 0.f;
-                        uint16_t* to = G + (size_t)(row + e) * ldg + col;
-                        if constexpr (PLANES == 1) {
-                            *to = rne_bf16(v);
-                        } else {
-                            uint16_t x[3];
-                            split3(v, x);
+                            if (col[b] == t4[e] - v0) p -= 1.f;
+                        to_parts<PARTS>(col[b] < N ? f * p : 0.f, v[b]);
+                    }
+                    uint16_t* to = G + (size_t)(row + e) * ldg + col[0];
 #pragma unroll
-                            for (int q = 0; q < 3; ++q) to[q * plane] = x[q];
-                        }
+                    for (int q = 0; q < PARTS; ++q) {
+                        if constexpr (FN == 2)
+                            *reinterpret_cast<uint32_t*>(to + q * plane) = v[0][q] | ((uint32_t)v[1][q] << 16);
+                        else
+                            to[q * plane] = v[0][q];
                     }
                 }
             }
     }
 };
 
-// dH: fp32 sums over the pieces, one block per split of the piece.
+// fp32 sums over the pieces (dH), one block per split.
 struct EpiAcc {
+    static constexpr bool PAIR = false;
     float* C;
     int ldc, first;
     long long split;
     template <int FM, int FN>
-    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane) const {
-        float* p = C + blockIdx.y * split;
+    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int s) const {
+        float* p = C + s * split;
 #pragma unroll
         for (int a = 0; a < FM; ++a)
 #pragma unroll
@@ -526,31 +856,50 @@ struct EpiAcc {
     }
 };
 
-// dW: the piece's rows of the gradient, in its type.
+// A gradient's rows and their scales: dH's packed rows go to their places, times w_n 2^(E - 14) with
+// two parts; dW's stay in order, times 2^(X - 14).
 template <typename OT>
-struct EpiOut {
+struct Grad {
     OT* C;
     int ldc, accumulate;
+    const int *row, *exp;
+    const float* w;
+    __device__ int scale() const { return exp ? *exp - 14 : 0; }
+    __device__ float weight(int i) const { return w ? w[i] : 1.f; }
+    __device__ OT* at(int i) const { return C + (size_t)(row ? row[i] : i) * ldc; }
+    __device__ void put(OT* to, float v) const {
+        if constexpr (sizeof(OT) == 4) {
+            *to = accumulate ? *to + v : v;
+        } else {
+            if (accumulate) v += bf16_bits_to_f32(*to);
+            *to = rne_bf16(v);
+        }
+    }
+};
+
+// A gradient from its only split and piece.
+template <int PARTS, typename OT>
+struct EpiOut {
+    static constexpr bool PAIR = false;
+    Grad<OT> out;
     template <int FM, int FN>
-    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane) const {
+    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int) const {
+        const int s = PARTS == 1 ? 0 : out.scale();
 #pragma unroll
         for (int a = 0; a < FM; ++a)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int row = row0 + reg_row(a, r, lane);
                 if (row >= M) continue;
+                OT* to = out.at(row);
+                const float w = PARTS == 1 ? 1.f : out.weight(row);
 #pragma unroll
                 for (int b = 0; b < FN; ++b) {
                     const int col = col0 + 32 * b + (lane & 31);
                     if (col >= N) continue;
-                    OT* to = C + (size_t)row * ldc + col;
                     float v = acc[a][b][r];
-                    if constexpr (sizeof(OT) == 4) {
-                        *to = accumulate ? *to + v : v;
-                    } else {
-                        if (accumulate) v += bf16_bits_to_f32(*to);
-                        *to = rne_bf16(v);
-                    }
+                    if constexpr (PARTS == 2) v = __builtin_ldexpf(v, s) * w;
+                    out.put(to + col, v);
                 }
             }
     }
@@ -564,17 +913,42 @@ __device__ inline void lse_merge(float& m, float& s, float m2, float s2) {
     m = mx;
 }
 
-// A work-group per 64 packed rows, 16 waves that share the piece's 128-row blocks; their results
-// meet in LDS in wave order.  state: what earlier pieces left (first: nothing).  The last piece
-// writes lse and loss = factor (lse + base).
+// The end of a row's join: what earlier pieces left (first: nothing) merged with this piece's, kept
+// for the next, or the row's lse and loss = factor (lse + base) from the last.
+struct JoinOut {
+    Rows rows;
+    float2* state;
+    int first, last;
+    const float* base;
+    float factor;
+    float *loss, *lse;
+    __device__ void put(int i, float m, float s) const {
+        if (!first) {
+            const float2 p = state[i];
+            float m0 = p.x, s0 = p.y;
+            lse_merge(m0, s0, m, s);
+            m = m0;
+            s = s0;
+        }
+        if (!last) {
+            state[i] = float2{m, s};
+            return;
+        }
+        const int n = rows.row[i];
+        const float l = m + __logf(s);
+        if (lse) lse[n] = l;
+        loss[n] = factor * (l + base[i]);
+    }
+};
+
+// A work-group per 64 packed rows, 16 waves that share the piece's blocks of table rows; their
+// results meet in LDS in wave order.
 __global__ void __launch_bounds__(1024) lse_join(const float2* __restrict__ part, int ldp, int blocks,
-                                                 Rows rows, float2* __restrict__ state, int first,
-                                                 int last, const float* __restrict__ base, float factor,
-                                                 float* __restrict__ loss, float* __restrict__ lse) {
+                                                 JoinOut out) {
     __shared__ float2 red[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int i = blockIdx.x * 64 + lane;
-    const int cnt = *rows.cnt;
+    const int cnt = *out.rows.cnt;
     if ((int)blockIdx.x * 64 >= cnt) return;
     float m = -INFINITY, s = 0.f;
     if (i < cnt)
@@ -585,26 +959,39 @@ __global__ void __launch_bounds__(1024) lse_join(const float2* __restrict__ part
     red[w][lane] = float2{m, s};
     __syncthreads();
     if (w != 0 || i >= cnt) return;
-    if (!first) {
-        const float2 p = state[i];
-        m = p.x;
-        s = p.y;
-        lse_merge(m, s, red[0][lane].x, red[0][lane].y);
-    }
+    m = red[0][lane].x;
+    s = red[0][lane].y;
     for (int x = 1; x < 16; ++x) lse_merge(m, s, red[x][lane].x, red[x][lane].y);
-    if (!last) {
-        state[i] = float2{m, s};
-        return;
+    out.put(i, m, s);
+}
+
+// Few rows: a work-group per packed row, its 256 threads share the blocks.  The lanes' results
+// meet at distances 1 to 32, the waves' in wave order.
+__global__ void __launch_bounds__(256) lse_join_few(const float2* __restrict__ part, int ldp, int blocks,
+                                                    JoinOut out) {
+    __shared__ float2 red[4];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int i = blockIdx.x;
+    if (i >= *out.rows.cnt) return;
+    float m = -INFINITY, s = 0.f;
+    for (int b = threadIdx.x; b < blocks; b += 256) {
+        const float2 p = part[(size_t)b * ldp + i];
+        lse_merge(m, s, p.x, p.y);
     }
-    const int n = rows.row[i];
-    const float l = m + __logf(s);
-    if (lse) lse[n] = l;
-    loss[n] = factor * (l + base[i]);
+    for (int x = 1; x < 64; x <<= 1) {
+        const float m2 = __shfl_xor(m, x, 64), s2 = __shfl_xor(s, x, 64);
+        lse_merge(m, s, m2, s2);
+    }
+    if (lane == 0) red[w] = float2{m, s};
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int x = 1; x < 4; ++x) lse_merge(m, s, red[x].x, red[x].y);
+    out.put(i, m, s);
 }
 
 // The entries of G at the teacher's tokens inside a piece, from the fp32 logits: w (p - q), q
 // summed where a token occurs more than once (each of its entries writes the same value).
-template <int PLANES>
+template <int PARTS>
 __global__ void __launch_bounds__(256) teacher_entries(Rows rows, Teacher t, int V, int v0, int R,
                                                        const float* __restrict__ q,
                                                        const float* __restrict__ z,
@@ -613,49 +1000,50 @@ __global__ void __launch_bounds__(256) teacher_entries(Rows rows, Teacher t, int
     const int i = blockIdx.x;
     if (i >= *rows.cnt) return;
     const size_t at = (size_t)rows.row[i] * t.K, from = (size_t)i * t.K;
-    const float w = rows.w[i], lse = rows.lse[i];
+    const float w = PARTS == 1 ? rows.w[i] : 0x1p14f, lse = rows.lse[i];
     for (int k = threadIdx.x; k < t.K; k += 256) {
         const int id = t.id[at + k];
         if (id < v0 || id >= v0 + R || !entry_counts(t, at + k, V)) continue;
         float sum = 0.f;
         for (int j = 0; j < t.K; ++j)
             if (t.id[at + j] == id) sum += q[from + j];
-        const float v = w * (__expf(z[from + k] - lse) - sum);
+        uint16_t parts[PARTS];
+        to_parts<PARTS>(w * (__expf(z[from + k] - lse) - sum), parts);
         uint16_t* to = G + (size_t)i * ldg + (id - v0);
-        if constexpr (PLANES == 1) {
-            *to = rne_bf16(v);
-        } else {
-            uint16_t x[3];
-            split3(v, x);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) to[p * plane] = x[p];
-        }
+        for (int p = 0; p < PARTS; ++p) to[p * plane] = parts[p];
     }
 }
 
-// dH (+)= the splits' sums, row by row in the callers' order; zero (or unchanged) for padding.
+// A gradient (+)= the sum of its splits, in their order.  Four columns per thread.
 template <typename OT>
-__global__ void __launch_bounds__(256) dh_finish(const int* __restrict__ inv, int N, int D,
-                                                 const float* __restrict__ acc, int lda, int splits,
-                                                 long long split, OT* __restrict__ dH, int ldd,
-                                                 int accumulate) {
-    const int lane = threadIdx.x & 63;
-    const long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= N) return;
-    const int i = inv[n];
-    if (i < 0 && accumulate) return;
-    for (int c = lane; c < D; c += 64) {
-        float v = 0.f;
-        if (i >= 0)
-            for (int s = 0; s < splits; ++s) v += acc[s * split + (size_t)i * lda + c];
-        OT* to = dH + (size_t)n * ldd + c;
-        if constexpr (sizeof(OT) == 4) {
-            *to = accumulate ? *to + v : v;
-        } else {
-            if (accumulate) v += bf16_bits_to_f32(*to);
-            *to = rne_bf16(v);
-        }
-    }
+struct Finish {
+    Grad<OT> out;
+    const float* acc;
+    int rows, lda, splits;
+    long long split;
+    const int* cnt;          // rows that count, or null: all
+    long long groups;        // work-groups of 256 threads
+};
+template <int PARTS, typename OT>
+__global__ void __launch_bounds__(256) finish(Finish<OT> h, Finish<OT> w, int D) {
+    const bool second = blockIdx.x >= h.groups;
+    const Finish<OT>& f = second ? w : h;
+    const int quads = (D + 3) / 4;
+    const long long t = (blockIdx.x - (second ? h.groups : 0)) * 256 + threadIdx.x;
+    const long long i = t / quads;
+    const int c = 4 * (int)(t % quads);
+    if (i >= (f.cnt ? *f.cnt : f.rows)) return;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < f.splits; ++s)
+        v += *reinterpret_cast<const f32x4*>(f.acc + s * f.split + (size_t)i * f.lda + c);
+    const int e = PARTS == 1 ? 0 : f.out.scale();
+    const float wi = PARTS == 1 ? 1.f : f.out.weight((int)i);
+    OT* to = f.out.at((int)i) + c;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (c + q < D) f.out.put(to + q, PARTS == 1 ? v[q] : __builtin_ldexpf(v[q], e) * wi);
 }
 
 // The gradient of no rows at all (N = 0).
@@ -682,47 +1070,94 @@ struct Head {
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+// A product's tile.
+enum Kind { T256, T128, T64 };
+int side(Kind t) { return t == T256 ? 256 : t == T128 ? 128 : 64; }
+int wave_rows(Kind t) { return side(t) / 2; }
+long long tiles_of(Kind t, long long M, long long N) {
+    return ((M + side(t) - 1) / side(t)) * ((N + side(t) - 1) / side(t));
+}
+// Splits of K over work-groups where sums of splits are added afterwards: towards one round of
+// work-groups, at least 512 k each.
+int splits_of(Kind t, long long M, long long N, long long K) {
+    const long long tiles = tiles_of(t, M, N), want = t == T256 ? 256 : 512;
+    long long s = tiles > 0 ? want / tiles : 1;
+    if (s > K / 512) s = K / 512;
+    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+// Estimated time of a product in us, the rule that picks its tile: rounds of work-groups (a last
+// round that is not full counts half of what it lacks) times their 32-k stages, each of the time
+// measured with one work-group on a CU or with as many as fit.  Measured / estimated, 256, 128 and
+// 64 wide: 1000 x 5000 x 256 fp32 29, 23, 24 / 28, 19, 23 us; 1000 x 2048 x 1024 bf16 28, 16, 11 /
+// 36, 16, 11; 32000 x 600 x 2048 bf16 119, 115, 161 / 118, 126, 202.
+double estimate(Kind t, long long M, long long N, long long K, int parts, bool split) {
+    static const double alone[] = {1.0, 0.45, 0.19}, full[] = {1.0, 0.68, 0.30};
+    static const int fit[] = {1, 2, 2};
+    const int s = split ? splits_of(t, M, N, K) : 1;
+    const double groups = (double)tiles_of(t, M, N) * s;
+    const double stages = (double)((K + 31) / 32) * (parts == 2 ? 3 : 1) / s + 4;
+    double rounds = groups / (256 * fit[t]);
+    const double whole = (double)(long long)(rounds + 0.9999);
+    rounds = rounds <= 1 ? 1 : (rounds + whole) / 2;
+    return rounds * stages * (groups <= 256 ? alone[t] : full[t]) +
+           (s > 1 ? 3 + (double)s * M * N * 8 / 4e6 : 0);
+}
+Kind pick(long long M, long long N, long long K, int parts, bool split) {
+    Kind best = T64;
+    for (Kind t : {T128, T256})
+        if (estimate(t, M, N, K, parts, split) < estimate(best, M, N, K, parts, split)) best = t;
+    return best;
+}
+
 // The workspace: a part whose size the shapes give, and a piece whose size is what is left.
 struct Plan {
-    int planes, Dp, Nt;       // parts of an operand, padded columns, rows padded to whole tiles
+    int parts, Dp, Nt;        // parts of an operand, padded columns, rows padded to whole tiles
     bool direct;              // the table is read in place
-    size_t ints, w, lse, base, q, z, state, Hp, acc;
-    int splits;
+    Kind lse, g, dh, dw;      // the products' tiles
+    int splits, wsplits;      // of dH and dW
+    size_t ints, w, lses, base, q, z, state, Hp, Xp, acc, wacc;
     size_t piece;             // first byte of the piece's buffers
     size_t per_block;         // bytes of a piece per 256 table rows
 };
 
 Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* W, int ldw) {
     Plan p{};
-    p.planes = dtype == DH_F32 ? 3 : 1;
+    p.parts = dtype == DH_F32 ? 2 : 1;
     p.Dp = (D + 31) / 32 * 32;
     p.Nt = (int)(((long long)N + 255) / 256 * 256);
     // In place: whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
     p.direct = dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
+    p.lse = pick(V, N, D, p.parts, false);
+    p.g = pick(N, V, D, p.parts, false);
+    p.dh = pick(N, D, V, p.parts, true);
+    p.dw = pick(V, D, N, p.parts, true);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += up256(bytes);
         return here;
     };
-    p.ints = take(((size_t)4 * p.Nt + 64) * 4);   // cnt, flags, row, inv, target
+    p.ints = take(((size_t)4 * p.Nt + p.Nt / PACK + 64 + SCAN) * 4);   // cnt and scales, row, target, ...
     p.w = take((size_t)p.Nt * 4);
-    p.lse = take((size_t)p.Nt * 4);
+    p.lses = take((size_t)p.Nt * 4);
     p.base = take((size_t)p.Nt * 4);
     p.q = take((size_t)N * K * 4);
     p.z = take((size_t)N * K * 4);
-    p.Hp = take((size_t)p.planes * N * p.Dp * 2);
+    p.Hp = take((size_t)p.parts * N * p.Dp * 2);
     if (backward) {
-        const long long tiles = (long long)(p.Nt / 256) * ((D + 255) / 256);
-        p.splits = tiles >= 256 ? 1 : (int)(256 / (tiles > 0 ? tiles : 1));
-        if (p.splits > 8) p.splits = 8;
+        p.splits = splits_of(p.dh, N, D, V);
         p.acc = take((size_t)p.splits * N * p.Dp * 4);
-        p.per_block = (size_t)p.planes * N * 256 * 2;
+        if (p.parts == 2) p.Xp = take((size_t)p.parts * N * p.Dp * 2);
+        p.per_block = (size_t)p.parts * N * 256 * 2;
+        // dW's sums over splits of the rows: a piece's, fp32.
+        p.wsplits = splits_of(p.dw, V, D, N);
+        if (p.wsplits > 1) p.per_block += (size_t)p.wsplits * 256 * p.Dp * 4;
     } else {
         p.state = take((size_t)p.Nt * 8);
-        p.per_block = (size_t)p.Nt * 2 * 8;
+        p.per_block = (size_t)p.Nt * (256 / wave_rows(p.lse)) * 8;
+        if (p.parts == 2) p.per_block += 1024;
     }
-    if (!p.direct) p.per_block += (size_t)p.planes * 256 * p.Dp * 2;
+    if (!p.direct) p.per_block += (size_t)p.parts * 256 * p.Dp * 2;
     p.piece = at;
     return p;
 }
@@ -764,104 +1199,123 @@ int check_head(const Head& h, int K, const void* ws, size_t ws_bytes, int backwa
 struct Work {
     Plan p;
     Rows rows;
-    float *base, *q, *z;
-    uint16_t* Hp;
+    Exps exps;
     int* flags;
+    float *base, *q, *z, *acc;
+    float2* state;
+    uint16_t *Hp, *Xp;   // Xp: the other operand of dW
     char* piece;
 };
 
-Work lay_out(const Plan& p, void* ws, int N) {
+Work lay_out(const Plan& p, void* ws) {
     char* b = (char*)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
     int* ints = (int*)(b + p.ints);
+    auto array = [&](int k) { return ints + 64 + (size_t)k * p.Nt; };
     Work w{};
     w.p = p;
-    w.rows = {ints, ints + 64, ints + 64 + p.Nt, ints + 64 + 2 * (size_t)p.Nt, (float*)(b + p.w),
-              (float*)(b + p.lse)};
-    w.flags = ints + 64 + 3 * (size_t)p.Nt;
+    w.rows = {ints, array(0), array(1), array(2), (float*)(b + p.w), (float*)(b + p.lses)};
+    w.flags = array(3);
+    w.exps = {nullptr, ints + 1, ints + 2, array(4), (float*)(array(4) + p.Nt / PACK)};
     w.base = (float*)(b + p.base);
     w.q = (float*)(b + p.q);
     w.z = (float*)(b + p.z);
+    w.state = (float2*)(b + p.state);
+    w.acc = (float*)(b + p.acc);
     w.Hp = (uint16_t*)(b + p.Hp);
+    w.Xp = p.parts == 2 ? (uint16_t*)(b + p.Xp) : w.Hp;
     w.piece = b + p.piece;
     return w;
 }
 
-template <typename T, int PLANES>
-int prepare_rows(const Head& h, const Work& w, float* loss, float* lse_out, const float* lse_in,
-                 const float* dloss) {
-    const int* target = h.target;
-    if (!target) {
+// Packs the rows; `more` work-groups of the launch stage table rows or scan the table.
+template <typename T, int PARTS>
+int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
+    a.targets = {h.target, h.teacher, h.V};
+    if (!h.target && (long long)h.N * h.teacher.K > 1 << 16) {
         teacher_flags<<<(h.N + 3) / 4, 256, 0, stream()>>>(h.teacher, h.N, h.V, w.flags);
         DH_TRY(check_launch(h.op));
-        target = w.flags;
+        a.targets.target = w.flags;
     }
-    pack_rows<T, PLANES><<<(h.N + 63) / 64, 1024, 0, stream()>>>(
-        target, h.N, h.V, h.D, (const T*)h.H, h.ldh, w.Hp, w.p.Dp, (long long)h.N * w.p.Dp, w.rows, loss,
-        lse_out, lse_in, dloss, h.wscale);
+    a.N = h.N;
+    a.D = h.D;
+    a.H = h.H;
+    a.ldh = h.ldh;
+    a.W = h.W;
+    a.ldw = h.ldw;
+    a.Hp = w.Hp;
+    a.Dp = w.p.Dp;
+    a.plane = (long long)h.N * w.p.Dp;
+    a.rows = w.rows;
+    a.exps = w.exps;
+    a.groups = (h.N + PACK - 1) / PACK;
+    a.c = h.c;
+    a.wscale = h.wscale;
+    pack_rows<T, PARTS><<<a.groups + more, 1024, 0, stream()>>>(a);
     DH_TRY(check_launch(h.op));
-    if (!h.target)
-        teacher_dots<T><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, (const T*)h.H, h.ldh,
-                                                   (const T*)h.W, h.ldw, h.D, w.q, w.z, w.base);
-    else if (loss)
-        target_dot<T><<<(h.N + 3) / 4, 256, 0, stream()>>>(w.rows, (const T*)h.H, h.ldh, (const T*)h.W,
-                                                           h.ldw, h.D, h.c, w.base);
+    if (h.target) return DH_OK;
+    teacher_dots<T><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, (const T*)h.H, h.ldh, (const T*)h.W,
+                                               h.ldw, h.D, w.q, w.z, w.base);
     return check_launch(h.op);
 }
 
-// The table rows of a piece as a product's operand: in place, or staged at `at`.
-template <typename T, int PLANES>
-int piece_table(const Head& h, const Plan& p, int v0, int R, uint16_t* at, const uint16_t*& W, int& ld,
-                long long& plane) {
-    if (p.direct) {
-        W = (const uint16_t*)h.W + (size_t)v0 * h.ldw;
-        ld = h.ldw;
-        plane = 0;
-        return DH_OK;
-    }
-    W = at;
-    ld = p.Dp;
-    plane = (long long)R * p.Dp;
-    stage_table<T, PLANES><<<(R + 3) / 4, 256, 0, stream()>>>((const T*)h.W, h.ldw, v0, R, h.D, at, p.Dp,
-                                                             plane);
-    return check_launch(h.op);
-}
-
-template <bool AK, bool BK, int TOK, int PLANES, class Epi>
-int product(const char* op, Prod g, int splits, const Epi& epi) {
-    const long long tiles = ((g.M + 255LL) / 256) * ((g.N + 255LL) / 256);
-    const int stages = (g.K + 31) / 32;
+template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
+int launch(const char* op, Prod g, int splits, const Epi& epi) {
+    const long long tiles = ((g.M + S::T - 1LL) / S::T) * ((g.N + S::T - 1LL) / S::T);
+    const int stages = (g.K + S::BK - 1) / S::BK;
     g.kstages = (stages + splits - 1) / splits;
-    vocab_gemm<AK, BK, TOK, PLANES, Epi><<<dim3((unsigned)tiles, splits), 512, 0, stream()>>>(g, epi);
+    vocab_gemm<S, AK, BK, TOK, PARTS, Epi><<<dim3((unsigned)tiles, splits), S::THREADS, 0, stream()>>>(g, epi);
     return check_launch(op);
 }
+template <bool AK, bool BK, int TOK, int PARTS, class Epi>
+int product(const char* op, Kind t, const Prod& g, int splits, const Epi& epi) {
+    if (t == T256) return launch<Shape<256>, AK, BK, TOK, PARTS>(op, g, splits, epi);
+    if (t == T128) return launch<Shape<128>, AK, BK, TOK, PARTS>(op, g, splits, epi);
+    return launch<Shape<64>, AK, BK, TOK, PARTS>(op, g, splits, epi);
+}
 
-template <typename T, int PLANES>
+template <typename T, int PARTS>
 int forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_bytes) {
     const Plan p = make_plan(h.dtype, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, 0, h.W, h.ldw);
-    const Work w = lay_out(p, ws, h.N);
-    float2* state = (float2*)((char*)w.piece - p.piece + p.state);
-    DH_TRY((prepare_rows<T, PLANES>(h, w, loss, lse, nullptr, nullptr)));
+    Work w = lay_out(p, ws);
     const int rows = piece_rows(p, h.V, ws_bytes);
+    const int wr = wave_rows(p.lse);
     float2* part = (float2*)w.piece;
-    uint16_t* staged = (uint16_t*)(w.piece + (size_t)(rows / 128) * p.Nt * 8);
-    for (int v0 = 0; v0 < h.V; v0 += rows) {
-        const int R = h.V - v0 < rows ? h.V - v0 : rows;
-        Prod g{};
-        DH_TRY((piece_table<T, PLANES>(h, p, v0, R, staged, g.A, g.lda, g.pa)));
-        g.B = w.Hp;
-        g.ldb = p.Dp;
-        g.pb = (long long)h.N * p.Dp;
-        g.M = R;
-        g.N = h.N;
-        g.K = p.direct ? h.D : p.Dp;
-        g.cnt = w.rows.cnt;
-        DH_TRY((product<true, true, TOK_N, PLANES>(h.op, g, 1, EpiLse{h.c, part, p.Nt})));
-        lse_join<<<p.Nt / 64, 1024, 0, stream()>>>(part, p.Nt, (R + 127) / 128, w.rows, state, v0 == 0,
-                                                   v0 + R >= h.V, w.base, h.factor, loss, lse);
-        DH_TRY(check_launch(h.op));
-        if (h.V - v0 <= rows) break;   // v0 + rows may pass the largest int
+    uint16_t* staged = (uint16_t*)(w.piece + (size_t)(rows / wr) * p.Nt * 8);
+    w.exps.e = (int*)(staged + (size_t)PARTS * rows * p.Dp);
+    const long long wplane = (long long)rows * p.Dp;
+    Pack a{};
+    a.loss = loss;
+    a.lse_out = lse;
+    if (h.target) a.base = w.base;
+    if (!p.direct) {   // the first piece's table rows go with the packing
+        a.R = h.V < rows ? h.V : rows;
+        a.tables = (a.R + 15) / 16;
+        a.staged = staged;
+        a.wplane = wplane;
     }
-    return DH_OK;
+    DH_TRY((prepare_rows<T, PARTS>(h, w, a, a.tables)));
+    for (int v0 = 0;; v0 += rows) {
+        const int R = h.V - v0 < rows ? h.V - v0 : rows;
+        const bool last = h.V - v0 <= rows;
+        Prod g{staged, w.Hp, p.Dp, p.Dp, wplane, (long long)h.N * p.Dp, R, h.N, p.Dp, 0, w.rows.cnt};
+        if (p.direct) {
+            g.A = (const uint16_t*)h.W + (size_t)v0 * h.ldw;
+            g.lda = h.ldw;
+            g.K = h.D;
+        } else if (v0 > 0) {
+            stage_table<T, PARTS><<<(R + 3) / 4, 256, 0, stream()>>>((const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp,
+                                                                    wplane, w.exps.e);
+            DH_TRY(check_launch(h.op));
+        }
+        DH_TRY((product<true, true, TOK_N, PARTS>(h.op, p.lse, g, 1,
+                                                  EpiLse<PARTS>{h.c, w.exps.e, w.rows.hexp, part, p.Nt})));
+        const JoinOut out{w.rows, w.state, v0 == 0, last, w.base, h.factor, loss, lse};
+        const int blocks = (R + wr - 1) / wr;
+        if (h.N <= 512) lse_join_few<<<h.N, 256, 0, stream()>>>(part, p.Nt, blocks, out);
+        else lse_join<<<p.Nt / 64, 1024, 0, stream()>>>(part, p.Nt, blocks, out);
+        DH_TRY(check_launch(h.op));
+        if (last) return DH_OK;
+    }
 }
 
 struct Grads {
@@ -872,61 +1326,116 @@ struct Grads {
     int lddw, acc_dW, type;
 };
 
-template <typename T, int PLANES>
+// dH and dW of a piece, in one launch where both take the same small tile.
+template <int PARTS, class EpiH, class EpiW>
+int gradients(const char* op, const Plan& p, const Prod* gh, const EpiH& eh, const Prod* gw, const EpiW& ew) {
+    if (gh && gw && p.dh == T64 && p.dw == T64) {
+        using S = Shape<64>;
+        auto per = [](int K, int splits) { return ((K + S::BK - 1) / S::BK + splits - 1) / splits; };
+        Prod a = *gh, b = *gw;
+        a.kstages = per(a.K, p.splits);
+        b.kstages = per(b.K, p.wsplits);
+        const long long th = tiles_of(p.dh, a.M, a.N), tw = tiles_of(p.dw, b.M, b.N);
+        vocab_grads<S, PARTS, EpiH, EpiW>
+            <<<(unsigned)(th * p.splits + tw * p.wsplits), S::THREADS, 0, stream()>>>(
+                a, eh, (int)th, (int)(th * p.splits), b, ew, (int)tw);
+        return check_launch(op);
+    }
+    if (gh) DH_TRY((product<true, false, TOK_M, PARTS>(op, p.dh, *gh, p.splits, eh)));
+    if (gw) DH_TRY((product<false, false, TOK_K, PARTS>(op, p.dw, *gw, p.wsplits, ew)));
+    return DH_OK;
+}
+
+template <typename T, int PARTS, typename OT>
 int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
-    const Plan p = make_plan(h.dtype, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, 1, h.W, h.ldw);
-    const Work w = lay_out(p, ws, h.N);
-    float* acc = (float*)((char*)w.piece - p.piece + p.acc);
-    DH_TRY((prepare_rows<T, PLANES>(h, w, nullptr, nullptr, d.lse, d.dloss)));
+    Plan p = make_plan(h.dtype, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, 1, h.W, h.ldw);
+    Work w = lay_out(p, ws);
     const int rows = piece_rows(p, h.V, ws_bytes);
-    const long long hplane = (long long)h.N * p.Dp, split = hplane;
+    const bool one = h.V <= rows;   // a single piece
+    const long long hplane = (long long)h.N * p.Dp, wplane = (long long)rows * p.Dp;
     uint16_t* G = (uint16_t*)w.piece;
     const long long gplane = (long long)h.N * rows;
-    uint16_t* staged = G + PLANES * gplane;
-    for (int v0 = 0; v0 < h.V; v0 += rows) {
+    float* wacc = (float*)(G + PARTS * gplane);
+    uint16_t* staged = (uint16_t*)(wacc + (p.wsplits > 1 ? p.wsplits * wplane : 0));
+    Pack a{};
+    a.lse_in = d.lse;
+    a.dloss = d.dloss;
+    if (d.dH && !d.acc_dH) {
+        a.dH = d.dH;
+        a.lddh = d.lddh;
+        a.dh_f32 = d.type == DH_F32;
+    }
+    int more = 0, scan = 0;
+    if (PARTS == 2) {
+        scan = more = h.V < 16 * SCAN ? (h.V + 15) / 16 : SCAN;
+    } else if (!p.direct) {
+        a.R = one ? h.V : rows;
+        more = a.tables = (a.R + 15) / 16;
+        a.staged = staged;
+        a.wplane = wplane;
+    }
+    DH_TRY((prepare_rows<T, PARTS>(h, w, a, more)));
+    const Grad<OT> to_dH{(OT*)d.dH, d.lddh, d.acc_dH, w.rows.row, PARTS == 2 ? w.exps.E : nullptr,
+                         PARTS == 2 ? w.rows.w : nullptr};
+    for (int v0 = 0;; v0 += rows) {
         const int R = h.V - v0 < rows ? h.V - v0 : rows;
-        const uint16_t* W;
-        int ldw;
-        long long wplane;
-        DH_TRY((piece_table<T, PLANES>(h, p, v0, R, staged, W, ldw, wplane)));
-        const int K = p.direct ? h.D : p.Dp;
-        Prod g{w.Hp, W, p.Dp, ldw, hplane, wplane, h.N, R, K, 0, w.rows.cnt};
-        if (h.target) {
-            DH_TRY((product<true, true, TOK_M, PLANES>(
-                h.op, g, 1, EpiG<PLANES, true>{h.c, w.rows.lse, w.rows.w, w.rows.target, v0, G, rows, gplane})));
-        } else {
-            DH_TRY((product<true, true, TOK_M, PLANES>(
-                h.op, g, 1, EpiG<PLANES, false>{h.c, w.rows.lse, w.rows.w, nullptr, v0, G, rows, gplane})));
-            teacher_entries<PLANES><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G,
-                                                               rows, gplane);
+        const bool last = h.V - v0 <= rows;
+        const uint16_t* W = staged;
+        int ldw = p.Dp, K = p.Dp;
+        if (p.direct) {
+            W = (const uint16_t*)h.W + (size_t)v0 * h.ldw;
+            ldw = h.ldw;
+            K = h.D;
+        } else if (PARTS == 2) {
+            const int tables = (R + 3) / 4;
+            stage_scaled<<<tables + (v0 == 0 ? (h.N + 3) / 4 : 0), 256, 0, stream()>>>(
+                (const float*)h.W, h.ldw, v0, R, h.D, staged, p.Dp, wplane, w.exps, (h.N + PACK - 1) / PACK,
+                scan, tables, w.rows, (const float*)h.H, h.ldh, w.Xp, hplane);
+            DH_TRY(check_launch(h.op));
+        } else if (v0 > 0) {
+            stage_table<T, PARTS><<<(R + 3) / 4, 256, 0, stream()>>>((const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp,
+                                                                    wplane, nullptr);
             DH_TRY(check_launch(h.op));
         }
-        if (d.dH) {
-            Prod gh{G, W, rows, ldw, gplane, wplane, h.N, h.D, R, 0, w.rows.cnt};
-            DH_TRY((product<true, false, TOK_M, PLANES>(h.op, gh, p.splits,
-                                                        EpiAcc{acc, p.Dp, v0 == 0, split})));
+        const Prod g{w.Hp, W, p.Dp, ldw, hplane, wplane, h.N, R, K, 0, w.rows.cnt};
+        if (h.target) {
+            DH_TRY((product<true, true, TOK_M, PARTS>(
+                h.op, p.g, g, 1,
+                EpiG<PARTS, true>{h.c, w.rows.lse, w.rows.w, w.rows.target, w.rows.hexp, w.exps.E, v0, G, rows,
+                                  gplane})));
+        } else {
+            DH_TRY((product<true, true, TOK_M, PARTS>(
+                h.op, p.g, g, 1,
+                EpiG<PARTS, false>{h.c, w.rows.lse, w.rows.w, nullptr, w.rows.hexp, w.exps.E, v0, G, rows,
+                                   gplane})));
+            teacher_entries<PARTS><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, rows,
+                                                              gplane);
+            DH_TRY(check_launch(h.op));
         }
-        if (d.dW) {
-            Prod gw{G, w.Hp, rows, p.Dp, gplane, hplane, R, h.D, h.N, 0, w.rows.cnt};
-            if (d.type == DH_F32)
-                DH_TRY((product<false, false, TOK_K, PLANES>(
-                    h.op, gw, 1, EpiOut<float>{(float*)d.dW + (size_t)v0 * d.lddw, d.lddw, d.acc_dW})));
-            else
-                DH_TRY((product<false, false, TOK_K, PLANES>(
-                    h.op, gw, 1, EpiOut<uint16_t>{(uint16_t*)d.dW + (size_t)v0 * d.lddw, d.lddw, d.acc_dW})));
+        const Prod gh{G, W, rows, ldw, gplane, wplane, h.N, h.D, R, 0, w.rows.cnt};
+        const Prod gw{G, w.Xp, rows, p.Dp, gplane, hplane, R, h.D, h.N, 0, w.rows.cnt};
+        const Prod *ph = d.dH ? &gh : nullptr, *pw = d.dW ? &gw : nullptr;
+        const Grad<OT> to_dW{d.dW ? (OT*)d.dW + (size_t)v0 * d.lddw : nullptr, d.lddw, d.acc_dW, nullptr,
+                             PARTS == 2 ? w.exps.X : nullptr, nullptr};
+        // Straight to the gradient, or as sums that the last launch adds.
+        const bool direct_h = one && p.splits == 1, direct_w = p.wsplits == 1;
+        const EpiAcc sum_h{w.acc, p.Dp, v0 == 0, hplane}, sum_w{wacc, p.Dp, 1, wplane};
+        const EpiOut<PARTS, OT> out_h{to_dH}, out_w{to_dW};
+        if (direct_h && direct_w) DH_TRY((gradients<PARTS>(h.op, p, ph, out_h, pw, out_w)));
+        else if (direct_h) DH_TRY((gradients<PARTS>(h.op, p, ph, out_h, pw, sum_w)));
+        else if (direct_w) DH_TRY((gradients<PARTS>(h.op, p, ph, sum_h, pw, out_w)));
+        else DH_TRY((gradients<PARTS>(h.op, p, ph, sum_h, pw, sum_w)));
+        Finish<OT> fh{to_dH, w.acc, h.N, p.Dp, p.splits, hplane, w.rows.cnt, 0};
+        Finish<OT> fw{to_dW, wacc, R, p.Dp, p.wsplits, wplane, nullptr, 0};
+        auto groups = [&](long long rows_) { return (rows_ * ((h.D + 3) / 4) + 255) / 256; };
+        if (ph && last && !direct_h) fh.groups = groups(h.N);
+        if (pw && !direct_w) fw.groups = groups(R);
+        if (fh.groups + fw.groups > 0) {
+            finish<PARTS, OT><<<(unsigned)(fh.groups + fw.groups), 256, 0, stream()>>>(fh, fw, h.D);
+            DH_TRY(check_launch(h.op));
         }
-        if (h.V - v0 <= rows) break;
+        if (last) return DH_OK;
     }
-    if (d.dH) {
-        if (d.type == DH_F32)
-            dh_finish<<<(h.N + 3) / 4, 256, 0, stream()>>>(w.rows.inv, h.N, h.D, acc, p.Dp, p.splits, split,
-                                                           (float*)d.dH, d.lddh, d.acc_dH);
-        else
-            dh_finish<<<(h.N + 3) / 4, 256, 0, stream()>>>(w.rows.inv, h.N, h.D, acc, p.Dp, p.splits, split,
-                                                           (uint16_t*)d.dH, d.lddh, d.acc_dH);
-        DH_TRY(check_launch(h.op));
-    }
-    return DH_OK;
 }
 
 int run_forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_bytes) {
@@ -936,7 +1445,7 @@ int run_forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_byte
         return set_error(DH_ERR_INVALID, "%s: null pointer", h.op);
     DH_TRY(ensure_init());
     if (h.N == 0) return DH_OK;
-    return h.dtype == DH_F32 ? forward<float, 3>(h, loss, lse, ws, ws_bytes)
+    return h.dtype == DH_F32 ? forward<float, 2>(h, loss, lse, ws, ws_bytes)
                              : forward<uint16_t, 1>(h, loss, lse, ws, ws_bytes);
 }
 
@@ -959,8 +1468,9 @@ int run_backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
             clear_rows<<<2048, 256, 0, stream()>>>((uint16_t*)d.dW, h.V, h.D, d.lddw);
         return check_launch(h.op);
     }
-    return h.dtype == DH_F32 ? backward<float, 3>(h, d, ws, ws_bytes)
-                             : backward<uint16_t, 1>(h, d, ws, ws_bytes);
+    if (h.dtype == DH_F32) return backward<float, 2, float>(h, d, ws, ws_bytes);
+    return d.type == DH_F32 ? backward<uint16_t, 1, float>(h, d, ws, ws_bytes)
+                            : backward<uint16_t, 1, uint16_t>(h, d, ws, ws_bytes);
 }
 
 Head xent_head(const char* op, int dtype, int N, int V, int D, float scale, const void* H, int ldh,

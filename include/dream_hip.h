@@ -334,7 +334,9 @@ int dh_unary(int op, int dtype, const void* d_A, void* d_C, size_t n, double lo,
  * query says (the losses take larger pieces of the vocabulary out of more, which is faster); no
  * call here allocates, so all of them can be captured.  Calls that may overlap in time, two
  * captured graphs among them, need workspaces of their own; nothing is kept there between calls.
- * The losses take an fp32 operand to 2^-24 of itself or 2^-134, whichever is more.
+ * The losses take an fp32 operand to 2^-23 of itself or 2^-51 of the largest value of its row
+ * (forward) or of its matrix (gradients), whichever is more, and softmax - q to 2^-23 of itself or
+ * 2^-51.
  * Deterministic: no floating-point atomics.
  *
  * Y[n] = scale W[id[n]] for N tokens. */

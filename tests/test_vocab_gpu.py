@@ -2,8 +2,8 @@
 
 Tolerances (u = 2^-24, the largest relative error of one fp32 rounding; ub = 2^-8 of one to bf16).
 A product of length D with operands rounded to their type before the call is exact up to its fp32
-sum, whose error is at most about sqrt(D) u of |h| |w| for operands of random sign; the parts of
-an fp32 operand are exact to 2^-24, and the pairs left out are below 2^-24 of a product.  With
+sum, whose error is at most about sqrt(D) u of |h| |w| for operands of random sign; an fp32 operand
+is taken to 2^-23 of itself or 2^-51 of its row's largest value.  With
 |z| up to about 20 that gives logits to 1e-5, and as d exp(z) = exp(z) dz every probability to 1e-5
 of itself; sums of them keep that.  So fp32 results are held to 2e-5 of the largest value of the
 result (for the loss: of its largest, at least 1).  bf16 gradients: one rounding of G (ub of
@@ -367,25 +367,42 @@ def test_xent_extremes():
 
 
 @pytest.mark.gpu
-def test_xent_table_beyond_bf16():
-    """fp32 values whose nearest bf16 is infinite (the largest finite ones) keep their value.  The
-    parts of a value end at bf16's smallest positive number, 2^-133, so they miss at most 2^-134 of
-    it: against a table entry of 2^128 that is 2^-6 of a logit (H's 1e-37 here)."""
-    N, V, D = 4, 40, 8
-    c = Loss(N, V, D, "f32")
-    big = np.float32(3.4e38)
-    W = c.W.copy()
-    W[3, 0] = big
-    H = c.H.copy()
-    H[:, 0] = np.array([1e-37, -1e-37, 2e-38, 0.0])
-    c.Hb, c.H = store(H, "f32")
-    c.Wb, c.W = store(W, "f32")
-    loss, lse = DB.empty((N,), np.float32), DB.empty((N,), np.float32)
-    size = c.least(0)
-    c.fwd(loss, lse, DB(size), size)
+@pytest.mark.parametrize("k", [-100, -30, 60, 100])
+def test_loss_operands_of_any_scale(k):
+    """H 2^k and W 2^-k have the logits, the losses and, scaled back, the gradients of H and W, bit
+    for bit: the products take each row at a scale of its own."""
+    outs = []
+    for j in (0, k):
+        c = Loss(70, 300, 40, "f32", seed=3)
+        H, W = np.ldexp(c.H, j), np.ldexp(c.W, -j)
+        c.Hb, c.H = store(H, "f32")
+        c.Wb, c.W = store(W, "f32")
+        size = max(c.least(0), c.least(1))
+        ws = DB(size)
+        loss, lse = DB.empty((c.N,), np.float32), DB.empty((c.N,), np.float32)
+        dH, dW = DB.empty((c.N, c.D), np.float32), DB.empty((c.V, c.D), np.float32)
+        c.fwd(loss, lse, ws, size)
+        c.bwd(lse, c.dlb, dH, c.D, False, dW, c.D, False, hip.F32, ws, size)
+        outs.append([loss.numpy(), lse.numpy(), np.ldexp(dH.numpy(), j), np.ldexp(dW.numpy(), -j)])
+    for a, b in zip(*outs):
+        assert (a == b).all()
+
+
+@pytest.mark.gpu
+def test_loss_rows_of_many_scales():
+    """Rows of H and of W, and loss weights, whose sizes differ by factors of up to 2^24."""
+    N, V, D = 150, 400, 48
+    c = Loss(N, V, D, "f32", seed=4)
+    r = np.random.default_rng(5)
+    c.Hb, c.H = store(np.ldexp(c.H, -r.integers(0, 24, (N, 1))), "f32")
+    c.Wb, c.W = store(np.ldexp(c.W, -r.integers(0, 24, (V, 1))), "f32")
+    c.dloss = np.ldexp(c.dloss, -r.integers(0, 24, N)).astype(np.float32)
+    c.dlb = DB.from_numpy(c.dloss)
+    got = run_loss(c)
     ref = c.ref()
-    err = np.abs(loss.numpy().astype(np.float64) - ref[0]).max()
-    assert err <= F32_TOL * np.abs(ref[0]).max() + 2.0 ** -134 * float(big), err
+    # every row of dH to its own size, as its sum's terms have the row's weight
+    err = np.abs(got[2] - ref[2]).max(1) / (c.dloss * np.abs(c.W).max())
+    assert err.max() <= F32_TOL, err.max()
 
 
 @pytest.mark.gpu
