@@ -421,38 +421,33 @@ __global__ void __launch_bounds__(256) stage_scaled(const float* __restrict__ W,
 }
 
 // ---- teachers ------------------------------------------------------------------------------------
-// A work-group per packed row: the teacher's probabilities q (N x K, zero where there is no
-// entry), the student's logits z at its tokens, and base[i] = sum q (log q - z).
+// A work-group per packed row, a wave per 2 of its K entries: the teacher's probabilities q (N x K,
+// zero where there is no entry), the student's logits z at its tokens, and base[i] =
+// sum q (log q - z).  Latency-bound: the entries' rows of W lie anywhere.
 template <typename T>
-__global__ void __launch_bounds__(256) teacher_dots(Rows rows, Teacher t, int V,
-                                                    const T* __restrict__ H, int ldh,
-                                                    const T* __restrict__ W, int ldw, int D,
-                                                    float* __restrict__ q, float* __restrict__ z,
-                                                    float* __restrict__ base) {
-    __shared__ float red[4];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+__global__ void __launch_bounds__(1024) teacher_dots(Rows rows, Teacher t, int V,
+                                                     const T* __restrict__ H, int ldh,
+                                                     const T* __restrict__ W, int ldw, int D,
+                                                     float* __restrict__ q, float* __restrict__ z,
+                                                     float* __restrict__ base) {
+    __shared__ float red[16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int i = blockIdx.x;
     if (i >= *rows.cnt) return;
     const int n = rows.row[i];
     const size_t at = (size_t)n * t.K, to = (size_t)i * t.K;
-    auto all = [&](float v, auto op) {
-        v = wave_reduce(v, op);
-        __syncthreads();
-        if (lane == 0) red[w] = v;
-        __syncthreads();
-        return op(op(red[0], red[1]), op(red[2], red[3]));
-    };
+    // Largest logit and sum of exponentials: every wave for itself, over all entries.
     float mx = -INFINITY;
-    for (int k = threadIdx.x; k < t.K; k += 256)
+    for (int k = lane; k < t.K; k += 64)
         if (entry_counts(t, at + k, V)) mx = fmaxf(mx, t.logit[at + k]);
-    mx = all(mx, OpMax());
+    mx = wave_reduce(mx, OpMax());
     float sum = 0.f;
-    for (int k = threadIdx.x; k < t.K; k += 256)
+    for (int k = lane; k < t.K; k += 64)
         if (entry_counts(t, at + k, V)) sum += __expf((t.logit[at + k] - mx) * t.inv_t);
-    sum = all(sum, OpSum());
+    sum = wave_reduce(sum, OpSum());
     const float log_sum = __logf(sum);
     float part = 0.f;
-    for (int k = w; k < t.K; k += 4) {
+    for (int k = w; k < t.K; k += waves) {
         float zk = 0.f, qk = 0.f;
         if (entry_counts(t, at + k, V)) {
             const float d = row_dot(H + (size_t)n * ldh, W + (size_t)t.id[at + k] * ldw, D, lane);
@@ -467,10 +462,11 @@ __global__ void __launch_bounds__(256) teacher_dots(Rows rows, Teacher t, int V,
             z[to + k] = zk;
         }
     }
-    __syncthreads();   // red[] may still be read
     if (lane == 0) red[w] = part;
     __syncthreads();
-    if (threadIdx.x == 0) base[i] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x != 0) return;
+    for (int x = 1; x < waves; ++x) part += red[x];
+    base[i] = part;
 }
 
 // ---- products -------------------------------------------------------------------------------------
@@ -1253,7 +1249,8 @@ int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
     pack_rows<T, PARTS><<<a.groups + more, 1024, 0, stream()>>>(a);
     DH_TRY(check_launch(h.op));
     if (h.target) return DH_OK;
-    teacher_dots<T><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, (const T*)h.H, h.ldh, (const T*)h.W,
+    const int waves = h.teacher.K <= 2 ? 1 : h.teacher.K >= 32 ? 16 : (h.teacher.K + 1) / 2;
+    teacher_dots<T><<<h.N, 64 * waves, 0, stream()>>>(w.rows, h.teacher, h.V, (const T*)h.H, h.ldh, (const T*)h.W,
                                                h.ldw, h.D, w.q, w.z, w.base);
     return check_launch(h.op);
 }

@@ -344,7 +344,7 @@ int dh_embedding_fwd(int dtype, int N, int V, int D, float scale, const int* d_i
                      const void* d_W, int ldw, void* d_Y, int ldy);
 /* dW[v] = scale * sum of dY[n] over id[n] = v, every row of the table (zero without a token); with
  * accumulate the rows that have tokens get it added, the others are not touched. */
-size_t dh_embedding_bwd_workspace(int N, int V, int D);   /* <= 18 N + N D / 2 + V + 8 D + 8192 */
+size_t dh_embedding_bwd_workspace(int N, int V, int D);   /* <= (N + 16)(D + 511) / 2 + 18 N + V + 16384 */
 int dh_embedding_bwd(int dtype, int N, int V, int D, float scale, const int* d_ids,
                      const void* d_dY, int lddy, void* d_dW, int lddw, int grad_type,
                      int accumulate, void* d_ws, size_t ws_bytes);

@@ -77,7 +77,7 @@ def run_embedding(ids, V, D, dtype, grad, ldx=0, accumulate=False, scale=1.5, se
     ib = ints(ids if N else [0])
     hip.embedding_fwd(DT[dtype], N, V, D, scale, ib, dW_, D + ldx, Yb, D + ldx)
     size = hip.embedding_bwd_workspace(N, V, D)
-    assert size <= 18 * N + N * D // 2 + V + 8 * D + 8192
+    assert size <= (N + 16) * (D + 511) // 2 + 18 * N + V + 16384
     ws = DB(max(size, 16))
     hip.embedding_bwd(DT[dtype], N, V, D, scale, ib, dYb, D + ldx, gb, D + ldx, DT[grad], accumulate,
                       ws, size)
@@ -99,7 +99,8 @@ def run_embedding(ids, V, D, dtype, grad, ldx=0, accumulate=False, scale=1.5, se
 @pytest.mark.parametrize("dtype,grad", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
 @pytest.mark.parametrize("N,V,D", [(1, 1, 1), (1, 65, 32), (16, 3, 7), (17, 300, 64), (255, 65, 33),
                                    (1000, 512, 130), (1024, 511, 520), (8192, 70000, 16),
-                                   (8193, 1000, 24), (20000, 300000, 9)])
+                                   (8193, 1000, 24), (20000, 300000, 9), (2048, 700, 1040),
+                                   (2049, 700, 1040), (9000, 5000, 1029)])
 def test_embedding(N, V, D, dtype, grad):
     r = np.random.default_rng(N + V)
     ids = np.minimum((V ** r.random(N)).astype(np.int64) - 1, V - 1)
@@ -107,7 +108,7 @@ def test_embedding(N, V, D, dtype, grad):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N", [5, 400, 9000])
+@pytest.mark.parametrize("N", [5, 400, 2100, 9000])
 @pytest.mark.parametrize("kind", ["all_same", "padding", "all_padding", "descending", "ends"])
 def test_embedding_orders(N, kind):
     V, D = 50, 40
