@@ -492,13 +492,12 @@ enum { TOK_M, TOK_N, TOK_K };
 //        c ^ 4 (k / 2 % 2); a fragment is two transposing reads
 // A resource per stage whose base is the stage's first element and whose range ends with the
 // operand's rows: operands of any size keep 32-bit offsets, and what lies behind the rows reads as
-// zero.  PAIR (KC): tile row 32 b + i of each 64 is row 2 i + b, so that a lane's two blocks of 32
-// columns are neighbours.
-template <bool KC, int T, int BK, int WAVES, bool PAIR>
+// zero.
+template <bool KC, int T, int BK, int WAVES>
 struct Operand {
     static constexpr int PER = T * BK / 512 / WAVES;   // blocks per wave
     static constexpr int CPR = KC ? BK / 8 : T / 8;    // chunks in a row
-    static_assert(PER >= 1 && (!PAIR || KC), "tile shapes");
+    static_assert(PER >= 1, "tile shapes");
     uint32_t off[PER];
     uint32_t last[KC ? PER : 1];   // offsets in the stage that K ends in
     const uint16_t* base;          // the tile's first element
@@ -515,9 +514,8 @@ struct Operand {
         rows = KC ? min(extent - t0, T) : t0;
 #pragma unroll
         for (int t = 0; t < PER; ++t) {
-            int r = 64 / CPR * (PER * wave + t) + lane / CPR;   // row of the LDS tile
+            const int r = 64 / CPR * (PER * wave + t) + lane / CPR;   // row of the LDS tile
             const int c = (lane % CPR) ^ swizzle(r);
-            if (PAIR) r = (r & ~63) + 2 * (r & 31) + ((r >> 5) & 1);
             off[t] = 2u * ((uint32_t)r * ld + 8 * c);
             // chunks past K (a multiple of 8) lie outside the resource
             if (KC) last[t] = 8 * c < K % BK ? off[t] : 0xFFFFFFF0u;
@@ -525,11 +523,13 @@ struct Operand {
     }
     __device__ void issue(long long plane, int kt, uint16_t* lds, int wave) const {
         const uint16_t* p = base + plane + (KC ? (size_t)kt * BK : (size_t)kt * BK * ld);
-        const uint32_t bytes = KC ? 2u * ((uint32_t)rows * ld - (uint32_t)(BK * kt))
-                                  : 2u * ((uint32_t)min(K - BK * kt, BK) * ld - (uint32_t)rows);
+        const int left = min(K - BK * kt, BK);   // none: all of the stage reads as zero
+        const uint32_t bytes = left <= 0 ? 0u
+                               : KC ? 2u * ((uint32_t)rows * ld - (uint32_t)(BK * kt))
+                                    : 2u * ((uint32_t)left * ld - (uint32_t)rows);
         const u32x4 rs = make_rsrc(p, bytes);
         const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(lds) + 1024u * PER * wave);
-        const bool end = KC && BK * kt + BK > K;
+        const bool end = KC && left < BK;
 #pragma unroll
         for (int t = 0; t < PER; ++t)
             lds_dma16_buf_so(KC && end ? last[KC ? t : 0] : off[t], rs, 0u, to + 1024u * t);
@@ -573,6 +573,7 @@ __device__ inline void mfma_parts(const bf16x8 (&fa)[FM], const bf16x8 (&fb)[FN]
 template <int T_>
 struct Shape {
     static constexpr int T = T_, BK = T == 64 ? 64 : 32, NS = 4;
+    static constexpr int DEEP = 3 * T * 64 + NS * T * 32;   // elements of gemm_deep's rings
     static constexpr int WAVES = T == 256 ? 8 : 4;
     static constexpr int WAVES_N = T == 256 ? 4 : 2;
     static constexpr int WM = T * WAVES_N / WAVES, WN = T / WAVES_N;
@@ -581,18 +582,39 @@ struct Shape {
     static constexpr int THREADS = 64 * WAVES;
 };
 
+// Row of register r of block a, relative to the wave's first row.
+__device__ inline int reg_row(int a, int r, int lane) { return 32 * a + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// 32 rows of a wave's tile of 16-bit values through its piece of LDS, so that they are written as
+// 16-byte pieces of rows: element by element (a lane has one column of 16 rows) the stores of a 256 x 256
+// tile took 38 us, as much as 40 of its stages.  put(row, chunk column, 8 values) writes a piece.
+constexpr int LDS_TILE = 32 * (64 + 8);   // elements; rows 16 bytes longer, so that the halves' banks differ
+template <int FN, class Put>
+__device__ inline void store_rows(uint16_t* lds, const uint16_t (&v)[FN][16], int row0, int lane, const Put& put) {
+    constexpr int LD = 32 * FN + 8, CHUNKS = 4 * FN;
+#pragma unroll
+    for (int b = 0; b < FN; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) lds[reg_row(0, r, lane) * LD + 32 * b + (lane & 31)] = v[b][r];
+#pragma unroll
+    for (int i = 0; i < 32 * CHUNKS / 64; ++i) {
+        const int r = 64 / CHUNKS * i + lane / CHUNKS, c = 8 * (lane % CHUNKS);
+        put(row0 + r, c, *reinterpret_cast<const h8*>(lds + r * LD + c));
+    }
+}
+
 // One tile of one split: stages of BK k through a ring of four in LDS filled by direct DMA three
 // stages ahead; a stage's 16-k steps run while the next operands are read (the schedule of the
 // bf16 GEMM's 8-wave form).  Epi::run gets the tile's accumulators: register r of block (a, b) is
-// row m0 + wm + 32 a + 8 (r / 4) + 4 h + r % 4, column n0 + wn + 32 b + l32, or with Epi::PAIR and
-// two blocks n0 + wn + 2 l32 + b (lane = 32 h + l32).
+// row m0 + wm + 32 a + 8 (r / 4) + 4 h + r % 4, column n0 + wn + 32 b + l32 (lane = 32 h + l32).
 template <class S, bool AK, bool BK_, int TOK, int PARTS, class Epi>
 __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, int tile, int tiles,
                                  int split) {
     constexpr int FM = S::FM, FN = S::FN, BK = S::BK, NS = S::NS, STEPS = BK / 16;
-    constexpr bool PAIR = BK_ && Epi::PAIR && FN == 2;
-    using OA = Operand<AK, S::T, BK, S::WAVES, false>;
-    using OB = Operand<BK_, S::T, BK, S::WAVES, PAIR>;
+    using OA = Operand<AK, S::T, BK, S::WAVES>;
+    using OB = Operand<BK_, S::T, BK, S::WAVES>;
     constexpr int BOFF = S::T * BK, LOADS = OA::PER + OB::PER;
     const int cnt = *g.cnt;
     const int M = TOK == TOK_M ? cnt : g.M, N = TOK == TOK_N ? cnt : g.N;
@@ -685,13 +707,144 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
         inner(total - 1);
         mma(1);
     }
-    epi.template run<FM, FN>(acc, M, N, m0 + wm, n0 + wn, lane, split);
+    if constexpr (Epi::LDS) __syncthreads();   // the ring is free
+    epi.template run<FM, FN>(acc, M, N, m0 + wm, n0 + wn, lane, split, ring + wave * LDS_TILE);
+}
+
+// The 256-wide tile with a k-contiguous A: A in 64-k stages (whole 128-byte lines of a row, where 32-k
+// stages fetch each half by itself) through a ring of three beside B's 32-k stages in a ring of
+// four, 160 KB; the bf16 GEMM's schedule for such operands.  A pair of stages (64 k) at a time:
+// pair p of A is fetched in stage 2 p - 4, stage s of B in stage s - 3, and past the end the last
+// ones again into slots that nobody reads any more, so that the waits are constants: when stage s
+// ends, stage s + 1 has landed and 12 (s even) or 8 (odd) younger loads may be in flight.  An odd
+// last stage lies past K and reads as zero.
+template <class S, bool BK_, int TOK, int PARTS, class Epi>
+__device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, int tile, int tiles, int split) {
+    constexpr int FM = S::FM, FN = S::FN, T = S::T;
+    using OA = Operand<true, T, 64, S::WAVES>;
+    using OB = Operand<BK_, T, 32, S::WAVES>;
+    static_assert(OA::PER == 4 && OB::PER == 2, "the waits below");
+    const int cnt = *g.cnt;
+    const int M = TOK == TOK_M ? cnt : g.M, N = TOK == TOK_N ? cnt : g.N;
+    int tm, tn;
+    xcd_tile_order(tile, tiles, (g.M + T - 1) / T, (g.N + T - 1) / T, 4, tm, tn);
+    const int m0 = tm * T, n0 = tn * T;
+    if (m0 >= M || n0 >= N) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = (wave / S::WAVES_N) * S::WM, wn = (wave % S::WAVES_N) * S::WN;
+
+    f32x16 acc[FM][FN];
+#pragma unroll
+    for (int a = 0; a < FM; ++a)
+#pragma unroll
+        for (int b = 0; b < FN; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+
+    const int p0 = split * g.kstages;   // in pairs
+    const int np = max(0, min((g.K + 63) / 64 - p0, g.kstages));
+    const int pairs = PARTS == 1 ? np : 3 * np;
+    if (pairs > 0) {
+        OA sa;
+        OB sb;
+        sa.init(g.A, g.lda, m0, M, g.K, wave, lane);
+        sb.init(g.B, g.ldb, n0, N, g.K, wave, lane);
+        uint16_t* const ring_a = ring;
+        uint16_t* const ring_b = ring + 3 * T * 64;
+        int ap = 0, akind = 0, aslot = 0, an = 0;   // the next pair of A, and how many are fetched
+        auto issue_a = [&]() {
+            sa.issue(PARTS == 2 && akind == 0 ? g.pa : 0, p0 + ap, ring_a + aslot * T * 64, wave);
+            aslot = aslot == 2 ? 0 : aslot + 1;
+            if (++an < pairs && ++ap == np) {
+                ap = 0;
+                ++akind;
+            }
+        };
+        int bs = 0, bkind = 0, bslot = 0, bn = 0;
+        auto issue_b = [&]() {
+            sb.issue(PARTS == 2 && bkind == 1 ? g.pb : 0, 2 * p0 + bs, ring_b + bslot * T * 32, wave);
+            bslot = (bslot + 1) & 3;
+            if (++bn < 2 * pairs && ++bs == 2 * np) {
+                bs = 0;
+                ++bkind;
+            }
+        };
+        bf16x8 fa[2][FM], fb[2][FN];
+        // The products of fragments f, and under them the reads of the other ones (16-k step ka of
+        // A's slot la, kb of B's lb) and then the DMA.
+        auto step = [&](int f, const uint16_t* la, int ka, const uint16_t* lb, int kb, auto dma) {
+#pragma unroll
+            for (int i = 0; i < FM * FN; ++i) {
+                const int a = i / FN, b = i % FN;
+                if constexpr (PARTS == 1)
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[f][a], fb[f][b], acc[a][b], 0, 0, 0);
+                else
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                        __builtin_bit_cast(f16x8, fa[f][a]), __builtin_bit_cast(f16x8, fb[f][b]), acc[a][b], 0,
+                        0, 0);
+                if (i < FM) fa[f ^ 1][i] = OA::frag(la, wm + 32 * i, ka, lane);
+                else if (i < FM + FN) fb[f ^ 1][i - FM] = OB::frag(lb, wn + 32 * (i - FM), kb, lane);
+                if (i == FM + FN) dma();
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto none = [] {};
+        issue_a();
+        issue_b();
+        issue_b();
+        issue_a();
+        issue_b();
+        wait_vmcnt<8>();
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < FM; ++x) fa[0][x] = OA::frag(ring_a, wm + 32 * x, 0, lane);
+#pragma unroll
+        for (int x = 0; x < FN; ++x) fb[0][x] = OB::frag(ring_b, wn + 32 * x, 0, lane);
+        int sla = 0;   // A's slot of the pair at hand
+        for (int p = 0; p < pairs; ++p) {
+            if (PARTS == 2 && p == 2 * np)
+#pragma unroll
+                for (int a = 0; a < FM; ++a)
+#pragma unroll
+                    for (int b = 0; b < FN; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[a][b][r] *= 0x1p-11f;
+            const uint16_t* la = ring_a + sla * T * 64;
+            sla = sla == 2 ? 0 : sla + 1;
+            const uint16_t* next = ring_a + sla * T * 64;
+            const uint16_t* lb = ring_b + ((2 * p) & 3) * T * 32;
+            const uint16_t* lb1 = ring_b + ((2 * p + 1) & 3) * T * 32;
+            const uint16_t* lb2 = ring_b + ((2 * p + 2) & 3) * T * 32;
+            step(0, la, 1, lb, 1, [&] {
+                issue_b();
+                issue_a();
+            });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            wait_vmcnt<12>();
+            __syncthreads();
+            step(1, la, 2, lb1, 0, none);
+            step(0, la, 3, lb1, 1, [&] { issue_b(); });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            wait_vmcnt<8>();
+            __syncthreads();
+            step(1, next, 0, lb2, 0, none);   // after the last pair: what is there, unused
+        }
+        wait_vmcnt<0>();   // what was fetched again lands before the LDS is given away
+    }
+    if constexpr (Epi::LDS) __syncthreads();   // the ring is free
+    epi.template run<FM, FN>(acc, M, N, m0 + wm, n0 + wn, lane, split, ring + wave * LDS_TILE);
 }
 
 template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
 __global__ void __launch_bounds__(S::THREADS) vocab_gemm(Prod g, Epi epi) {
-    __shared__ __attribute__((aligned(16))) uint16_t ring[S::NS * S::STAGE];
-    gemm_tile<S, AK, BK, TOK, PARTS>(ring, g, epi, blockIdx.x, gridDim.x, blockIdx.y);
+    if constexpr (S::T == 256 && AK) {
+        __shared__ __attribute__((aligned(16))) uint16_t ring[S::DEEP];
+        gemm_deep<S, BK, TOK, PARTS>(ring, g, epi, blockIdx.x, gridDim.x, blockIdx.y);
+    } else {
+        __shared__ __attribute__((aligned(16))) uint16_t ring[S::NS * S::STAGE];
+        gemm_tile<S, AK, BK, TOK, PARTS>(ring, g, epi, blockIdx.x, gridDim.x, blockIdx.y);
+    }
 }
 
 // dH and dW of a piece in one launch: the first `first` work-groups are dH's, splits one after the
@@ -708,23 +861,19 @@ __global__ void __launch_bounds__(S::THREADS) vocab_grads(Prod gh, EpiH eh, int 
                                                  (b - first) / tiles_w);
 }
 
-// Row of register r of block a, relative to the wave's first row.
-__device__ inline int reg_row(int a, int r, int lane) { return 32 * a + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
-
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-
 // Forward: rows are table rows, columns packed rows.  A lane holds half of the wave's logits of
 // each of its columns, lane + 32 the other half: their maximum and sum of exponentials go to
 // part[the wave's block of 32 FM rows][column].
 template <int PARTS>
 struct EpiLse {
-    static constexpr bool PAIR = false;
+    static constexpr bool LDS = false;
     float c;
     const int *e, *h;      // exponents of the table's and the packed rows' scales (two parts)
     float2* part;
     int ldp;
     template <int FM, int FN>
-    __device__ void run(f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int) const {
+    __device__ void run(f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int,
+                        uint16_t*) const {
         if (row0 >= M) return;   // the wave has no table row: its block is not joined either
         const bool full = row0 + 32 * FM <= M;
         float kc[FN];
@@ -771,11 +920,10 @@ struct EpiLse {
 
 // Backward: rows are packed rows, columns the piece's table rows.  One part: G = w (p - q), rounded
 // once to bf16, the type that the products take.  Two parts: 2^14 (p - q) to 22 bits.  Columns past
-// the table's end up to the tile's are zero.  Two blocks of columns are neighbours in a lane, so a
-// store instruction writes whole 128-byte lines of two rows.
+// the table's end up to the tile's are zero.
 template <int PARTS, bool HARD>
 struct EpiG {
-    static constexpr bool PAIR = true;
+    static constexpr bool LDS = true;
     float c;
     const float *lse, *w;
     const int *target, *h, *E;
@@ -784,13 +932,12 @@ struct EpiG {
     int ldg;
     long long plane;
     template <int FM, int FN>
-    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int) const {
-        int col[FN];
+    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int,
+                        uint16_t* lds) const {
+        const int table = PARTS == 1 ? 0 : *E, col = col0 + (lane & 31);
 #pragma unroll
-        for (int b = 0; b < FN; ++b) col[b] = col0 + (FN == 2 ? 2 * (lane & 31) + b : lane & 31);
-        const int table = PARTS == 1 ? 0 : *E;
-#pragma unroll
-        for (int a = 0; a < FM; ++a)
+        for (int a = 0; a < FM; ++a) {
+            uint16_t v[PARTS][FN][16];
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int row = row0 + reg_row(a, 4 * r4, lane);
@@ -802,38 +949,38 @@ struct EpiG {
                 if constexpr (HARD) t4 = *reinterpret_cast<const i32x4*>(target + row);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (row + e >= M) continue;
                     const float k = PARTS == 1 ? c : __builtin_ldexpf(c, h4[e] + table);
                     const float f = PARTS == 1 ? w4[e] : 0x1p14f;
-                    uint16_t v[FN][PARTS];
 #pragma unroll
                     for (int b = 0; b < FN; ++b) {
                         float p = __expf(__builtin_fmaf(k, acc[a][b][4 * r4 + e], -l4[e]));
                         if constexpr (HARD)
-                            if (col[b] == t4[e] - v0) p -= 1.f;
-                        to_parts<PARTS>(col[b] < N ? f * p : 0.f, v[b]);
-                    }
-                    uint16_t* to = G + (size_t)(row + e) * ldg + col[0];
+                            if (col + 32 * b == t4[e] - v0) p -= 1.f;
+                        uint16_t x[PARTS];
+                        to_parts<PARTS>(col + 32 * b < N ? f * p : 0.f, x);
 #pragma unroll
-                    for (int q = 0; q < PARTS; ++q) {
-                        if constexpr (FN == 2)
-                            *reinterpret_cast<uint32_t*>(to + q * plane) = v[0][q] | ((uint32_t)v[1][q] << 16);
-                        else
-                            to[q * plane] = v[0][q];
+                        for (int q = 0; q < PARTS; ++q) v[q][b][4 * r4 + e] = x[q];
                     }
                 }
             }
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+                store_rows<FN>(lds, v[q], row0 + 32 * a, lane, [&](int row, int cc, h8 x) {
+                    if (row < M) *reinterpret_cast<h8*>(G + q * plane + (size_t)row * ldg + col0 + cc) = x;
+                });
+        }
     }
 };
 
 // fp32 sums over the pieces (dH), one block per split.
 struct EpiAcc {
-    static constexpr bool PAIR = false;
+    static constexpr bool LDS = false;
     float* C;
     int ldc, first;
     long long split;
     template <int FM, int FN>
-    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int s) const {
+    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int s,
+                        uint16_t*) const {
         float* p = C + s * split;
 #pragma unroll
         for (int a = 0; a < FM; ++a)
@@ -873,13 +1020,39 @@ struct Grad {
     }
 };
 
-// A gradient from its only split and piece.
+// A gradient from its only split and piece.  bf16 that is not added to what is there goes through LDS.
 template <int PARTS, typename OT>
 struct EpiOut {
-    static constexpr bool PAIR = false;
+    static constexpr bool LDS = sizeof(OT) == 2;
     Grad<OT> out;
     template <int FM, int FN>
-    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int) const {
+    __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int,
+                        uint16_t* lds) const {
+        if constexpr (LDS) {
+            static_assert(PARTS == 1, "bf16 results come from one part");
+            if (!out.accumulate) {
+#pragma unroll
+                for (int a = 0; a < FM; ++a) {
+                    uint16_t v[FN][16];
+#pragma unroll
+                    for (int b = 0; b < FN; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) v[b][r] = rne_bf16(acc[a][b][r]);
+                    store_rows<FN>(lds, v, row0 + 32 * a, lane, [&](int row, int cc, h8 x) {
+                        if (row >= M || col0 + cc >= N) return;
+                        OT* to = out.at(row) + col0 + cc;
+                        if (col0 + cc + 8 <= N) {
+                            *reinterpret_cast<h8a*>(to) = x;   // at any alignment
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (col0 + cc + e < N) to[e] = x[e];
+                        }
+                    });
+                }
+                return;
+            }
+        }
         const int s = PARTS == 1 ? 0 : out.scale();
 #pragma unroll
         for (int a = 0; a < FM; ++a)
@@ -1105,9 +1278,14 @@ Kind pick(long long M, long long N, long long K, int parts, bool split) {
     return best;
 }
 
+// The distance of rows of `cols` 16-bit values in the workspace: a half line more than a multiple of
+// 512 bytes would be, as rows at such distances lie in few of the memory's channels and sets, and a
+// tile's stage reads a piece of each of its rows.
+int apart(int cols) { return cols % 256 == 0 ? cols + 64 : cols; }
+
 // The workspace: a part whose size the shapes give, and a piece whose size is what is left.
 struct Plan {
-    int parts, Dp, Nt;        // parts of an operand, padded columns, rows padded to whole tiles
+    int parts, Kp, Dp, Nt;    // parts of an operand, padded columns, their rows' distance, padded rows
     bool direct;              // the table is read in place
     Kind lse, g, dh, dw;      // the products' tiles
     int splits, wsplits;      // of dH and dW
@@ -1119,7 +1297,8 @@ struct Plan {
 Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* W, int ldw) {
     Plan p{};
     p.parts = dtype == DH_F32 ? 2 : 1;
-    p.Dp = (D + 31) / 32 * 32;
+    p.Kp = (D + 31) / 32 * 32;
+    p.Dp = apart(p.Kp);
     p.Nt = (int)(((long long)N + 255) / 256 * 256);
     // In place: whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
     p.direct = dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
@@ -1144,7 +1323,7 @@ Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* 
         p.splits = splits_of(p.dh, N, D, V);
         p.acc = take((size_t)p.splits * N * p.Dp * 4);
         if (p.parts == 2) p.Xp = take((size_t)p.parts * N * p.Dp * 2);
-        p.per_block = (size_t)p.parts * N * 256 * 2;
+        p.per_block = (size_t)p.parts * N * (256 + 64) * 2;
         // dW's sums over splits of the rows: a piece's, fp32.
         p.wsplits = splits_of(p.dw, V, D, N);
         if (p.wsplits > 1) p.per_block += (size_t)p.wsplits * 256 * p.Dp * 4;
@@ -1258,7 +1437,8 @@ int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
 template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
 int launch(const char* op, Prod g, int splits, const Epi& epi) {
     const long long tiles = ((g.M + S::T - 1LL) / S::T) * ((g.N + S::T - 1LL) / S::T);
-    const int stages = (g.K + S::BK - 1) / S::BK;
+    const int bk = S::T == 256 && AK ? 64 : S::BK;   // gemm_deep counts pairs
+    const int stages = (g.K + bk - 1) / bk;
     g.kstages = (stages + splits - 1) / splits;
     vocab_gemm<S, AK, BK, TOK, PARTS, Epi><<<dim3((unsigned)tiles, splits), S::THREADS, 0, stream()>>>(g, epi);
     return check_launch(op);
@@ -1294,7 +1474,7 @@ int forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_bytes) {
     for (int v0 = 0;; v0 += rows) {
         const int R = h.V - v0 < rows ? h.V - v0 : rows;
         const bool last = h.V - v0 <= rows;
-        Prod g{staged, w.Hp, p.Dp, p.Dp, wplane, (long long)h.N * p.Dp, R, h.N, p.Dp, 0, w.rows.cnt};
+        Prod g{staged, w.Hp, p.Dp, p.Dp, wplane, (long long)h.N * p.Dp, R, h.N, p.Kp, 0, w.rows.cnt};
         if (p.direct) {
             g.A = (const uint16_t*)h.W + (size_t)v0 * h.ldw;
             g.lda = h.ldw;
@@ -1351,7 +1531,8 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     const bool one = h.V <= rows;   // a single piece
     const long long hplane = (long long)h.N * p.Dp, wplane = (long long)rows * p.Dp;
     uint16_t* G = (uint16_t*)w.piece;
-    const long long gplane = (long long)h.N * rows;
+    const int ldg = apart(rows);
+    const long long gplane = (long long)h.N * ldg;
     float* wacc = (float*)(G + PARTS * gplane);
     uint16_t* staged = (uint16_t*)(wacc + (p.wsplits > 1 ? p.wsplits * wplane : 0));
     Pack a{};
@@ -1378,7 +1559,7 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         const int R = h.V - v0 < rows ? h.V - v0 : rows;
         const bool last = h.V - v0 <= rows;
         const uint16_t* W = staged;
-        int ldw = p.Dp, K = p.Dp;
+        int ldw = p.Dp, K = p.Kp;
         if (p.direct) {
             W = (const uint16_t*)h.W + (size_t)v0 * h.ldw;
             ldw = h.ldw;
@@ -1398,19 +1579,19 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         if (h.target) {
             DH_TRY((product<true, true, TOK_M, PARTS>(
                 h.op, p.g, g, 1,
-                EpiG<PARTS, true>{h.c, w.rows.lse, w.rows.w, w.rows.target, w.rows.hexp, w.exps.E, v0, G, rows,
+                EpiG<PARTS, true>{h.c, w.rows.lse, w.rows.w, w.rows.target, w.rows.hexp, w.exps.E, v0, G, ldg,
                                   gplane})));
         } else {
             DH_TRY((product<true, true, TOK_M, PARTS>(
                 h.op, p.g, g, 1,
-                EpiG<PARTS, false>{h.c, w.rows.lse, w.rows.w, nullptr, w.rows.hexp, w.exps.E, v0, G, rows,
+                EpiG<PARTS, false>{h.c, w.rows.lse, w.rows.w, nullptr, w.rows.hexp, w.exps.E, v0, G, ldg,
                                    gplane})));
-            teacher_entries<PARTS><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, rows,
+            teacher_entries<PARTS><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, ldg,
                                                               gplane);
             DH_TRY(check_launch(h.op));
         }
-        const Prod gh{G, W, rows, ldw, gplane, wplane, h.N, h.D, R, 0, w.rows.cnt};
-        const Prod gw{G, w.Xp, rows, p.Dp, gplane, hplane, R, h.D, h.N, 0, w.rows.cnt};
+        const Prod gh{G, W, ldg, ldw, gplane, wplane, h.N, h.D, R, 0, w.rows.cnt};
+        const Prod gw{G, w.Xp, ldg, p.Dp, gplane, hplane, R, h.D, h.N, 0, w.rows.cnt};
         const Prod *ph = d.dH ? &gh : nullptr, *pw = d.dW ? &gw : nullptr;
         const Grad<OT> to_dW{d.dW ? (OT*)d.dW + (size_t)v0 * d.lddw : nullptr, d.lddw, d.acc_dW, nullptr,
                              PARTS == 2 ? w.exps.X : nullptr, nullptr};
