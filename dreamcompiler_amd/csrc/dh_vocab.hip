@@ -490,49 +490,70 @@ enum { TOK_M, TOK_N, TOK_K };
 //        a fragment is one 16-byte read
 //   else [BK k][T]: chunk c of row k at c ^ 4 (k % 4), for T = 64 (two rows in the 64 banks)
 //        c ^ 4 (k / 2 % 2); a fragment is two transposing reads
-// A resource per stage whose base is the stage's first element and whose range ends with the
-// operand's rows: operands of any size keep 32-bit offsets, and what lies behind the rows reads as
-// zero.
+// Loads go through a buffer resource whose range ends with the operand's rows, so what lies behind
+// them reads as zero; it begins with the tile (KC; the stage's place in the rows is a scalar
+// offset) or with the stage, so operands of any size keep 32-bit offsets.
 template <bool KC, int T, int BK, int WAVES>
 struct Operand {
     static constexpr int PER = T * BK / 512 / WAVES;   // blocks per wave
     static constexpr int CPR = KC ? BK / 8 : T / 8;    // chunks in a row
     static_assert(PER >= 1, "tile shapes");
     uint32_t off[PER];
-    uint32_t last[KC ? PER : 1];   // offsets in the stage that K ends in
+    u32x4 rs;
+    uint32_t soff;
     const uint16_t* base;          // the tile's first element
-    int ld, rows, K;               // rows: of the tile (KC), or its first column
+    long long plane;
+    int ld, K, rows;               // rows: of the tile (KC), or its first column
 
     __device__ static int swizzle(int r) {
         if (KC) return BK == 32 ? (r >> 2) & 3 : (r >> 1) & 7;
         return T == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
     }
-    __device__ void init(const uint16_t* p, int ld_, int t0, int extent, int K_, int wave, int lane) {
+    __device__ static int row_of(int t, int wave, int lane) { return 64 / CPR * (PER * wave + t) + lane / CPR; }
+    __device__ static int chunk_of(int t, int wave, int lane) {
+        return (lane % CPR) ^ swizzle(row_of(t, wave, lane));
+    }
+    __device__ void init(const uint16_t* p, long long plane_, int ld_, int t0, int extent, int K_, int wave,
+                         int lane) {
         ld = ld_;
         K = K_;
+        plane = plane_;
         base = KC ? p + (size_t)t0 * ld : p + t0;
         rows = KC ? min(extent - t0, T) : t0;
 #pragma unroll
-        for (int t = 0; t < PER; ++t) {
-            const int r = 64 / CPR * (PER * wave + t) + lane / CPR;   // row of the LDS tile
-            const int c = (lane % CPR) ^ swizzle(r);
-            off[t] = 2u * ((uint32_t)r * ld + 8 * c);
-            // chunks past K (a multiple of 8) lie outside the resource
-            if (KC) last[t] = 8 * c < K % BK ? off[t] : 0xFFFFFFF0u;
+        for (int t = 0; t < PER; ++t)
+            off[t] = 2u * ((uint32_t)row_of(t, wave, lane) * ld + 8 * chunk_of(t, wave, lane));
+    }
+    // Stage kt of a part is the next one.
+    __device__ void start(int part, int kt) {
+        rs = make_rsrc(base + part * plane + (KC ? 0 : (size_t)kt * BK * ld),
+                       2u * (KC ? (uint32_t)rows * ld : (uint32_t)(BK * ld - rows)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rs[e] = __builtin_amdgcn_readfirstlane(rs[e]);
+        soff = __builtin_amdgcn_readfirstlane(KC ? 2u * BK * kt : 0u);
+    }
+    __device__ void next() {
+        if (KC) {
+            soff += 2 * BK;
+        } else {
+            const uint64_t a = (((uint64_t)rs[1] << 32) | rs[0]) + 2u * BK * ld;
+            rs[0] = (uint32_t)a;
+            rs[1] = (uint32_t)(a >> 32);
         }
     }
-    __device__ void issue(long long plane, int kt, uint16_t* lds, int wave) const {
-        const uint16_t* p = base + plane + (KC ? (size_t)kt * BK : (size_t)kt * BK * ld);
-        const int left = min(K - BK * kt, BK);   // none: all of the stage reads as zero
-        const uint32_t bytes = left <= 0 ? 0u
-                               : KC ? 2u * ((uint32_t)rows * ld - (uint32_t)(BK * kt))
-                                    : 2u * ((uint32_t)left * ld - (uint32_t)rows);
-        const u32x4 rs = make_rsrc(p, bytes);
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(lds) + 1024u * PER * wave);
-        const bool end = KC && left < BK;
+    __device__ void issue(uint32_t to) const {
+#pragma unroll
+        for (int t = 0; t < PER; ++t) lds_dma16_buf_so(off[t], rs, soff, to + 1024u * t);
+    }
+    // A stage kt that ends behind K: zeros from there on (KC: K is a multiple of 8).
+    __device__ void issue_end(uint32_t to, int kt, int wave, int lane) const {
+        const int left = K - BK * kt;
+        u32x4 r = rs;
+        if (!KC) r[2] = left <= 0 ? 0u : 2u * (uint32_t)(left * ld - rows);
 #pragma unroll
         for (int t = 0; t < PER; ++t)
-            lds_dma16_buf_so(KC && end ? last[KC ? t : 0] : off[t], rs, 0u, to + 1024u * t);
+            lds_dma16_buf_so(!KC || 8 * chunk_of(t, wave, lane) < left ? off[t] : 0xFFFFFFF0u, r, soff,
+                             to + 1024u * t);
     }
     // Tile rows o .. o + 31, 16-k step kk of the stage.
     __device__ static bf16x8 frag(const uint16_t* lds, int o, int kk, int lane) {
@@ -616,7 +637,7 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
     using OA = Operand<AK, S::T, BK, S::WAVES>;
     using OB = Operand<BK_, S::T, BK, S::WAVES>;
     constexpr int BOFF = S::T * BK, LOADS = OA::PER + OB::PER;
-    const int cnt = *g.cnt;
+    const int cnt = __builtin_amdgcn_readfirstlane(*g.cnt);
     const int M = TOK == TOK_M ? cnt : g.M, N = TOK == TOK_N ? cnt : g.N;
     const int Kall = TOK == TOK_K ? cnt : g.K;
     int tm, tn;
@@ -642,17 +663,34 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
     if (total > 0) {
         OA sa;
         OB sb;
-        sa.init(g.A, g.lda, m0, M, Kall, wave, lane);
-        sb.init(g.B, g.ldb, n0, N, Kall, wave, lane);
-        int ikt = 0, ipair = 0, islot = 0;   // the next stage to fetch
+        sa.init(g.A, g.pa, g.lda, m0, M, Kall, wave, lane);
+        sb.init(g.B, g.pb, g.ldb, n0, N, Kall, wave, lane);
+        // the parts' pairs: lo hi, hi lo, hi hi
+        sa.start(PARTS == 2 ? 1 : 0, kt0);
+        sb.start(0, kt0);
+        const int tail = (kt0 + nk) * BK > Kall ? nk - 1 : -1;   // the stage that ends behind K
+        constexpr uint32_t RING = 2u * NS * S::STAGE;
+        const uint32_t ring0 = lds_addr(ring);
+        const uint32_t wave_a = 1024u * OA::PER * wave, wave_b = 2u * BOFF + 1024u * OB::PER * wave;
+        int ikt = 0, ipair = 0;   // the next stage to fetch
+        uint32_t slot = 0;
         auto issue = [&]() {
-            uint16_t* st = ring + islot * S::STAGE;
-            sa.issue(PARTS == 2 && ipair == 0 ? g.pa : 0, kt0 + ikt, st, wave);
-            sb.issue(PARTS == 2 && ipair == 1 ? g.pb : 0, kt0 + ikt, st + BOFF, wave);
-            islot = (islot + 1) % NS;
-            if (++ikt == nk) {
+            const uint32_t to = __builtin_amdgcn_readfirstlane(ring0 + slot);
+            if (__builtin_expect(ikt != tail, 1)) {
+                sa.issue(to + wave_a);
+                sb.issue(to + wave_b);
+            } else {
+                sa.issue_end(to + wave_a, kt0 + ikt, wave, lane);
+                sb.issue_end(to + wave_b, kt0 + ikt, wave, lane);
+            }
+            slot = slot == RING - 2u * S::STAGE ? 0u : slot + 2u * S::STAGE;
+            sa.next();
+            sb.next();
+            if (++ikt == nk && PARTS == 2) {
                 ikt = 0;
                 ++ipair;
+                sa.start(0, kt0);
+                sb.start(ipair == 1, kt0);
             }
         };
         auto landed = [&](int ahead) {   // all but the youngest `ahead` stages
@@ -695,11 +733,20 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
         landed(pre - 1);
         __syncthreads();
         read(0, 0, fa[0], fb[0]);
-        for (int s = 0; s < total - 1; ++s) {
-            if (s + NS - 1 < total) issue();
+        int s = 0;
+        for (; s < total - NS + 1; ++s) {
+            issue();
             inner(s);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            landed(min(total - 1, s + NS - 1) - (s + 1));
+            wait_vmcnt<(NS - 2) * LOADS>();
+            __syncthreads();
+            read(s + 1, 0, fa[0], fb[0]);
+            mma(1);
+        }
+        for (; s < total - 1; ++s) {   // all is fetched
+            inner(s);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            landed(total - 2 - s);
             __syncthreads();
             read(s + 1, 0, fa[0], fb[0]);
             mma(1);
@@ -724,7 +771,7 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
     using OA = Operand<true, T, 64, S::WAVES>;
     using OB = Operand<BK_, T, 32, S::WAVES>;
     static_assert(OA::PER == 4 && OB::PER == 2, "the waits below");
-    const int cnt = *g.cnt;
+    const int cnt = __builtin_amdgcn_readfirstlane(*g.cnt);
     const int M = TOK == TOK_M ? cnt : g.M, N = TOK == TOK_N ? cnt : g.N;
     int tm, tn;
     xcd_tile_order(tile, tiles, (g.M + T - 1) / T, (g.N + T - 1) / T, 4, tm, tn);
@@ -748,26 +795,45 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
     if (pairs > 0) {
         OA sa;
         OB sb;
-        sa.init(g.A, g.lda, m0, M, g.K, wave, lane);
-        sb.init(g.B, g.ldb, n0, N, g.K, wave, lane);
+        sa.init(g.A, g.pa, g.lda, m0, M, g.K, wave, lane);
+        sb.init(g.B, g.pb, g.ldb, n0, N, g.K, wave, lane);
+        sa.start(PARTS == 2 ? 1 : 0, p0);
+        sb.start(0, 2 * p0);
+        const uint32_t ring_a0 = lds_addr(ring) + 1024u * OA::PER * wave;
+        const uint32_t ring_b0 = lds_addr(ring) + 2u * 3 * T * 64 + 1024u * OB::PER * wave;
         uint16_t* const ring_a = ring;
         uint16_t* const ring_b = ring + 3 * T * 64;
-        int ap = 0, akind = 0, aslot = 0, an = 0;   // the next pair of A, and how many are fetched
+        const bool tail = (p0 + np) * 64 > g.K;
+        int ap = 0, akind = 0, an = 0;   // the next pair of A, and how many are fetched
+        uint32_t aslot = 0;
         auto issue_a = [&]() {
-            sa.issue(PARTS == 2 && akind == 0 ? g.pa : 0, p0 + ap, ring_a + aslot * T * 64, wave);
-            aslot = aslot == 2 ? 0 : aslot + 1;
-            if (++an < pairs && ++ap == np) {
-                ap = 0;
-                ++akind;
+            const uint32_t to = __builtin_amdgcn_readfirstlane(ring_a0 + aslot);
+            if (__builtin_expect(!tail || ap != np - 1, 1)) sa.issue(to);
+            else sa.issue_end(to, p0 + ap, wave, lane);
+            aslot = aslot == 2u * 2 * T * 64 ? 0u : aslot + 2u * T * 64;
+            if (++an < pairs) {
+                sa.next();
+                if (++ap == np) {
+                    ap = 0;
+                    ++akind;
+                    sa.start(0, p0);
+                }
             }
         };
-        int bs = 0, bkind = 0, bslot = 0, bn = 0;
+        int bs = 0, bkind = 0, bn = 0;
+        uint32_t bslot = 0;
         auto issue_b = [&]() {
-            sb.issue(PARTS == 2 && bkind == 1 ? g.pb : 0, 2 * p0 + bs, ring_b + bslot * T * 32, wave);
-            bslot = (bslot + 1) & 3;
-            if (++bn < 2 * pairs && ++bs == 2 * np) {
-                bs = 0;
-                ++bkind;
+            const uint32_t to = __builtin_amdgcn_readfirstlane(ring_b0 + bslot);
+            if (__builtin_expect(!tail || bs < 2 * np - 2, 1)) sb.issue(to);
+            else sb.issue_end(to, 2 * p0 + bs, wave, lane);
+            bslot = (bslot + 2u * T * 32) & (2u * 4 * T * 32 - 1);
+            if (++bn < 2 * pairs) {
+                sb.next();
+                if (++bs == 2 * np) {
+                    bs = 0;
+                    ++bkind;
+                    sb.start(bkind == 1, 2 * p0);
+                }
             }
         };
         bf16x8 fa[2][FM], fb[2][FN];
