@@ -25,6 +25,8 @@
 // where k runs along the row (H, and W in the forward), else all of the operand (W in the
 // backward, where its rows are summed over; G, whose entries are p - q; and w_n H_n, the other
 // operand of dW).
+#include <type_traits>
+
 #include "dh_common.hpp"
 #include "dh_gemm_bf16.hpp"
 
@@ -541,19 +543,13 @@ struct Operand {
             rs[1] = (uint32_t)(a >> 32);
         }
     }
-    __device__ void issue(uint32_t to) const {
-#pragma unroll
-        for (int t = 0; t < PER; ++t) lds_dma16_buf_so(off[t], rs, soff, to + 1024u * t);
-    }
-    // A stage kt that ends behind K: zeros from there on (KC: K is a multiple of 8).
-    __device__ void issue_end(uint32_t to, int kt, int wave, int lane) const {
+    __device__ void issue_one(uint32_t to, int t) const { lds_dma16_buf_so(off[t], rs, soff, to + 1024u * t); }
+    // Of a stage kt that ends behind K: zeros from there on (KC: K is a multiple of 8).
+    __device__ void issue_end(uint32_t to, int t, int kt, int wave, int lane) const {
         const int left = K - BK * kt;
         u32x4 r = rs;
         if (!KC) r[2] = left <= 0 ? 0u : 2u * (uint32_t)(left * ld - rows);
-#pragma unroll
-        for (int t = 0; t < PER; ++t)
-            lds_dma16_buf_so(!KC || 8 * chunk_of(t, wave, lane) < left ? off[t] : 0xFFFFFFF0u, r, soff,
-                             to + 1024u * t);
+        lds_dma16_buf_so(!KC || 8 * chunk_of(t, wave, lane) < left ? off[t] : 0xFFFFFFF0u, r, soff, to + 1024u * t);
     }
     // Tile rows o .. o + 31, 16-k step kk of the stage.
     __device__ static bf16x8 frag(const uint16_t* lds, int o, int kk, int lane) {
@@ -607,6 +603,7 @@ struct Shape {
 __device__ inline int reg_row(int a, int r, int lane) { return 32 * a + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+constexpr float LOG2E = 1.4426950408889634f;
 
 // 32 rows of a wave's tile of 16-bit values through its piece of LDS, so that they are written as
 // 16-byte pieces of rows: element by element (a lane has one column of 16 rows) the stores of a 256 x 256
@@ -677,11 +674,15 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
         auto issue = [&]() {
             const uint32_t to = __builtin_amdgcn_readfirstlane(ring0 + slot);
             if (__builtin_expect(ikt != tail, 1)) {
-                sa.issue(to + wave_a);
-                sb.issue(to + wave_b);
+#pragma unroll
+                for (int t = 0; t < OA::PER; ++t) sa.issue_one(to + wave_a, t);
+#pragma unroll
+                for (int t = 0; t < OB::PER; ++t) sb.issue_one(to + wave_b, t);
             } else {
-                sa.issue_end(to + wave_a, kt0 + ikt, wave, lane);
-                sb.issue_end(to + wave_b, kt0 + ikt, wave, lane);
+#pragma unroll
+                for (int t = 0; t < OA::PER; ++t) sa.issue_end(to + wave_a, t, kt0 + ikt, wave, lane);
+#pragma unroll
+                for (int t = 0; t < OB::PER; ++t) sb.issue_end(to + wave_b, t, kt0 + ikt, wave, lane);
             }
             slot = slot == RING - 2u * S::STAGE ? 0u : slot + 2u * S::STAGE;
             sa.next();
@@ -806,12 +807,18 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
         const bool tail = (p0 + np) * 64 > g.K;
         int ap = 0, akind = 0, an = 0;   // the next pair of A, and how many are fetched
         uint32_t aslot = 0;
-        auto issue_a = [&]() {
-            const uint32_t to = __builtin_amdgcn_readfirstlane(ring_a0 + aslot);
-            if (__builtin_expect(!tail || ap != np - 1, 1)) sa.issue(to);
-            else sa.issue_end(to, p0 + ap, wave, lane);
+        // Load t of the next pair; with the last one goes on to the pair behind it.  INSIDE: neither
+        // the last pair of the part, nor one that ends behind K.
+        auto load_a = [&](int t, auto inside) {
+            constexpr bool INSIDE = decltype(inside)::value;
+            const uint32_t to = ring_a0 + aslot;
+            if (INSIDE || __builtin_expect(!tail || ap != np - 1, 1)) sa.issue_one(to, t);
+            else sa.issue_end(to, t, p0 + ap, wave, lane);
+            if (t + 1 < OA::PER) return;
             aslot = aslot == 2u * 2 * T * 64 ? 0u : aslot + 2u * T * 64;
-            if (++an < pairs) {
+            if (INSIDE) {
+                sa.next();
+            } else if (++an < pairs) {
                 sa.next();
                 if (++ap == np) {
                     ap = 0;
@@ -822,12 +829,16 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
         };
         int bs = 0, bkind = 0, bn = 0;
         uint32_t bslot = 0;
-        auto issue_b = [&]() {
-            const uint32_t to = __builtin_amdgcn_readfirstlane(ring_b0 + bslot);
-            if (__builtin_expect(!tail || bs < 2 * np - 2, 1)) sb.issue(to);
-            else sb.issue_end(to, 2 * p0 + bs, wave, lane);
+        auto load_b = [&](int t, auto inside) {
+            constexpr bool INSIDE = decltype(inside)::value;
+            const uint32_t to = ring_b0 + bslot;
+            if (INSIDE || __builtin_expect(!tail || bs < 2 * np - 2, 1)) sb.issue_one(to, t);
+            else sb.issue_end(to, t, 2 * p0 + bs, wave, lane);
+            if (t + 1 < OB::PER) return;
             bslot = (bslot + 2u * T * 32) & (2u * 4 * T * 32 - 1);
-            if (++bn < 2 * pairs) {
+            if (INSIDE) {
+                sb.next();
+            } else if (++bn < 2 * pairs) {
                 sb.next();
                 if (++bs == 2 * np) {
                     bs = 0;
@@ -836,9 +847,19 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
                 }
             }
         };
+        constexpr std::false_type anywhere{};
+        auto issue_a = [&] {
+#pragma unroll
+            for (int t = 0; t < OA::PER; ++t) load_a(t, anywhere);
+        };
+        auto issue_b = [&] {
+#pragma unroll
+            for (int t = 0; t < OB::PER; ++t) load_b(t, anywhere);
+        };
         bf16x8 fa[2][FM], fb[2][FN];
-        // The products of fragments f, and under them the reads of the other ones (16-k step ka of
-        // A's slot la, kb of B's lb) and then the DMA.
+        // The products of fragments f, and under each a read of the other ones (16-k step ka of A's
+        // slot la, kb of B's lb) and a load: a wave that issues them in a row leaves its SIMD's matrix
+        // core idle.
         auto step = [&](int f, const uint16_t* la, int ka, const uint16_t* lb, int kb, auto dma) {
 #pragma unroll
             for (int i = 0; i < FM * FN; ++i) {
@@ -851,11 +872,11 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
                         0, 0);
                 if (i < FM) fa[f ^ 1][i] = OA::frag(la, wm + 32 * i, ka, lane);
                 else if (i < FM + FN) fb[f ^ 1][i - FM] = OB::frag(lb, wn + 32 * (i - FM), kb, lane);
-                if (i == FM + FN) dma();
+                dma(i);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto none = [] {};
+        auto none = [](int) {};
         issue_a();
         issue_b();
         issue_b();
@@ -867,34 +888,42 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
         for (int x = 0; x < FM; ++x) fa[0][x] = OA::frag(ring_a, wm + 32 * x, 0, lane);
 #pragma unroll
         for (int x = 0; x < FN; ++x) fb[0][x] = OB::frag(ring_b, wn + 32 * x, 0, lane);
-        int sla = 0;   // A's slot of the pair at hand
-        for (int p = 0; p < pairs; ++p) {
-            if (PARTS == 2 && p == 2 * np)
+        uint32_t sla = 0, slb = 0;   // elements to the slots of the pair at hand
+        auto pair = [&](auto inside) {
+            const uint16_t* la = ring_a + sla;
+            sla = sla == 2 * T * 64 ? 0 : sla + T * 64;
+            const uint16_t* next = ring_a + sla;
+            const uint16_t *lb = ring_b + slb, *lb1 = lb + T * 32;
+            slb ^= 2 * T * 32;
+            const uint16_t* lb2 = ring_b + slb;
+            step(0, la, 1, lb, 1, [&](int i) {
+                if (i >= 2 && i < 4) load_b(i - 2, inside);
+                else if (i >= 4) load_a(i - 4, inside);
+            });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            wait_vmcnt<12>();
+            __syncthreads();
+            step(1, la, 2, lb1, 0, none);
+            step(0, la, 3, lb1, 1, [&](int i) {
+                if (i >= 6) load_b(i - 6, inside);
+            });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            wait_vmcnt<8>();
+            __syncthreads();
+            step(1, next, 0, lb2, 0, none);   // after the last pair: what is there, unused
+        };
+        for (int kind = 0; kind < (PARTS == 1 ? 1 : 3); ++kind) {
+            if (kind == 2)
 #pragma unroll
                 for (int a = 0; a < FM; ++a)
 #pragma unroll
                     for (int b = 0; b < FN; ++b)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) acc[a][b][r] *= 0x1p-11f;
-            const uint16_t* la = ring_a + sla * T * 64;
-            sla = sla == 2 ? 0 : sla + 1;
-            const uint16_t* next = ring_a + sla * T * 64;
-            const uint16_t* lb = ring_b + ((2 * p) & 3) * T * 32;
-            const uint16_t* lb1 = ring_b + ((2 * p + 1) & 3) * T * 32;
-            const uint16_t* lb2 = ring_b + ((2 * p + 2) & 3) * T * 32;
-            step(0, la, 1, lb, 1, [&] {
-                issue_b();
-                issue_a();
-            });
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            wait_vmcnt<12>();
-            __syncthreads();
-            step(1, la, 2, lb1, 0, none);
-            step(0, la, 3, lb1, 1, [&] { issue_b(); });
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            wait_vmcnt<8>();
-            __syncthreads();
-            step(1, next, 0, lb2, 0, none);   // after the last pair: what is there, unused
+            int p = 0;
+            for (; p < np - 3; ++p) pair(std::true_type{});   // fetches pair p + 2 and stage 2 p + 4
+            an += p, ap += p, bn += 2 * p, bs += 2 * p;
+            for (; p < np; ++p) pair(anywhere);
         }
         wait_vmcnt<0>();   // what was fetched again lands before the LDS is given away
     }
@@ -942,11 +971,15 @@ struct EpiLse {
                         uint16_t*) const {
         if (row0 >= M) return;   // the wave has no table row: its block is not joined either
         const bool full = row0 + 32 * FM <= M;
+        // Two parts: the logits in place; one part: they are c times the accumulators, and
+        // exp(c (x - mx)) = 2^(k x - k mx) with k = c log2(e), one multiply-add an exponential.
+        // -inf past the table's end.
         float kc[FN];
 #pragma unroll
         for (int b = 0; b < FN; ++b)
-            kc[b] = PARTS == 1 ? c : __builtin_ldexpf(c, h[col0 + 32 * b + (lane & 31)]);
-        // logits in place; -inf past the table's end
+            kc[b] = PARTS == 1 ? 1.f : __builtin_ldexpf(c, h[col0 + 32 * b + (lane & 31)]);
+        const float k = PARTS == 1 ? c * LOG2E : LOG2E;
+        if (PARTS == 2 || !full)
 #pragma unroll
         for (int a = 0; a < FM; ++a)
 #pragma unroll
@@ -959,7 +992,8 @@ struct EpiLse {
 #pragma unroll
                     for (int b = 0; b < FN; ++b) {
                         const float z =
-                            acc[a][b][4 * r4 + q] * (PARTS == 1 ? kc[b] : __builtin_ldexpf(kc[b], e4[q]));
+                            PARTS == 1 ? acc[a][b][4 * r4 + q]
+                                       : acc[a][b][4 * r4 + q] * __builtin_ldexpf(kc[b], e4[q]);
                         acc[a][b][4 * r4 + q] = full || row + q < M ? z : -INFINITY;
                     }
             }
@@ -972,14 +1006,18 @@ struct EpiLse {
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[a][b][r]);
             mx = fmaxf(mx, xor32(mx));
             const float m = mx == -INFINITY ? 0.f : mx;   // all -inf: a sum of zeros, not of NaN
+            const float km = k * m;
             float s = 0.f;
 #pragma unroll
             for (int a = 0; a < FM; ++a)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s += __expf(acc[a][b][r] - m);
+                for (int r = 0; r < 16; ++r)
+                    s += __builtin_amdgcn_exp2f(PARTS == 1 ? __builtin_fmaf(k, acc[a][b][r], -km)
+                                                           : k * (acc[a][b][r] - m));
             s += xor32(s);
             const int col = col0 + 32 * b + (lane & 31);
-            if (lane < 32 && col < N) part[(size_t)(row0 / (32 * FM)) * ldp + col] = float2{mx, s};
+            if (lane < 32 && col < N)
+                part[(size_t)(row0 / (32 * FM)) * ldp + col] = float2{PARTS == 1 ? c * mx : mx, s};
         }
     }
 };
@@ -1001,6 +1039,7 @@ struct EpiG {
     __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int,
                         uint16_t* lds) const {
         const int table = PARTS == 1 ? 0 : *E, col = col0 + (lane & 31);
+        const float k1 = c * LOG2E;   // one part: 2^(k1 x - log2(e) lse)
 #pragma unroll
         for (int a = 0; a < FM; ++a) {
             uint16_t v[PARTS][FN][16];
@@ -1015,17 +1054,19 @@ struct EpiG {
                 if constexpr (HARD) t4 = *reinterpret_cast<const i32x4*>(target + row);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float k = PARTS == 1 ? c : __builtin_ldexpf(c, h4[e] + table);
+                    const float k = PARTS == 1 ? k1 : __builtin_ldexpf(c, h4[e] + table);
+                    const float l = PARTS == 1 ? l4[e] * LOG2E : l4[e];
                     const float f = PARTS == 1 ? w4[e] : 0x1p14f;
 #pragma unroll
                     for (int b = 0; b < FN; ++b) {
-                        float p = __expf(__builtin_fmaf(k, acc[a][b][4 * r4 + e], -l4[e]));
+                        const float x = __builtin_fmaf(k, acc[a][b][4 * r4 + e], -l);
+                        float p = __builtin_amdgcn_exp2f(PARTS == 1 ? x : x * LOG2E);
                         if constexpr (HARD)
                             if (col + 32 * b == t4[e] - v0) p -= 1.f;
-                        uint16_t x[PARTS];
-                        to_parts<PARTS>(col + 32 * b < N ? f * p : 0.f, x);
+                        uint16_t parts[PARTS];
+                        to_parts<PARTS>(col + 32 * b < N ? f * p : 0.f, parts);
 #pragma unroll
-                        for (int q = 0; q < PARTS; ++q) v[q][b][4 * r4 + e] = x[q];
+                        for (int q = 0; q < PARTS; ++q) v[q][b][4 * r4 + e] = parts[q];
                     }
                 }
             }
