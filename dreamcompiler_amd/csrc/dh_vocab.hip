@@ -25,6 +25,7 @@
 // where k runs along the row (H, and W in the forward), else all of the operand (W in the
 // backward, where its rows are summed over; G, whose entries are p - q; and w_n H_n, the other
 // operand of dW).
+#include <algorithm>
 #include <type_traits>
 
 #include "dh_common.hpp"
@@ -1322,6 +1323,416 @@ __global__ void __launch_bounds__(256) finish(Finish<OT> h, Finish<OT> w, int D)
         if (c + q < D) f.out.put(to + q, PARTS == 1 ? v[q] : __builtin_ldexpf(v[q], e) * wi);
 }
 
+// ---- few rows --------------------------------------------------------------------------------------
+// Up to FEW rows: bound by reading the table, so it is read as it is, at any alignment, once for
+// the forward and twice for the gradient, straight into the fp32 matrix cores (v_mfma_f32_16x16x4:
+// at 16 rows they take 17 TB/s of fp32 values or 9 of bf16), with no packing: a row that does not
+// count reads as zeros, and its G is zero.  G is fp32, [table row][FEW].
+constexpr int FEW = 16;
+constexpr int FEW_MAX_V = 1 << 21;
+
+struct Few {
+    Targets targets;
+    int N, D;
+    const void* H;
+    int ldh;
+    const void* W;
+    int ldw;
+    float c;
+    float2* part;        // [work-group of few_lse][FEW]
+    float* G;
+    const float *lse, *dloss;
+    float wscale, factor;
+    float *loss, *lse_out;
+    // dH's splits of the table rows, [split][FEW][Dp]
+    float* acc;
+    int Dp, splits, rows_per_split, hblocks, hslabs;
+    // dW
+    int wrows, wslabs, wlanes;   // table rows of a work-group, slabs of columns, lanes of a row
+};
+
+// One wave's operands of a step of 32 k: lane l has 8 values from k + 8 (l / 16) of the rows l % 16 of
+// RT tiles of the table, and of token l % 16.  The order of k within the step is the same on
+// both sides, so it does not matter which instruction takes which.
+template <typename T, int RT> struct FewStep;
+template <int RT> struct FewStep<float, RT> {   // v_mfma_f32_16x16x4_f32: a value of each lane at a time
+    static constexpr int AHEAD = 1;
+    float x[RT][8], y[8];
+    __device__ static void get(const float* p, int k, int D, float (&v)[8]) { load8(p, k, D, v); }
+    __device__ void zero() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = 0.f;
+    }
+    __device__ void mma(f32x4 (&acc)[RT]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int a = 0; a < RT; ++a) acc[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[a][e], y[e], acc[a], 0, 0, 0);
+    }
+};
+template <int RT> struct FewStep<uint16_t, RT> {   // v_mfma_f32_16x16x32_bf16: all 8; half the registers, more ahead
+    static constexpr int AHEAD = 3;
+    h8 x[RT], y;
+    __device__ static void get(const uint16_t* p, int k, int D, h8& v) {
+        if (k + 8 <= D) {
+            v = *reinterpret_cast<const h8a*>(p + k);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = k + e < D ? p[k + e] : (uint16_t)0;
+        }
+    }
+    __device__ void zero() { y = h8{}; }
+    __device__ void mma(f32x4 (&acc)[RT]) const {
+#pragma unroll
+        for (int a = 0; a < RT; ++a)
+            acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[a]),
+                                                             __builtin_bit_cast(bf16x8, y), acc[a], 0, 0, 0);
+    }
+};
+
+// 16 RT rows of logits against FEW tokens: the work-group's KW waves share the k of all rows (steps of
+// 32 k in turn), and their sums meet in LDS in wave order.  Thread t < 64 RT ends with row t / 4,
+// tokens 4 (t % 4) .. + 3.
+template <typename T, int KW, int RT>
+__device__ inline f32x4 few_logits(const Few& f, int v0, uint32_t keep, float (*red)[16 * RT][FEW]) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int m = lane & 15, k8 = 8 * (lane >> 4);
+    const int V = f.targets.V, D = f.D;
+    const T* rows[RT];
+#pragma unroll
+    for (int a = 0; a < RT; ++a)   // past the end: the last row again, unused
+        rows[a] = (const T*)f.W + (size_t)min(v0 + 16 * a + m, V - 1) * f.ldw;
+    const T* h = (const T*)f.H + (size_t)m * f.ldh;
+    const bool on = (keep >> m) & 1;
+    f32x4 acc[RT];
+#pragma unroll
+    for (int a = 0; a < RT; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int AHEAD = FewStep<T, RT>::AHEAD, NB = AHEAD + 1, HOP = 32 * KW;
+    FewStep<T, RT> step[NB];
+    auto fetch = [&](int k, FewStep<T, RT>& st) {
+#pragma unroll
+        for (int a = 0; a < RT; ++a) FewStep<T, RT>::get(rows[a], k + k8, D, st.x[a]);
+        if (on) FewStep<T, RT>::get(h, k + k8, D, st.y);
+        else st.zero();
+    };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+        if (32 * w + HOP * u < D) fetch(32 * w + HOP * u, step[u]);
+    for (int k = 32 * w; k < D; k += HOP * NB) {
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+            const int here = k + HOP * u;
+            if (here >= D) break;
+            if (here + HOP * AHEAD < D) fetch(here + HOP * AHEAD, step[(u + AHEAD) % NB]);
+            step[u].mma(acc);
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < RT; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) red[w][16 * a + 4 * (lane >> 4) + r][m] = acc[a][r];
+    __syncthreads();
+    const int row = (threadIdx.x % (64 * RT)) >> 2, n4 = 4 * (threadIdx.x & 3);
+    f32x4 z = *reinterpret_cast<const f32x4*>(&red[0][row][n4]);
+#pragma unroll
+    for (int p = 1; p < KW; ++p) z += *reinterpret_cast<const f32x4*>(&red[p][row][n4]);
+    return z;
+}
+
+// The rows that count, as bits.
+__device__ inline uint32_t few_keep(const Few& f) {
+    const int lane = threadIdx.x & 63;
+    return (uint32_t)__ballot(lane < f.N && f.targets.has(lane));
+}
+
+template <typename T, int KW, int RT>
+__global__ void __launch_bounds__(64 * KW) few_lse(Few f) {
+    __shared__ float red[KW][16 * RT][FEW];
+    __shared__ float stat[2][RT][FEW];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int v0 = blockIdx.x * 16 * RT, row = threadIdx.x >> 2, n4 = 4 * (threadIdx.x & 3);
+    f32x4 z = few_logits<T, KW, RT>(f, v0, few_keep(f), red);
+    const bool own = w < RT, in = v0 + row < f.targets.V;
+    f32x4 mx;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        z[q] = in ? f.c * z[q] : -INFINITY;
+        mx[q] = z[q];
+        for (int x = 4; x < 64; x <<= 1) mx[q] = fmaxf(mx[q], __shfl_xor(mx[q], x, 64));
+        if (own && lane < 4) stat[0][w][n4 + q] = mx[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float m = stat[0][0][n4 + q];
+        for (int x = 1; x < RT; ++x) m = fmaxf(m, stat[0][x][n4 + q]);
+        mx[q] = m;
+        float s = __expf(z[q] - (m == -INFINITY ? 0.f : m));
+        for (int x = 4; x < 64; x <<= 1) s += __shfl_xor(s, x, 64);
+        if (own && lane < 4) stat[1][w][n4 + q] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < 4)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float s = stat[1][0][n4 + q];
+            for (int x = 1; x < RT; ++x) s += stat[1][x][n4 + q];
+            f.part[(size_t)blockIdx.x * FEW + n4 + q] = float2{mx[q], s};
+        }
+}
+
+// A row's teacher: largest logit and logarithm of the sum of exponentials, by every wave.
+__device__ inline void teacher_stats(const Teacher& t, size_t at, int V, float& mx, float& log_sum) {
+    const int lane = threadIdx.x & 63;
+    mx = -INFINITY;
+    for (int k = lane; k < t.K; k += 64)
+        if (entry_counts(t, at + k, V)) mx = fmaxf(mx, t.logit[at + k]);
+    mx = wave_reduce(mx, OpMax());
+    float sum = 0.f;
+    for (int k = lane; k < t.K; k += 64)
+        if (entry_counts(t, at + k, V)) sum += __expf((t.logit[at + k] - mx) * t.inv_t);
+    log_sum = __logf(wave_reduce(sum, OpSum()));
+}
+
+// A work-group per row: joins the parts, takes the logits at the row's targets and writes loss and
+// lse.
+template <typename T>
+__global__ void __launch_bounds__(1024) few_loss(Few f, int blocks) {
+    __shared__ float2 red[16];
+    __shared__ float redf[16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int n = blockIdx.x;
+    const Targets& tg = f.targets;
+    if (!tg.has(n)) {
+        if (threadIdx.x == 0) {
+            f.loss[n] = 0.f;
+            if (f.lse_out) f.lse_out[n] = 0.f;
+        }
+        return;
+    }
+    float m = -INFINITY, s = 0.f;
+    for (int b = threadIdx.x; b < blocks; b += 1024) {
+        const float2 p = f.part[(size_t)b * FEW + n];
+        lse_merge(m, s, p.x, p.y);
+    }
+    for (int x = 1; x < 64; x <<= 1) {
+        const float m2 = __shfl_xor(m, x, 64), s2 = __shfl_xor(s, x, 64);
+        lse_merge(m, s, m2, s2);
+    }
+    const T* h = (const T*)f.H + (size_t)n * f.ldh;
+    const T* W = (const T*)f.W;
+    float base = 0.f;   // of this wave
+    if (tg.target) {
+        if (w == 0) base = -(f.c * row_dot(h, W + (size_t)tg.target[n] * f.ldw, f.D, lane));
+    } else {
+        const size_t at = (size_t)n * tg.t.K;
+        float mx, log_sum;
+        teacher_stats(tg.t, at, tg.V, mx, log_sum);
+        for (int k = w; k < tg.t.K; k += 16)
+            if (entry_counts(tg.t, at + k, tg.V)) {
+                const float z = f.c * row_dot(h, W + (size_t)tg.t.id[at + k] * f.ldw, f.D, lane);
+                const float lq = (tg.t.logit[at + k] - mx) * tg.t.inv_t - log_sum, q = __expf(lq);
+                if (!(q == 0.f)) base += q * (lq - z);
+            }
+    }
+    if (lane == 0) {
+        red[w] = float2{m, s};
+        redf[w] = base;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int x = 1; x < 16; ++x) {
+        lse_merge(m, s, red[x].x, red[x].y);
+        base += redf[x];
+    }
+    const float l = m + __logf(s);
+    if (f.lse_out) f.lse_out[n] = l;
+    f.loss[n] = f.factor * (l + base);
+}
+
+// G = w (softmax - [target]); what a teacher takes off follows.
+template <typename T, int KW, int RT>
+__global__ void __launch_bounds__(64 * KW) few_g(Few f) {
+    __shared__ float red[KW][16 * RT][FEW];
+    const int v0 = blockIdx.x * 16 * RT, v = v0 + (threadIdx.x >> 2), n4 = 4 * (threadIdx.x & 3);
+    const uint32_t keep = few_keep(f);
+    const f32x4 z = few_logits<T, KW, RT>(f, v0, keep, red);
+    if (threadIdx.x >= 64 * RT || v >= f.targets.V) return;
+    f32x4 g = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if ((keep >> (n4 + q)) & 1) {
+            const int n = n4 + q;
+            float p = __expf(__builtin_fmaf(f.c, z[q], -f.lse[n]));
+            if (f.targets.target && f.targets.target[n] == v) p -= 1.f;
+            g[q] = (f.dloss ? f.dloss[n] : 1.f) * f.wscale * p;
+        }
+    *reinterpret_cast<f32x4*>(f.G + (size_t)v * FEW + n4) = g;
+}
+
+// A work-group per row: the first entry of each token takes off the sum of its entries.
+__global__ void __launch_bounds__(256) few_teacher(Few f) {
+    const int n = blockIdx.x;
+    const Teacher& t = f.targets.t;
+    const int V = f.targets.V;
+    const size_t at = (size_t)n * t.K;
+    float mx, log_sum;
+    teacher_stats(t, at, V, mx, log_sum);
+    const float w = (f.dloss ? f.dloss[n] : 1.f) * f.wscale;
+    for (int k = threadIdx.x; k < t.K; k += 256) {
+        if (!entry_counts(t, at + k, V)) continue;
+        const int id = t.id[at + k];
+        float q = 0.f;
+        bool first = true;
+        for (int j = 0; j < t.K; ++j)
+            if (t.id[at + j] == id && entry_counts(t, at + j, V)) {
+                first &= j >= k;
+                q += __expf((t.logit[at + j] - mx) * t.inv_t - log_sum);
+            }
+        if (first) f.G[(size_t)id * FEW + n] -= w * q;
+    }
+}
+
+// R values of a row from column c, zero past its end; any alignment.
+template <int R, typename T>
+__device__ inline void load_piece(const T* __restrict__ p, int c, int D, float* v) {
+    typedef T piece __attribute__((ext_vector_type(R), aligned(sizeof(T))));
+    if (c + R <= D) {
+        const piece x = *reinterpret_cast<const piece*>(p + c);
+#pragma unroll
+        for (int e = 0; e < R; ++e) {
+            if constexpr (sizeof(T) == 4) v[e] = x[e];
+            else v[e] = bf16_bits_to_f32(x[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < R; ++e) {
+            if constexpr (sizeof(T) == 4) v[e] = c + e < D ? p[c + e] : 0.f;
+            else v[e] = c + e < D ? bf16_bits_to_f32(p[c + e]) : 0.f;
+        }
+    }
+}
+
+// dH and dW.  Work-groups [0, hblocks): a split of the table rows and a slab of 16 C columns (C = 4
+// or 8 values of 16 bytes); its 4 waves take a quarter of the rows each, 4 rows an instruction:
+// lane l has G of token l % 16 and C columns of the table at row l / 16, and the products with
+// column j of each piece go to accumulator j.  The others: rows of dW by slabs of 64 C' columns, a
+// lane's C' columns of all rows of H in registers, G by scalar loads; narrow tables take several rows
+// at a time, 1 / lanes of a wave each.
+template <typename T, typename OT, int NT>
+__global__ void __launch_bounds__(256) few_grads(Few f, const float* __restrict__ G, Grad<OT> dW) {
+    constexpr int C = 16 / sizeof(T), CW = 16 / sizeof(OT);
+    __shared__ float red[3][FEW][16 * C];
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int V = f.targets.V, D = f.D;
+    if ((int)blockIdx.x < f.hblocks) {
+        const int slab = blockIdx.x % f.hslabs, split = blockIdx.x / f.hslabs;
+        const int c0 = 16 * C * slab + C * (lane & 15), r4 = lane >> 4, n = lane & 15;
+        const int per = f.rows_per_split / 4;   // a multiple of 4
+        const int begin = split * f.rows_per_split + w * per, end = min(begin + per, V);
+        const T* W = (const T*)f.W;
+        f32x4 acc[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int FLY = 4;
+        for (int v0 = begin; v0 < end; v0 += 4 * FLY) {
+            float g[FLY], x[FLY][8];
+#pragma unroll
+            for (int u = 0; u < FLY; ++u) {
+                const int v = v0 + 4 * u + r4, at = v < end ? v : begin;
+                g[u] = G[(size_t)at * FEW + n];
+                if (v >= end) g[u] = 0.f;
+                load_piece<C>(W + (size_t)at * f.ldw, c0, D, x[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < FLY; ++u)
+#pragma unroll
+                for (int j = 0; j < C; ++j)
+                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[u], x[u][j], acc[j], 0, 0, 0);
+        }
+        // acc[j][r]: token 4 (lane / 16) + r, column C (lane % 16) + j of the slab
+        if (w > 0)
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) red[w - 1][4 * r4 + r][C * n + j] = acc[j][r];
+        __syncthreads();
+        if (w > 0) return;
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = acc[j][r];
+                for (int p = 0; p < 3; ++p) v += red[p][4 * r4 + r][C * n + j];
+                if (c0 + j < D) f.acc[((size_t)split * FEW + 4 * r4 + r) * f.Dp + c0 + j] = v;
+            }
+        return;
+    }
+    const int b = blockIdx.x - f.hblocks;
+    const int slab = b % f.wslabs, v0 = b / f.wslabs * f.wrows, end = min(v0 + f.wrows, V);
+    const int lanes = f.wlanes, each = 64 / lanes;   // lanes of a row, rows of a wave
+    const int c0 = 64 * CW * slab + CW * (lane & (lanes - 1));
+    const uint32_t keep = few_keep(f);
+    float h[NT][CW];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float x[8] = {};
+        if ((keep >> n) & 1) load_piece<CW>((const T*)f.H + (size_t)n * f.ldh, c0, D, x);
+#pragma unroll
+        for (int j = 0; j < CW; ++j) h[n][j] = x[j];
+    }
+    auto put = [&](int v, const float* __restrict__ g) {
+        float s[CW] = {};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float gn = g[n];
+#pragma unroll
+            for (int j = 0; j < CW; ++j) s[j] = __builtin_fmaf(gn, h[n][j], s[j]);
+        }
+        OT* to = dW.at(v) + c0;
+        if (!dW.accumulate && c0 + CW <= D) {
+            if constexpr (CW == 4) {
+                *reinterpret_cast<f4a*>(to) = f4a{s[0], s[1], s[2], s[3]};
+            } else {
+                h8a x;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = rne_bf16(s[j]);
+                *reinterpret_cast<h8a*>(to) = x;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < CW; ++j)
+                if (c0 + j < D) dW.put(to + j, s[j]);
+        }
+    };
+    if (each == 1) {
+        for (int v = v0 + w; v < end; v += 4) put(v, G + (size_t)v * FEW);
+    } else {
+        for (int v = v0 + w * each + lane / lanes; v < end; v += 4 * each) put(v, G + (size_t)v * FEW);
+    }
+}
+
+// dH (+)= the sum of its splits: a work-group per row and 64 columns, its 16 waves share the splits
+// and meet in LDS in wave order.
+template <typename OT>
+__global__ void __launch_bounds__(1024) few_finish(Few f, Grad<OT> dH) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int n = blockIdx.y, c = blockIdx.x * 64 + lane;
+    const bool on = f.targets.has(n);
+    if (!on && dH.accumulate) return;
+    float v = 0.f;
+    if (on && c < f.D)
+#pragma unroll 4
+        for (int s = w; s < f.splits; s += 16) v += f.acc[((size_t)s * FEW + n) * f.Dp + c];
+    red[w][lane] = v;
+    __syncthreads();
+    if (w != 0 || c >= f.D) return;
+    for (int x = 1; x < 16; ++x) v += red[x][lane];
+    dH.put(dH.C + (size_t)n * dH.ldc + c, v);
+}
+
 // The gradient of no rows at all (N = 0).
 template <typename OT>
 __global__ void __launch_bounds__(256) clear_rows(OT* __restrict__ p, int R, int D, int ld) {
@@ -1444,8 +1855,48 @@ Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* 
     return p;
 }
 
+// Few rows: nothing is packed or staged, the workspace does not depend on alignments.
+bool is_few(int N, int V) { return N <= FEW && V <= FEW_MAX_V; }
+
+struct FewPlan {
+    int Dp, rows, waves, blocks;   // of few_lse and few_g: table rows and waves of a work-group
+    int splits, rows_per_split, hslabs, wslabs, wrows, wlanes;
+    size_t G, acc, total;   // the parts of the forward lie at G
+};
+FewPlan few_plan(int dtype, int grad_type, int V, int D, int backward) {
+    FewPlan p{};
+    const int C = dtype == DH_F32 ? 4 : 8, CW = grad_type == DH_F32 ? 4 : 8;
+    p.Dp = (D + 3) / 4 * 4;
+    // 64 rows and 4 waves; few work-groups of those: 16 rows, and a long k shared by 16 waves, which
+    // shortens its chain of loads (2000 x 4000 fp32: 41 / 18 us).
+    const bool small = V <= 64 * 256;
+    p.rows = small ? 16 : 64;
+    p.waves = small && D >= 512 ? 16 : 4;
+    p.blocks = (V + p.rows - 1) / p.rows;
+    if (!backward) {
+        p.total = up256((size_t)p.blocks * FEW * 8);
+        return p;
+    }
+    // About 1024 work-groups of 4 waves for dH and 4096 for dW.
+    p.hslabs = (D + 16 * C - 1) / (16 * C);
+    const int splits = std::max(1, std::min(1024 / p.hslabs, (V + 63) / 64));
+    p.rows_per_split = ((V + splits - 1) / splits + 15) / 16 * 16;
+    p.splits = (V + p.rows_per_split - 1) / p.rows_per_split;
+    p.wslabs = (D + 64 * CW - 1) / (64 * CW);
+    p.wlanes = 64;
+    while (p.wlanes > 1 && p.wlanes / 2 * CW >= D) p.wlanes /= 2;
+    const int least = 16 * (64 / p.wlanes);   // rows of a work-group
+    const int chunks = std::max(1, std::min(4096 / p.wslabs, (V + least - 1) / least));
+    p.wrows = (V + chunks - 1) / chunks;
+    p.acc = up256((size_t)p.blocks * p.rows * FEW * 4);
+    p.total = p.acc + up256((size_t)p.splits * FEW * p.Dp * 4);
+    return p;
+}
+
 // The workspace that serves any alignment of the operands (staged tables take more).
 size_t least_ws(int dtype, int N, int V, int D, int K, int backward) {
+    if (is_few(N, V))   // whichever type the gradients have
+        return std::max(few_plan(dtype, DH_F32, V, D, backward).total, few_plan(dtype, dtype, V, D, backward).total);
     const Plan p = make_plan(dtype, N, V, D, K, backward, nullptr, 1);
     return p.piece + p.per_block + 512;
 }
@@ -1723,6 +2174,69 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     }
 }
 
+Few few_args(const Head& h) {
+    Few f{};
+    f.targets = {h.target, h.teacher, h.V};
+    f.N = h.N;
+    f.D = h.D;
+    f.H = h.H;
+    f.ldh = h.ldh;
+    f.W = h.W;
+    f.ldw = h.ldw;
+    f.c = h.c;
+    f.wscale = h.wscale;
+    f.factor = h.factor;
+    return f;
+}
+
+template <typename T>
+int few_forward(const Head& h, float* loss, float* lse, void* ws) {
+    const FewPlan p = few_plan(h.dtype, h.dtype, h.V, h.D, 0);
+    Few f = few_args(h);
+    f.part = (float2*)ws;
+    f.loss = loss;
+    f.lse_out = lse;
+    auto lse_parts = p.rows == 64 ? few_lse<T, 4, 4> : p.waves == 4 ? few_lse<T, 4, 1> : few_lse<T, 16, 1>;
+    lse_parts<<<p.blocks, 64 * p.waves, 0, stream()>>>(f);
+    DH_TRY(check_launch(h.op));
+    few_loss<T><<<h.N, 1024, 0, stream()>>>(f, p.blocks);
+    return check_launch(h.op);
+}
+
+template <typename T, typename OT>
+int few_backward(const Head& h, const Grads& d, void* ws) {
+    const FewPlan p = few_plan(h.dtype, d.type, h.V, h.D, 1);
+    Few f = few_args(h);
+    f.G = (float*)ws;
+    f.acc = (float*)((char*)ws + p.acc);
+    f.lse = d.lse;
+    f.dloss = d.dloss;
+    f.Dp = p.Dp;
+    f.splits = p.splits;
+    f.rows_per_split = p.rows_per_split;
+    f.hslabs = p.hslabs;
+    f.hblocks = d.dH ? p.hslabs * p.splits : 0;
+    f.wslabs = p.wslabs;
+    f.wrows = p.wrows;
+    f.wlanes = p.wlanes;
+    auto g = p.rows == 64 ? few_g<T, 4, 4> : p.waves == 4 ? few_g<T, 4, 1> : few_g<T, 16, 1>;
+    g<<<p.blocks, 64 * p.waves, 0, stream()>>>(f);
+    DH_TRY(check_launch(h.op));
+    if (!h.target && h.teacher.K > 0) {
+        few_teacher<<<h.N, 256, 0, stream()>>>(f);
+        DH_TRY(check_launch(h.op));
+    }
+    const Grad<OT> dW{(OT*)d.dW, d.lddw, d.acc_dW, nullptr, nullptr, nullptr};
+    const int wblocks = d.dW ? (h.V + p.wrows - 1) / p.wrows * p.wslabs : 0;
+    auto grads = h.N <= 4 ? few_grads<T, OT, 4> : h.N <= 8 ? few_grads<T, OT, 8> : few_grads<T, OT, 16>;
+    grads<<<f.hblocks + wblocks, 256, 0, stream()>>>(f, f.G, dW);
+    DH_TRY(check_launch(h.op));
+    if (!d.dH) return DH_OK;
+    few_finish<OT><<<dim3((h.D + 63) / 64, h.N), 1024, 0, stream()>>>(
+        f, Grad<OT>{(OT*)d.dH, d.lddh, d.acc_dH, nullptr, nullptr, nullptr});
+    return check_launch(h.op);
+}
+
 int run_forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_bytes) {
     const int K = h.target ? 0 : h.teacher.K;
     DH_TRY(check_head(h, K, ws, ws_bytes, 0));
@@ -1730,6 +2244,8 @@ int run_forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_byte
         return set_error(DH_ERR_INVALID, "%s: null pointer", h.op);
     DH_TRY(ensure_init());
     if (h.N == 0) return DH_OK;
+    if (is_few(h.N, h.V))
+        return h.dtype == DH_F32 ? few_forward<float>(h, loss, lse, ws) : few_forward<uint16_t>(h, loss, lse, ws);
     return h.dtype == DH_F32 ? forward<float, 2>(h, loss, lse, ws, ws_bytes)
                              : forward<uint16_t, 1>(h, loss, lse, ws, ws_bytes);
 }
@@ -1752,6 +2268,11 @@ int run_backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         else
             clear_rows<<<2048, 256, 0, stream()>>>((uint16_t*)d.dW, h.V, h.D, d.lddw);
         return check_launch(h.op);
+    }
+    if (is_few(h.N, h.V)) {
+        if (h.dtype == DH_F32) return few_backward<float, float>(h, d, ws);
+        return d.type == DH_F32 ? few_backward<uint16_t, float>(h, d, ws)
+                                : few_backward<uint16_t, uint16_t>(h, d, ws);
     }
     if (h.dtype == DH_F32) return backward<float, 2, float>(h, d, ws, ws_bytes);
     return d.type == DH_F32 ? backward<uint16_t, 1, float>(h, d, ws, ws_bytes)

@@ -286,7 +286,8 @@ def run_loss(c, grad=None, extra=0, accumulate=False):
 
 
 SHAPES = [(1, 1, 1), (1, 65, 32), (2, 3, 5), (31, 257, 64), (64, 1000, 100), (256, 256, 32),
-          (257, 300, 40), (300, 1025, 96), (513, 130, 264), (3, 5000, 72)]
+          (257, 300, 40), (300, 1025, 96), (513, 130, 264), (3, 5000, 72), (16, 3000, 129),
+          (5, 64, 1030), (9, 700, 300), (17, 3000, 129)]
 
 
 @pytest.mark.gpu
