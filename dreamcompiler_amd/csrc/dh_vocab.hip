@@ -932,15 +932,135 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
     epi.template run<FM, FN>(acc, M, N, m0 + wm, n0 + wn, lane, split, ring + wave * LDS_TILE);
 }
 
+// The 64-wide tile of two parts: a stage holds 64 k of both parts of both operands (32 KB, a ring of
+// four) and each of its 16-k steps makes all three products, the cross products in accumulators of
+// their own.  One chain of stages instead of three, and two thirds of the loads.
+template <class S, bool AK, bool BK_, int TOK, class Epi>
+__device__ inline void gemm_both(uint16_t* ring, const Prod& g, const Epi& epi, int tile, int tiles,
+                                 int split) {
+    constexpr int T = S::T, BK = S::BK, NS = S::NS, STEPS = BK / 16, SUB = T * BK;
+    static_assert(S::FM == 1 && S::FN == 1, "one block per wave");
+    using OA = Operand<AK, T, BK, S::WAVES>;
+    using OB = Operand<BK_, T, BK, S::WAVES>;
+    constexpr int LOADS = 2 * (OA::PER + OB::PER);
+    const int cnt = __builtin_amdgcn_readfirstlane(*g.cnt);
+    const int M = TOK == TOK_M ? cnt : g.M, N = TOK == TOK_N ? cnt : g.N;
+    const int Kall = TOK == TOK_K ? cnt : g.K;
+    int tm, tn;
+    xcd_tile_order(tile, tiles, (g.M + T - 1) / T, (g.N + T - 1) / T, 4, tm, tn);
+    const int m0 = tm * T, n0 = tn * T;
+    if (m0 >= M || n0 >= N) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = (wave / S::WAVES_N) * S::WM, wn = (wave % S::WAVES_N) * S::WN;
+
+    f32x16 acc[1][1], cross;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[0][0][r] = cross[r] = 0.f;
+    const int kt0 = split * g.kstages;
+    const int total = max(0, min((Kall + BK - 1) / BK - kt0, g.kstages));
+    if (total > 0) {
+        OA sa[2];
+        OB sb[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            sa[p].init(g.A, g.pa, g.lda, m0, M, Kall, wave, lane);
+            sb[p].init(g.B, g.pb, g.ldb, n0, N, Kall, wave, lane);
+            sa[p].start(p, kt0);
+            sb[p].start(p, kt0);
+        }
+        const int tail = (kt0 + total) * BK > Kall ? total - 1 : -1;   // the stage that ends behind K
+        constexpr uint32_t RING = 2u * NS * 4 * SUB;
+        const uint32_t ring0 = lds_addr(ring) + 1024u * OA::PER * wave;
+        static_assert(OA::PER == OB::PER, "one offset of the wave");
+        int ikt = 0;   // the next stage to fetch
+        uint32_t slot = 0;
+        auto issue = [&]() {
+            const uint32_t to = ring0 + slot;
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int t = 0; t < OA::PER; ++t) {
+                    if (__builtin_expect(ikt != tail, 1)) {
+                        sa[p].issue_one(to + 2u * SUB * p, t);
+                        sb[p].issue_one(to + 2u * SUB * (2 + p), t);
+                    } else {
+                        sa[p].issue_end(to + 2u * SUB * p, t, kt0 + ikt, wave, lane);
+                        sb[p].issue_end(to + 2u * SUB * (2 + p), t, kt0 + ikt, wave, lane);
+                    }
+                }
+            slot = slot == RING - 2u * 4 * SUB ? 0u : slot + 2u * 4 * SUB;
+            ++ikt;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                sa[p].next();
+                sb[p].next();
+            }
+        };
+        auto landed = [&](int ahead) {   // all but the youngest `ahead` stages
+            if (ahead >= 2) wait_vmcnt<2 * LOADS>();
+            else if (ahead == 1) wait_vmcnt<LOADS>();
+            else wait_vmcnt<0>();
+        };
+        f16x8 fa[2][2], fb[2][2];   // [buffer][part]
+        auto read = [&](int s, int kk, int f) {
+            const uint16_t* st = ring + (s % NS) * 4 * SUB;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                fa[f][p] = __builtin_bit_cast(f16x8, OA::frag(st + p * SUB, wm, kk, lane));
+                fb[f][p] = __builtin_bit_cast(f16x8, OB::frag(st + (2 + p) * SUB, wn, kk, lane));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto mma = [&](int f) {
+            cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[f][1], fb[f][0], cross, 0, 0, 0);
+            acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[f][0], fb[f][0], acc[0][0], 0, 0, 0);
+            cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[f][0], fb[f][1], cross, 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        const int pre = min(total, NS - 1);
+        for (int s = 0; s < pre; ++s) issue();
+        landed(pre - 1);
+        __syncthreads();
+        read(0, 0, 0);
+        for (int s = 0; s < total; ++s) {
+            if (s + NS - 1 < total) issue();
+#pragma unroll
+            for (int kk = 0; kk < STEPS - 1; ++kk) {
+                read(s, kk + 1, (kk + 1) & 1);
+                mma(kk & 1);
+            }
+            if (s + 1 < total) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                landed(min(total - 1, s + NS - 1) - (s + 1));
+                __syncthreads();
+                read(s + 1, 0, 0);
+            }
+            mma(1);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[0][0][r] = __builtin_fmaf(cross[r], 0x1p-11f, acc[0][0][r]);
+    if constexpr (Epi::LDS) __syncthreads();   // the ring is free
+    epi.template run<1, 1>(acc, M, N, m0 + wm, n0 + wn, lane, split, ring + wave * LDS_TILE);
+}
+
+// The form that a shape and its operands take, and its LDS in elements.
+template <class S, bool AK, int PARTS>
+constexpr int ring_of() {
+    return S::T == 256 && AK ? S::DEEP : S::NS * S::STAGE * (S::T == 64 && PARTS == 2 ? 2 : 1);
+}
+template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
+__device__ inline void gemm_form(uint16_t* ring, const Prod& g, const Epi& epi, int tile, int tiles, int split) {
+    if constexpr (S::T == 256 && AK) gemm_deep<S, BK, TOK, PARTS>(ring, g, epi, tile, tiles, split);
+    else if constexpr (S::T == 64 && PARTS == 2) gemm_both<S, AK, BK, TOK>(ring, g, epi, tile, tiles, split);
+    else gemm_tile<S, AK, BK, TOK, PARTS>(ring, g, epi, tile, tiles, split);
+}
+
 template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
 __global__ void __launch_bounds__(S::THREADS) vocab_gemm(Prod g, Epi epi) {
-    if constexpr (S::T == 256 && AK) {
-        __shared__ __attribute__((aligned(16))) uint16_t ring[S::DEEP];
-        gemm_deep<S, BK, TOK, PARTS>(ring, g, epi, blockIdx.x, gridDim.x, blockIdx.y);
-    } else {
-        __shared__ __attribute__((aligned(16))) uint16_t ring[S::NS * S::STAGE];
-        gemm_tile<S, AK, BK, TOK, PARTS>(ring, g, epi, blockIdx.x, gridDim.x, blockIdx.y);
-    }
+    __shared__ __attribute__((aligned(16))) uint16_t ring[ring_of<S, AK, PARTS>()];
+    gemm_form<S, AK, BK, TOK, PARTS>(ring, g, epi, blockIdx.x, gridDim.x, blockIdx.y);
 }
 
 // dH and dW of a piece in one launch: the first `first` work-groups are dH's, splits one after the
@@ -948,12 +1068,12 @@ __global__ void __launch_bounds__(S::THREADS) vocab_gemm(Prod g, Epi epi) {
 template <class S, int PARTS, class EpiH, class EpiW>
 __global__ void __launch_bounds__(S::THREADS) vocab_grads(Prod gh, EpiH eh, int tiles_h, int first, Prod gw,
                                                           EpiW ew, int tiles_w) {
-    __shared__ __attribute__((aligned(16))) uint16_t ring[S::NS * S::STAGE];
+    __shared__ __attribute__((aligned(16))) uint16_t ring[ring_of<S, true, PARTS>()];
     const int b = blockIdx.x;
     if (b < first)
-        gemm_tile<S, true, false, TOK_M, PARTS>(ring, gh, eh, b % tiles_h, tiles_h, b / tiles_h);
+        gemm_form<S, true, false, TOK_M, PARTS>(ring, gh, eh, b % tiles_h, tiles_h, b / tiles_h);
     else
-        gemm_tile<S, false, false, TOK_K, PARTS>(ring, gw, ew, (b - first) % tiles_w, tiles_w,
+        gemm_form<S, false, false, TOK_K, PARTS>(ring, gw, ew, (b - first) % tiles_w, tiles_w,
                                                  (b - first) / tiles_w);
 }
 
@@ -1764,35 +1884,38 @@ int wave_rows(Kind t) { return side(t) / 2; }
 long long tiles_of(Kind t, long long M, long long N) {
     return ((M + side(t) - 1) / side(t)) * ((N + side(t) - 1) / side(t));
 }
-// Splits of K over work-groups where sums of splits are added afterwards: towards one round of
-// work-groups, at least 512 k each.
-int splits_of(Kind t, long long M, long long N, long long K) {
-    const long long tiles = tiles_of(t, M, N), want = t == T256 ? 256 : 512;
-    long long s = tiles > 0 ? want / tiles : 1;
-    if (s > K / 512) s = K / 512;
-    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
-}
-// Estimated time of a product in us, the rule that picks its tile: rounds of work-groups (a last
-// round that is not full counts half of what it lacks) times their 32-k stages, each of the time
-// measured with one work-group on a CU or with as many as fit.  Measured / estimated, 256, 128 and
-// 64 wide: 1000 x 5000 x 256 fp32 29, 23, 24 / 28, 19, 23 us; 1000 x 2048 x 1024 bf16 28, 16, 11 /
-// 36, 16, 11; 32000 x 600 x 2048 bf16 119, 115, 161 / 118, 126, 202.
-double estimate(Kind t, long long M, long long N, long long K, int parts, bool split) {
+// Estimated time of a product in us, the rule that picks its tile and how many splits of K are added
+// afterwards: rounds of work-groups (a last round that is not full counts half of what it lacks)
+// times their 32-k stages, each of the time measured with one work-group on a CU or with as many as
+// fit; the sums of splits are written, read and cost a launch.
+double estimate(Kind t, long long M, long long N, long long K, int parts, int splits) {
     static const double alone[] = {1.0, 0.45, 0.19}, full[] = {1.0, 0.68, 0.30};
-    static const int fit[] = {1, 2, 2};
-    const int s = split ? splits_of(t, M, N, K) : 1;
-    const double groups = (double)tiles_of(t, M, N) * s;
-    const double stages = (double)((K + 31) / 32) * (parts == 2 ? 3 : 1) / s + 4;
-    double rounds = groups / (256 * fit[t]);
+    const bool both = t == T64 && parts == 2;   // gemm_both: three products a stage, one group a CU
+    const int fit = t == T256 || both ? 1 : 2;
+    const double groups = (double)tiles_of(t, M, N) * splits;
+    const double stages = (double)((K + 31) / 32) * (parts == 2 && !both ? 3 : 1) / splits + 4;
+    double rounds = groups / (256 * fit);
     const double whole = (double)(long long)(rounds + 0.9999);
     rounds = rounds <= 1 ? 1 : (rounds + whole) / 2;
-    return rounds * stages * (groups <= 256 ? alone[t] : full[t]) +
-           (s > 1 ? 3 + (double)s * M * N * 8 / 4e6 : 0);
+    const double stage = both ? 0.30 : groups <= 256 ? alone[t] : full[t];
+    return rounds * stages * stage + (splits > 1 ? 4 + (double)splits * M * N * 8 / 4e6 : 0);
 }
-Kind pick(long long M, long long N, long long K, int parts, bool split) {
-    Kind best = T64;
-    for (Kind t : {T128, T256})
-        if (estimate(t, M, N, K, parts, split) < estimate(best, M, N, K, parts, split)) best = t;
+struct Choice {
+    Kind kind;
+    int splits;
+};
+Choice pick(long long M, long long N, long long K, int parts, bool split) {
+    Choice best{T64, 1};
+    double least = estimate(T64, M, N, K, parts, 1);
+    for (Kind t : {T64, T128, T256})
+        for (int s = 1; s <= 64 && s * 128 <= std::max(128LL, K); s = s < 8 ? s + 1 : s + 4) {
+            const double e = estimate(t, M, N, K, parts, s);
+            if (e < least) {
+                least = e;
+                best = {t, s};
+            }
+            if (!split) break;
+        }
     return best;
 }
 
@@ -1820,10 +1943,13 @@ Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* 
     p.Nt = (int)(((long long)N + 255) / 256 * 256);
     // In place: whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
     p.direct = dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
-    p.lse = pick(V, N, D, p.parts, false);
-    p.g = pick(N, V, D, p.parts, false);
-    p.dh = pick(N, D, V, p.parts, true);
-    p.dw = pick(V, D, N, p.parts, true);
+    p.lse = pick(V, N, D, p.parts, false).kind;
+    p.g = pick(N, V, D, p.parts, false).kind;
+    const Choice dh = pick(N, D, V, p.parts, true), dw = pick(V, D, N, p.parts, true);
+    p.dh = dh.kind;
+    p.dw = dw.kind;
+    p.splits = dh.splits;
+    p.wsplits = dw.splits;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -1838,12 +1964,10 @@ Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* 
     p.z = take((size_t)N * K * 4);
     p.Hp = take((size_t)p.parts * N * p.Dp * 2);
     if (backward) {
-        p.splits = splits_of(p.dh, N, D, V);
         p.acc = take((size_t)p.splits * N * p.Dp * 4);
         if (p.parts == 2) p.Xp = take((size_t)p.parts * N * p.Dp * 2);
         p.per_block = (size_t)p.parts * N * (256 + 64) * 2;
         // dW's sums over splits of the rows: a piece's, fp32.
-        p.wsplits = splits_of(p.dw, V, D, N);
         if (p.wsplits > 1) p.per_block += (size_t)p.wsplits * 256 * p.Dp * 4;
     } else {
         p.state = take((size_t)p.Nt * 8);
