@@ -170,7 +170,8 @@ struct Rows {
     int* row;          // packed -> row
     int* target;
     int* hexp;
-    float *w, *lse;    // backward only
+    float *w, *lse;    // backward only; one part: w is the row's share of the largest weight,
+    float* wtop;       // which stands here
 };
 // Two parts: the scales of the other operands.
 struct Exps {
@@ -278,6 +279,7 @@ constexpr int PACK = 16;     // rows of a work-group, one per wave
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
     __shared__ int red[16];
+    __shared__ float tops[16];
     __shared__ int own[PACK];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const T* H = (const T*)a.H;
@@ -313,19 +315,39 @@ __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
     }
     const int n0 = blockIdx.x * PACK;
     int before = 0;
-    for (int n = threadIdx.x; n < n0; n += 1024) before += a.targets.has(n);
+    float top = 0.f;   // the largest size of a weight
+    const bool shares = PARTS == 1 && a.lse_in && a.dloss;
+    for (int n = threadIdx.x; n < (shares ? a.N : n0); n += 1024)
+        if (a.targets.has(n)) {
+            before += n < n0;
+            if (shares) {
+                const float x = __builtin_fabsf(a.dloss[n]);
+                top = x < INFINITY ? fmaxf(top, x) : top;
+            }
+        }
     for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m, 64);
-    if (lane == 0) red[w] = before;
+    if (shares) top = wave_reduce(top, OpMax());
+    if (lane == 0) {
+        red[w] = before;
+        tops[w] = top;
+    }
     if (threadIdx.x < PACK) own[threadIdx.x] = n0 + (int)threadIdx.x < a.N && a.targets.has(n0 + threadIdx.x);
     __syncthreads();
     before = 0;
-    for (int x = 0; x < 16; ++x) before += red[x];
+    for (int x = 0; x < 16; ++x) {
+        before += red[x];
+        top = fmaxf(top, tops[x]);
+    }
+    if (!(top > 0.f)) top = 1.f;
     int count = 0, i = before;
     for (int x = 0; x < PACK; ++x) {
         if (x < w) i += own[x];
         count += own[x];
     }
-    if ((int)blockIdx.x == a.groups - 1 && threadIdx.x == 0) *a.rows.cnt = before + count;
+    if ((int)blockIdx.x == a.groups - 1 && threadIdx.x == 0) {
+        *a.rows.cnt = before + count;
+        if (PARTS == 1 && a.lse_in) *a.rows.wtop = top * a.wscale;
+    }
     const int n = n0 + w;
     const bool keep = own[w];
     int most = NO_EXP;
@@ -342,7 +364,8 @@ __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
             a.rows.target[i] = target;
             a.rows.hexp[i] = h;
             if (a.lse_in) {
-                const float wn = (a.dloss ? a.dloss[n] : 1.f) * a.wscale;
+                const float d = a.dloss ? a.dloss[n] : 1.f;
+                const float wn = PARTS == 1 ? d / top : d * a.wscale;
                 a.rows.lse[i] = a.lse_in[n];
                 a.rows.w[i] = wn;
                 most = exponent(wn) + h;   // |w_n H_n| < 2^(15 + this)
@@ -1144,7 +1167,10 @@ struct EpiLse {
 };
 
 // Backward: rows are packed rows, columns the piece's table rows.  One part: G = w (p - q), rounded
-// once to bf16, the type that the products take.  Two parts: 2^14 (p - q) to 22 bits.  Columns past
+// once to bf16, the type that the products take; w is the row's share of the largest weight, so that
+// with equal weights the entry at an unlikely target lies just above -1, where bf16 rounds by 2^-9 of
+// it at most; times the weight itself it could be off by 2^-8, in the same direction in all rows that
+// share the target.  The gradients' last step multiplies by the largest weight.  Two parts: 2^14 (p - q) to 22 bits.  Columns past
 // the table's end up to the tile's are zero.
 template <int PARTS, bool HARD>
 struct EpiG {
@@ -1228,7 +1254,7 @@ struct EpiAcc {
 };
 
 // A gradient's rows and their scales: dH's packed rows go to their places, times w_n 2^(E - 14) with
-// two parts; dW's stay in order, times 2^(X - 14).
+// two parts; dW's stay in order, times 2^(X - 14).  One part: both times the largest weight, *w.
 template <typename OT>
 struct Grad {
     OT* C;
@@ -1236,7 +1262,7 @@ struct Grad {
     const int *row, *exp;
     const float* w;
     __device__ int scale() const { return exp ? *exp - 14 : 0; }
-    __device__ float weight(int i) const { return w ? w[i] : 1.f; }
+    template <int PARTS> __device__ float weight(int i) const { return PARTS == 1 ? *w : w ? w[i] : 1.f; }
     __device__ OT* at(int i) const { return C + (size_t)(row ? row[i] : i) * ldc; }
     __device__ void put(OT* to, float v) const {
         if constexpr (sizeof(OT) == 4) {
@@ -1259,13 +1285,14 @@ struct EpiOut {
         if constexpr (LDS) {
             static_assert(PARTS == 1, "bf16 results come from one part");
             if (!out.accumulate) {
+                const float w = out.template weight<1>(0);
 #pragma unroll
                 for (int a = 0; a < FM; ++a) {
                     uint16_t v[FN][16];
 #pragma unroll
                     for (int b = 0; b < FN; ++b)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) v[b][r] = rne_bf16(acc[a][b][r]);
+                        for (int r = 0; r < 16; ++r) v[b][r] = rne_bf16(acc[a][b][r] * w);
                     store_rows<FN>(lds, v, row0 + 32 * a, lane, [&](int row, int cc, h8 x) {
                         if (row >= M || col0 + cc >= N) return;
                         OT* to = out.at(row) + col0 + cc;
@@ -1289,14 +1316,14 @@ struct EpiOut {
                 const int row = row0 + reg_row(a, r, lane);
                 if (row >= M) continue;
                 OT* to = out.at(row);
-                const float w = PARTS == 1 ? 1.f : out.weight(row);
+                const float w = out.template weight<PARTS>(row);
 #pragma unroll
                 for (int b = 0; b < FN; ++b) {
                     const int col = col0 + 32 * b + (lane & 31);
                     if (col >= N) continue;
                     float v = acc[a][b][r];
-                    if constexpr (PARTS == 2) v = __builtin_ldexpf(v, s) * w;
-                    out.put(to + col, v);
+                    if constexpr (PARTS == 2) v = __builtin_ldexpf(v, s);
+                    out.put(to + col, v * w);
                 }
             }
     }
@@ -1436,11 +1463,11 @@ __global__ void __launch_bounds__(256) finish(Finish<OT> h, Finish<OT> w, int D)
     for (int s = 0; s < f.splits; ++s)
         v += *reinterpret_cast<const f32x4*>(f.acc + s * f.split + (size_t)i * f.lda + c);
     const int e = PARTS == 1 ? 0 : f.out.scale();
-    const float wi = PARTS == 1 ? 1.f : f.out.weight((int)i);
+    const float wi = f.out.template weight<PARTS>((int)i);
     OT* to = f.out.at((int)i) + c;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-        if (c + q < D) f.out.put(to + q, PARTS == 1 ? v[q] : __builtin_ldexpf(v[q], e) * wi);
+        if (c + q < D) f.out.put(to + q, (PARTS == 1 ? v[q] : __builtin_ldexpf(v[q], e)) * wi);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------
@@ -1979,7 +2006,6 @@ Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* 
     return p;
 }
 
-// Few rows: nothing is packed or staged, the workspace does not depend on alignments.
 bool is_few(int N, int V) { return N <= FEW && V <= FEW_MAX_V; }
 
 struct FewPlan {
@@ -2070,7 +2096,7 @@ Work lay_out(const Plan& p, void* ws) {
     auto array = [&](int k) { return ints + 64 + (size_t)k * p.Nt; };
     Work w{};
     w.p = p;
-    w.rows = {ints, array(0), array(1), array(2), (float*)(b + p.w), (float*)(b + p.lses)};
+    w.rows = {ints, array(0), array(1), array(2), (float*)(b + p.w), (float*)(b + p.lses), (float*)(ints + 3)};
     w.flags = array(3);
     w.exps = {nullptr, ints + 1, ints + 2, array(4), (float*)(array(4) + p.Nt / PACK)};
     w.base = (float*)(b + p.base);
@@ -2236,7 +2262,7 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     }
     DH_TRY((prepare_rows<T, PARTS>(h, w, a, more)));
     const Grad<OT> to_dH{(OT*)d.dH, d.lddh, d.acc_dH, w.rows.row, PARTS == 2 ? w.exps.E : nullptr,
-                         PARTS == 2 ? w.rows.w : nullptr};
+                         PARTS == 2 ? w.rows.w : w.rows.wtop};
     for (int v0 = 0;; v0 += rows) {
         const int R = h.V - v0 < rows ? h.V - v0 : rows;
         const bool last = h.V - v0 <= rows;
@@ -2276,7 +2302,7 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         const Prod gw{G, w.Xp, ldg, p.Dp, gplane, hplane, R, h.D, h.N, 0, w.rows.cnt};
         const Prod *ph = d.dH ? &gh : nullptr, *pw = d.dW ? &gw : nullptr;
         const Grad<OT> to_dW{d.dW ? (OT*)d.dW + (size_t)v0 * d.lddw : nullptr, d.lddw, d.acc_dW, nullptr,
-                             PARTS == 2 ? w.exps.X : nullptr, nullptr};
+                             PARTS == 2 ? w.exps.X : nullptr, PARTS == 2 ? nullptr : w.rows.wtop};
         // Straight to the gradient, or as sums that the last launch adds.
         const bool direct_h = one && p.splits == 1, direct_w = p.wsplits == 1;
         const EpiAcc sum_h{w.acc, p.Dp, v0 == 0, hplane}, sum_w{wacc, p.Dp, 1, wplane};
