@@ -618,7 +618,8 @@ EmbWs emb_ws(int N, int V, int D) {
 int check_emb(const char* op, int dtype, int N, int V, int D, float scale) {
     if (dtype != DH_F32 && dtype != DH_BF16)
         return set_error(DH_ERR_INVALID, "%s: dtype must be fp32 or bf16", op);
-    if (N < 0 || V < 1 || D < 1 || V == 0x7FFFFFFF || D > 1 << 24)
+    // 2^20 below the ends of int, which the strides of the kernels' loops stay under
+    if (N < 0 || V < 1 || D < 1 || N > 0x7FF00000 || V > 0x7FF00000 || D > 1 << 24)
         return set_error(DH_ERR_INVALID, "%s: shape N=%d V=%d D=%d", op, N, V, D);
     if (!(scale - scale == 0.f)) return set_error(DH_ERR_INVALID, "%s: scale must be finite", op);
     return DH_OK;

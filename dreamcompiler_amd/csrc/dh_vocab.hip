@@ -1486,7 +1486,8 @@ struct Few {
     const void* W;
     int ldw;
     float c;
-    float2* part;        // [work-group of few_lse][FEW]
+    float2* part;        // [work-group of few_lse][ldpart]
+    int ldpart;
     float* G;
     const float *lse, *dloss;
     float wscale, factor;
@@ -1499,27 +1500,30 @@ struct Few {
 };
 
 // One wave's operands of a step of 32 k: lane l has 8 values from k + 8 (l / 16) of the rows l % 16 of
-// RT tiles of the table, and of token l % 16.  The order of k within the step is the same on
+// RT tiles of the table, and of token l % 16 of TG groups.  The order of k within the step is the same on
 // both sides, so it does not matter which instruction takes which.
-template <typename T, int RT> struct FewStep;
-template <int RT> struct FewStep<float, RT> {   // v_mfma_f32_16x16x4_f32: a value of each lane at a time
+template <typename T, int RT, int TG> struct FewStep;
+template <int RT, int TG> struct FewStep<float, RT, TG> {   // v_mfma_f32_16x16x4_f32: a value of each lane at a time
     static constexpr int AHEAD = 1;
-    float x[RT][8], y[8];
+    float x[RT][8], y[TG][8];
     __device__ static void get(const float* p, int k, int D, float (&v)[8]) { load8(p, k, D, v); }
-    __device__ void zero() {
+    __device__ void zero(int t) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = 0.f;
+        for (int e = 0; e < 8; ++e) y[t][e] = 0.f;
     }
-    __device__ void mma(f32x4 (&acc)[RT]) const {
+    __device__ void mma(f32x4 (&acc)[TG][RT]) const {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int a = 0; a < RT; ++a) acc[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[a][e], y[e], acc[a], 0, 0, 0);
+            for (int t = 0; t < TG; ++t)
+#pragma unroll
+                for (int a = 0; a < RT; ++a)
+                    acc[t][a] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[a][e], y[t][e], acc[t][a], 0, 0, 0);
     }
 };
-template <int RT> struct FewStep<uint16_t, RT> {   // v_mfma_f32_16x16x32_bf16: all 8; half the registers, more ahead
+template <int RT, int TG> struct FewStep<uint16_t, RT, TG> {   // v_mfma_f32_16x16x32_bf16: all 8; more ahead
     static constexpr int AHEAD = 3;
-    h8 x[RT], y;
+    h8 x[RT], y[TG];
     __device__ static void get(const uint16_t* p, int k, int D, h8& v) {
         if (k + 8 <= D) {
             v = *reinterpret_cast<const h8a*>(p + k);
@@ -1528,20 +1532,22 @@ template <int RT> struct FewStep<uint16_t, RT> {   // v_mfma_f32_16x16x32_bf16: 
             for (int e = 0; e < 8; ++e) v[e] = k + e < D ? p[k + e] : (uint16_t)0;
         }
     }
-    __device__ void zero() { y = h8{}; }
-    __device__ void mma(f32x4 (&acc)[RT]) const {
+    __device__ void zero(int t) { y[t] = h8{}; }
+    __device__ void mma(f32x4 (&acc)[TG][RT]) const {
 #pragma unroll
-        for (int a = 0; a < RT; ++a)
-            acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[a]),
-                                                             __builtin_bit_cast(bf16x8, y), acc[a], 0, 0, 0);
+        for (int t = 0; t < TG; ++t)
+#pragma unroll
+            for (int a = 0; a < RT; ++a)
+                acc[t][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8, x[a]), __builtin_bit_cast(bf16x8, y[t]), acc[t][a], 0, 0, 0);
     }
 };
 
-// 16 RT rows of logits against FEW tokens: the work-group's KW waves share the k of all rows (steps of
+// 16 RT rows of logits against 16 TG tokens: the work-group's KW waves share the k of all rows (steps of
 // 32 k in turn), and their sums meet in LDS in wave order.  Thread t < 64 RT ends with row t / 4,
-// tokens 4 (t % 4) .. + 3.
-template <typename T, int KW, int RT>
-__device__ inline f32x4 few_logits(const Few& f, int v0, uint32_t keep, float (*red)[16 * RT][FEW]) {
+// tokens 4 (t % 4) .. + 3 of each 16.
+template <typename T, int KW, int RT, int TG>
+__device__ inline void few_logits(const Few& f, int v0, uint32_t keep, float (*red)[16 * RT][16 * TG], f32x4 (&z)[TG]) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int m = lane & 15, k8 = 8 * (lane >> 4);
     const int V = f.targets.V, D = f.D;
@@ -1550,17 +1556,21 @@ __device__ inline f32x4 few_logits(const Few& f, int v0, uint32_t keep, float (*
     for (int a = 0; a < RT; ++a)   // past the end: the last row again, unused
         rows[a] = (const T*)f.W + (size_t)min(v0 + 16 * a + m, V - 1) * f.ldw;
     const T* h = (const T*)f.H + (size_t)m * f.ldh;
-    const bool on = (keep >> m) & 1;
-    f32x4 acc[RT];
+    f32x4 acc[TG][RT];
 #pragma unroll
-    for (int a = 0; a < RT; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int AHEAD = FewStep<T, RT>::AHEAD, NB = AHEAD + 1, HOP = 32 * KW;
-    FewStep<T, RT> step[NB];
-    auto fetch = [&](int k, FewStep<T, RT>& st) {
+    for (int t = 0; t < TG; ++t)
 #pragma unroll
-        for (int a = 0; a < RT; ++a) FewStep<T, RT>::get(rows[a], k + k8, D, st.x[a]);
-        if (on) FewStep<T, RT>::get(h, k + k8, D, st.y);
-        else st.zero();
+        for (int a = 0; a < RT; ++a) acc[t][a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    using Step = FewStep<T, RT, TG>;
+    constexpr int AHEAD = Step::AHEAD, NB = AHEAD + 1, HOP = 32 * KW;
+    Step step[NB];
+    auto fetch = [&](int k, Step& st) {
+#pragma unroll
+        for (int a = 0; a < RT; ++a) Step::get(rows[a], k + k8, D, st.x[a]);
+#pragma unroll
+        for (int t = 0; t < TG; ++t)
+            if ((keep >> (16 * t + m)) & 1) Step::get(h + (size_t)16 * t * f.ldh, k + k8, D, st.y[t]);
+            else st.zero(t);
     };
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
@@ -1575,15 +1585,19 @@ __device__ inline f32x4 few_logits(const Few& f, int v0, uint32_t keep, float (*
         }
     }
 #pragma unroll
-    for (int a = 0; a < RT; ++a)
+    for (int t = 0; t < TG; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) red[w][16 * a + 4 * (lane >> 4) + r][m] = acc[a][r];
+        for (int a = 0; a < RT; ++a)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) red[w][16 * a + 4 * (lane >> 4) + r][16 * t + m] = acc[t][a][r];
     __syncthreads();
     const int row = (threadIdx.x % (64 * RT)) >> 2, n4 = 4 * (threadIdx.x & 3);
-    f32x4 z = *reinterpret_cast<const f32x4*>(&red[0][row][n4]);
 #pragma unroll
-    for (int p = 1; p < KW; ++p) z += *reinterpret_cast<const f32x4*>(&red[p][row][n4]);
-    return z;
+    for (int t = 0; t < TG; ++t) {
+        z[t] = *reinterpret_cast<const f32x4*>(&red[0][row][16 * t + n4]);
+#pragma unroll
+        for (int p = 1; p < KW; ++p) z[t] += *reinterpret_cast<const f32x4*>(&red[p][row][16 * t + n4]);
+    }
 }
 
 // The rows that count, as bits.
@@ -1592,40 +1606,47 @@ __device__ inline uint32_t few_keep(const Few& f) {
     return (uint32_t)__ballot(lane < f.N && f.targets.has(lane));
 }
 
-template <typename T, int KW, int RT>
+template <typename T, int KW, int RT, int TG>
 __global__ void __launch_bounds__(64 * KW) few_lse(Few f) {
-    __shared__ float red[KW][16 * RT][FEW];
-    __shared__ float stat[2][RT][FEW];
+    __shared__ float red[KW][16 * RT][16 * TG];
+    __shared__ float stat[2][RT][16 * TG];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int v0 = blockIdx.x * 16 * RT, row = threadIdx.x >> 2, n4 = 4 * (threadIdx.x & 3);
-    f32x4 z = few_logits<T, KW, RT>(f, v0, few_keep(f), red);
+    f32x4 z[TG], mx[TG];
+    few_logits<T, KW, RT, TG>(f, v0, few_keep(f), red, z);
     const bool own = w < RT, in = v0 + row < f.targets.V;
-    f32x4 mx;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        z[q] = in ? f.c * z[q] : -INFINITY;
-        mx[q] = z[q];
-        for (int x = 4; x < 64; x <<= 1) mx[q] = fmaxf(mx[q], __shfl_xor(mx[q], x, 64));
-        if (own && lane < 4) stat[0][w][n4 + q] = mx[q];
-    }
+    for (int t = 0; t < TG; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float m = z[t][q] = in ? f.c * z[t][q] : -INFINITY;
+            for (int x = 4; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+            if (own && lane < 4) stat[0][w][16 * t + n4 + q] = m;
+        }
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        float m = stat[0][0][n4 + q];
-        for (int x = 1; x < RT; ++x) m = fmaxf(m, stat[0][x][n4 + q]);
-        mx[q] = m;
-        float s = __expf(z[q] - (m == -INFINITY ? 0.f : m));
-        for (int x = 4; x < 64; x <<= 1) s += __shfl_xor(s, x, 64);
-        if (own && lane < 4) stat[1][w][n4 + q] = s;
-    }
+    for (int t = 0; t < TG; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int n = 16 * t + n4 + q;
+            float m = stat[0][0][n];
+            for (int x = 1; x < RT; ++x) m = fmaxf(m, stat[0][x][n]);
+            mx[t][q] = m;
+            float s = __expf(z[t][q] - (m == -INFINITY ? 0.f : m));
+            for (int x = 4; x < 64; x <<= 1) s += __shfl_xor(s, x, 64);
+            if (own && lane < 4) stat[1][w][n] = s;
+        }
     __syncthreads();
     if (threadIdx.x < 4)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float s = stat[1][0][n4 + q];
-            for (int x = 1; x < RT; ++x) s += stat[1][x][n4 + q];
-            f.part[(size_t)blockIdx.x * FEW + n4 + q] = float2{mx[q], s};
-        }
+        for (int t = 0; t < TG; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = 16 * t + n4 + q;
+                float s = stat[1][0][n];
+                for (int x = 1; x < RT; ++x) s += stat[1][x][n];
+                f.part[(size_t)blockIdx.x * f.ldpart + n] = float2{mx[t][q], s};
+            }
 }
 
 // A row's teacher: largest logit and logarithm of the sum of exponentials, by every wave.
@@ -1659,7 +1680,7 @@ __global__ void __launch_bounds__(1024) few_loss(Few f, int blocks) {
     }
     float m = -INFINITY, s = 0.f;
     for (int b = threadIdx.x; b < blocks; b += 1024) {
-        const float2 p = f.part[(size_t)b * FEW + n];
+        const float2 p = f.part[(size_t)b * f.ldpart + n];
         lse_merge(m, s, p.x, p.y);
     }
     for (int x = 1; x < 64; x <<= 1) {
@@ -1703,14 +1724,15 @@ __global__ void __launch_bounds__(64 * KW) few_g(Few f) {
     __shared__ float red[KW][16 * RT][FEW];
     const int v0 = blockIdx.x * 16 * RT, v = v0 + (threadIdx.x >> 2), n4 = 4 * (threadIdx.x & 3);
     const uint32_t keep = few_keep(f);
-    const f32x4 z = few_logits<T, KW, RT>(f, v0, keep, red);
+    f32x4 z[1];
+    few_logits<T, KW, RT, 1>(f, v0, keep, red, z);
     if (threadIdx.x >= 64 * RT || v >= f.targets.V) return;
     f32x4 g = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         if ((keep >> (n4 + q)) & 1) {
             const int n = n4 + q;
-            float p = __expf(__builtin_fmaf(f.c, z[q], -f.lse[n]));
+            float p = __expf(__builtin_fmaf(f.c, z[0][q], -f.lse[n]));
             if (f.targets.target && f.targets.target[n] == v) p -= 1.f;
             g[q] = (f.dloss ? f.dloss[n] : 1.f) * f.wscale * p;
         }
@@ -1962,14 +1984,18 @@ struct Plan {
     size_t per_block;         // bytes of a piece per 256 table rows
 };
 
+// Whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
+bool in_place(int dtype, int D, const void* W, int ldw) {
+    return dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
+}
+
 Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* W, int ldw) {
     Plan p{};
     p.parts = dtype == DH_F32 ? 2 : 1;
     p.Kp = (D + 31) / 32 * 32;
     p.Dp = apart(p.Kp);
     p.Nt = (int)(((long long)N + 255) / 256 * 256);
-    // In place: whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
-    p.direct = dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
+    p.direct = in_place(dtype, D, W, ldw);
     p.lse = pick(V, N, D, p.parts, false).kind;
     p.g = pick(N, V, D, p.parts, false).kind;
     const Choice dh = pick(N, D, V, p.parts, true), dw = pick(V, D, N, p.parts, true);
@@ -2006,14 +2032,18 @@ Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* 
     return p;
 }
 
-bool is_few(int N, int V) { return N <= FEW && V <= FEW_MAX_V; }
+// The forward also takes twice as many rows, where the table cannot be read in place: staging costs
+// more than the fp32 matrix cores at half their useful rate (18 x 41216 x 2357 fp32: OLDT / NEWT us).
+bool is_few(int N, int V, bool staged, int backward) {
+    return N <= (staged && !backward ? 2 * FEW : FEW) && V <= FEW_MAX_V;
+}
 
 struct FewPlan {
     int Dp, rows, waves, blocks;   // of few_lse and few_g: table rows and waves of a work-group
     int splits, rows_per_split, hslabs, wslabs, wrows, wlanes;
     size_t G, acc, total;   // the parts of the forward lie at G
 };
-FewPlan few_plan(int dtype, int grad_type, int V, int D, int backward) {
+FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int backward) {
     FewPlan p{};
     const int C = dtype == DH_F32 ? 4 : 8, CW = grad_type == DH_F32 ? 4 : 8;
     p.Dp = (D + 3) / 4 * 4;
@@ -2024,7 +2054,7 @@ FewPlan few_plan(int dtype, int grad_type, int V, int D, int backward) {
     p.waves = small && D >= 512 ? 16 : 4;
     p.blocks = (V + p.rows - 1) / p.rows;
     if (!backward) {
-        p.total = up256((size_t)p.blocks * FEW * 8);
+        p.total = up256((size_t)p.blocks * (N <= FEW ? FEW : 2 * FEW) * 8);
         return p;
     }
     // About 1024 work-groups of 4 waves for dH and 4096 for dW.
@@ -2045,10 +2075,15 @@ FewPlan few_plan(int dtype, int grad_type, int V, int D, int backward) {
 
 // The workspace that serves any alignment of the operands (staged tables take more).
 size_t least_ws(int dtype, int N, int V, int D, int K, int backward) {
-    if (is_few(N, V))   // whichever type the gradients have
-        return std::max(few_plan(dtype, DH_F32, V, D, backward).total, few_plan(dtype, dtype, V, D, backward).total);
-    const Plan p = make_plan(dtype, N, V, D, K, backward, nullptr, 1);
-    return p.piece + p.per_block + 512;
+    size_t need = 0;
+    if (is_few(N, V, true, backward))   // whichever type the gradients have
+        need = std::max(few_plan(dtype, DH_F32, N, V, D, backward).total,
+                        few_plan(dtype, dtype, N, V, D, backward).total);
+    if (!is_few(N, V, false, backward)) {
+        const Plan p = make_plan(dtype, N, V, D, K, backward, nullptr, 1);
+        need = std::max(need, p.piece + p.per_block + 512);
+    }
+    return need;
 }
 
 // Table rows of a piece: as many blocks of 256 as fit, the same for every piece.
@@ -2341,12 +2376,16 @@ Few few_args(const Head& h) {
 
 template <typename T>
 int few_forward(const Head& h, float* loss, float* lse, void* ws) {
-    const FewPlan p = few_plan(h.dtype, h.dtype, h.V, h.D, 0);
+    const FewPlan p = few_plan(h.dtype, h.dtype, h.N, h.V, h.D, 0);
     Few f = few_args(h);
     f.part = (float2*)ws;
     f.loss = loss;
     f.lse_out = lse;
-    auto lse_parts = p.rows == 64 ? few_lse<T, 4, 4> : p.waves == 4 ? few_lse<T, 4, 1> : few_lse<T, 16, 1>;
+    const bool two = h.N > FEW;
+    f.ldpart = two ? 2 * FEW : FEW;
+    auto lse_parts = p.rows == 64  ? two ? few_lse<T, 4, 4, 2> : few_lse<T, 4, 4, 1>
+                     : p.waves == 4 ? two ? few_lse<T, 4, 1, 2> : few_lse<T, 4, 1, 1>
+                                    : two ? few_lse<T, 16, 1, 2> : few_lse<T, 16, 1, 1>;
     lse_parts<<<p.blocks, 64 * p.waves, 0, stream()>>>(f);
     DH_TRY(check_launch(h.op));
     few_loss<T><<<h.N, 1024, 0, stream()>>>(f, p.blocks);
@@ -2355,7 +2394,7 @@ int few_forward(const Head& h, float* loss, float* lse, void* ws) {
 
 template <typename T, typename OT>
 int few_backward(const Head& h, const Grads& d, void* ws) {
-    const FewPlan p = few_plan(h.dtype, d.type, h.V, h.D, 1);
+    const FewPlan p = few_plan(h.dtype, d.type, h.N, h.V, h.D, 1);
     Few f = few_args(h);
     f.G = (float*)ws;
     f.acc = (float*)((char*)ws + p.acc);
@@ -2394,7 +2433,7 @@ int run_forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_byte
         return set_error(DH_ERR_INVALID, "%s: null pointer", h.op);
     DH_TRY(ensure_init());
     if (h.N == 0) return DH_OK;
-    if (is_few(h.N, h.V))
+    if (is_few(h.N, h.V, !in_place(h.dtype, h.D, h.W, h.ldw), 0))
         return h.dtype == DH_F32 ? few_forward<float>(h, loss, lse, ws) : few_forward<uint16_t>(h, loss, lse, ws);
     return h.dtype == DH_F32 ? forward<float, 2>(h, loss, lse, ws, ws_bytes)
                              : forward<uint16_t, 1>(h, loss, lse, ws, ws_bytes);
@@ -2419,7 +2458,7 @@ int run_backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
             clear_rows<<<2048, 256, 0, stream()>>>((uint16_t*)d.dW, h.V, h.D, d.lddw);
         return check_launch(h.op);
     }
-    if (is_few(h.N, h.V)) {
+    if (is_few(h.N, h.V, true, 1)) {
         if (h.dtype == DH_F32) return few_backward<float, float>(h, d, ws);
         return d.type == DH_F32 ? few_backward<uint16_t, float>(h, d, ws)
                                 : few_backward<uint16_t, uint16_t>(h, d, ws);

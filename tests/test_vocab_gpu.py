@@ -10,6 +10,8 @@ result (for the loss: of its largest, at least 1).  bf16 gradients: one rounding
 each term of a sum, in random directions) and one of the result (ub of it): 2 ub = 2^-7 of the
 result's largest value; the embedding's bf16 results are rounded once: ub.
 """
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -443,3 +445,353 @@ def test_loss_gradient_against_differences(K):
         b[v, d] -= small
         diff = (total(H0, a) - total(H0, b)) / (float(a[v, d]) - float(b[v, d]))
         assert abs(diff - gW[v, d]) <= 4e-3 * max(1.0, np.abs(gW).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("N", [1, 4, 8, 16, 18, 32, 33])
+@pytest.mark.parametrize("D", [40, 77])
+def test_few_rows_of_a_long_table(N, D, dtype):
+    """V above 2^14, where few rows take the table in blocks of 64 of its rows; D = 77 takes 16-bit
+    tables at odd addresses."""
+    run_loss(Loss(N, 17001, D, dtype, pad=0.2 if N > 2 else 0.0))
+    run_loss(Loss(N, 17001, D, dtype, K=9, T=2.0, pad=0.2 if N > 2 else 0.0), accumulate=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [None, 4])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("N", [5, 13, 29])
+def test_few_rows_padding_holds_anything(N, K, dtype):
+    c = Loss(N, 300, 47, dtype, K=K, pad=0.5, seed=1)
+    assert c.keep.any() and not c.keep.all()
+    clean = run_loss(c)
+    H = c.H.copy()
+    H[~c.keep] = np.where(np.arange((~c.keep).sum())[:, None] % 2 == 0, np.nan, np.inf)
+    c.Hb, _ = store(H, dtype)
+    d = c.dloss.copy()
+    d[~c.keep] = np.nan
+    c.dlb = DB.from_numpy(d)
+    for a, b in zip(clean, run_loss(c)):
+        assert (a == b).all()
+    c.ids = ints(np.full(c.N * (K or 1), -1))
+    c.keep[:] = False
+    c.q[:] = 0
+    if K:
+        c.ok[:] = False
+    c.H = np.zeros_like(c.H)
+    run_loss(c)
+
+
+@pytest.mark.gpu
+def test_few_rows_of_a_table_past_the_short_form():
+    """V above 2^21: the form for many rows also takes few of them."""
+    run_loss(Loss(2, (1 << 21) + 3, 8, "bf16"), "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [None, 3])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("N,V,D", [(7, 500, 40), (130, 700, 96), (300, 5000, 200)])
+def test_loss_without_some_results(N, V, D, K, dtype):
+    """lse, dH, dW and dloss may be missing: what is left does not change, nor does a second run."""
+    c = Loss(N, V, D, dtype, K=K, pad=0.2)
+    size = max(c.least(0), c.least(1)) + (4 << 20)
+    ws = DB(size)
+    t = np.uint16 if dtype == "bf16" else np.float32
+
+    def run(with_lse, with_H, with_W, dloss):
+        loss, lse = (DB.from_numpy(np.zeros(N, np.float32)) for _ in range(2))
+        dH, dW = DB.from_numpy(np.zeros((N, D), t)), DB.from_numpy(np.zeros((V, D), t))
+        c.fwd(loss, lse if with_lse else None, ws, size)
+        if not with_lse:
+            return loss.numpy(), None, None
+        c.bwd(lse, dloss, dH if with_H else None, D, False, dW if with_W else None, D, False, DT[dtype],
+              ws, size)
+        return loss.numpy(), dH.numpy(), dW.numpy()
+
+    both = run(True, True, True, c.dlb)
+    assert all((a == b).all() for a, b in zip(both, run(True, True, True, c.dlb)))
+    assert (run(False, True, True, c.dlb)[0] == both[0]).all()
+    assert (run(True, True, False, c.dlb)[1] == both[1]).all()
+    assert (run(True, False, True, c.dlb)[2] == both[2]).all()
+    run(True, False, False, c.dlb)
+    ones = run(True, True, True, DB.from_numpy(np.ones(N, np.float32)))
+    assert all((a == b).all() for a, b in zip(ones, run(True, True, True, None)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,grad", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("weights", ["equal", "zero", "tiny", "wide"])
+def test_loss_weights(weights, dtype, grad):
+    """One loss weight for all rows as a mean has it, none, tiny ones, and weights of both signs over
+    a range of 2^40: the gradients hold what they hold for weights of about 1."""
+    N, V, D = 150, 400, 48
+    c = Loss(N, V, D, dtype, seed=6, pad=0.1)
+    r = np.random.default_rng(7)
+    c.dloss = {"equal": np.full(N, 1 / 1719), "zero": np.zeros(N), "tiny": np.full(N, 2.0 ** -100) * (1 + r.random(N)),
+               "wide": np.ldexp(r.standard_normal(N), r.integers(-40, 1, N))}[weights].astype(np.float32)
+    c.dlb = DB.from_numpy(c.dloss)
+    size = max(c.least(0), c.least(1))
+    ws = DB(size)
+    loss, lse = DB.empty((N,), np.float32), DB.empty((N,), np.float32)
+    bufs = [store(np.full(s, np.nan), grad)[0] for s in ((N, D), (V, D))]
+    c.fwd(loss, lse, ws, size)
+    c.bwd(lse, c.dlb, bufs[0], D, False, bufs[1], D, False, DT[grad], ws, size)
+    ref, tol = c.ref(), F32_TOL if dtype == "f32" else BF16_TOL
+    for k in (0, 1):
+        got = fetch(bufs[k], ((N, D), (V, D))[k], grad)[0]
+        close(got, ref[2 + k], tol, floor=np.abs(c.dloss).max() * np.abs((c.W, c.H)[k]).max())
+        if weights == "zero":
+            assert (got == 0).all()
+
+
+def part(buf, first, rows, D, dtype):
+    """Rows first .. first + rows - 1 of a large device matrix of rows of D values."""
+    t = np.dtype(np.uint16 if dtype == "bf16" else np.float32)
+    out = np.empty((rows, D), t)
+    hip.check(hip.load().dh_memcpy_d2h(out.ctypes.data, buf.ptr + first * D * t.itemsize, out.nbytes), "d2h")
+    return (bits_to_f32(out) if dtype == "bf16" else out).astype(np.float64)
+
+
+@pytest.mark.gpu
+def test_table_past_32_bit_offsets():
+    """V D above 2^31: rows at the table's ends.  The table repeats with a period, so the reference
+    needs one period and how often each of its rows occurs."""
+    V, D, P = 262200, 8200, 97
+    assert V * D > 2 ** 31
+    r = np.random.default_rng(1)
+    pat = bf16_bits((r.standard_normal((P, D)) * 0.1).astype(np.float32))
+    Wp = bits_to_f32(pat).astype(np.float64)
+    W = np.empty((V, D), np.uint16)
+    for s in range(0, V, P):
+        W[s:s + P] = pat[:V - s]
+    Wb = DB.from_numpy(W)
+    del W
+    times = np.bincount(np.arange(V) % P, minlength=P)
+    dWb = DB(V * D * 2)
+    edge = 300
+    spots = np.concatenate([np.arange(edge), np.arange(V - edge, V)])
+    for N in (3, 20):
+        Hb, H = store(r.standard_normal((N, D)) * (20.0 / np.sqrt(D)), "bf16")
+        target = spots[r.integers(0, 2 * edge, N)]
+        target[:3] = V - 1, 0, V - 2
+        size = max(hip.linear_xent_workspace(hip.BF16, N, V, D, b) for b in (0, 1)) + (64 << 20)
+        ws, tb = DB(size), ints(target)
+        loss, lse = DB.empty((N,), np.float32), DB.empty((N,), np.float32)
+        dHb = store(np.zeros((N, D)), "bf16")[0]
+        hip.linear_xent_fwd(hip.BF16, N, V, D, 1.0, Hb, D, Wb, D, tb, loss, lse, ws, size)
+        hip.linear_xent_bwd(hip.BF16, N, V, D, 1.0, Hb, D, Wb, D, tb, lse, None, dHb, D, False, dWb, D, False,
+                            hip.BF16, ws, size)
+        z = H @ Wp.T
+        m = z.max(1, keepdims=True)
+        rl = (m + np.log((times * np.exp(z - m)).sum(1, keepdims=True)))
+        p = np.exp(z - rl)
+        close(lse.numpy().astype(np.float64), rl[:, 0], F32_TOL)
+        close(loss.numpy().astype(np.float64), rl[:, 0] - z[np.arange(N), target % P], F32_TOL)
+        G = np.zeros((N, 2 * edge))
+        G[:] = p[:, spots % P]
+        for n in range(N):
+            G[n, np.searchsorted(spots, target[n])] -= 1.0
+        close(fetch(dHb, (N, D), "bf16")[0], (p * times) @ Wp - Wp[target % P], BF16_TOL, floor=np.abs(Wp).max())
+        got = np.concatenate([part(dWb, 0, edge, D, "bf16"), part(dWb, V - edge, edge, D, "bf16")])
+        close(got, G.T @ H, BF16_TOL, floor=np.abs(H).max())
+        # the embedding of the same tokens, and its gradient over what is there
+        Yb = store(np.zeros((N, D)), "bf16")[0]
+        hip.embedding_fwd(hip.BF16, N, V, D, 2.0, tb, Wb, D, Yb, D)
+        close(fetch(Yb, (N, D), "bf16")[0], 2.0 * Wp[target % P], BF16_ONCE)
+        hip.embedding_bwd(hip.BF16, N, V, D, 1.0, tb, Hb, D, dWb, D, hip.BF16, False, ws, size)
+        want = np.zeros((2 * edge, D))
+        np.add.at(want, np.searchsorted(spots, target), H)
+        got = np.concatenate([part(dWb, 0, edge, D, "bf16"), part(dWb, V - edge, edge, D, "bf16")])
+        close(got, want, BF16_ONCE)
+
+
+# ------------------------------------------------------------------------------ together
+
+class Tied:
+    """A small language model's two ends, fp32: x = s W[id], y = its layer norm, h = y P, cross entropy
+    and distillation of h W^T, and the gradients of W (from all three) and of P."""
+    N, V, D, K, S, T = 96, 500, 64, 4, 8.0, 2.0
+
+    def __init__(self):
+        r = np.random.default_rng(11)
+        N, V, D, K = self.N, self.V, self.D, self.K
+        self.W0 = (r.standard_normal((V, D)) * 0.2).astype(np.float32)
+        self.P0 = (r.standard_normal((D, D)) * 0.2).astype(np.float32)
+        self.id0 = r.integers(0, V, N)
+        self.t0 = r.integers(0, V, N)
+        self.id0[-5:] = self.t0[-5:] = -1           # the batch's padding
+        self.top0 = np.argsort(r.random((N, V)), 1)[:, :K]
+        self.top0[-5:] = -1
+        self.logit0 = (r.standard_normal((N, K)) * 2).astype(np.float32)
+        self.w1, self.w2 = np.full(N, 0.7 / N, np.float32), np.full(N, 0.3 / N, np.float32)
+        up = DB.from_numpy
+        self.W, self.P, self.id, self.t = up(self.W0), up(self.P0), ints(self.id0), ints(self.t0)
+        self.top, self.logit, self.a, self.b = ints(self.top0), up(self.logit0), up(self.w1), up(self.w2)
+        f = lambda *s: DB.empty(s, np.float32)  # noqa: E731
+        self.x, self.y, self.h, self.dh, self.dy, self.dx = (f(N, D) for _ in range(6))
+        self.dW, self.dP = f(V, D), f(D, D)
+        self.l1, self.l2, self.lse1, self.lse2 = (f(N) for _ in range(4))
+        self.size = max(hip.embedding_bwd_workspace(N, V, D),
+                        *(hip.linear_xent_workspace(0, N, V, D, b) for b in (0, 1)),
+                        *(hip.linear_distill_workspace(0, N, V, D, K, b) for b in (0, 1)))
+        self.ws = DB(self.size)
+
+    def head(self, backward):
+        N, V, D, F = self.N, self.V, self.D, hip.F32
+        w = (self.ws, self.size)
+        x = (F, N, V, D, 1.0, self.h, D, self.W, D, self.t)
+        d = (F, N, V, D, self.K, self.T, self.h, D, self.W, D, self.top, self.logit)
+        hip.linear_xent_fwd(*x, self.l1, self.lse1, *w)
+        hip.linear_distill_fwd(*d, self.l2, self.lse2, *w)
+        if backward:
+            hip.linear_xent_bwd(*x, self.lse1, self.a, self.dh, D, False, self.dW, D, False, F, *w)
+            hip.linear_distill_bwd(*d, self.lse2, self.b, self.dh, D, True, self.dW, D, True, F, *w)
+
+    def step(self):
+        N, V, D, F = self.N, self.V, self.D, hip.F32
+        hip.embedding_fwd(F, N, V, D, self.S, self.id, self.W, D, self.x, D)
+        hip.layer_norm(self.x, self.y, N, D)
+        hip.gemm_f32(False, False, N, D, D, self.y, D, self.P, D, 0.0, self.h, D)
+        self.head(True)
+        hip.gemm_f32(True, False, D, D, N, self.y, D, self.dh, D, 0.0, self.dP, D)
+        hip.gemm_f32(False, True, N, D, D, self.dh, D, self.P, D, 0.0, self.dy, D)
+        hip.layer_norm_bwd(self.x, self.y, self.dy, self.dx, N, D)
+        hip.embedding_bwd(F, N, V, D, self.S, self.id, self.dx, D, self.dW, D, F, True, self.ws, self.size)
+
+    def ref(self):
+        N, V, D = self.N, self.V, self.D
+        W, P = self.W0.astype(np.float64), self.P0.astype(np.float64)
+        x, _ = emb_ref(self.id0, W, np.zeros((N, D)), self.S)
+        inv = 1 / np.sqrt(x.var(1, keepdims=True) + 1e-5)
+        y = (x - x.mean(1, keepdims=True)) * inv
+        h, keep = y @ P, self.t0 >= 0
+        q1, q2 = np.zeros((N, V)), np.zeros((N, V))
+        q1[np.nonzero(keep)[0], self.t0[keep]] = 1
+        e = np.exp(self.logit0.astype(np.float64) / self.T)
+        np.put_along_axis(q2, np.maximum(self.top0, 0), e / e.sum(1, keepdims=True), 1)
+        r1 = loss_ref(h, W, q1, 1.0, 1.0, 1.0, self.w1, keep)
+        r2 = loss_ref(h, W, q2, 1 / self.T, self.T ** 2, self.T, self.w2, keep)
+        dh = r1[2] + r2[2]
+        dy = dh @ P.T
+        dx = inv * (dy - dy.mean(1, keepdims=True) - y * (dy * y).mean(1, keepdims=True))
+        return r1[0], r2[0], r1[3] + r2[3] + emb_ref(self.id0, W, dx, self.S)[1], y.T @ dh
+
+
+@pytest.mark.gpu
+def test_tied_table_step():
+    """Four kinds of step between the losses and the result, each good to F32_TOL of its largest
+    value, which is up to four times a typical one: 16 F32_TOL of the results' largest."""
+    m = Tied()
+    m.step()
+    got = [b.numpy().astype(np.float64) for b in (m.l1, m.l2, m.dW, m.dP)]
+    for g, want in zip(got, m.ref()):
+        close(g, want, 16 * F32_TOL)
+    # steps against the gradient lower the loss: the directional derivative over a small step of W
+    # as the embedding and both heads see it, second order below 1e-2 of it
+    total = lambda: float(m.w1 @ m.l1.numpy().astype(np.float64) + m.w2 @ m.l2.numpy().astype(np.float64))  # noqa: E731
+    before, g = total(), got[2]
+    step = 1e-2 / np.linalg.norm(g)
+    moved = []
+    for s in (1, -1):
+        m.W = DB.from_numpy((m.W0 + s * step * g).astype(np.float32))
+        m.step()
+        moved.append(total())
+    slope = (moved[0] - moved[1]) / (2 * step)
+    assert moved[1] < before < moved[0]
+    assert abs(slope - (g * g).sum()) <= 1e-2 * (g * g).sum()
+
+
+def _runtime():
+    rt = ctypes.CDLL("libamdhip64.so")
+    v, p = ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)
+    for name, args in (("hipStreamCreate", [p]), ("hipStreamDestroy", [v]), ("hipStreamSynchronize", [v]),
+                       ("hipStreamBeginCapture", [v, ctypes.c_int]), ("hipStreamEndCapture", [v, p]),
+                       ("hipGraphInstantiate", [p, v, v, v, ctypes.c_size_t]), ("hipGraphLaunch", [v, v]),
+                       ("hipGraphExecDestroy", [v]), ("hipGraphDestroy", [v])):
+        f = getattr(rt, name)
+        f.restype, f.argtypes = ctypes.c_int, args
+    return rt
+
+
+class Recorded:
+    """A loss's forward and backward and an embedding's, with a workspace of their own."""
+
+    def __init__(self, N, V, D, dtype, K, seed):
+        self.c = c = Loss(N, V, D, dtype, K=K, pad=0.2, seed=seed)
+        t = np.uint16 if dtype == "bf16" else np.float32
+        self.size = max(c.least(0), c.least(1), hip.embedding_bwd_workspace(N, V, D)) + (1 << 20)
+        self.ws = DB(self.size)
+        self.id = ints(np.random.default_rng(seed).integers(-1, V, N))
+        self.out = [DB.empty((N,), np.float32), DB.empty((N,), np.float32), DB.empty((N, D), t), DB.empty((V, D), t),
+                    DB.empty((N, D), t), DB.empty((V, D), t)]
+
+    def run(self):
+        c, (loss, lse, dH, dW, Y, dE) = self.c, self.out
+        dt = DT[c.dtype]
+        c.fwd(loss, lse, self.ws, self.size)
+        c.bwd(lse, c.dlb, dH, c.D, False, dW, c.D, False, dt, self.ws, self.size)
+        hip.embedding_fwd(dt, c.N, c.V, c.D, 1.0, self.id, c.Wb, c.ld, Y, c.D)
+        hip.embedding_bwd(dt, c.N, c.V, c.D, 1.0, self.id, dH, c.D, dE, c.D, dt, False, self.ws, self.size)
+
+    def wipe(self):
+        for b in self.out:
+            g = np.full(b.shape, 7, b.dtype)
+            hip.check(hip.load().dh_memcpy_h2d(b.ptr, g.ctypes.data, g.nbytes), "h2d")
+        hip.sync()
+
+    def values(self):
+        return [b.numpy() for b in self.out]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("a,b", [((200, 3000, 72, "bf16", None), (12, 900, 50, "f32", 5)),
+                                 ((9, 20000, 64, "bf16", 4), (2100, 300, 40, "f32", None)),
+                                 ((9000, 40, 24, "bf16", None), (300, 700, 130, "f32", 40))])
+def test_graphs_on_other_streams(a, b):
+    """Recorded with nothing allocated, on streams of the caller's; two graphs replayed at once, three
+    times, their results wiped between: what the library's own stream gives, bit for bit."""
+    jobs = [Recorded(*a, seed=1), Recorded(*b, seed=2)]
+    want = []
+    for j in jobs:
+        j.run()
+        want.append(j.values())
+    R, lib = _runtime(), hip.load()
+    streams, graphs, exes = ([ctypes.c_void_p() for _ in jobs] for _ in range(3))
+    ref = ctypes.byref
+    try:
+        for j, s, g, x in zip(jobs, streams, graphs, exes):
+            assert R.hipStreamCreate(ref(s)) == 0
+            hip.check(lib.dh_set_stream(s), "dh_set_stream")
+            j.wipe()
+            j.run()                                              # eager on that stream
+            assert all(np.array_equal(v, w) for v, w in zip(j.values(), want[jobs.index(j)]))
+            assert R.hipStreamBeginCapture(s, 0) == 0
+            try:
+                j.run()
+            finally:
+                end = R.hipStreamEndCapture(s, ref(g))
+            assert end == 0 and R.hipGraphInstantiate(ref(x), g, None, None, 0) == 0
+        lib.dh_set_stream(None)
+        for _ in range(3):
+            for j in jobs:
+                j.wipe()
+            for x, s in zip(exes, streams):
+                assert R.hipGraphLaunch(x, s) == 0
+            for s in streams:
+                assert R.hipStreamSynchronize(s) == 0
+            for j, w in zip(jobs, want):
+                assert all(np.array_equal(v, u) for v, u in zip(j.values(), w))
+            jobs[0].run()                                        # the program's own work between
+            hip.sync()
+    finally:
+        lib.dh_set_stream(None)
+        for s, g, x in zip(streams, graphs, exes):
+            if x.value:
+                R.hipGraphExecDestroy(x)
+            if g.value:
+                R.hipGraphDestroy(g)
+            if s.value:
+                R.hipStreamSynchronize(s)
+                R.hipStreamDestroy(s)
