@@ -1471,7 +1471,7 @@ __global__ void __launch_bounds__(256) finish(Finish<OT> h, Finish<OT> w, int D)
 }
 
 // ---- few rows --------------------------------------------------------------------------------------
-// Up to FEW rows: bound by reading the table, so it is read as it is, at any alignment, once for
+// Few rows: bound by reading the table, so it is read as it is, at any alignment, once for
 // the forward and twice for the gradient, straight into the fp32 matrix cores (v_mfma_f32_16x16x4:
 // at 16 rows they take 17 TB/s of fp32 values or 9 of bf16), with no packing: a row that does not
 // count reads as zeros, and its G is zero.  G is fp32, [table row][FEW].
@@ -1984,18 +1984,14 @@ struct Plan {
     size_t per_block;         // bytes of a piece per 256 table rows
 };
 
-// Whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
-bool in_place(int dtype, int D, const void* W, int ldw) {
-    return dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
-}
-
 Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* W, int ldw) {
     Plan p{};
     p.parts = dtype == DH_F32 ? 2 : 1;
     p.Kp = (D + 31) / 32 * 32;
     p.Dp = apart(p.Kp);
     p.Nt = (int)(((long long)N + 255) / 256 * 256);
-    p.direct = in_place(dtype, D, W, ldw);
+    // In place: whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
+    p.direct = dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
     p.lse = pick(V, N, D, p.parts, false).kind;
     p.g = pick(N, V, D, p.parts, false).kind;
     const Choice dh = pick(N, D, V, p.parts, true), dw = pick(V, D, N, p.parts, true);
@@ -2032,10 +2028,18 @@ Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* 
     return p;
 }
 
-// The forward also takes twice as many rows, where the table cannot be read in place: staging costs
-// more than the fp32 matrix cores at half their useful rate (18 x 41216 x 2357 fp32: OLDT / NEWT us).
-bool is_few(int N, int V, bool staged, int backward) {
-    return N <= (staged && !backward ? 2 * FEW : FEW) && V <= FEW_MAX_V;
+// Which calls take this form, measured against the form for many rows (us, that one's behind the stroke):
+//   forward, up to FEW rows      fp32 16 x 32000 x 1024: under half; bf16 16 x 131072 x 2048 116 / 116,
+//                                16 x 50001 x 1001 48 / 60, 1 x 131072 x 2048 107 / 115
+//   forward, up to 2 FEW, fp32   as there the table would be staged: 18 x 41216 x 2357 155 / 248; bf16 tables
+//                                are read in place or cheap to stage: 32 x 50001 x 1001 63 / 60
+//   gradient, fp32               with its forward 16 x 32000 x 1024 111 / 240
+//   gradient, bf16               up to 4 rows (4 x 50001 x 1000 109 / 113, x 1001 153 / 175; 4 x 131072 x 2048
+//                                557 / 503) or up to 2^22 table values (16 x 8000 x 512 37 / 37, 16 x 1000 x
+//                                1024 24 / 34); beyond, fp32 multiply-adds bound it: 16 x 50001 x 1000 180 / 117
+bool is_few(int dtype, int N, int V, int D, int backward) {
+    if (V > FEW_MAX_V || N > (dtype == DH_F32 && !backward ? 2 * FEW : FEW)) return false;
+    return dtype == DH_F32 || !backward || N <= 4 || (long long)V * D <= 1 << 22;
 }
 
 struct FewPlan {
@@ -2047,10 +2051,10 @@ FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int backward) {
     FewPlan p{};
     const int C = dtype == DH_F32 ? 4 : 8, CW = grad_type == DH_F32 ? 4 : 8;
     p.Dp = (D + 3) / 4 * 4;
-    // 64 rows and 4 waves; few work-groups of those: 16 rows, and a long k shared by 16 waves, which
+    // 64 rows (32 for two groups of tokens) and 4 waves; few work-groups of those: 16 rows, and a long k shared by 16 waves, which
     // shortens its chain of loads (2000 x 4000 fp32: 41 / 18 us).
     const bool small = V <= 64 * 256;
-    p.rows = small ? 16 : 64;
+    p.rows = small ? 16 : N <= FEW ? 64 : 32;
     p.waves = small && D >= 512 ? 16 : 4;
     p.blocks = (V + p.rows - 1) / p.rows;
     if (!backward) {
@@ -2075,15 +2079,11 @@ FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int backward) {
 
 // The workspace that serves any alignment of the operands (staged tables take more).
 size_t least_ws(int dtype, int N, int V, int D, int K, int backward) {
-    size_t need = 0;
-    if (is_few(N, V, true, backward))   // whichever type the gradients have
-        need = std::max(few_plan(dtype, DH_F32, N, V, D, backward).total,
+    if (is_few(dtype, N, V, D, backward))   // whichever type the gradients have
+        return std::max(few_plan(dtype, DH_F32, N, V, D, backward).total,
                         few_plan(dtype, dtype, N, V, D, backward).total);
-    if (!is_few(N, V, false, backward)) {
-        const Plan p = make_plan(dtype, N, V, D, K, backward, nullptr, 1);
-        need = std::max(need, p.piece + p.per_block + 512);
-    }
-    return need;
+    const Plan p = make_plan(dtype, N, V, D, K, backward, nullptr, 1);
+    return p.piece + p.per_block + 512;
 }
 
 // Table rows of a piece: as many blocks of 256 as fit, the same for every piece.
@@ -2381,11 +2381,13 @@ int few_forward(const Head& h, float* loss, float* lse, void* ws) {
     f.part = (float2*)ws;
     f.loss = loss;
     f.lse_out = lse;
-    const bool two = h.N > FEW;
-    f.ldpart = two ? 2 * FEW : FEW;
-    auto lse_parts = p.rows == 64  ? two ? few_lse<T, 4, 4, 2> : few_lse<T, 4, 4, 1>
-                     : p.waves == 4 ? two ? few_lse<T, 4, 1, 2> : few_lse<T, 4, 1, 1>
-                                    : two ? few_lse<T, 16, 1, 2> : few_lse<T, 16, 1, 1>;
+    auto lse_parts = p.rows == 64 ? few_lse<T, 4, 4, 1> : p.waves == 4 ? few_lse<T, 4, 1, 1> : few_lse<T, 16, 1, 1>;
+    f.ldpart = FEW;
+    if constexpr (sizeof(T) == 4)
+        if (h.N > FEW) {
+            lse_parts = p.rows == 32 ? few_lse<T, 4, 2, 2> : p.waves == 4 ? few_lse<T, 4, 1, 2> : few_lse<T, 16, 1, 2>;
+            f.ldpart = 2 * FEW;
+        }
     lse_parts<<<p.blocks, 64 * p.waves, 0, stream()>>>(f);
     DH_TRY(check_launch(h.op));
     few_loss<T><<<h.N, 1024, 0, stream()>>>(f, p.blocks);
@@ -2433,7 +2435,7 @@ int run_forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_byte
         return set_error(DH_ERR_INVALID, "%s: null pointer", h.op);
     DH_TRY(ensure_init());
     if (h.N == 0) return DH_OK;
-    if (is_few(h.N, h.V, !in_place(h.dtype, h.D, h.W, h.ldw), 0))
+    if (is_few(h.dtype, h.N, h.V, h.D, 0))
         return h.dtype == DH_F32 ? few_forward<float>(h, loss, lse, ws) : few_forward<uint16_t>(h, loss, lse, ws);
     return h.dtype == DH_F32 ? forward<float, 2>(h, loss, lse, ws, ws_bytes)
                              : forward<uint16_t, 1>(h, loss, lse, ws, ws_bytes);
@@ -2458,7 +2460,7 @@ int run_backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
             clear_rows<<<2048, 256, 0, stream()>>>((uint16_t*)d.dW, h.V, h.D, d.lddw);
         return check_launch(h.op);
     }
-    if (is_few(h.N, h.V, true, 1)) {
+    if (is_few(h.dtype, h.N, h.V, h.D, 1)) {
         if (h.dtype == DH_F32) return few_backward<float, float>(h, d, ws);
         return d.type == DH_F32 ? few_backward<uint16_t, float>(h, d, ws)
                                 : few_backward<uint16_t, uint16_t>(h, d, ws);

@@ -289,7 +289,7 @@ def run_loss(c, grad=None, extra=0, accumulate=False):
 
 SHAPES = [(1, 1, 1), (1, 65, 32), (2, 3, 5), (31, 257, 64), (64, 1000, 100), (256, 256, 32),
           (257, 300, 40), (300, 1025, 96), (513, 130, 264), (3, 5000, 72), (16, 3000, 129),
-          (5, 64, 1030), (9, 700, 300), (17, 3000, 129)]
+          (5, 64, 1030), (9, 700, 300), (17, 3000, 129), (5, 70000, 61), (16, 65600, 64)]
 
 
 @pytest.mark.gpu
@@ -544,6 +544,35 @@ def test_loss_weights(weights, dtype, grad):
         close(got, ref[2 + k], tol, floor=np.abs(c.dloss).max() * np.abs((c.W, c.H)[k]).max())
         if weights == "zero":
             assert (got == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [None, 3])
+@pytest.mark.parametrize("dtype,grad", [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16")])
+def test_loss_of_no_rows(K, dtype, grad):
+    """Nothing is read; dW is zero, or stays as it was where it is added to."""
+    V, D, ld = 70, 33, 35
+    t = np.uint16 if grad == "bf16" else np.float32
+    for acc in (False, True):
+        dW = DB.from_numpy(np.full((V, ld), 7, t))
+        head = (DT[dtype], 0, V, D) + ((1.0,) if K is None else (K, 2.0)) + (None, D, None, D)
+        ids = (None,) if K is None else (None, None)
+        if K is None:
+            hip.linear_xent_fwd(*head, *ids, None, None, None, 0)
+            hip.linear_xent_bwd(*head, *ids, None, None, None, D, False, dW, ld, acc, DT[grad], None, 0)
+        else:
+            hip.linear_distill_fwd(*head, *ids, None, None, None, 0)
+            hip.linear_distill_bwd(*head, *ids, None, None, None, D, False, dW, ld, acc, DT[grad], None, 0)
+        got = dW.numpy()
+        assert (got[:, :D] == (7 if acc else 0)).all() and (got[:, D:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("N,V,D,ldx", [(1, 300, 40, 0), (7, 17001, 24, 3), (16, 129, 700, 0)])
+def test_few_rows_with_gradients_in_floats(N, V, D, ldx, accumulate):
+    run_loss(Loss(N, V, D, "bf16", ldx=ldx), "f32", accumulate=accumulate)
+    run_loss(Loss(N, V, D, "bf16", K=5, T=2.0, ldx=ldx), "f32", accumulate=accumulate)
 
 
 def part(buf, first, rows, D, dtype):
