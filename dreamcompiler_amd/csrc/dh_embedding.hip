@@ -21,8 +21,12 @@
 namespace dh {
 namespace {
 
-constexpr int EMB_DIRECT = 2048;   // tokens that are not sorted
-constexpr int EMB_TILE = 8192;     // tokens one work-group sorts
+// Tokens that are not sorted: forward and gradient of 300 / 1000 / 2048 x 50001 x 1024 bf16 take 19 / 22 / 29 us
+// so and 33 / 34 / 36 sorted, of 2048 x 500 x 1024 fp32 15 and 23.
+constexpr int EMB_DIRECT = 2048;
+// Tokens one work-group sorts: 8192 ids below 50001 in 26 us, the cleared rows beside; the launches per
+// pass that more tokens take cost 20 us for each of the two passes.
+constexpr int EMB_TILE = 8192;
 constexpr int EMB_CHUNK = 16;      // sorted tokens added by one wave
 constexpr int EMB_BITS = 9, EMB_BINS = 1 << EMB_BITS;
 
@@ -91,7 +95,8 @@ inline bool whole_lines(const void* p, int ld, size_t size) {
 }
 
 // ---- lookup ------------------------------------------------------------------------------------
-// A wave per row and slab of 512 columns.
+// A wave per row and slab of 512 columns.  65536 x 2048 fp32: 174 us, 3.1 TB/s written and as much read
+// (partly from cache, as tokens repeat).
 template <typename T, int R>
 __global__ void __launch_bounds__(256) embedding_fwd_kernel(const int* __restrict__ ids, int N, int V,
                                                             int D, float scale,
@@ -479,6 +484,7 @@ __device__ inline void load_part(const float* p, float (&v)[8]) {
 // of 512 columns, rows fetched four at a time.  part[chunk][0] is the sum of the run that came in
 // from the chunk before, part[chunk][1] that of the run that goes on behind it; a run that does
 // both is in part[chunk][0].  The other work-groups (with `present`) clear `rows` table rows each.
+// 65536 x 131072 x 2048 fp32: 398 us for 0.54 GB read and 1.07 GB written, 4.1 TB/s (a copy: 4.8).
 template <typename T, typename OT, int R>
 __global__ void __launch_bounds__(256) embedding_sum(const int* __restrict__ key,
                                                      const int* __restrict__ pos, int N,

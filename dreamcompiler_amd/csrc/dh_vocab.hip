@@ -1080,6 +1080,13 @@ __device__ inline void gemm_form(uint16_t* ring, const Prod& g, const Epi& epi, 
     else gemm_tile<S, AK, BK, TOK, PARTS>(ring, g, epi, tile, tiles, split);
 }
 
+// The four products.  Bound by the matrix cores under the card's power limit (1.54 to 1.65 GHz).  Measured for
+// 8192 rows x 131072 x 2048 bf16, 4.4 TFLOP each, in ms, PFLOP/s and share of the time that the matrix
+// cores are busy: statistics 3.58 / 1.23 / 76%, G 4.02 / 1.09 / 64% (exponentials, and 16-bit G
+// through LDS), dH 3.26 / 1.35 / 84%, dW 3.84 / 1.14 / 67% (both operands by transposing reads, 32-k
+// stages); a bf16 product of 8192^3 by the vendor's library reaches 1.23 here.  2048 x 32000 x 1024 fp32,
+// 0.134 TFLOP each, in us and TFLOP/s of fp32: 373 / 360, 408 / 329, 346 / 388, 419 / 321; the fp32 matrix
+// cores themselves end at 157.
 template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
 __global__ void __launch_bounds__(S::THREADS) vocab_gemm(Prod g, Epi epi) {
     __shared__ __attribute__((aligned(16))) uint16_t ring[ring_of<S, AK, PARTS>()];
@@ -1366,7 +1373,7 @@ struct JoinOut {
 };
 
 // A work-group per 64 packed rows, 16 waves that share the piece's blocks of table rows; their
-// results meet in LDS in wave order.
+// results meet in LDS in wave order.  8192 rows x 1024 blocks: 41 us.
 __global__ void __launch_bounds__(1024) lse_join(const float2* __restrict__ part, int ldp, int blocks,
                                                  JoinOut out) {
     __shared__ float2 red[16][64];
@@ -1389,7 +1396,9 @@ __global__ void __launch_bounds__(1024) lse_join(const float2* __restrict__ part
     out.put(i, m, s);
 }
 
-// Few rows: a work-group per packed row, its 256 threads share the blocks.  The lanes' results
+// Up to 512 rows, which are few work-groups of the other kind (forward of 100 x 32000 x 256 bf16 14.9 against
+// 24.5 us, of 512 23.4 against 27.2).
+// A work-group per packed row, its 256 threads share the blocks.  The lanes' results
 // meet at distances 1 to 32, the waves' in wave order.
 __global__ void __launch_bounds__(256) lse_join_few(const float2* __restrict__ part, int ldp, int blocks,
                                                     JoinOut out) {
@@ -1606,6 +1615,8 @@ __device__ inline uint32_t few_keep(const Few& f) {
     return (uint32_t)__ballot(lane < f.N && f.targets.has(lane));
 }
 
+// Reads the table once: 1 x 131072 x 2048 bf16 101 us, 5.3 TB/s; 16 x 41216 x 2357 fp32 (rows at odd
+// 4-byte places) 117 us, 3.3 TB/s.
 template <typename T, int KW, int RT, int TG>
 __global__ void __launch_bounds__(64 * KW) few_lse(Few f) {
     __shared__ float red[KW][16 * RT][16 * TG];
