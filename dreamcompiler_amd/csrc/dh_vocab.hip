@@ -214,7 +214,8 @@ struct Targets {
 };
 
 // flag[n] = 0 where row n has an entry, -1 where it has none: for so many entries that pack_rows
-// had better not look for them again and again.  A wave per row.
+// had better not look for them again and again (2048 rows x 32: packing 16.0 us alone, 8.3 with the
+// flags, which take 5.1).  A wave per row.
 __global__ void __launch_bounds__(256) teacher_flags(Teacher t, int N, int V, int* __restrict__ flag) {
     const int lane = threadIdx.x & 63;
     const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -447,47 +448,78 @@ __global__ void __launch_bounds__(256) stage_scaled(const float* __restrict__ W,
 }
 
 // ---- teachers ------------------------------------------------------------------------------------
-// A work-group per packed row, a wave per 2 of its K entries: the teacher's probabilities q (N x K,
-// zero where there is no entry), the student's logits z at its tokens, and base[i] =
-// sum q (log q - z).  Latency-bound: the entries' rows of W lie anywhere.
-template <typename T>
-__global__ void __launch_bounds__(1024) teacher_dots(Rows rows, Teacher t, int V,
-                                                     const T* __restrict__ H, int ldh,
-                                                     const T* __restrict__ W, int ldw, int D,
-                                                     float* __restrict__ q, float* __restrict__ z,
-                                                     float* __restrict__ base) {
-    __shared__ float red[16];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int i = blockIdx.x;
-    if (i >= *rows.cnt) return;
-    const int n = rows.row[i];
-    const size_t at = (size_t)n * t.K, to = (size_t)i * t.K;
-    // Largest logit and sum of exponentials: every wave for itself, over all entries.
-    float mx = -INFINITY;
+// A row's teacher: largest logit and logarithm of the sum of exponentials, by every wave.
+__device__ inline void teacher_stats(const Teacher& t, size_t at, int V, float& mx, float& log_sum) {
+    const int lane = threadIdx.x & 63;
+    mx = -INFINITY;
     for (int k = lane; k < t.K; k += 64)
         if (entry_counts(t, at + k, V)) mx = fmaxf(mx, t.logit[at + k]);
     mx = wave_reduce(mx, OpMax());
     float sum = 0.f;
     for (int k = lane; k < t.K; k += 64)
         if (entry_counts(t, at + k, V)) sum += __expf((t.logit[at + k] - mx) * t.inv_t);
-    sum = wave_reduce(sum, OpSum());
-    const float log_sum = __logf(sum);
+    log_sum = __logf(wave_reduce(sum, OpSum()));
+}
+
+// A work-group per packed row: the teacher's probabilities q (N x K, zero where there is no entry), the
+// student's logits z at its tokens, and base[i] = sum q (log q - z).  The entries' rows of W lie
+// anywhere, so a wave has four of them in flight: 2048 x 32 entries x 1024 bf16 31 us, 4.3 TB/s (two a wave, one
+// after the other: 39), 4096 x 100 x 2048 330 us, 5.1 TB/s (360).
+constexpr int TEACHER_FLY = 4;
+template <typename T>
+__global__ void __launch_bounds__(512) teacher_dots(Rows rows, Teacher t, int V,
+                                                    const T* __restrict__ H, int ldh,
+                                                    const T* __restrict__ W, int ldw, int D,
+                                                    float* __restrict__ q, float* __restrict__ z,
+                                                    float* __restrict__ base) {
+    __shared__ float red[8];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int i = blockIdx.x;
+    if (i >= *rows.cnt) return;
+    const int n = rows.row[i];
+    const size_t at = (size_t)n * t.K, to = (size_t)i * t.K;
+    const T* h = H + (size_t)n * ldh;
+    for (int k0 = w; k0 < t.K; k0 += TEACHER_FLY * waves) {
+        const T* row[TEACHER_FLY];
+        float s[TEACHER_FLY] = {};
+#pragma unroll
+        for (int f = 0; f < TEACHER_FLY; ++f) {   // no entry: the table's first row, unused
+            const int k = k0 + f * waves, id = k < t.K ? t.id[at + k] : -1;
+            row[f] = W + (counts(id, V) ? (size_t)id * ldw : 0);
+        }
+        for (int c = 8 * lane; c < D; c += 512) {
+            float x[8], y[TEACHER_FLY][8];
+            load8(h, c, D, x);
+#pragma unroll
+            for (int f = 0; f < TEACHER_FLY; ++f) load8(row[f], c, D, y[f]);
+#pragma unroll
+            for (int f = 0; f < TEACHER_FLY; ++f)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[f] = __builtin_fmaf(x[e], y[f][e], s[f]);
+        }
+#pragma unroll
+        for (int f = 0; f < TEACHER_FLY; ++f) {
+            s[f] = wave_reduce(s[f], OpSum());
+            const int k = k0 + f * waves;
+            if (lane == 0 && k < t.K) z[to + k] = t.inv_t * s[f];
+        }
+    }
+    // Largest logit and sum of exponentials: every wave for itself, over all entries.
+    float mx, log_sum;
+    teacher_stats(t, at, V, mx, log_sum);
+    __syncthreads();   // z is there
     float part = 0.f;
-    for (int k = w; k < t.K; k += waves) {
-        float zk = 0.f, qk = 0.f;
+    for (int k = threadIdx.x; k < t.K; k += blockDim.x) {
+        float qk = 0.f;
         if (entry_counts(t, at + k, V)) {
-            const float d = row_dot(H + (size_t)n * ldh, W + (size_t)t.id[at + k] * ldw, D, lane);
-            zk = t.inv_t * d;
             const float lq = (t.logit[at + k] - mx) * t.inv_t - log_sum;
             qk = __expf(lq);
             // exp underflows below about -104: the entry's share of the loss is zero there
-            if (!(qk == 0.f)) part += qk * (lq - zk);
+            if (!(qk == 0.f)) part += qk * (lq - z[to + k]);
         }
-        if (lane == 0) {
-            q[to + k] = qk;
-            z[to + k] = zk;
-        }
+        q[to + k] = qk;
     }
+    part = wave_reduce(part, OpSum());
     if (lane == 0) red[w] = part;
     __syncthreads();
     if (threadIdx.x != 0) return;
@@ -1660,19 +1692,6 @@ __global__ void __launch_bounds__(64 * KW) few_lse(Few f) {
             }
 }
 
-// A row's teacher: largest logit and logarithm of the sum of exponentials, by every wave.
-__device__ inline void teacher_stats(const Teacher& t, size_t at, int V, float& mx, float& log_sum) {
-    const int lane = threadIdx.x & 63;
-    mx = -INFINITY;
-    for (int k = lane; k < t.K; k += 64)
-        if (entry_counts(t, at + k, V)) mx = fmaxf(mx, t.logit[at + k]);
-    mx = wave_reduce(mx, OpMax());
-    float sum = 0.f;
-    for (int k = lane; k < t.K; k += 64)
-        if (entry_counts(t, at + k, V)) sum += __expf((t.logit[at + k] - mx) * t.inv_t);
-    log_sum = __logf(wave_reduce(sum, OpSum()));
-}
-
 // A work-group per row: joins the parts, takes the logits at the row's targets and writes loss and
 // lse.
 template <typename T>
@@ -2160,7 +2179,7 @@ Work lay_out(const Plan& p, void* ws) {
 template <typename T, int PARTS>
 int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
     a.targets = {h.target, h.teacher, h.V};
-    if (!h.target && (long long)h.N * h.teacher.K > 1 << 16) {
+    if (!h.target && (long long)h.N * h.teacher.K > 1 << 15) {
         teacher_flags<<<(h.N + 3) / 4, 256, 0, stream()>>>(h.teacher, h.N, h.V, w.flags);
         DH_TRY(check_launch(h.op));
         a.targets.target = w.flags;
@@ -2182,7 +2201,9 @@ int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
     pack_rows<T, PARTS><<<a.groups + more, 1024, 0, stream()>>>(a);
     DH_TRY(check_launch(h.op));
     if (h.target) return DH_OK;
-    const int waves = h.teacher.K <= 2 ? 1 : h.teacher.K >= 32 ? 16 : (h.teacher.K + 1) / 2;
+    // Up to 8 waves, with as few idle places in their last turn as that leaves.
+    const int turns = std::max(1, (h.teacher.K + 8 * TEACHER_FLY - 1) / (8 * TEACHER_FLY));
+    const int waves = std::max(1, (h.teacher.K + TEACHER_FLY * turns - 1) / (TEACHER_FLY * turns));
     teacher_dots<T><<<h.N, 64 * waves, 0, stream()>>>(w.rows, h.teacher, h.V, (const T*)h.H, h.ldh, (const T*)h.W,
                                                h.ldw, h.D, w.q, w.z, w.base);
     return check_launch(h.op);
