@@ -1527,6 +1527,7 @@ struct Few {
     const void* W;
     int ldw;
     float c;
+    uint32_t* keep;      // the rows that count, as bits, from few_mark; null: they have a target
     float2* part;        // [work-group of few_lse][ldpart]
     int ldpart;
     float* G;
@@ -1641,10 +1642,29 @@ __device__ inline void few_logits(const Few& f, int v0, uint32_t keep, float (*r
     }
 }
 
-// The rows that count, as bits.
+// The rows that count, as bits: a teacher's from a launch of its own, as a row without entries is known
+// for one only after all K (16 x 32000 x 1024 fp32, K = 100, forward and gradient: every work-group looking for
+// itself 245 us with half of the rows padding, 141 so; without padding 140 and 144).
+__global__ void __launch_bounds__(1024) few_mark(Few f) {
+    __shared__ uint32_t bits[16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const Teacher& t = f.targets.t;
+    uint32_t mine = 0;
+    for (int n = w; n < f.N; n += 16) {
+        bool any = false;
+        for (int k = lane; k < t.K; k += 64) any |= entry_counts(t, (size_t)n * t.K + k, f.targets.V);
+        if (__ballot(any)) mine |= 1u << n;
+    }
+    if (lane == 0) bits[w] = mine;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int x = 1; x < 16; ++x) mine |= bits[x];
+    *f.keep = mine;
+}
 __device__ inline uint32_t few_keep(const Few& f) {
+    if (f.keep) return *f.keep;
     const int lane = threadIdx.x & 63;
-    return (uint32_t)__ballot(lane < f.N && f.targets.has(lane));
+    return (uint32_t)__ballot(lane < f.N && counts(f.targets.target[lane < f.N ? lane : 0], f.targets.V));
 }
 
 // Reads the table once: 1 x 131072 x 2048 bf16 101 us, 5.3 TB/s; 16 x 41216 x 2357 fp32 (rows at odd
@@ -1701,7 +1721,7 @@ __global__ void __launch_bounds__(1024) few_loss(Few f, int blocks) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int n = blockIdx.x;
     const Targets& tg = f.targets;
-    if (!tg.has(n)) {
+    if (!((few_keep(f) >> n) & 1)) {
         if (threadIdx.x == 0) {
             f.loss[n] = 0.f;
             if (f.lse_out) f.lse_out[n] = 0.f;
@@ -1919,7 +1939,7 @@ __global__ void __launch_bounds__(1024) few_finish(Few f, Grad<OT> dH) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int n = blockIdx.y, c = blockIdx.x * 64 + lane;
-    const bool on = f.targets.has(n);
+    const bool on = (few_keep(f) >> n) & 1;
     if (!on && dH.accumulate) return;
     float v = 0.f;
     if (on && c < f.D)
@@ -2075,7 +2095,7 @@ bool is_few(int dtype, int N, int V, int D, int backward) {
 struct FewPlan {
     int Dp, rows, waves, blocks;   // of few_lse and few_g: table rows and waves of a work-group
     int splits, rows_per_split, hslabs, wslabs, wrows, wlanes;
-    size_t G, acc, total;   // the parts of the forward lie at G
+    size_t G, acc, keep, total;   // the parts of the forward lie at G
 };
 FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int backward) {
     FewPlan p{};
@@ -2088,7 +2108,8 @@ FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int backward) {
     p.waves = small && D >= 512 ? 16 : 4;
     p.blocks = (V + p.rows - 1) / p.rows;
     if (!backward) {
-        p.total = up256((size_t)p.blocks * (N <= FEW ? FEW : 2 * FEW) * 8);
+        p.keep = up256((size_t)p.blocks * (N <= FEW ? FEW : 2 * FEW) * 8);
+        p.total = p.keep + 256;
         return p;
     }
     // About 1024 work-groups of 4 waves for dH and 4096 for dW.
@@ -2103,7 +2124,8 @@ FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int backward) {
     const int chunks = std::max(1, std::min(4096 / p.wslabs, (V + least - 1) / least));
     p.wrows = (V + chunks - 1) / chunks;
     p.acc = up256((size_t)p.blocks * p.rows * FEW * 4);
-    p.total = p.acc + up256((size_t)p.splits * FEW * p.Dp * 4);
+    p.keep = p.acc + up256((size_t)p.splits * FEW * p.Dp * 4);
+    p.total = p.keep + 256;
     return p;
 }
 
@@ -2406,10 +2428,19 @@ Few few_args(const Head& h) {
     return f;
 }
 
+// The rows that count, where a teacher tells.
+int few_rows(const Head& h, Few& f, const FewPlan& p, void* ws) {
+    if (h.target) return DH_OK;
+    f.keep = (uint32_t*)((char*)ws + p.keep);
+    few_mark<<<1, 1024, 0, stream()>>>(f);
+    return check_launch(h.op);
+}
+
 template <typename T>
 int few_forward(const Head& h, float* loss, float* lse, void* ws) {
     const FewPlan p = few_plan(h.dtype, h.dtype, h.N, h.V, h.D, 0);
     Few f = few_args(h);
+    DH_TRY(few_rows(h, f, p, ws));
     f.part = (float2*)ws;
     f.loss = loss;
     f.lse_out = lse;
@@ -2430,6 +2461,7 @@ template <typename T, typename OT>
 int few_backward(const Head& h, const Grads& d, void* ws) {
     const FewPlan p = few_plan(h.dtype, d.type, h.N, h.V, h.D, 1);
     Few f = few_args(h);
+    DH_TRY(few_rows(h, f, p, ws));
     f.G = (float*)ws;
     f.acc = (float*)((char*)ws + p.acc);
     f.lse = d.lse;
