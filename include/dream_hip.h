@@ -358,7 +358,8 @@ int dh_linear_xent_fwd(int dtype, int N, int V, int D, float scale, const void* 
 /* Its gradient from the forward's lse: G = dloss[n] scale (softmax(z) - onehot(target)),
  * dH = G W, dW = G^T H.  d_dloss (N, fp32) may be NULL: ones.  d_dH or d_dW may be NULL: not
  * computed.  acc_dH / acc_dW add into them.  bf16: G is rounded to bf16 once before the products
- * (as any bf16 training does), so bf16 inputs give gradients to bf16 precision also in DH_F32.
+ * (as any bf16 training does), so bf16 inputs give gradients to bf16 precision also in DH_F32; it
+ * holds shares of the largest dloss, so rows 2^-110 of that and below may give none.
  * dH must not overlap H, nor dW W. */
 int dh_linear_xent_bwd(int dtype, int N, int V, int D, float scale, const void* d_H, int ldh,
                        const void* d_W, int ldw, const int* d_target, const float* d_lse,

@@ -130,6 +130,26 @@ def test_embedding_orders(N, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("grad", ["f32", "bf16"])
+@pytest.mark.parametrize("off", [0, 1, 5, 33])
+@pytest.mark.parametrize("N,V,D", [(0, 3000, 61), (6, 20000, 61), (6, 9, 1), (40, 70000, 7)])
+def test_embedding_clears_a_table_without_gaps(N, V, D, off, grad):
+    """Tables that begin at any value: every row is written, and nothing before or behind them."""
+    t, fill = (np.uint16, 0x7FC0) if grad == "bf16" else (np.float32, np.float32(7))
+    r = np.random.default_rng(N)
+    ids, dY = r.integers(0, V, N), r.integers(-8, 9, (max(N, 1), D)).astype(np.float32)   # exact in both
+    dYb = store(dY, grad)[0]
+    full = DB.from_numpy(np.full(V * D + off + 300, fill, t))
+    hip.embedding_bwd(DT[grad], N, V, D, 1.0, ints(ids if N else [0]), dYb, D,
+                      full.ptr + off * np.dtype(t).itemsize, D, DT[grad], False, None, 0)
+    raw = full.numpy()
+    assert (raw[:off] == fill).all() and (raw[off + V * D:] == fill).all()
+    got = raw[off:off + V * D].reshape(V, D)
+    want = emb_ref(ids, np.zeros((V, D)), dY[:N].astype(np.float64), 1.0)[1]
+    assert ((bits_to_f32(got) if grad == "bf16" else got) == want).all()
+
+
+@pytest.mark.gpu
 def test_embedding_no_tokens():
     run_embedding([], 5, 12, "f32", "f32")
     run_embedding([], 5, 12, "bf16", "f32", accumulate=True)
