@@ -15,13 +15,18 @@
 // products.  Rows without a target (padding) are taken out first: the rows that count are packed
 // side by side, so padding costs no product and nothing in it, NaN included, reaches a sum.
 //
-// All four products run on the 16-bit matrix cores with fp32 accumulators.  bf16 operands are taken
-// as they are.  An fp32 operand is scaled by a power of two and split into two fp16 parts of 11
-// significant bits, x = hi + 2^-11 lo; a product is 2^-11 (lo hi + hi lo) + hi hi: the two cross
-// products are added first, the accumulators scaled by 2^-11 (exactly), then the third is added.
-// Three 16-bit products at 16 times the rate of an fp32 one.  With the operand's largest value
-// scaled below 2^15, the others are taken to 2^-23 of themselves or 2^-51 of it, whichever is more,
-// and the product left out (lo lo) is below 2^-24 of a product.  What the scale is common to: a row
+// All four products run on the 16-bit matrix cores with fp32 accumulators.  The forward takes bf16
+// operands as they are.  Every other operand is scaled by a power of two and held in fp16 parts of 11
+// significant bits, one or two, x = hi + 2^-11 lo; a product of two by two is 2^-11 (lo hi + hi lo) +
+// hi hi: the cross products are added first, the accumulators scaled by 2^-11 (exactly), then the
+// third is added (lo lo is left out).  Three 16-bit products at 16 times the rate of an fp32 one.
+//   fp32 inputs            two parts of all operands
+//   bf16, gradients bf16   one part: H and W fit exactly, G and w_n H_n are rounded to 11 bits, whose
+//                          2^-11 is an eighth of the result's own rounding (to bf16 G would lose as much
+//                          as the result does, and at the targets in one direction); as many products
+//   bf16, gradients fp32   one part of H and W, two of G and w_n H_n: 1, 2 and 3 products
+// With the operand's largest value scaled below 2^15, the others are taken to 2^-23 (one part: 2^-11) of
+// themselves or 2^-51 (2^-39) of it, whichever is more.  What the scale is common to: a row
 // where k runs along the row (H, and W in the forward), else all of the operand (W in the
 // backward, where its rows are summed over; G, whose entries are p - q; and w_n H_n, the other
 // operand of dW).
@@ -79,19 +84,23 @@ __device__ inline void split2(float x, uint16_t (&p)[2]) {
     p[0] = __builtin_bit_cast(uint16_t, hi);
     p[1] = __builtin_bit_cast(uint16_t, lo);
 }
-// What the products take of a value: its nearest bf16, or its two fp16 parts.
-template <int PARTS>
-__device__ inline void to_parts(float x, uint16_t (&p)[PARTS]) {
-    if constexpr (PARTS == 1) p[0] = rne_bf16(x);
+// What the products take of a value: its nearest bf16 (BF), or that many fp16 parts.
+constexpr int BF = 0;
+constexpr int parts_of(int P) { return P == 2 ? 2 : 1; }
+template <int P>
+__device__ inline void to_parts(float x, uint16_t (&p)[parts_of(P)]) {
+    if constexpr (P == BF) p[0] = rne_bf16(x);
+    else if constexpr (P == 1) p[0] = __builtin_bit_cast(uint16_t, (_Float16)x);
     else split2(x, p);
 }
-template <int PARTS>
+template <int P>
 __device__ inline void store_parts(uint16_t* __restrict__ dst, long long plane, const float (&v)[8]) {
+    constexpr int PARTS = parts_of(P);
     h8 o[PARTS];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         uint16_t x[PARTS];
-        to_parts<PARTS>(v[e], x);
+        to_parts<P>(v[e], x);
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) o[p][e] = x[p];
     }
@@ -113,16 +122,16 @@ __device__ inline float larger(float mx, const float (&x)[8]) {
     return mx;
 }
 
-// One row of D values as parts with zeros up to Dp, by one wave.  Two parts: OWN, at the row's own
+// One row of D values as parts with zeros up to Dp, by one wave.  fp16: OWN, at the row's own
 // scale, which is returned; else v 2^-e f (f at most 1 in size, so nothing overflows on the way).
-template <typename T, int PARTS, bool OWN>
+template <typename T, int P, bool OWN>
 __device__ inline int convert_row(const T* __restrict__ src, int D, uint16_t* __restrict__ dst, int Dp,
                                   long long plane, int lane, int e = 0, float f = 1.f) {
-    if constexpr (PARTS == 1) {
+    if constexpr (P == BF) {
         for (int c = 8 * lane; c < Dp; c += 512) {
             float v[8];
             load8(src, c, D, v);
-            store_parts<1>(dst + c, plane, v);
+            store_parts<BF>(dst + c, plane, v);
         }
         return 0;
     } else {
@@ -147,7 +156,7 @@ __device__ inline int convert_row(const T* __restrict__ src, int D, uint16_t* __
         auto put = [&](int c, float (&x)[8]) {
 #pragma unroll
             for (int q = 0; q < 8; ++q) x[q] = OWN ? x[q] * scale : (x[q] * scale) * f;
-            store_parts<PARTS>(dst + c, plane, x);
+            store_parts<P>(dst + c, plane, x);
         };
 #pragma unroll
         for (int t = 0; t < KEEP; ++t)
@@ -162,22 +171,23 @@ __device__ inline int convert_row(const T* __restrict__ src, int D, uint16_t* __
 }
 
 // ---- packing ------------------------------------------------------------------------------------
-// What a packed row i is: its row n, target, loss weight and lse (backward), and its scale (two
-// parts).  Arrays are padded to whole tiles of rows, so that a tile's epilogue may load past the
-// last row.
+// What a packed row i is: its row n, target, loss weight and lse (backward), and its scale (fp16).
+// Arrays are padded to whole tiles of rows, so that a tile's epilogue may load past the last row.
 struct Rows {
     int* cnt;          // rows that count
     int* row;          // packed -> row
     int* target;
     int* hexp;
-    float *w, *lse;    // backward only; one part: w is the row's share of the largest weight,
-    float* wtop;       // which stands here
+    float *w, *lse;    // backward only
 };
-// Two parts: the scales of the other operands.
+// fp16: the scales of the other operands.
 struct Exps {
     int* e;            // forward: of the piece's table rows
     int *X, *E;        // backward: of w_n H_n and of the table
-    int* group;        // per group of packed rows, the largest scale that w_n H_n asks for
+    float* wtop;       // one part: the largest weight.  w_n / wtop H_n is the operand then, which is
+                       // exact where all weights are equal
+    int* group;        // per group of packed rows, the largest scale that w_n H_n asks for,
+    float* gtop;       // and its largest weight
     float* wmax;       // per work-group of the scan, the table's largest value
 };
 constexpr int SCAN = 1024;   // most work-groups that look for it
@@ -278,8 +288,8 @@ constexpr int PACK = 16;     // rows of a work-group, one per wave
 // Work-group b < groups packs rows 16 b .. 16 b + 15: it counts the rows that count before them (the
 // targets are few and stay in cache), then converts its own.  Forward: also the padding's zeros and,
 // for cross entropy, base = -z at the target (the loss is lse + base).  The work-groups behind
-// stage table rows, or (backward, two parts) look for the table's largest value.
-template <typename T, int PARTS>
+// stage table rows (forward), or look for the table's largest value (backward).
+template <typename T, int P>
 __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
     __shared__ int red[16];
     __shared__ float tops[16];
@@ -293,12 +303,12 @@ __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
         if (b < a.tables) {
             const int r = 16 * b + w;
             if (r >= a.R) return;
-            const int e = convert_row<T, PARTS, true>(W + (size_t)r * a.ldw, D, a.staged + (size_t)r * a.Dp,
-                                                      a.Dp, a.wplane, lane);
-            if (PARTS == 2 && lane == 0) a.exps.e[r] = e;
+            const int e = convert_row<T, P, true>(W + (size_t)r * a.ldw, D, a.staged + (size_t)r * a.Dp,
+                                                  a.Dp, a.wplane, lane);
+            if (P != BF && lane == 0) a.exps.e[r] = e;
             return;
         }
-        if constexpr (PARTS == 2) {
+        if constexpr (P != BF) {
             const int scan = gridDim.x - a.groups;
             float mx = 0.f;
             for (long long v = 16LL * b + w; v < V; v += 16LL * scan)
@@ -318,44 +328,25 @@ __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
     }
     const int n0 = blockIdx.x * PACK;
     int before = 0;
-    float top = 0.f;   // the largest size of a weight
-    const bool shares = PARTS == 1 && a.lse_in && a.dloss;
-    for (int n = threadIdx.x; n < (shares ? a.N : n0); n += 1024)
-        if (a.targets.has(n)) {
-            before += n < n0;
-            if (shares) {
-                const float x = __builtin_fabsf(a.dloss[n]);
-                top = x < INFINITY ? fmaxf(top, x) : top;
-            }
-        }
+    for (int n = threadIdx.x; n < n0; n += 1024) before += a.targets.has(n);
     for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m, 64);
-    if (shares) top = wave_reduce(top, OpMax());
-    if (lane == 0) {
-        red[w] = before;
-        tops[w] = top;
-    }
+    if (lane == 0) red[w] = before;
     if (threadIdx.x < PACK) own[threadIdx.x] = n0 + (int)threadIdx.x < a.N && a.targets.has(n0 + threadIdx.x);
     __syncthreads();
     before = 0;
-    for (int x = 0; x < 16; ++x) {
-        before += red[x];
-        top = fmaxf(top, tops[x]);
-    }
-    if (!(top > 0.f)) top = 1.f;
+    for (int x = 0; x < 16; ++x) before += red[x];
     int count = 0, i = before;
     for (int x = 0; x < PACK; ++x) {
         if (x < w) i += own[x];
         count += own[x];
     }
-    if ((int)blockIdx.x == a.groups - 1 && threadIdx.x == 0) {
-        *a.rows.cnt = before + count;
-        if (PARTS == 1 && a.lse_in) *a.rows.wtop = top * a.wscale;
-    }
+    if ((int)blockIdx.x == a.groups - 1 && threadIdx.x == 0) *a.rows.cnt = before + count;
     const int n = n0 + w;
     const bool keep = own[w];
     int most = NO_EXP;
+    float top = 0.f;   // the weight's size, where finite
     if (keep) {
-        const int h = convert_row<T, PARTS, true>(H + (size_t)n * a.ldh, D, a.Hp + (size_t)i * a.Dp, a.Dp,
+        const int h = convert_row<T, P, true>(H + (size_t)n * a.ldh, D, a.Hp + (size_t)i * a.Dp, a.Dp,
                                                   a.plane, lane);
         const int target = a.targets.target ? a.targets.target[n] : 0;
         if (a.base) {
@@ -367,11 +358,11 @@ __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
             a.rows.target[i] = target;
             a.rows.hexp[i] = h;
             if (a.lse_in) {
-                const float d = a.dloss ? a.dloss[n] : 1.f;
-                const float wn = PARTS == 1 ? d / top : d * a.wscale;
+                const float wn = (a.dloss ? a.dloss[n] : 1.f) * a.wscale, size = __builtin_fabsf(wn);
                 a.rows.lse[i] = a.lse_in[n];
                 a.rows.w[i] = wn;
                 most = exponent(wn) + h;   // |w_n H_n| < 2^(15 + this)
+                top = size < INFINITY ? size : 0.f;
             }
         }
     } else if (n < a.N) {
@@ -384,69 +375,89 @@ __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
             else zero_row((uint16_t*)a.dH + (size_t)n * a.lddh, D, lane);
         }
     }
-    if (PARTS == 2 && a.lse_in) {
+    if (P != BF && a.lse_in) {
         __syncthreads();   // red[] has been read
-        if (lane == 0) red[w] = most;
+        if (lane == 0) {
+            red[w] = most;
+            tops[w] = top;
+        }
         __syncthreads();
         if (threadIdx.x == 0) {
-            for (int x = 1; x < 16; ++x) most = max(most, red[x]);
+            for (int x = 1; x < 16; ++x) {
+                most = max(most, red[x]);
+                top = fmaxf(top, tops[x]);
+            }
             a.exps.group[blockIdx.x] = most;
+            a.exps.gtop[blockIdx.x] = top;
         }
     }
 }
 
-// Forward, or one part: rows v0 .. v0 + R - 1 of the table as parts, a wave per row.
-template <typename T, int PARTS>
+// Forward: rows v0 .. v0 + R - 1 of the table as parts, a wave per row.
+template <typename T, int P>
 __global__ void __launch_bounds__(256) stage_table(const T* __restrict__ W, int ldw, int v0, int R, int D,
                                                    uint16_t* __restrict__ dst, int Dp, long long plane,
                                                    int* __restrict__ exps) {
     const int lane = threadIdx.x & 63;
     const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= R) return;
-    const int e = convert_row<T, PARTS, true>(W + (size_t)(v0 + r) * ldw, D, dst + (size_t)r * Dp, Dp, plane,
-                                              lane);
-    if (PARTS == 2 && lane == 0) exps[r] = e;
+    const int e = convert_row<T, P, true>(W + (size_t)(v0 + r) * ldw, D, dst + (size_t)r * Dp, Dp, plane,
+                                          lane);
+    if (P != BF && lane == 0) exps[r] = e;
 }
 
-// Backward of two parts: the same at the table's scale, which each work-group finds from the scan's
-// results; the work-groups behind (first piece) convert the packed rows of w_n H_n at theirs.  The
-// first work-group writes both scales down for the products.
-__global__ void __launch_bounds__(256) stage_scaled(const float* __restrict__ W, int ldw, int v0, int R,
+// Backward: the same at the table's scale, which each work-group finds from the scan's results; the
+// work-groups behind (first piece) convert the packed rows of w_n H_n (one part: w_n / wtop H_n) at theirs,
+// in XP parts.  The first work-group writes the scales down for the products.
+template <typename T, int P, int XP>
+__global__ void __launch_bounds__(256) stage_scaled(const T* __restrict__ W, int ldw, int v0, int R,
                                                     int D, uint16_t* __restrict__ dst, int Dp,
                                                     long long plane, Exps exps, int groups, int scan, int tables,
-                                                    Rows rows, const float* __restrict__ H, int ldh,
+                                                    Rows rows, const T* __restrict__ H, int ldh,
                                                     uint16_t* __restrict__ Xp, long long xplane) {
-    __shared__ float redf[4];
+    __shared__ float redf[4], redw[4];
     __shared__ int redi[4];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    float mx = 0.f;
+    float mx = 0.f, top = 0.f;
     for (int g = threadIdx.x; g < scan; g += 256) mx = fmaxf(mx, exps.wmax[g]);
     mx = wave_reduce(mx, OpMax());
     int x = NO_EXP;
-    for (int g = threadIdx.x; g < groups; g += 256) x = max(x, exps.group[g]);
+    for (int g = threadIdx.x; g < groups; g += 256) {
+        x = max(x, exps.group[g]);
+        if (XP == 1) top = fmaxf(top, exps.gtop[g]);
+    }
     for (int m = 1; m < 64; m <<= 1) x = max(x, __shfl_xor(x, m, 64));
+    if (XP == 1) top = wave_reduce(top, OpMax());
     if (lane == 0) {
         redf[w] = mx;
+        redw[w] = top;
         redi[w] = x;
     }
     __syncthreads();
     const int E = scale_of(fmaxf(fmaxf(redf[0], redf[1]), fmaxf(redf[2], redf[3])));
-    const int X = max(max(redi[0], redi[1]), max(redi[2], redi[3]));
+    int X = max(max(redi[0], redi[1]), max(redi[2], redi[3]));
+    if (XP == 1) {
+        top = fmaxf(fmaxf(redw[0], redw[1]), fmaxf(redw[2], redw[3]));
+        if (!(top > 0.f)) top = 1.f;   // all weights are zero
+        X = X - exponent(top) + 1;     // |w_n / top| < 2^(its exponent - top's + 1)
+    }
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *exps.E = E;
         *exps.X = X;
+        *exps.wtop = top;
     }
     if ((int)blockIdx.x < tables) {
         const int r = blockIdx.x * 4 + w;
         if (r < R)
-            convert_row<float, 2, false>(W + (size_t)(v0 + r) * ldw, D, dst + (size_t)r * Dp, Dp, plane, lane, E);
+            convert_row<T, P, false>(W + (size_t)(v0 + r) * ldw, D, dst + (size_t)r * Dp, Dp, plane, lane, E);
         return;
     }
     const int i = (blockIdx.x - tables) * 4 + w;
     if (i >= *rows.cnt) return;
     const int h = rows.hexp[i];
-    convert_row<float, 2, false>(H + (size_t)rows.row[i] * ldh, D, Xp + (size_t)i * Dp, Dp, xplane, lane, h,
-                                 __builtin_ldexpf(rows.w[i], h - X));
+    const float wn = XP == 1 ? rows.w[i] / top : rows.w[i];
+    convert_row<T, XP, false>(H + (size_t)rows.row[i] * ldh, D, Xp + (size_t)i * Dp, Dp, xplane, lane, h,
+                              __builtin_ldexpf(wn, h - X));
 }
 
 // ---- teachers ------------------------------------------------------------------------------------
@@ -530,9 +541,9 @@ __global__ void __launch_bounds__(512) teacher_dots(Rows rows, Teacher t, int V,
 }
 
 // ---- products -------------------------------------------------------------------------------------
-// C (M x N) = sum over k of A and B, operands of PARTS 16-bit parts.  AK: A is stored [m][k], else
-// [k][m]; BK: B is stored [n][k], else [k][n].  One of M, N and K counts packed rows: its extent
-// is *cnt.
+// C (M x N) = sum over k of A and B, operands of PA and PB fp16 parts (or both BF).  AK: A is stored
+// [m][k], else [k][m]; BK: B is stored [n][k], else [k][n].  One of M, N and K counts packed rows: its
+// extent is *cnt.
 struct Prod {
     const uint16_t *A, *B;
     int lda, ldb;
@@ -628,18 +639,26 @@ struct Operand {
     }
 };
 
-template <int PARTS, int FM, int FN>
+// The 16-bit products that make one of such operands, in this order: low parts of A by B (two of A),
+// A by low parts of B (two of B), high by high.
+constexpr int kinds_of(int PA, int PB) { return 1 + (PA == 2) + (PB == 2); }
+constexpr int part_a(int PA, int kind) { return PA == 2 && kind == 0; }
+constexpr int part_b(int PA, int PB, int kind) { return PB == 2 && kind == (PA == 2); }
+
+template <int PA>
+__device__ inline void mfma16(const bf16x8& a, const bf16x8& b, f32x16& acc) {
+    if constexpr (PA == BF)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+    else
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc,
+                                                     0, 0, 0);
+}
+template <int PA, int FM, int FN>
 __device__ inline void mfma_parts(const bf16x8 (&fa)[FM], const bf16x8 (&fb)[FN], f32x16 (&acc)[FM][FN]) {
 #pragma unroll
     for (int a = 0; a < FM; ++a)
 #pragma unroll
-        for (int b = 0; b < FN; ++b) {
-            if constexpr (PARTS == 1)
-                acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[a], fb[b], acc[a][b], 0, 0, 0);
-            else
-                acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    __builtin_bit_cast(f16x8, fa[a]), __builtin_bit_cast(f16x8, fb[b]), acc[a][b], 0, 0, 0);
-        }
+        for (int b = 0; b < FN; ++b) mfma16<PA>(fa[a], fb[b], acc[a][b]);
 }
 
 // Tiles: 256 x 256 by 8 waves of 128 x 64 and 128 x 128 by 4 waves of 64 x 64, stages of 32 k; 64 x 64
@@ -685,7 +704,7 @@ __device__ inline void store_rows(uint16_t* lds, const uint16_t (&v)[FN][16], in
 // stages ahead; a stage's 16-k steps run while the next operands are read (the schedule of the
 // bf16 GEMM's 8-wave form).  Epi::run gets the tile's accumulators: register r of block (a, b) is
 // row m0 + wm + 32 a + 8 (r / 4) + 4 h + r % 4, column n0 + wn + 32 b + l32 (lane = 32 h + l32).
-template <class S, bool AK, bool BK_, int TOK, int PARTS, class Epi>
+template <class S, bool AK, bool BK_, int TOK, int PA, int PB, class Epi>
 __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, int tile, int tiles,
                                  int split) {
     constexpr int FM = S::FM, FN = S::FN, BK = S::BK, NS = S::NS, STEPS = BK / 16;
@@ -713,21 +732,21 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
 
     const int kt0 = split * g.kstages;
     const int nk = max(0, min((Kall + BK - 1) / BK - kt0, g.kstages));
-    // two parts: lo hi, hi lo, then (from stage `cross` on) hi hi
-    const int total = PARTS == 1 ? nk : 3 * nk, cross = 2 * nk;
+    // the last kind, from stage `cross` on, is high by high
+    constexpr int KINDS = kinds_of(PA, PB);
+    const int total = KINDS * nk, cross = (KINDS - 1) * nk;
     if (total > 0) {
         OA sa;
         OB sb;
         sa.init(g.A, g.pa, g.lda, m0, M, Kall, wave, lane);
         sb.init(g.B, g.pb, g.ldb, n0, N, Kall, wave, lane);
-        // the parts' pairs: lo hi, hi lo, hi hi
-        sa.start(PARTS == 2 ? 1 : 0, kt0);
-        sb.start(0, kt0);
+        sa.start(part_a(PA, 0), kt0);
+        sb.start(part_b(PA, PB, 0), kt0);
         const int tail = (kt0 + nk) * BK > Kall ? nk - 1 : -1;   // the stage that ends behind K
         constexpr uint32_t RING = 2u * NS * S::STAGE;
         const uint32_t ring0 = lds_addr(ring);
         const uint32_t wave_a = 1024u * OA::PER * wave, wave_b = 2u * BOFF + 1024u * OB::PER * wave;
-        int ikt = 0, ipair = 0;   // the next stage to fetch
+        int ikt = 0, kind = 0;   // the next stage to fetch
         uint32_t slot = 0;
         auto issue = [&]() {
             const uint32_t to = __builtin_amdgcn_readfirstlane(ring0 + slot);
@@ -745,11 +764,11 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
             slot = slot == RING - 2u * S::STAGE ? 0u : slot + 2u * S::STAGE;
             sa.next();
             sb.next();
-            if (++ikt == nk && PARTS == 2) {
+            if (++ikt == nk && KINDS > 1) {
                 ikt = 0;
-                ++ipair;
-                sa.start(0, kt0);
-                sb.start(ipair == 1, kt0);
+                ++kind;
+                sa.start(part_a(PA, kind), kt0);
+                sb.start(part_b(PA, PB, kind), kt0);
             }
         };
         auto landed = [&](int ahead) {   // all but the youngest `ahead` stages
@@ -758,7 +777,7 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
             else wait_vmcnt<0>();
         };
         auto scale_cross = [&](int s) {
-            if (PARTS == 2 && s == cross)
+            if (KINDS > 1 && s == cross)
 #pragma unroll
                 for (int a = 0; a < FM; ++a)
 #pragma unroll
@@ -776,7 +795,7 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
         };
         bf16x8 fa[2][FM], fb[2][FN];
         auto mma = [&](int f) {
-            mfma_parts<PARTS, FM, FN>(fa[f], fb[f], acc);
+            mfma_parts<PA, FM, FN>(fa[f], fb[f], acc);
             __builtin_amdgcn_sched_barrier(0);
         };
         auto inner = [&](int s) {   // all steps but the last, whose operands it reads
@@ -824,7 +843,7 @@ __device__ inline void gemm_tile(uint16_t* ring, const Prod& g, const Epi& epi, 
 // ones again into slots that nobody reads any more, so that the waits are constants: when stage s
 // ends, stage s + 1 has landed and 12 (s even) or 8 (odd) younger loads may be in flight.  An odd
 // last stage lies past K and reads as zero.
-template <class S, bool BK_, int TOK, int PARTS, class Epi>
+template <class S, bool BK_, int TOK, int PA, int PB, class Epi>
 __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, int tile, int tiles, int split) {
     constexpr int FM = S::FM, FN = S::FN, T = S::T;
     using OA = Operand<true, T, 64, S::WAVES>;
@@ -850,14 +869,15 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
 
     const int p0 = split * g.kstages;   // in pairs
     const int np = max(0, min((g.K + 63) / 64 - p0, g.kstages));
-    const int pairs = PARTS == 1 ? np : 3 * np;
+    constexpr int KINDS = kinds_of(PA, PB);
+    const int pairs = KINDS * np;
     if (pairs > 0) {
         OA sa;
         OB sb;
         sa.init(g.A, g.pa, g.lda, m0, M, g.K, wave, lane);
         sb.init(g.B, g.pb, g.ldb, n0, N, g.K, wave, lane);
-        sa.start(PARTS == 2 ? 1 : 0, p0);
-        sb.start(0, 2 * p0);
+        sa.start(part_a(PA, 0), p0);
+        sb.start(part_b(PA, PB, 0), 2 * p0);
         const uint32_t ring_a0 = lds_addr(ring) + 1024u * OA::PER * wave;
         const uint32_t ring_b0 = lds_addr(ring) + 2u * 3 * T * 64 + 1024u * OB::PER * wave;
         uint16_t* const ring_a = ring;
@@ -881,7 +901,7 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
                 if (++ap == np) {
                     ap = 0;
                     ++akind;
-                    sa.start(0, p0);
+                    sa.start(part_a(PA, akind), p0);
                 }
             }
         };
@@ -901,7 +921,7 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
                 if (++bs == 2 * np) {
                     bs = 0;
                     ++bkind;
-                    sb.start(bkind == 1, 2 * p0);
+                    sb.start(part_b(PA, PB, bkind), 2 * p0);
                 }
             }
         };
@@ -922,12 +942,7 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
 #pragma unroll
             for (int i = 0; i < FM * FN; ++i) {
                 const int a = i / FN, b = i % FN;
-                if constexpr (PARTS == 1)
-                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[f][a], fb[f][b], acc[a][b], 0, 0, 0);
-                else
-                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                        __builtin_bit_cast(f16x8, fa[f][a]), __builtin_bit_cast(f16x8, fb[f][b]), acc[a][b], 0,
-                        0, 0);
+                mfma16<PA>(fa[f][a], fb[f][b], acc[a][b]);
                 if (i < FM) fa[f ^ 1][i] = OA::frag(la, wm + 32 * i, ka, lane);
                 else if (i < FM + FN) fb[f ^ 1][i - FM] = OB::frag(lb, wn + 32 * (i - FM), kb, lane);
                 dma(i);
@@ -970,8 +985,8 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
             __syncthreads();
             step(1, next, 0, lb2, 0, none);   // after the last pair: what is there, unused
         };
-        for (int kind = 0; kind < (PARTS == 1 ? 1 : 3); ++kind) {
-            if (kind == 2)
+        for (int kind = 0; kind < KINDS; ++kind) {
+            if (KINDS > 1 && kind == KINDS - 1)
 #pragma unroll
                 for (int a = 0; a < FM; ++a)
 #pragma unroll
@@ -989,7 +1004,7 @@ __device__ inline void gemm_deep(uint16_t* ring, const Prod& g, const Epi& epi, 
     epi.template run<FM, FN>(acc, M, N, m0 + wm, n0 + wn, lane, split, ring + wave * LDS_TILE);
 }
 
-// The 64-wide tile of two parts: a stage holds 64 k of both parts of both operands (32 KB, a ring of
+// The 64-wide tile of two parts by two: a stage holds 64 k of both parts of both operands (32 KB, a ring of
 // four) and each of its 16-k steps makes all three products, the cross products in accumulators of
 // their own.  One chain of stages instead of three, and two thirds of the loads.
 template <class S, bool AK, bool BK_, int TOK, class Epi>
@@ -1103,15 +1118,15 @@ __device__ inline void gemm_both(uint16_t* ring, const Prod& g, const Epi& epi, 
 }
 
 // The form that a shape and its operands take, and its LDS in elements.
-template <class S, bool AK, int PARTS>
+template <class S, bool AK, int PA, int PB>
 constexpr int ring_of() {
-    return S::T == 256 && AK ? S::DEEP : S::NS * S::STAGE * (S::T == 64 && PARTS == 2 ? 2 : 1);
+    return S::T == 256 && AK ? S::DEEP : S::NS * S::STAGE * (S::T == 64 && PA == 2 && PB == 2 ? 2 : 1);
 }
-template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
+template <class S, bool AK, bool BK, int TOK, int PA, int PB, class Epi>
 __device__ inline void gemm_form(uint16_t* ring, const Prod& g, const Epi& epi, int tile, int tiles, int split) {
-    if constexpr (S::T == 256 && AK) gemm_deep<S, BK, TOK, PARTS>(ring, g, epi, tile, tiles, split);
-    else if constexpr (S::T == 64 && PARTS == 2) gemm_both<S, AK, BK, TOK>(ring, g, epi, tile, tiles, split);
-    else gemm_tile<S, AK, BK, TOK, PARTS>(ring, g, epi, tile, tiles, split);
+    if constexpr (S::T == 256 && AK) gemm_deep<S, BK, TOK, PA, PB>(ring, g, epi, tile, tiles, split);
+    else if constexpr (S::T == 64 && PA == 2 && PB == 2) gemm_both<S, AK, BK, TOK>(ring, g, epi, tile, tiles, split);
+    else gemm_tile<S, AK, BK, TOK, PA, PB>(ring, g, epi, tile, tiles, split);
 }
 
 // The four products.  Bound by the matrix cores under the card's power limit (1.54 to 1.65 GHz).  Measured for
@@ -1121,34 +1136,34 @@ __device__ inline void gemm_form(uint16_t* ring, const Prod& g, const Epi& epi, 
 // stages); a bf16 product of 8192^3 by the vendor's library reaches 1.23 here.  2048 x 32000 x 1024 fp32,
 // 0.134 TFLOP each, in us and TFLOP/s of fp32: 373 / 360, 408 / 329, 346 / 388, 419 / 321; the fp32 matrix
 // cores themselves end at 157.
-template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
+template <class S, bool AK, bool BK, int TOK, int PA, int PB, class Epi>
 __global__ void __launch_bounds__(S::THREADS) vocab_gemm(Prod g, Epi epi) {
-    __shared__ __attribute__((aligned(16))) uint16_t ring[ring_of<S, AK, PARTS>()];
-    gemm_form<S, AK, BK, TOK, PARTS>(ring, g, epi, blockIdx.x, gridDim.x, blockIdx.y);
+    __shared__ __attribute__((aligned(16))) uint16_t ring[ring_of<S, AK, PA, PB>()];
+    gemm_form<S, AK, BK, TOK, PA, PB>(ring, g, epi, blockIdx.x, gridDim.x, blockIdx.y);
 }
 
 // dH and dW of a piece in one launch: the first `first` work-groups are dH's, splits one after the
-// other.
-template <class S, int PARTS, class EpiH, class EpiW>
+// other.  W in P parts, G and w_n H_n in GP.
+template <class S, int P, int GP, class EpiH, class EpiW>
 __global__ void __launch_bounds__(S::THREADS) vocab_grads(Prod gh, EpiH eh, int tiles_h, int first, Prod gw,
                                                           EpiW ew, int tiles_w) {
-    __shared__ __attribute__((aligned(16))) uint16_t ring[ring_of<S, true, PARTS>()];
+    __shared__ __attribute__((aligned(16))) uint16_t ring[std::max(ring_of<S, true, GP, P>(), ring_of<S, false, GP, GP>())];
     const int b = blockIdx.x;
     if (b < first)
-        gemm_form<S, true, false, TOK_M, PARTS>(ring, gh, eh, b % tiles_h, tiles_h, b / tiles_h);
+        gemm_form<S, true, false, TOK_M, GP, P>(ring, gh, eh, b % tiles_h, tiles_h, b / tiles_h);
     else
-        gemm_form<S, false, false, TOK_K, PARTS>(ring, gw, ew, (b - first) % tiles_w, tiles_w,
-                                                 (b - first) / tiles_w);
+        gemm_form<S, false, false, TOK_K, GP, GP>(ring, gw, ew, (b - first) % tiles_w, tiles_w,
+                                                  (b - first) / tiles_w);
 }
 
 // Forward: rows are table rows, columns packed rows.  A lane holds half of the wave's logits of
 // each of its columns, lane + 32 the other half: their maximum and sum of exponentials go to
 // part[the wave's block of 32 FM rows][column].
-template <int PARTS>
+template <int P>
 struct EpiLse {
     static constexpr bool LDS = false;
     float c;
-    const int *e, *h;      // exponents of the table's and the packed rows' scales (two parts)
+    const int *e, *h;      // exponents of the table's and the packed rows' scales (fp16)
     float2* part;
     int ldp;
     template <int FM, int FN>
@@ -1156,28 +1171,28 @@ struct EpiLse {
                         uint16_t*) const {
         if (row0 >= M) return;   // the wave has no table row: its block is not joined either
         const bool full = row0 + 32 * FM <= M;
-        // Two parts: the logits in place; one part: they are c times the accumulators, and
+        // fp16: the logits in place; bf16: they are c times the accumulators, and
         // exp(c (x - mx)) = 2^(k x - k mx) with k = c log2(e), one multiply-add an exponential.
         // -inf past the table's end.
         float kc[FN];
 #pragma unroll
         for (int b = 0; b < FN; ++b)
-            kc[b] = PARTS == 1 ? 1.f : __builtin_ldexpf(c, h[col0 + 32 * b + (lane & 31)]);
-        const float k = PARTS == 1 ? c * LOG2E : LOG2E;
-        if (PARTS == 2 || !full)
+            kc[b] = P == BF ? 1.f : __builtin_ldexpf(c, h[col0 + 32 * b + (lane & 31)]);
+        const float k = P == BF ? c * LOG2E : LOG2E;
+        if (P != BF || !full)
 #pragma unroll
         for (int a = 0; a < FM; ++a)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int row = row0 + reg_row(a, 4 * r4, lane);
                 i32x4 e4;
-                if constexpr (PARTS == 2) e4 = *reinterpret_cast<const i32x4*>(e + row);
+                if constexpr (P != BF) e4 = *reinterpret_cast<const i32x4*>(e + row);
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
 #pragma unroll
                     for (int b = 0; b < FN; ++b) {
                         const float z =
-                            PARTS == 1 ? acc[a][b][4 * r4 + q]
+                            P == BF ? acc[a][b][4 * r4 + q]
                                        : acc[a][b][4 * r4 + q] * __builtin_ldexpf(kc[b], e4[q]);
                         acc[a][b][4 * r4 + q] = full || row + q < M ? z : -INFINITY;
                     }
@@ -1197,27 +1212,24 @@ struct EpiLse {
             for (int a = 0; a < FM; ++a)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s += __builtin_amdgcn_exp2f(PARTS == 1 ? __builtin_fmaf(k, acc[a][b][r], -km)
+                    s += __builtin_amdgcn_exp2f(P == BF ? __builtin_fmaf(k, acc[a][b][r], -km)
                                                            : k * (acc[a][b][r] - m));
             s += xor32(s);
             const int col = col0 + 32 * b + (lane & 31);
             if (lane < 32 && col < N)
-                part[(size_t)(row0 / (32 * FM)) * ldp + col] = float2{PARTS == 1 ? c * mx : mx, s};
+                part[(size_t)(row0 / (32 * FM)) * ldp + col] = float2{P == BF ? c * mx : mx, s};
         }
     }
 };
 
-// Backward: rows are packed rows, columns the piece's table rows.  One part: G = w (p - q), rounded
-// once to bf16, the type that the products take; w is the row's share of the largest weight, so that
-// with equal weights the entry at an unlikely target lies just above -1, where bf16 rounds by 2^-9 of
-// it at most; times the weight itself it could be off by 2^-8, in the same direction in all rows that
-// share the target.  The gradients' last step multiplies by the largest weight.  Two parts: 2^14 (p - q) to 22 bits.  Columns past
-// the table's end up to the tile's are zero.
-template <int PARTS, bool HARD>
+// Backward: rows are packed rows, columns the piece's table rows.  G = 2^14 (p - q) in GP fp16 parts,
+// without the row's weight, whose range over the rows it need not hold.  Columns past the table's end
+// up to the tile's are zero.
+template <int GP, bool HARD>
 struct EpiG {
     static constexpr bool LDS = true;
     float c;
-    const float *lse, *w;
+    const float* lse;
     const int *target, *h, *E;
     int v0;
     uint16_t* G;
@@ -1226,40 +1238,38 @@ struct EpiG {
     template <int FM, int FN>
     __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int,
                         uint16_t* lds) const {
-        const int table = PARTS == 1 ? 0 : *E, col = col0 + (lane & 31);
-        const float k1 = c * LOG2E;   // one part: 2^(k1 x - log2(e) lse)
+        const int table = *E, col = col0 + (lane & 31);
+        // One part: 2^(k x - log2(e) lse) with the factor log2(e) in k, one multiply-add an exponential.
+        const float c1 = GP == 1 ? c * LOG2E : c;
 #pragma unroll
         for (int a = 0; a < FM; ++a) {
-            uint16_t v[PARTS][FN][16];
+            uint16_t v[GP][FN][16];
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int row = row0 + reg_row(a, 4 * r4, lane);
                 const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + row);
-                f32x4 w4;
-                i32x4 t4, h4;
-                if constexpr (PARTS == 1) w4 = *reinterpret_cast<const f32x4*>(w + row);
-                if constexpr (PARTS == 2) h4 = *reinterpret_cast<const i32x4*>(h + row);
+                const i32x4 h4 = *reinterpret_cast<const i32x4*>(h + row);
+                i32x4 t4;
                 if constexpr (HARD) t4 = *reinterpret_cast<const i32x4*>(target + row);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float k = PARTS == 1 ? k1 : __builtin_ldexpf(c, h4[e] + table);
-                    const float l = PARTS == 1 ? l4[e] * LOG2E : l4[e];
-                    const float f = PARTS == 1 ? w4[e] : 0x1p14f;
+                    const float k = __builtin_ldexpf(c1, h4[e] + table);
+                    const float l = GP == 1 ? l4[e] * LOG2E : l4[e];
 #pragma unroll
                     for (int b = 0; b < FN; ++b) {
                         const float x = __builtin_fmaf(k, acc[a][b][4 * r4 + e], -l);
-                        float p = __builtin_amdgcn_exp2f(PARTS == 1 ? x : x * LOG2E);
+                        float p = __builtin_amdgcn_exp2f(GP == 1 ? x : x * LOG2E);
                         if constexpr (HARD)
                             if (col + 32 * b == t4[e] - v0) p -= 1.f;
-                        uint16_t parts[PARTS];
-                        to_parts<PARTS>(col + 32 * b < N ? f * p : 0.f, parts);
+                        uint16_t parts[GP];
+                        to_parts<GP>(col + 32 * b < N ? 0x1p14f * p : 0.f, parts);
 #pragma unroll
-                        for (int q = 0; q < PARTS; ++q) v[q][b][4 * r4 + e] = parts[q];
+                        for (int q = 0; q < GP; ++q) v[q][b][4 * r4 + e] = parts[q];
                     }
                 }
             }
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q)
+            for (int q = 0; q < GP; ++q)
                 store_rows<FN>(lds, v[q], row0 + 32 * a, lane, [&](int row, int cc, h8 x) {
                     if (row < M) *reinterpret_cast<h8*>(G + q * plane + (size_t)row * ldg + col0 + cc) = x;
                 });
@@ -1294,16 +1304,17 @@ struct EpiAcc {
     }
 };
 
-// A gradient's rows and their scales: dH's packed rows go to their places, times w_n 2^(E - 14) with
-// two parts; dW's stay in order, times 2^(X - 14).  One part: both times the largest weight, *w.
+// A gradient's rows and their scales: dH's packed rows go to their places, times w_n 2^(E - 14); dW's
+// stay in order, times 2^(X - 14), and wtop where w_n H_n has one part.
 template <typename OT>
 struct Grad {
     OT* C;
     int ldc, accumulate;
     const int *row, *exp;
     const float* w;
-    __device__ int scale() const { return exp ? *exp - 14 : 0; }
-    template <int PARTS> __device__ float weight(int i) const { return PARTS == 1 ? *w : w ? w[i] : 1.f; }
+    int own;               // w is the rows', else one for all
+    __device__ int scale() const { return *exp - 14; }
+    __device__ float weight(int i) const { return w ? w[own ? i : 0] : 1.f; }
     __device__ OT* at(int i) const { return C + (size_t)(row ? row[i] : i) * ldc; }
     __device__ void put(OT* to, float v) const {
         if constexpr (sizeof(OT) == 4) {
@@ -1316,24 +1327,26 @@ struct Grad {
 };
 
 // A gradient from its only split and piece.  bf16 that is not added to what is there goes through LDS.
-template <int PARTS, typename OT>
+template <typename OT>
 struct EpiOut {
     static constexpr bool LDS = sizeof(OT) == 2;
     Grad<OT> out;
     template <int FM, int FN>
     __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int,
                         uint16_t* lds) const {
+        const int s = out.scale();
         if constexpr (LDS) {
-            static_assert(PARTS == 1, "bf16 results come from one part");
             if (!out.accumulate) {
-                const float w = out.template weight<1>(0);
 #pragma unroll
                 for (int a = 0; a < FM; ++a) {
                     uint16_t v[FN][16];
 #pragma unroll
-                    for (int b = 0; b < FN; ++b)
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = row0 + reg_row(a, r, lane);
+                        const float w = row < M ? out.weight(row) : 0.f;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) v[b][r] = rne_bf16(acc[a][b][r] * w);
+                        for (int b = 0; b < FN; ++b) v[b][r] = rne_bf16(__builtin_ldexpf(acc[a][b][r], s) * w);
+                    }
                     store_rows<FN>(lds, v, row0 + 32 * a, lane, [&](int row, int cc, h8 x) {
                         if (row >= M || col0 + cc >= N) return;
                         OT* to = out.at(row) + col0 + cc;
@@ -1349,7 +1362,6 @@ struct EpiOut {
                 return;
             }
         }
-        const int s = PARTS == 1 ? 0 : out.scale();
 #pragma unroll
         for (int a = 0; a < FM; ++a)
 #pragma unroll
@@ -1357,14 +1369,12 @@ struct EpiOut {
                 const int row = row0 + reg_row(a, r, lane);
                 if (row >= M) continue;
                 OT* to = out.at(row);
-                const float w = out.template weight<PARTS>(row);
+                const float w = out.weight(row);
 #pragma unroll
                 for (int b = 0; b < FN; ++b) {
                     const int col = col0 + 32 * b + (lane & 31);
                     if (col >= N) continue;
-                    float v = acc[a][b][r];
-                    if constexpr (PARTS == 2) v = __builtin_ldexpf(v, s);
-                    out.put(to + col, v * w);
+                    out.put(to + col, __builtin_ldexpf(acc[a][b][r], s) * w);
                 }
             }
     }
@@ -1456,9 +1466,9 @@ __global__ void __launch_bounds__(256) lse_join_few(const float2* __restrict__ p
     out.put(i, m, s);
 }
 
-// The entries of G at the teacher's tokens inside a piece, from the fp32 logits: w (p - q), q
+// The entries of G at the teacher's tokens inside a piece, from the fp32 logits: p - q, q
 // summed where a token occurs more than once (each of its entries writes the same value).
-template <int PARTS>
+template <int GP>
 __global__ void __launch_bounds__(256) teacher_entries(Rows rows, Teacher t, int V, int v0, int R,
                                                        const float* __restrict__ q,
                                                        const float* __restrict__ z,
@@ -1467,18 +1477,18 @@ __global__ void __launch_bounds__(256) teacher_entries(Rows rows, Teacher t, int
     const int i = blockIdx.x;
     if (i >= *rows.cnt) return;
     const size_t at = (size_t)rows.row[i] * t.K, from = (size_t)i * t.K;
-    const float w = PARTS == 1 ? rows.w[i] : 0x1p14f, lse = rows.lse[i];
+    const float lse = rows.lse[i];
     for (int k = threadIdx.x; k < t.K; k += 256) {
         const int id = t.id[at + k];
         if (id < v0 || id >= v0 + R || !entry_counts(t, at + k, V)) continue;
         float sum = 0.f;
         for (int j = 0; j < t.K; ++j)
             if (t.id[at + j] == id) sum += q[from + j];
-        uint16_t parts[PARTS];
-        to_parts<PARTS>(w * (__expf(z[from + k] - lse) - sum), parts);
+        uint16_t parts[GP];
+        to_parts<GP>(0x1p14f * (__expf(z[from + k] - lse) - sum), parts);
         uint16_t* to = G + (size_t)i * ldg + (id - v0);
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) to[p * plane] = parts[p];
+        for (int p = 0; p < GP; ++p) to[p * plane] = parts[p];
     }
 }
 
@@ -1492,7 +1502,7 @@ struct Finish {
     const int* cnt;          // rows that count, or null: all
     long long groups;        // work-groups of 256 threads
 };
-template <int PARTS, typename OT>
+template <typename OT>
 __global__ void __launch_bounds__(256) finish(Finish<OT> h, Finish<OT> w, int D) {
     const bool second = blockIdx.x >= h.groups;
     const Finish<OT>& f = second ? w : h;
@@ -1505,12 +1515,12 @@ __global__ void __launch_bounds__(256) finish(Finish<OT> h, Finish<OT> w, int D)
 #pragma unroll 4
     for (int s = 0; s < f.splits; ++s)
         v += *reinterpret_cast<const f32x4*>(f.acc + s * f.split + (size_t)i * f.lda + c);
-    const int e = PARTS == 1 ? 0 : f.out.scale();
-    const float wi = f.out.template weight<PARTS>((int)i);
+    const int e = f.out.scale();
+    const float wi = f.out.weight((int)i);
     OT* to = f.out.at((int)i) + c;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-        if (c + q < D) f.out.put(to + q, (PARTS == 1 ? v[q] : __builtin_ldexpf(v[q], e)) * wi);
+        if (c + q < D) f.out.put(to + q, __builtin_ldexpf(v[q], e) * wi);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------
@@ -1989,12 +1999,12 @@ long long tiles_of(Kind t, long long M, long long N) {
 // afterwards: rounds of work-groups (a last round that is not full counts half of what it lacks)
 // times their 32-k stages, each of the time measured with one work-group on a CU or with as many as
 // fit; the sums of splits are written, read and cost a launch.
-double estimate(Kind t, long long M, long long N, long long K, int parts, int splits) {
+double estimate(Kind t, long long M, long long N, long long K, int kinds, int splits) {
     static const double alone[] = {1.0, 0.45, 0.19}, full[] = {1.0, 0.68, 0.30};
-    const bool both = t == T64 && parts == 2;   // gemm_both: three products a stage, one group a CU
+    const bool both = t == T64 && kinds == 3;   // gemm_both: three products a stage, one group a CU
     const int fit = t == T256 || both ? 1 : 2;
     const double groups = (double)tiles_of(t, M, N) * splits;
-    const double stages = (double)((K + 31) / 32) * (parts == 2 && !both ? 3 : 1) / splits + 4;
+    const double stages = (double)((K + 31) / 32) * (both ? 1 : kinds) / splits + 4;
     double rounds = groups / (256 * fit);
     const double whole = (double)(long long)(rounds + 0.9999);
     rounds = rounds <= 1 ? 1 : (rounds + whole) / 2;
@@ -2005,12 +2015,12 @@ struct Choice {
     Kind kind;
     int splits;
 };
-Choice pick(long long M, long long N, long long K, int parts, bool split) {
+Choice pick(long long M, long long N, long long K, int kinds, bool split) {
     Choice best{T64, 1};
-    double least = estimate(T64, M, N, K, parts, 1);
+    double least = estimate(T64, M, N, K, kinds, 1);
     for (Kind t : {T64, T128, T256})
         for (int s = 1; s <= 64 && s * 128 <= std::max(128LL, K); s = s < 8 ? s + 1 : s + 4) {
-            const double e = estimate(t, M, N, K, parts, s);
+            const double e = estimate(t, M, N, K, kinds, s);
             if (e < least) {
                 least = e;
                 best = {t, s};
@@ -2027,7 +2037,8 @@ int apart(int cols) { return cols % 256 == 0 ? cols + 64 : cols; }
 
 // The workspace: a part whose size the shapes give, and a piece whose size is what is left.
 struct Plan {
-    int parts, Kp, Dp, Nt;    // parts of an operand, padded columns, their rows' distance, padded rows
+    int parts, gparts;        // of H and W; of G and w_n H_n
+    int Kp, Dp, Nt;           // padded columns, their rows' distance, padded rows
     bool direct;              // the table is read in place
     Kind lse, g, dh, dw;      // the products' tiles
     int splits, wsplits;      // of dH and dW
@@ -2036,17 +2047,21 @@ struct Plan {
     size_t per_block;         // bytes of a piece per 256 table rows
 };
 
-Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* W, int ldw) {
+// gtype: the gradients' type, or a negative one for the forward.
+Plan make_plan(int dtype, int gtype, int N, int V, int D, int K, const void* W, int ldw) {
     Plan p{};
+    const bool backward = gtype >= 0;
     p.parts = dtype == DH_F32 ? 2 : 1;
+    p.gparts = gtype == DH_F32 ? 2 : 1;
     p.Kp = (D + 31) / 32 * 32;
     p.Dp = apart(p.Kp);
     p.Nt = (int)(((long long)N + 255) / 256 * 256);
-    // In place: whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
-    p.direct = dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
-    p.lse = pick(V, N, D, p.parts, false).kind;
-    p.g = pick(N, V, D, p.parts, false).kind;
-    const Choice dh = pick(N, D, V, p.parts, true), dw = pick(V, D, N, p.parts, true);
+    // In place (forward): whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
+    p.direct = !backward && dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
+    p.lse = pick(V, N, D, kinds_of(p.parts, p.parts), false).kind;
+    p.g = pick(N, V, D, kinds_of(p.parts, p.parts), false).kind;
+    const Choice dh = pick(N, D, V, kinds_of(p.gparts, p.parts), true),
+                 dw = pick(V, D, N, kinds_of(p.gparts, p.gparts), true);
     p.dh = dh.kind;
     p.dw = dw.kind;
     p.splits = dh.splits;
@@ -2057,7 +2072,7 @@ Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* 
         at += up256(bytes);
         return here;
     };
-    p.ints = take(((size_t)4 * p.Nt + p.Nt / PACK + 64 + SCAN) * 4);   // cnt and scales, row, target, ...
+    p.ints = take(((size_t)4 * p.Nt + 2 * (p.Nt / PACK) + 64 + SCAN) * 4);   // cnt and scales, row, target, ...
     p.w = take((size_t)p.Nt * 4);
     p.lses = take((size_t)p.Nt * 4);
     p.base = take((size_t)p.Nt * 4);
@@ -2066,8 +2081,8 @@ Plan make_plan(int dtype, int N, int V, int D, int K, int backward, const void* 
     p.Hp = take((size_t)p.parts * N * p.Dp * 2);
     if (backward) {
         p.acc = take((size_t)p.splits * N * p.Dp * 4);
-        if (p.parts == 2) p.Xp = take((size_t)p.parts * N * p.Dp * 2);
-        p.per_block = (size_t)p.parts * N * (256 + 64) * 2;
+        p.Xp = take((size_t)p.gparts * N * p.Dp * 2);
+        p.per_block = (size_t)p.gparts * N * (256 + 64) * 2;
         // dW's sums over splits of the rows: a piece's, fp32.
         if (p.wsplits > 1) p.per_block += (size_t)p.wsplits * 256 * p.Dp * 4;
     } else {
@@ -2136,8 +2151,12 @@ size_t least_ws(int dtype, int N, int V, int D, int K, int backward) {
     if (is_few(dtype, N, V, D, backward))   // whichever type the gradients have
         return std::max(few_plan(dtype, DH_F32, N, V, D, backward).total,
                         few_plan(dtype, dtype, N, V, D, backward).total);
-    const Plan p = make_plan(dtype, N, V, D, K, backward, nullptr, 1);
-    return p.piece + p.per_block + 512;
+    size_t need = 0;
+    for (int g : {(int)DH_F32, dtype}) {
+        const Plan p = make_plan(dtype, backward ? g : -1, N, V, D, K, nullptr, 1);
+        need = std::max(need, p.piece + p.per_block + 512);
+    }
+    return need;
 }
 
 // Table rows of a piece: as many blocks of 256 as fit, the same for every piece.
@@ -2185,22 +2204,24 @@ Work lay_out(const Plan& p, void* ws) {
     auto array = [&](int k) { return ints + 64 + (size_t)k * p.Nt; };
     Work w{};
     w.p = p;
-    w.rows = {ints, array(0), array(1), array(2), (float*)(b + p.w), (float*)(b + p.lses), (float*)(ints + 3)};
+    w.rows = {ints, array(0), array(1), array(2), (float*)(b + p.w), (float*)(b + p.lses)};
     w.flags = array(3);
-    w.exps = {nullptr, ints + 1, ints + 2, array(4), (float*)(array(4) + p.Nt / PACK)};
+    const int groups = p.Nt / PACK;
+    w.exps = {nullptr, ints + 1, ints + 2, (float*)(ints + 3), array(4), (float*)(array(4) + groups),
+              (float*)(array(4) + 2 * groups)};
     w.base = (float*)(b + p.base);
     w.q = (float*)(b + p.q);
     w.z = (float*)(b + p.z);
     w.state = (float2*)(b + p.state);
     w.acc = (float*)(b + p.acc);
     w.Hp = (uint16_t*)(b + p.Hp);
-    w.Xp = p.parts == 2 ? (uint16_t*)(b + p.Xp) : w.Hp;
+    w.Xp = (uint16_t*)(b + p.Xp);
     w.piece = b + p.piece;
     return w;
 }
 
 // Packs the rows; `more` work-groups of the launch stage table rows or scan the table.
-template <typename T, int PARTS>
+template <typename T, int P>
 int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
     a.targets = {h.target, h.teacher, h.V};
     if (!h.target && (h.teacher.K > 16 || (long long)h.N * h.teacher.K > 1 << 15)) {
@@ -2222,7 +2243,7 @@ int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
     a.groups = (h.N + PACK - 1) / PACK;
     a.c = h.c;
     a.wscale = h.wscale;
-    pack_rows<T, PARTS><<<a.groups + more, 1024, 0, stream()>>>(a);
+    pack_rows<T, P><<<a.groups + more, 1024, 0, stream()>>>(a);
     DH_TRY(check_launch(h.op));
     if (h.target) return DH_OK;
     // Up to 8 waves, with as few idle places in their last turn as that leaves.
@@ -2233,31 +2254,31 @@ int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
     return check_launch(h.op);
 }
 
-template <class S, bool AK, bool BK, int TOK, int PARTS, class Epi>
+template <class S, bool AK, bool BK, int TOK, int PA, int PB, class Epi>
 int launch(const char* op, Prod g, int splits, const Epi& epi) {
     const long long tiles = ((g.M + S::T - 1LL) / S::T) * ((g.N + S::T - 1LL) / S::T);
     const int bk = S::T == 256 && AK ? 64 : S::BK;   // gemm_deep counts pairs
     const int stages = (g.K + bk - 1) / bk;
     g.kstages = (stages + splits - 1) / splits;
-    vocab_gemm<S, AK, BK, TOK, PARTS, Epi><<<dim3((unsigned)tiles, splits), S::THREADS, 0, stream()>>>(g, epi);
+    vocab_gemm<S, AK, BK, TOK, PA, PB, Epi><<<dim3((unsigned)tiles, splits), S::THREADS, 0, stream()>>>(g, epi);
     return check_launch(op);
 }
-template <bool AK, bool BK, int TOK, int PARTS, class Epi>
+template <bool AK, bool BK, int TOK, int PA, int PB, class Epi>
 int product(const char* op, Kind t, const Prod& g, int splits, const Epi& epi) {
-    if (t == T256) return launch<Shape<256>, AK, BK, TOK, PARTS>(op, g, splits, epi);
-    if (t == T128) return launch<Shape<128>, AK, BK, TOK, PARTS>(op, g, splits, epi);
-    return launch<Shape<64>, AK, BK, TOK, PARTS>(op, g, splits, epi);
+    if (t == T256) return launch<Shape<256>, AK, BK, TOK, PA, PB>(op, g, splits, epi);
+    if (t == T128) return launch<Shape<128>, AK, BK, TOK, PA, PB>(op, g, splits, epi);
+    return launch<Shape<64>, AK, BK, TOK, PA, PB>(op, g, splits, epi);
 }
 
-template <typename T, int PARTS>
+template <typename T, int P>
 int forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_bytes) {
-    const Plan p = make_plan(h.dtype, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, 0, h.W, h.ldw);
+    const Plan p = make_plan(h.dtype, -1, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, h.W, h.ldw);
     Work w = lay_out(p, ws);
     const int rows = piece_rows(p, h.V, ws_bytes);
     const int wr = wave_rows(p.lse);
     float2* part = (float2*)w.piece;
     uint16_t* staged = (uint16_t*)(w.piece + (size_t)(rows / wr) * p.Nt * 8);
-    w.exps.e = (int*)(staged + (size_t)PARTS * rows * p.Dp);
+    w.exps.e = (int*)(staged + (size_t)p.parts * rows * p.Dp);
     const long long wplane = (long long)rows * p.Dp;
     Pack a{};
     a.loss = loss;
@@ -2269,7 +2290,7 @@ int forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_bytes) {
         a.staged = staged;
         a.wplane = wplane;
     }
-    DH_TRY((prepare_rows<T, PARTS>(h, w, a, a.tables)));
+    DH_TRY((prepare_rows<T, P>(h, w, a, a.tables)));
     for (int v0 = 0;; v0 += rows) {
         const int R = h.V - v0 < rows ? h.V - v0 : rows;
         const bool last = h.V - v0 <= rows;
@@ -2279,12 +2300,12 @@ int forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_bytes) {
             g.lda = h.ldw;
             g.K = h.D;
         } else if (v0 > 0) {
-            stage_table<T, PARTS><<<(R + 3) / 4, 256, 0, stream()>>>((const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp,
+            stage_table<T, P><<<(R + 3) / 4, 256, 0, stream()>>>((const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp,
                                                                     wplane, w.exps.e);
             DH_TRY(check_launch(h.op));
         }
-        DH_TRY((product<true, true, TOK_N, PARTS>(h.op, p.lse, g, 1,
-                                                  EpiLse<PARTS>{h.c, w.exps.e, w.rows.hexp, part, p.Nt})));
+        DH_TRY((product<true, true, TOK_N, P, P>(h.op, p.lse, g, 1,
+                                                  EpiLse<P>{h.c, w.exps.e, w.rows.hexp, part, p.Nt})));
         const JoinOut out{w.rows, w.state, v0 == 0, last, w.base, h.factor, loss, lse};
         const int blocks = (R + wr - 1) / wr;
         if (h.N <= 512) lse_join_few<<<h.N, 256, 0, stream()>>>(part, p.Nt, blocks, out);
@@ -2303,7 +2324,7 @@ struct Grads {
 };
 
 // dH and dW of a piece, in one launch where both take the same small tile.
-template <int PARTS, class EpiH, class EpiW>
+template <int P, int GP, class EpiH, class EpiW>
 int gradients(const char* op, const Plan& p, const Prod* gh, const EpiH& eh, const Prod* gw, const EpiW& ew) {
     if (gh && gw && p.dh == T64 && p.dw == T64) {
         using S = Shape<64>;
@@ -2312,19 +2333,20 @@ int gradients(const char* op, const Plan& p, const Prod* gh, const EpiH& eh, con
         a.kstages = per(a.K, p.splits);
         b.kstages = per(b.K, p.wsplits);
         const long long th = tiles_of(p.dh, a.M, a.N), tw = tiles_of(p.dw, b.M, b.N);
-        vocab_grads<S, PARTS, EpiH, EpiW>
+        vocab_grads<S, P, GP, EpiH, EpiW>
             <<<(unsigned)(th * p.splits + tw * p.wsplits), S::THREADS, 0, stream()>>>(
                 a, eh, (int)th, (int)(th * p.splits), b, ew, (int)tw);
         return check_launch(op);
     }
-    if (gh) DH_TRY((product<true, false, TOK_M, PARTS>(op, p.dh, *gh, p.splits, eh)));
-    if (gw) DH_TRY((product<false, false, TOK_K, PARTS>(op, p.dw, *gw, p.wsplits, ew)));
+    if (gh) DH_TRY((product<true, false, TOK_M, GP, P>(op, p.dh, *gh, p.splits, eh)));
+    if (gw) DH_TRY((product<false, false, TOK_K, GP, GP>(op, p.dw, *gw, p.wsplits, ew)));
     return DH_OK;
 }
 
-template <typename T, int PARTS, typename OT>
+// P parts of H and W, GP of G and w_n H_n.
+template <typename T, int P, int GP, typename OT>
 int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
-    Plan p = make_plan(h.dtype, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, 1, h.W, h.ldw);
+    const Plan p = make_plan(h.dtype, d.type, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, h.W, h.ldw);
     Work w = lay_out(p, ws);
     const int rows = piece_rows(p, h.V, ws_bytes);
     const bool one = h.V <= rows;   // a single piece
@@ -2332,7 +2354,7 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     uint16_t* G = (uint16_t*)w.piece;
     const int ldg = apart(rows);
     const long long gplane = (long long)h.N * ldg;
-    float* wacc = (float*)(G + PARTS * gplane);
+    float* wacc = (float*)(G + GP * gplane);
     uint16_t* staged = (uint16_t*)(wacc + (p.wsplits > 1 ? p.wsplits * wplane : 0));
     Pack a{};
     a.lse_in = d.lse;
@@ -2342,73 +2364,50 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         a.lddh = d.lddh;
         a.dh_f32 = d.type == DH_F32;
     }
-    int more = 0, scan = 0;
-    if (PARTS == 2) {
-        scan = more = h.V < 16 * SCAN ? (h.V + 15) / 16 : SCAN;
-    } else if (!p.direct) {
-        a.R = one ? h.V : rows;
-        more = a.tables = (a.R + 15) / 16;
-        a.staged = staged;
-        a.wplane = wplane;
-    }
-    DH_TRY((prepare_rows<T, PARTS>(h, w, a, more)));
-    const Grad<OT> to_dH{(OT*)d.dH, d.lddh, d.acc_dH, w.rows.row, PARTS == 2 ? w.exps.E : nullptr,
-                         PARTS == 2 ? w.rows.w : w.rows.wtop};
+    const int scan = h.V < 16 * SCAN ? (h.V + 15) / 16 : SCAN;
+    DH_TRY((prepare_rows<T, P>(h, w, a, scan)));
+    const Grad<OT> to_dH{(OT*)d.dH, d.lddh, d.acc_dH, w.rows.row, w.exps.E, w.rows.w, 1};
     for (int v0 = 0;; v0 += rows) {
         const int R = h.V - v0 < rows ? h.V - v0 : rows;
         const bool last = h.V - v0 <= rows;
-        const uint16_t* W = staged;
-        int ldw = p.Dp, K = p.Kp;
-        if (p.direct) {
-            W = (const uint16_t*)h.W + (size_t)v0 * h.ldw;
-            ldw = h.ldw;
-            K = h.D;
-        } else if (PARTS == 2) {
-            const int tables = (R + 3) / 4;
-            stage_scaled<<<tables + (v0 == 0 ? (h.N + 3) / 4 : 0), 256, 0, stream()>>>(
-                (const float*)h.W, h.ldw, v0, R, h.D, staged, p.Dp, wplane, w.exps, (h.N + PACK - 1) / PACK,
-                scan, tables, w.rows, (const float*)h.H, h.ldh, w.Xp, hplane);
-            DH_TRY(check_launch(h.op));
-        } else if (v0 > 0) {
-            stage_table<T, PARTS><<<(R + 3) / 4, 256, 0, stream()>>>((const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp,
-                                                                    wplane, nullptr);
-            DH_TRY(check_launch(h.op));
-        }
-        const Prod g{w.Hp, W, p.Dp, ldw, hplane, wplane, h.N, R, K, 0, w.rows.cnt};
+        const int tables = (R + 3) / 4;
+        stage_scaled<T, P, GP><<<tables + (v0 == 0 ? (h.N + 3) / 4 : 0), 256, 0, stream()>>>(
+            (const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp, wplane, w.exps, (h.N + PACK - 1) / PACK, scan, tables,
+            w.rows, (const T*)h.H, h.ldh, w.Xp, hplane);
+        DH_TRY(check_launch(h.op));
+        const Prod g{w.Hp, staged, p.Dp, p.Dp, hplane, wplane, h.N, R, p.Kp, 0, w.rows.cnt};
         if (h.target) {
-            DH_TRY((product<true, true, TOK_M, PARTS>(
+            DH_TRY((product<true, true, TOK_M, P, P>(
                 h.op, p.g, g, 1,
-                EpiG<PARTS, true>{h.c, w.rows.lse, w.rows.w, w.rows.target, w.rows.hexp, w.exps.E, v0, G, ldg,
-                                  gplane})));
+                EpiG<GP, true>{h.c, w.rows.lse, w.rows.target, w.rows.hexp, w.exps.E, v0, G, ldg, gplane})));
         } else {
-            DH_TRY((product<true, true, TOK_M, PARTS>(
+            DH_TRY((product<true, true, TOK_M, P, P>(
                 h.op, p.g, g, 1,
-                EpiG<PARTS, false>{h.c, w.rows.lse, w.rows.w, nullptr, w.rows.hexp, w.exps.E, v0, G, ldg,
-                                   gplane})));
-            teacher_entries<PARTS><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, ldg,
-                                                              gplane);
+                EpiG<GP, false>{h.c, w.rows.lse, nullptr, w.rows.hexp, w.exps.E, v0, G, ldg, gplane})));
+            teacher_entries<GP><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, ldg,
+                                                           gplane);
             DH_TRY(check_launch(h.op));
         }
-        const Prod gh{G, W, ldg, ldw, gplane, wplane, h.N, h.D, R, 0, w.rows.cnt};
+        const Prod gh{G, staged, ldg, p.Dp, gplane, wplane, h.N, h.D, R, 0, w.rows.cnt};
         const Prod gw{G, w.Xp, ldg, p.Dp, gplane, hplane, R, h.D, h.N, 0, w.rows.cnt};
         const Prod *ph = d.dH ? &gh : nullptr, *pw = d.dW ? &gw : nullptr;
-        const Grad<OT> to_dW{d.dW ? (OT*)d.dW + (size_t)v0 * d.lddw : nullptr, d.lddw, d.acc_dW, nullptr,
-                             PARTS == 2 ? w.exps.X : nullptr, PARTS == 2 ? nullptr : w.rows.wtop};
+        const Grad<OT> to_dW{d.dW ? (OT*)d.dW + (size_t)v0 * d.lddw : nullptr, d.lddw, d.acc_dW, nullptr, w.exps.X,
+                             GP == 1 ? w.exps.wtop : nullptr, 0};
         // Straight to the gradient, or as sums that the last launch adds.
         const bool direct_h = one && p.splits == 1, direct_w = p.wsplits == 1;
         const EpiAcc sum_h{w.acc, p.Dp, v0 == 0, hplane}, sum_w{wacc, p.Dp, 1, wplane};
-        const EpiOut<PARTS, OT> out_h{to_dH}, out_w{to_dW};
-        if (direct_h && direct_w) DH_TRY((gradients<PARTS>(h.op, p, ph, out_h, pw, out_w)));
-        else if (direct_h) DH_TRY((gradients<PARTS>(h.op, p, ph, out_h, pw, sum_w)));
-        else if (direct_w) DH_TRY((gradients<PARTS>(h.op, p, ph, sum_h, pw, out_w)));
-        else DH_TRY((gradients<PARTS>(h.op, p, ph, sum_h, pw, sum_w)));
+        const EpiOut<OT> out_h{to_dH}, out_w{to_dW};
+        if (direct_h && direct_w) DH_TRY((gradients<P, GP>(h.op, p, ph, out_h, pw, out_w)));
+        else if (direct_h) DH_TRY((gradients<P, GP>(h.op, p, ph, out_h, pw, sum_w)));
+        else if (direct_w) DH_TRY((gradients<P, GP>(h.op, p, ph, sum_h, pw, out_w)));
+        else DH_TRY((gradients<P, GP>(h.op, p, ph, sum_h, pw, sum_w)));
         Finish<OT> fh{to_dH, w.acc, h.N, p.Dp, p.splits, hplane, w.rows.cnt, 0};
         Finish<OT> fw{to_dW, wacc, R, p.Dp, p.wsplits, wplane, nullptr, 0};
         auto groups = [&](long long rows_) { return (rows_ * ((h.D + 3) / 4) + 255) / 256; };
         if (ph && last && !direct_h) fh.groups = groups(h.N);
         if (pw && !direct_w) fw.groups = groups(R);
         if (fh.groups + fw.groups > 0) {
-            finish<PARTS, OT><<<(unsigned)(fh.groups + fw.groups), 256, 0, stream()>>>(fh, fw, h.D);
+            finish<OT><<<(unsigned)(fh.groups + fw.groups), 256, 0, stream()>>>(fh, fw, h.D);
             DH_TRY(check_launch(h.op));
         }
         if (last) return DH_OK;
@@ -2483,14 +2482,14 @@ int few_backward(const Head& h, const Grads& d, void* ws) {
         few_teacher<<<h.N, 256, 0, stream()>>>(f);
         DH_TRY(check_launch(h.op));
     }
-    const Grad<OT> dW{(OT*)d.dW, d.lddw, d.acc_dW, nullptr, nullptr, nullptr};
+    const Grad<OT> dW{(OT*)d.dW, d.lddw, d.acc_dW, nullptr, nullptr, nullptr, 0};
     const int wblocks = d.dW ? (h.V + p.wrows - 1) / p.wrows * p.wslabs : 0;
     auto grads = h.N <= 4 ? few_grads<T, OT, 4> : h.N <= 8 ? few_grads<T, OT, 8> : few_grads<T, OT, 16>;
     grads<<<f.hblocks + wblocks, 256, 0, stream()>>>(f, f.G, dW);
     DH_TRY(check_launch(h.op));
     if (!d.dH) return DH_OK;
     few_finish<OT><<<dim3((h.D + 63) / 64, h.N), 1024, 0, stream()>>>(
-        f, Grad<OT>{(OT*)d.dH, d.lddh, d.acc_dH, nullptr, nullptr, nullptr});
+        f, Grad<OT>{(OT*)d.dH, d.lddh, d.acc_dH, nullptr, nullptr, nullptr, 0});
     return check_launch(h.op);
 }
 
@@ -2504,7 +2503,7 @@ int run_forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_byte
     if (is_few(h.dtype, h.N, h.V, h.D, 0))
         return h.dtype == DH_F32 ? few_forward<float>(h, loss, lse, ws) : few_forward<uint16_t>(h, loss, lse, ws);
     return h.dtype == DH_F32 ? forward<float, 2>(h, loss, lse, ws, ws_bytes)
-                             : forward<uint16_t, 1>(h, loss, lse, ws, ws_bytes);
+                             : forward<uint16_t, BF>(h, loss, lse, ws, ws_bytes);
 }
 
 int run_backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
@@ -2531,9 +2530,9 @@ int run_backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         return d.type == DH_F32 ? few_backward<uint16_t, float>(h, d, ws)
                                 : few_backward<uint16_t, uint16_t>(h, d, ws);
     }
-    if (h.dtype == DH_F32) return backward<float, 2, float>(h, d, ws, ws_bytes);
-    return d.type == DH_F32 ? backward<uint16_t, 1, float>(h, d, ws, ws_bytes)
-                            : backward<uint16_t, 1, uint16_t>(h, d, ws, ws_bytes);
+    if (h.dtype == DH_F32) return backward<float, 2, 2, float>(h, d, ws, ws_bytes);
+    return d.type == DH_F32 ? backward<uint16_t, 1, 2, float>(h, d, ws, ws_bytes)
+                            : backward<uint16_t, 1, 1, uint16_t>(h, d, ws, ws_bytes);
 }
 
 Head xent_head(const char* op, int dtype, int N, int V, int D, float scale, const void* H, int ldh,
