@@ -2100,13 +2100,12 @@ Plan make_plan(int dtype, int gtype, int N, int V, int D, int K, const void* W, 
 //                                16 x 50001 x 1001 48 / 60, 1 x 131072 x 2048 107 / 115
 //   forward, up to 2 FEW, fp32   as there the table would be staged: 18 x 41216 x 2357 155 / 248; bf16 tables
 //                                are read in place or cheap to stage: 32 x 50001 x 1001 63 / 60
-//   gradient, fp32               with its forward 16 x 32000 x 1024 111 / 240
-//   gradient, bf16               up to 4 rows (4 x 50001 x 1000 109 / 113, x 1001 153 / 175; 4 x 131072 x 2048
-//                                557 / 503) or up to 2^22 table values (16 x 8000 x 512 37 / 37, 16 x 1000 x
-//                                1024 24 / 34); beyond, fp32 multiply-adds bound it: 16 x 50001 x 1000 180 / 117
-bool is_few(int dtype, int N, int V, int D, int backward) {
-    if (V > FEW_MAX_V || N > (dtype == DH_F32 && !backward ? 2 * FEW : FEW)) return false;
-    return dtype == DH_F32 || !backward || N <= 4 || (long long)V * D <= 1 << 22;
+//   gradient, up to FEW rows     with its forward fp32 16 x 32000 x 1024 111 / 240; bf16 4 x 131072 x 2048 560 / 825,
+//                                16 x 131072 x 2048 738 / 835, 16 x 50001 x 1000 183 / 179, x 1001 250 / 202, 16 x
+//                                8000 x 512 38 / 50; bf16 inputs with fp32 gradients 16 x 131072 x 2048 803 / 1056.
+//                                Its G is fp32 for any of them: a row more or less does not change how exact they are.
+bool is_few(int dtype, int N, int V, int backward) {
+    return V <= FEW_MAX_V && N <= (dtype == DH_F32 && !backward ? 2 * FEW : FEW);
 }
 
 struct FewPlan {
@@ -2148,7 +2147,7 @@ FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int backward) {
 
 // The workspace that serves any alignment of the operands (staged tables take more).
 size_t least_ws(int dtype, int N, int V, int D, int K, int backward) {
-    if (is_few(dtype, N, V, D, backward))   // whichever type the gradients have
+    if (is_few(dtype, N, V, backward))   // whichever type the gradients have
         return std::max(few_plan(dtype, DH_F32, N, V, D, backward).total,
                         few_plan(dtype, dtype, N, V, D, backward).total);
     size_t need = 0;
@@ -2500,7 +2499,7 @@ int run_forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_byte
         return set_error(DH_ERR_INVALID, "%s: null pointer", h.op);
     DH_TRY(ensure_init());
     if (h.N == 0) return DH_OK;
-    if (is_few(h.dtype, h.N, h.V, h.D, 0))
+    if (is_few(h.dtype, h.N, h.V, 0))
         return h.dtype == DH_F32 ? few_forward<float>(h, loss, lse, ws) : few_forward<uint16_t>(h, loss, lse, ws);
     return h.dtype == DH_F32 ? forward<float, 2>(h, loss, lse, ws, ws_bytes)
                              : forward<uint16_t, BF>(h, loss, lse, ws, ws_bytes);
@@ -2525,7 +2524,7 @@ int run_backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
             clear_rows<<<2048, 256, 0, stream()>>>((uint16_t*)d.dW, h.V, h.D, d.lddw);
         return check_launch(h.op);
     }
-    if (is_few(h.dtype, h.N, h.V, h.D, 1)) {
+    if (is_few(h.dtype, h.N, h.V, 1)) {
         if (h.dtype == DH_F32) return few_backward<float, float>(h, d, ws);
         return d.type == DH_F32 ? few_backward<uint16_t, float>(h, d, ws)
                                 : few_backward<uint16_t, uint16_t>(h, d, ws);

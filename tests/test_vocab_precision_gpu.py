@@ -48,8 +48,8 @@ def sizes(c, lse, grad):
     return (dH, P.T @ H[k]), [FLOOR[grad] * x + 2.0 ** -126 for x in low]
 
 
-def check(c, grad, accumulate=False, extra=0):
-    """All four results to the bounds above."""
+def check(c, grad, accumulate=False, extra=0, part=2.0 ** -10):
+    """All four results to the bounds above; `part` is what one part of G and of w H loses."""
     dH, dW, loss, lse, old = gradients(c, grad, accumulate, extra)
     ref = c.ref()
     close(loss, ref[0], F32_TOL, floor=1.0)
@@ -58,7 +58,7 @@ def check(c, grad, accumulate=False, extra=0):
         want = want + add
         bound = F32_TOL * S + 2.0 ** -23 * np.abs(want) + low
         if grad == "bf16":
-            bound = 2.0 ** -8 * np.abs(want) + (1 + 2.0 ** -8) * (bound + 2.0 ** -10 * S)
+            bound = 2.0 ** -8 * np.abs(want) + (1 + 2.0 ** -8) * (bound + part * S)
         off = np.abs(got - want)
         worst = np.unravel_index(np.argmax(off / bound), off.shape)
         assert np.isfinite(got).all() and (off <= bound).all(), (name, worst, off[worst], bound[worst])
@@ -79,6 +79,13 @@ def test_gradients_do_not_get_coarser_with_a_row_more(N):
     """Over a table of more than 2^22 values."""
     check(Loss(N, 70000, 64, "bf16"), "f32")
     check(Loss(N, 70000, 64, "bf16"), "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 4, 5, 16])
+@pytest.mark.parametrize("V,D", [(300, 64), (70000, 64)])
+def test_few_rows_keep_G_in_floats(N, V, D):
+    check(Loss(N, V, D, "bf16", seed=1), "bf16", part=0.0)
 
 
 @pytest.mark.gpu
