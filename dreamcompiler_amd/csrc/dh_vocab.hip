@@ -35,6 +35,7 @@
 
 #include "dh_common.hpp"
 #include "dh_gemm_bf16.hpp"
+#include "dh_vocab_range.hpp"
 
 namespace dh {
 namespace {
@@ -561,9 +562,9 @@ enum { TOK_M, TOK_N, TOK_K };
 //        a fragment is one 16-byte read
 //   else [BK k][T]: chunk c of row k at c ^ 4 (k % 4), for T = 64 (two rows in the 64 banks)
 //        c ^ 4 (k / 2 % 2); a fragment is two transposing reads
-// Loads go through a buffer resource whose range ends with the operand's rows, so what lies behind
-// them reads as zero; it begins with the tile (KC; the stage's place in the rows is a scalar
-// offset) or with the stage, so operands of any size keep 32-bit offsets.
+// Loads go through a buffer resource whose range ends with the operand's last column of the last row
+// (dh_vocab_range.hpp), so what lies behind reads as zero; it begins with the tile (KC; the stage's place in
+// the rows is a scalar offset) or with the stage, so operands of any size keep 32-bit offsets.
 template <bool KC, int T, int BK, int WAVES>
 struct Operand {
     static constexpr int PER = T * BK / 512 / WAVES;   // blocks per wave
@@ -574,7 +575,8 @@ struct Operand {
     uint32_t soff;
     const uint16_t* base;          // the tile's first element
     long long plane;
-    int ld, K, rows;               // rows: of the tile (KC), or its first column
+    int ld, K, rows;               // rows: of the tile (KC)
+    int t0, extent;
 
     __device__ static int swizzle(int r) {
         if (KC) return BK == 32 ? (r >> 2) & 3 : (r >> 1) & 7;
@@ -584,13 +586,15 @@ struct Operand {
     __device__ static int chunk_of(int t, int wave, int lane) {
         return (lane % CPR) ^ swizzle(row_of(t, wave, lane));
     }
-    __device__ void init(const uint16_t* p, long long plane_, int ld_, int t0, int extent, int K_, int wave,
+    __device__ void init(const uint16_t* p, long long plane_, int ld_, int t0_, int extent_, int K_, int wave,
                          int lane) {
         ld = ld_;
         K = K_;
+        t0 = t0_;
+        extent = extent_;
         plane = plane_;
         base = KC ? p + (size_t)t0 * ld : p + t0;
-        rows = KC ? min(extent - t0, T) : t0;
+        rows = min(extent - t0, T);
 #pragma unroll
         for (int t = 0; t < PER; ++t)
             off[t] = 2u * ((uint32_t)row_of(t, wave, lane) * ld + 8 * chunk_of(t, wave, lane));
@@ -598,7 +602,7 @@ struct Operand {
     // Stage kt of a part is the next one.
     __device__ void start(int part, int kt) {
         rs = make_rsrc(base + part * plane + (KC ? 0 : (size_t)kt * BK * ld),
-                       2u * (KC ? (uint32_t)rows * ld : (uint32_t)(BK * ld - rows)));
+                       KC ? range_bytes(rows, ld, K, 0) : range_bytes(BK, ld, extent, t0));
 #pragma unroll
         for (int e = 0; e < 4; ++e) rs[e] = __builtin_amdgcn_readfirstlane(rs[e]);
         soff = __builtin_amdgcn_readfirstlane(KC ? 2u * BK * kt : 0u);
@@ -613,11 +617,11 @@ struct Operand {
         }
     }
     __device__ void issue_one(uint32_t to, int t) const { lds_dma16_buf_so(off[t], rs, soff, to + 1024u * t); }
-    // Of a stage kt that ends behind K: zeros from there on (KC: K is a multiple of 8).
+    // Of a stage kt that ends behind K: zeros from there on (KC: by whole chunks).
     __device__ void issue_end(uint32_t to, int t, int kt, int wave, int lane) const {
         const int left = K - BK * kt;
         u32x4 r = rs;
-        if (!KC) r[2] = left <= 0 ? 0u : 2u * (uint32_t)(left * ld - rows);
+        if (!KC) r[2] = range_bytes(min(left, BK), ld, extent, t0);
         lds_dma16_buf_so(!KC || 8 * chunk_of(t, wave, lane) < left ? off[t] : 0xFFFFFFF0u, r, soff, to + 1024u * t);
     }
     // Tile rows o .. o + 31, 16-k step kk of the stage.
