@@ -34,7 +34,6 @@
 #include <type_traits>
 
 #include "dh_common.hpp"
-#include "dh_gemm_bf16.hpp"
 #include "dh_vocab_range.hpp"
 
 namespace dh {
