@@ -196,6 +196,14 @@ __device__ inline uint32_t lds_addr(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
+// Between a wave's LDS stores and its reads of what other lanes stored (or the other way round).  The
+// accesses of a wave run in program order; this keeps the compiler to that order too, without an instruction.
+__device__ inline void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // N consecutive floats from p (16-byte loads for N a multiple of 4, one 8-byte load for 2;
 // p aligned to match).
 template <int N>

@@ -310,10 +310,10 @@ __device__ inline void tile_ranks(const int (&digit)[ITEMS], int bits, uint16_t 
             const int c = cnt[w][digit[j]];
             rank[j] = c + before;
             // the wave's lanes have read the count before its first peer raises it
-            __builtin_amdgcn_wave_barrier();
+            wave_fence();
             if (before == 0) cnt[w][digit[j]] = (uint16_t)(c + __popcll(peers));
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_fence();
     }
     __syncthreads();
     // Per digit: exclusive counts over the waves, then exclusive over the digits (512 threads).

@@ -688,6 +688,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // 32 rows of a wave's tile of 16-bit values through its piece of LDS, so that they are written as
 // 16-byte pieces of rows: element by element (a lane has one column of 16 rows) the stores of a 256 x 256
 // tile took 38 us, as much as 40 of its stages.  put(row, chunk column, 8 values) writes a piece.
+// The lanes read what others stored, and the next 32 rows go into the same LDS: fences before both.
 constexpr int LDS_TILE = 32 * (64 + 8);   // elements; rows 16 bytes longer, so that the halves' banks differ
 template <int FN, class Put>
 __device__ inline void store_rows(uint16_t* lds, const uint16_t (&v)[FN][16], int row0, int lane, const Put& put) {
@@ -696,11 +697,13 @@ __device__ inline void store_rows(uint16_t* lds, const uint16_t (&v)[FN][16], in
     for (int b = 0; b < FN; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) lds[reg_row(0, r, lane) * LD + 32 * b + (lane & 31)] = v[b][r];
+    wave_fence();
 #pragma unroll
     for (int i = 0; i < 32 * CHUNKS / 64; ++i) {
         const int r = 64 / CHUNKS * i + lane / CHUNKS, c = 8 * (lane % CHUNKS);
         put(row0 + r, c, *reinterpret_cast<const h8*>(lds + r * LD + c));
     }
+    wave_fence();
 }
 
 // One tile of one split: stages of BK k through a ring of four in LDS filled by direct DMA three
