@@ -19,14 +19,14 @@
 // operands as they are.  Every other operand is scaled by a power of two and held in fp16 parts of 11
 // significant bits, one or two, x = hi + 2^-11 lo; a product of two by two is 2^-11 (lo hi + hi lo) +
 // hi hi: the cross products are added first, the accumulators scaled by 2^-11 (exactly), then the
-// third is added (lo lo is left out).  Three 16-bit products at 16 times the rate of an fp32 one.
+// third is added (lo lo, at most 2^-22 of the product, is left out).  Three 16-bit products at 16 times the rate of an fp32 one.
 //   fp32 inputs            two parts of all operands
 //   bf16, gradients bf16   one part: H and W fit exactly, G and w_n H_n are rounded to 11 bits, whose
 //                          2^-11 is an eighth of the result's own rounding (to bf16 G would lose as much
 //                          as the result does, and at the targets in one direction); as many products
 //   bf16, gradients fp32   one part of H and W, two of G and w_n H_n: 1, 2 and 3 products
 // With the operand's largest value scaled below 2^15, the others are taken to 2^-23 (one part: 2^-11) of
-// themselves or 2^-51 (2^-39) of it, whichever is more.  What the scale is common to: a row
+// themselves or 2^-50 (2^-39) of it, whichever is more.  What the scale is common to: a row
 // where k runs along the row (H, and W in the forward), else all of the operand (W in the
 // backward, where its rows are summed over; G, whose entries are p - q; and w_n H_n, the other
 // operand of dW).

@@ -334,9 +334,10 @@ int dh_unary(int op, int dtype, const void* d_A, void* d_C, size_t n, double lo,
  * query says (the losses take larger pieces of the vocabulary out of more, which is faster); no
  * call here allocates, so all of them can be captured.  Calls that may overlap in time, two
  * captured graphs among them, need workspaces of their own; nothing is kept there between calls.
- * The losses take an fp32 operand to 2^-23 of itself or 2^-51 of the largest value of its row
- * (forward) or of its matrix (gradients), whichever is more, and softmax - q to 2^-23 of itself or
- * 2^-51.
+ * The losses take an fp32 operand to 2^-23 of itself or 2^-50 of the largest value of its row
+ * (forward) or of its matrix (gradients), whichever is more, softmax - q to 2^-23 of itself or 2^-50,
+ * and a product of two fp32 operands to 2^-21 of itself.  bf16 operands are exact in the forward, and in the
+ * gradients above 2^-32 of their matrix's largest value (below it to 2^-39 of that).
  * Deterministic: no floating-point atomics.
  *
  * Y[n] = scale W[id[n]] for N tokens. */
@@ -358,7 +359,7 @@ int dh_linear_xent_fwd(int dtype, int N, int V, int D, float scale, const void* 
 /* Its gradient from the forward's lse: G = dloss[n] scale (softmax(z) - onehot(target)),
  * dH = G W, dW = G^T H.  d_dloss (N, fp32) may be NULL: ones.  d_dH or d_dW may be NULL: not
  * computed.  acc_dH / acc_dW add into them.  bf16 gradients: softmax - onehot and the rows of
- * dloss H are taken to 2^-11 of themselves, or 2^-39 (of 1, and of the largest), before the products:
+ * dloss H are taken to 2^-11 of themselves, or 2^-38 (of 1, and of the largest), before the products:
  * an eighth of the result's own rounding.  DH_F32 gradients of bf16 inputs are as exact as those of fp32
  * inputs, for twice the products.
  * dH must not overlap H, nor dW W. */

@@ -138,3 +138,18 @@ def test_gradients_of_operands_of_any_scale(k):
     c.Wb, c.W = store(np.ldexp(c.W, -k), "bf16")
     for grad in ("f32", "bf16"):
         check(c, grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,V,D", [(70, 1000, 100), (40, 300, 1030)])
+def test_products_whose_low_parts_all_add_up(N, V, D):
+    """Every operand 2^e (1 + 2^-11): its high part is 2^e, and the product of the low parts, 2^-22 of each term and
+    the one that is left out, has one sign in all of them.  2^-22 of a logit of 20 is 5e-6, within what fp32 results
+    are held to."""
+    c = Loss(N, V, D, "f32", seed=2)
+    r = np.random.default_rng(1)
+    one = 1 + 2.0 ** -11
+    c.Hb, c.H = store(np.ldexp(one, r.integers(-3, 1, (N, D))), "f32")
+    c.Wb, c.W = store(np.ldexp(one, r.integers(-3, 1, (V, 1)) * np.ones((1, D), int) - int(np.log2(D)) + 4), "f32")
+    assert 5 < (c.H @ c.W.T).max() < 25
+    check(c, "f32")
