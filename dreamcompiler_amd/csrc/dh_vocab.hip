@@ -2036,15 +2036,10 @@ Choice pick(long long M, long long N, long long K, int kinds, bool split) {
     return best;
 }
 
-// The distance of rows of `cols` 16-bit values in the workspace: a half line more than a multiple of
-// 512 bytes would be, as rows at such distances lie in few of the memory's channels and sets, and a
-// tile's stage reads a piece of each of its rows.
-int apart(int cols) { return cols % 256 == 0 ? cols + 64 : cols; }
-
 // The workspace: a part whose size the shapes give, and a piece whose size is what is left.
 struct Plan {
     int parts, gparts;        // of H and W; of G and w_n H_n
-    int Kp, Dp, Nt;           // padded columns, their rows' distance, padded rows
+    int Dp, Nt;               // columns and rows as the workspace holds them
     bool direct;              // the table is read in place
     Kind lse, g, dh, dw;      // the products' tiles
     int splits, wsplits;      // of dH and dW
@@ -2059,8 +2054,7 @@ Plan make_plan(int dtype, int gtype, int N, int V, int D, int K, const void* W, 
     const bool backward = gtype >= 0;
     p.parts = dtype == DH_F32 ? 2 : 1;
     p.gparts = gtype == DH_F32 ? 2 : 1;
-    p.Kp = (D + 31) / 32 * 32;
-    p.Dp = apart(p.Kp);
+    p.Dp = (D + 31) / 32 * 32;
     p.Nt = (int)(((long long)N + 255) / 256 * 256);
     // In place (forward): whole 16-byte chunks at aligned addresses, 256 rows within 32-bit offsets.
     p.direct = !backward && dtype == DH_BF16 && D % 8 == 0 && ldw % 8 == 0 && ldw <= 1 << 22 && ((uintptr_t)W & 15) == 0;
@@ -2088,7 +2082,7 @@ Plan make_plan(int dtype, int gtype, int N, int V, int D, int K, const void* W, 
     if (backward) {
         p.acc = take((size_t)p.splits * N * p.Dp * 4);
         p.Xp = take((size_t)p.gparts * N * p.Dp * 2);
-        p.per_block = (size_t)p.gparts * N * (256 + 64) * 2;
+        p.per_block = (size_t)p.gparts * N * 256 * 2;
         // dW's sums over splits of the rows: a piece's, fp32.
         if (p.wsplits > 1) p.per_block += (size_t)p.wsplits * 256 * p.Dp * 4;
     } else {
@@ -2299,7 +2293,7 @@ int forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_bytes) {
     for (int v0 = 0;; v0 += rows) {
         const int R = h.V - v0 < rows ? h.V - v0 : rows;
         const bool last = h.V - v0 <= rows;
-        Prod g{staged, w.Hp, p.Dp, p.Dp, wplane, (long long)h.N * p.Dp, R, h.N, p.Kp, 0, w.rows.cnt};
+        Prod g{staged, w.Hp, p.Dp, p.Dp, wplane, (long long)h.N * p.Dp, R, h.N, p.Dp, 0, w.rows.cnt};
         if (p.direct) {
             g.A = (const uint16_t*)h.W + (size_t)v0 * h.ldw;
             g.lda = h.ldw;
@@ -2357,8 +2351,7 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     const bool one = h.V <= rows;   // a single piece
     const long long hplane = (long long)h.N * p.Dp, wplane = (long long)rows * p.Dp;
     uint16_t* G = (uint16_t*)w.piece;
-    const int ldg = apart(rows);
-    const long long gplane = (long long)h.N * ldg;
+    const long long gplane = (long long)h.N * rows;
     float* wacc = (float*)(G + GP * gplane);
     uint16_t* staged = (uint16_t*)(wacc + (p.wsplits > 1 ? p.wsplits * wplane : 0));
     Pack a{};
@@ -2380,21 +2373,21 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
             (const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp, wplane, w.exps, (h.N + PACK - 1) / PACK, scan, tables,
             w.rows, (const T*)h.H, h.ldh, w.Xp, hplane);
         DH_TRY(check_launch(h.op));
-        const Prod g{w.Hp, staged, p.Dp, p.Dp, hplane, wplane, h.N, R, p.Kp, 0, w.rows.cnt};
+        const Prod g{w.Hp, staged, p.Dp, p.Dp, hplane, wplane, h.N, R, p.Dp, 0, w.rows.cnt};
         if (h.target) {
             DH_TRY((product<true, true, TOK_M, P, P>(
                 h.op, p.g, g, 1,
-                EpiG<GP, true>{h.c, w.rows.lse, w.rows.target, w.rows.hexp, w.exps.E, v0, G, ldg, gplane})));
+                EpiG<GP, true>{h.c, w.rows.lse, w.rows.target, w.rows.hexp, w.exps.E, v0, G, rows, gplane})));
         } else {
             DH_TRY((product<true, true, TOK_M, P, P>(
                 h.op, p.g, g, 1,
-                EpiG<GP, false>{h.c, w.rows.lse, nullptr, w.rows.hexp, w.exps.E, v0, G, ldg, gplane})));
-            teacher_entries<GP><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, ldg,
+                EpiG<GP, false>{h.c, w.rows.lse, nullptr, w.rows.hexp, w.exps.E, v0, G, rows, gplane})));
+            teacher_entries<GP><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, rows,
                                                            gplane);
             DH_TRY(check_launch(h.op));
         }
-        const Prod gh{G, staged, ldg, p.Dp, gplane, wplane, h.N, h.D, R, 0, w.rows.cnt};
-        const Prod gw{G, w.Xp, ldg, p.Dp, gplane, hplane, R, h.D, h.N, 0, w.rows.cnt};
+        const Prod gh{G, staged, rows, p.Dp, gplane, wplane, h.N, h.D, R, 0, w.rows.cnt};
+        const Prod gw{G, w.Xp, rows, p.Dp, gplane, hplane, R, h.D, h.N, 0, w.rows.cnt};
         const Prod *ph = d.dH ? &gh : nullptr, *pw = d.dW ? &gw : nullptr;
         const Grad<OT> to_dW{d.dW ? (OT*)d.dW + (size_t)v0 * d.lddw : nullptr, d.lddw, d.acc_dW, nullptr, w.exps.X,
                              GP == 1 ? w.exps.wtop : nullptr, 0};
