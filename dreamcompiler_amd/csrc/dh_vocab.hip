@@ -269,6 +269,7 @@ struct Pack {
     Rows rows;
     Exps exps;
     int groups;              // of PACK rows
+    const int* counts;       // of count_rows, or null
     float c;
     // forward
     float *loss, *lse_out, *base;
@@ -284,6 +285,22 @@ struct Pack {
     long long wplane;
 };
 constexpr int PACK = 16;     // rows of a work-group, one per wave
+
+// How many of every COUNT rows count, for N above MANY: every group of pack_rows looking through all
+// rows before its own is quadratic in them (forward and gradient of N x 65 x 32 bf16, us, without / with these launches
+// and that of scales(): 8192 43.3 / 45.5, 16384 63.4 / 58.8, 65536 283 / 140, 2^20 35598 / 1913).
+constexpr int COUNT = 1024, MANY = 10240;
+__global__ void __launch_bounds__(COUNT) count_rows(Targets t, int N, int* __restrict__ counts) {
+    __shared__ int red[COUNT / 64];
+    const int n = blockIdx.x * COUNT + threadIdx.x;
+    const uint64_t mask = __ballot(n < N && t.has(n));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = __popcll(mask);
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    int sum = 0;
+    for (int x = 0; x < COUNT / 64; ++x) sum += red[x];
+    counts[blockIdx.x] = sum;
+}
 
 // Work-group b < groups packs rows 16 b .. 16 b + 15: it counts the rows that count before them (the
 // targets are few and stay in cache), then converts its own.  Forward: also the padding's zeros and,
@@ -328,7 +345,9 @@ __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
     }
     const int n0 = blockIdx.x * PACK;
     int before = 0;
-    for (int n = threadIdx.x; n < n0; n += 1024) before += a.targets.has(n);
+    if (a.counts)
+        for (int b = threadIdx.x; b < n0 / COUNT; b += 1024) before += a.counts[b];
+    for (int n = (a.counts ? n0 / COUNT * COUNT : 0) + threadIdx.x; n < n0; n += 1024) before += a.targets.has(n);
     for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m, 64);
     if (lane == 0) red[w] = before;
     if (threadIdx.x < PACK) own[threadIdx.x] = n0 + (int)threadIdx.x < a.N && a.targets.has(n0 + threadIdx.x);
@@ -406,45 +425,76 @@ __global__ void __launch_bounds__(256) stage_table(const T* __restrict__ W, int 
     if (P != BF && lane == 0) exps[r] = e;
 }
 
-// Backward: the same at the table's scale, which each work-group finds from the scan's results; the
-// work-groups behind (first piece) convert the packed rows of w_n H_n (one part: w_n / wtop H_n) at theirs,
-// in XP parts.  The first work-group writes the scales down for the products.
-template <typename T, int P, int XP>
-__global__ void __launch_bounds__(256) stage_scaled(const T* __restrict__ W, int ldw, int v0, int R,
-                                                    int D, uint16_t* __restrict__ dst, int Dp,
-                                                    long long plane, Exps exps, int groups, int scan, int tables,
-                                                    Rows rows, const T* __restrict__ H, int ldh,
-                                                    uint16_t* __restrict__ Xp, long long xplane) {
-    __shared__ float redf[4], redw[4];
-    __shared__ int redi[4];
+// Backward: the scales of the table and of w_n H_n (one part: w_n / wtop H_n), from the scan's results and the
+// groups', by a work-group of WAVES waves.
+template <int XP, int WAVES>
+__device__ inline void find_scales(const Exps& exps, int groups, int scan, int& E, int& X, float& top) {
+    __shared__ float redf[WAVES], redw[WAVES];
+    __shared__ int redi[WAVES];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    float mx = 0.f, top = 0.f;
-    for (int g = threadIdx.x; g < scan; g += 256) mx = fmaxf(mx, exps.wmax[g]);
+    float mx = 0.f;
+    for (int g = threadIdx.x; g < scan; g += 64 * WAVES) mx = fmaxf(mx, exps.wmax[g]);
     mx = wave_reduce(mx, OpMax());
-    int x = NO_EXP;
-    for (int g = threadIdx.x; g < groups; g += 256) {
-        x = max(x, exps.group[g]);
+    X = NO_EXP;
+    top = 0.f;
+    for (int g = threadIdx.x; g < groups; g += 64 * WAVES) {
+        X = max(X, exps.group[g]);
         if (XP == 1) top = fmaxf(top, exps.gtop[g]);
     }
-    for (int m = 1; m < 64; m <<= 1) x = max(x, __shfl_xor(x, m, 64));
+    for (int m = 1; m < 64; m <<= 1) X = max(X, __shfl_xor(X, m, 64));
     if (XP == 1) top = wave_reduce(top, OpMax());
     if (lane == 0) {
         redf[w] = mx;
         redw[w] = top;
-        redi[w] = x;
+        redi[w] = X;
     }
     __syncthreads();
-    const int E = scale_of(fmaxf(fmaxf(redf[0], redf[1]), fmaxf(redf[2], redf[3])));
-    int X = max(max(redi[0], redi[1]), max(redi[2], redi[3]));
+    for (int x = 0; x < WAVES; ++x) {
+        mx = fmaxf(mx, redf[x]);
+        top = fmaxf(top, redw[x]);
+        X = max(X, redi[x]);
+    }
+    E = scale_of(mx);
     if (XP == 1) {
-        top = fmaxf(fmaxf(redw[0], redw[1]), fmaxf(redw[2], redw[3]));
         if (!(top > 0.f)) top = 1.f;   // all weights are zero
         X = X - exponent(top) + 1;     // |w_n / top| < 2^(its exponent - top's + 1)
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        *exps.E = E;
-        *exps.X = X;
-        *exps.wtop = top;
+}
+// For N above MANY: once, instead of by every work-group of stage_scaled.
+template <int XP>
+__global__ void __launch_bounds__(1024) scales(Exps exps, int groups, int scan) {
+    int E, X;
+    float top;
+    find_scales<XP, 16>(exps, groups, scan, E, X, top);
+    if (threadIdx.x != 0) return;
+    *exps.E = E;
+    *exps.X = X;
+    *exps.wtop = top;
+}
+
+// Backward: rows of the table at its scale; the work-groups behind (first piece) convert the packed rows of
+// w_n H_n at theirs, in XP parts.  Unless the scales are known, each work-group finds them, and the first one
+// writes them down.
+template <typename T, int P, int XP>
+__global__ void __launch_bounds__(256) stage_scaled(const T* __restrict__ W, int ldw, int v0, int R,
+                                                    int D, uint16_t* __restrict__ dst, int Dp,
+                                                    long long plane, Exps exps, int groups, int scan, int known,
+                                                    int tables, Rows rows, const T* __restrict__ H, int ldh,
+                                                    uint16_t* __restrict__ Xp, long long xplane) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int E, X;
+    float top;
+    if (known) {
+        E = *exps.E;
+        X = *exps.X;
+        top = *exps.wtop;
+    } else {
+        find_scales<XP, 4>(exps, groups, scan, E, X, top);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            *exps.E = E;
+            *exps.X = X;
+            *exps.wtop = top;
+        }
     }
     if ((int)blockIdx.x < tables) {
         const int r = blockIdx.x * 4 + w;
@@ -2072,7 +2122,7 @@ Plan make_plan(int dtype, int gtype, int N, int V, int D, int K, const void* W, 
         at += up256(bytes);
         return here;
     };
-    p.ints = take(((size_t)4 * p.Nt + 2 * (p.Nt / PACK) + 64 + SCAN) * 4);   // cnt and scales, row, target, ...
+    p.ints = take(((size_t)4 * p.Nt + 2 * (p.Nt / PACK) + 64 + SCAN + p.Nt / COUNT + 1) * 4);   // cnt and scales, row, target, ...
     p.w = take((size_t)p.Nt * 4);
     p.lses = take((size_t)p.Nt * 4);
     p.base = take((size_t)p.Nt * 4);
@@ -2190,7 +2240,7 @@ struct Work {
     Plan p;
     Rows rows;
     Exps exps;
-    int* flags;
+    int *flags, *counts;
     float *base, *q, *z, *acc;
     float2* state;
     uint16_t *Hp, *Xp;   // Xp: the other operand of dW
@@ -2208,6 +2258,7 @@ Work lay_out(const Plan& p, void* ws) {
     const int groups = p.Nt / PACK;
     w.exps = {nullptr, ints + 1, ints + 2, (float*)(ints + 3), array(4), (float*)(array(4) + groups),
               (float*)(array(4) + 2 * groups)};
+    w.counts = array(4) + 2 * groups + SCAN;
     w.base = (float*)(b + p.base);
     w.q = (float*)(b + p.q);
     w.z = (float*)(b + p.z);
@@ -2227,6 +2278,11 @@ int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
         teacher_flags<<<(h.N + 3) / 4, 256, 0, stream()>>>(h.teacher, h.N, h.V, w.flags);
         DH_TRY(check_launch(h.op));
         a.targets.target = w.flags;
+    }
+    if (h.N > MANY) {
+        count_rows<<<(h.N + COUNT - 1) / COUNT, COUNT, 0, stream()>>>(a.targets, h.N, w.counts);
+        DH_TRY(check_launch(h.op));
+        a.counts = w.counts;
     }
     a.N = h.N;
     a.D = h.D;
@@ -2364,13 +2420,18 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     }
     const int scan = h.V < 16 * SCAN ? (h.V + 15) / 16 : SCAN;
     DH_TRY((prepare_rows<T, P>(h, w, a, scan)));
+    const int groups = (h.N + PACK - 1) / PACK;
+    if (h.N > MANY) {
+        scales<GP><<<1, 1024, 0, stream()>>>(w.exps, groups, scan);
+        DH_TRY(check_launch(h.op));
+    }
     const Grad<OT> to_dH{(OT*)d.dH, d.lddh, d.acc_dH, w.rows.row, w.exps.E, w.rows.w, 1};
     for (int v0 = 0;; v0 += rows) {
         const int R = h.V - v0 < rows ? h.V - v0 : rows;
         const bool last = h.V - v0 <= rows;
         const int tables = (R + 3) / 4;
         stage_scaled<T, P, GP><<<tables + (v0 == 0 ? (h.N + 3) / 4 : 0), 256, 0, stream()>>>(
-            (const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp, wplane, w.exps, (h.N + PACK - 1) / PACK, scan, tables,
+            (const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp, wplane, w.exps, groups, scan, v0 > 0 || h.N > MANY, tables,
             w.rows, (const T*)h.H, h.ldh, w.Xp, hplane);
         DH_TRY(check_launch(h.op));
         const Prod g{w.Hp, staged, p.Dp, p.Dp, hplane, wplane, h.N, R, p.Dp, 0, w.rows.cnt};
@@ -2401,9 +2462,9 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         else DH_TRY((gradients<P, GP>(h.op, p, ph, sum_h, pw, sum_w)));
         Finish<OT> fh{to_dH, w.acc, h.N, p.Dp, p.splits, hplane, w.rows.cnt, 0};
         Finish<OT> fw{to_dW, wacc, R, p.Dp, p.wsplits, wplane, nullptr, 0};
-        auto groups = [&](long long rows_) { return (rows_ * ((h.D + 3) / 4) + 255) / 256; };
-        if (ph && last && !direct_h) fh.groups = groups(h.N);
-        if (pw && !direct_w) fw.groups = groups(R);
+        auto finish_groups = [&](long long n) { return (n * ((h.D + 3) / 4) + 255) / 256; };
+        if (ph && last && !direct_h) fh.groups = finish_groups(h.N);
+        if (pw && !direct_w) fw.groups = finish_groups(R);
         if (fh.groups + fw.groups > 0) {
             finish<OT><<<(unsigned)(fh.groups + fw.groups), 256, 0, stream()>>>(fh, fw, h.D);
             DH_TRY(check_launch(h.op));
