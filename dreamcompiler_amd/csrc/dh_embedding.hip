@@ -648,11 +648,15 @@ EmbWs emb_ws(int N, int V, int D) {
     return w;
 }
 
-int check_emb(const char* op, int dtype, int N, int V, int D, float scale) {
+// The most tokens of a gradient: embedding_join has 256 threads per EMB_CHUNK of them, and a launch
+// less than 2^32.
+constexpr int EMB_MOST = EMB_CHUNK * ((1 << 24) - 1);
+
+int check_emb(const char* op, int dtype, int N, int V, int D, float scale, int most) {
     if (dtype != DH_F32 && dtype != DH_BF16)
         return set_error(DH_ERR_INVALID, "%s: dtype must be fp32 or bf16", op);
     // 2^20 below the ends of int, which the strides of the kernels' loops stay under
-    if (N < 0 || V < 1 || D < 1 || N > 0x7FF00000 || V > 0x7FF00000 || D > 1 << 24)
+    if (N < 0 || V < 1 || D < 1 || N > most || V > 0x7FF00000 || D > 1 << 24)
         return set_error(DH_ERR_INVALID, "%s: shape N=%d V=%d D=%d", op, N, V, D);
     if (!(scale - scale == 0.f)) return set_error(DH_ERR_INVALID, "%s: scale must be finite", op);
     return DH_OK;
@@ -736,7 +740,7 @@ extern "C" {
 
 int dh_embedding_fwd(int dtype, int N, int V, int D, float scale, const int* ids, const void* W,
                      int ldw, void* Y, int ldy) {
-    DH_TRY(check_emb("dh_embedding_fwd", dtype, N, V, D, scale));
+    DH_TRY(check_emb("dh_embedding_fwd", dtype, N, V, D, scale, 0x7FF00000));
     if (ldw < D || ldy < D)
         return set_error(DH_ERR_INVALID, "dh_embedding_fwd: leading dimension below D");
     if (N > 0 && (!ids || !W || !Y)) return set_error(DH_ERR_INVALID, "dh_embedding_fwd: null pointer");
@@ -760,7 +764,7 @@ size_t dh_embedding_bwd_workspace(int N, int V, int D) {
 int dh_embedding_bwd(int dtype, int N, int V, int D, float scale, const int* ids, const void* dY,
                      int lddy, void* dW, int lddw, int grad_type, int accumulate, void* ws,
                      size_t ws_bytes) {
-    DH_TRY(check_emb("dh_embedding_bwd", dtype, N, V, D, scale));
+    DH_TRY(check_emb("dh_embedding_bwd", dtype, N, V, D, scale, EMB_MOST));
     if (grad_type != DH_F32 && grad_type != dtype)
         return set_error(DH_ERR_INVALID, "dh_embedding_bwd: grad_type must be fp32 or the inputs' type");
     if (lddy < D || lddw < D)

@@ -39,6 +39,13 @@
 namespace dh {
 namespace {
 
+// Launches of more than 2^22 work-groups have a second dimension: a dimension has less than 2^32 threads.
+inline dim3 long_grid(long long n) {
+    const long long x = 1 << 22;
+    return dim3((unsigned)std::min(n, x), (unsigned)((n + x - 1) / x));
+}
+__device__ inline long long grid_index() { return (long long)blockIdx.y << 22 | blockIdx.x; }
+
 // ---- rows of either type ----------------------------------------------------------------------
 typedef float f4a __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t h8a __attribute__((ext_vector_type(8), aligned(2)));
@@ -537,7 +544,7 @@ __global__ void __launch_bounds__(512) teacher_dots(Rows rows, Teacher t, int V,
                                                     float* __restrict__ base) {
     __shared__ float red[8];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int i = blockIdx.x;
+    const int i = (int)grid_index();
     if (i >= *rows.cnt) return;
     const int n = rows.row[i];
     const size_t at = (size_t)n * t.K, to = (size_t)i * t.K;
@@ -1530,7 +1537,7 @@ __global__ void __launch_bounds__(256) teacher_entries(Rows rows, Teacher t, int
                                                        const float* __restrict__ z,
                                                        uint16_t* __restrict__ G, int ldg,
                                                        long long plane) {
-    const int i = blockIdx.x;
+    const int i = (int)grid_index();
     if (i >= *rows.cnt) return;
     const size_t at = (size_t)rows.row[i] * t.K, from = (size_t)i * t.K;
     const float lse = rows.lse[i];
@@ -1560,10 +1567,12 @@ struct Finish {
 };
 template <typename OT>
 __global__ void __launch_bounds__(256) finish(Finish<OT> h, Finish<OT> w, int D) {
-    const bool second = blockIdx.x >= h.groups;
+    const long long group = grid_index();
+    const bool second = group >= h.groups;
+    if (group >= h.groups + w.groups) return;
     const Finish<OT>& f = second ? w : h;
     const int quads = (D + 3) / 4;
-    const long long t = (blockIdx.x - (second ? h.groups : 0)) * 256 + threadIdx.x;
+    const long long t = (group - (second ? h.groups : 0)) * 256 + threadIdx.x;
     const long long i = t / quads;
     const int c = 4 * (int)(t % quads);
     if (i >= (f.cnt ? *f.cnt : f.rows)) return;
@@ -2208,12 +2217,20 @@ size_t least_ws(int dtype, int N, int V, int D, int K, int backward) {
     return need;
 }
 
+// The most rows that a loss takes, and the most values of H: a launch has less than 2^32 threads in
+// a dimension.
+constexpr int MOST_ROWS = 1 << 25;
+constexpr long long MOST_VALUES = 1LL << 35;
+
 // Table rows of a piece: as many blocks of 256 as fit, the same for every piece.
-int piece_rows(const Plan& p, int V, size_t ws_bytes) {
+int piece_rows(const Plan& p, int N, int V, int D, size_t ws_bytes) {
     const long long blocks = (V + 255LL) / 256;
     long long fit = (long long)((ws_bytes - 512 - p.piece) / p.per_block);
     if (fit > blocks) fit = blocks;
     if (fit > 4096) fit = 4096;   // 256 rows of G stay within 32-bit offsets
+    // 64-wide tiles of rows x N or D have a thread per 16 values.
+    const long long most = (1LL << 34) / std::max(N, D) / 256;   // at least 1, as N <= 2^25
+    if (fit > most) fit = most;
     const long long pieces = (blocks + fit - 1) / fit;
     return (int)((blocks + pieces - 1) / pieces) * 256;
 }
@@ -2221,7 +2238,8 @@ int piece_rows(const Plan& p, int V, size_t ws_bytes) {
 int check_head(const Head& h, int K, const void* ws, size_t ws_bytes, int backward) {
     if (h.dtype != DH_F32 && h.dtype != DH_BF16)
         return set_error(DH_ERR_INVALID, "%s: dtype must be fp32 or bf16", h.op);
-    if (h.N < 0 || h.V < 1 || h.D < 1 || K < 0 || h.N > 0x7FFFFE00 || h.V > 0x7FFFFE00 || h.D > 1 << 20)
+    if (h.N < 0 || h.V < 1 || h.D < 1 || K < 0 || h.N > MOST_ROWS || h.V > 0x7FFFFE00 || h.D > 1 << 20 ||
+        (long long)h.N * h.D > MOST_VALUES)
         return set_error(DH_ERR_INVALID, "%s: shape N=%d V=%d D=%d", h.op, h.N, h.V, h.D);
     if (h.ldh < h.D || h.ldw < h.D)
         return set_error(DH_ERR_INVALID, "%s: leading dimension below D", h.op);
@@ -2304,7 +2322,7 @@ int prepare_rows(const Head& h, const Work& w, Pack a, int more) {
     // Up to 8 waves, with as few idle places in their last turn as that leaves.
     const int turns = std::max(1, (h.teacher.K + 8 * TEACHER_FLY - 1) / (8 * TEACHER_FLY));
     const int waves = std::max(1, (h.teacher.K + TEACHER_FLY * turns - 1) / (TEACHER_FLY * turns));
-    teacher_dots<T><<<h.N, 64 * waves, 0, stream()>>>(w.rows, h.teacher, h.V, (const T*)h.H, h.ldh, (const T*)h.W,
+    teacher_dots<T><<<long_grid(h.N), 64 * waves, 0, stream()>>>(w.rows, h.teacher, h.V, (const T*)h.H, h.ldh, (const T*)h.W,
                                                h.ldw, h.D, w.q, w.z, w.base);
     return check_launch(h.op);
 }
@@ -2329,7 +2347,7 @@ template <typename T, int P>
 int forward(const Head& h, float* loss, float* lse, void* ws, size_t ws_bytes) {
     const Plan p = make_plan(h.dtype, -1, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, h.W, h.ldw);
     Work w = lay_out(p, ws);
-    const int rows = piece_rows(p, h.V, ws_bytes);
+    const int rows = piece_rows(p, h.N, h.V, h.D, ws_bytes);
     const int wr = wave_rows(p.lse);
     float2* part = (float2*)w.piece;
     uint16_t* staged = (uint16_t*)(w.piece + (size_t)(rows / wr) * p.Nt * 8);
@@ -2403,7 +2421,7 @@ template <typename T, int P, int GP, typename OT>
 int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     const Plan p = make_plan(h.dtype, d.type, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, h.W, h.ldw);
     Work w = lay_out(p, ws);
-    const int rows = piece_rows(p, h.V, ws_bytes);
+    const int rows = piece_rows(p, h.N, h.V, h.D, ws_bytes);
     const bool one = h.V <= rows;   // a single piece
     const long long hplane = (long long)h.N * p.Dp, wplane = (long long)rows * p.Dp;
     uint16_t* G = (uint16_t*)w.piece;
@@ -2443,7 +2461,7 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
             DH_TRY((product<true, true, TOK_M, P, P>(
                 h.op, p.g, g, 1,
                 EpiG<GP, false>{h.c, w.rows.lse, nullptr, w.rows.hexp, w.exps.E, v0, G, rows, gplane})));
-            teacher_entries<GP><<<h.N, 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, rows,
+            teacher_entries<GP><<<long_grid(h.N), 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, rows,
                                                            gplane);
             DH_TRY(check_launch(h.op));
         }
@@ -2466,7 +2484,7 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         if (ph && last && !direct_h) fh.groups = finish_groups(h.N);
         if (pw && !direct_w) fw.groups = finish_groups(R);
         if (fh.groups + fw.groups > 0) {
-            finish<OT><<<(unsigned)(fh.groups + fw.groups), 256, 0, stream()>>>(fh, fw, h.D);
+            finish<OT><<<long_grid(fh.groups + fw.groups), 256, 0, stream()>>>(fh, fw, h.D);
             DH_TRY(check_launch(h.op));
         }
         if (last) return DH_OK;

@@ -339,6 +339,8 @@ int dh_unary(int op, int dtype, const void* d_A, void* d_C, size_t n, double lo,
  * and a product of two fp32 operands to 2^-21 of itself.  bf16 operands are exact in the forward, and in the
  * gradients above 2^-32 of their matrix's largest value (below it to 2^-39 of that).
  * Deterministic: no floating-point atomics.
+ * Sizes: D up to 2^24 (embedding) or 2^20 (losses), N up to 2^31 - 2^20 tokens of a lookup, 2^28 - 16 of its
+ * gradient, 2^25 rows of a loss with N D up to 2^35; V up to 2^31 - 2^20.  More is refused.
  *
  * Y[n] = scale W[id[n]] for N tokens. */
 int dh_embedding_fwd(int dtype, int N, int V, int D, float scale, const int* d_ids,
