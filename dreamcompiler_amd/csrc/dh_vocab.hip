@@ -2629,6 +2629,30 @@ using namespace dh;
 
 extern "C" {
 
+int dh_linear_loss_plan(int dtype, int grad_type, int N, int V, int D, int K, size_t ws_bytes, int* plan) {
+    if ((dtype != DH_F32 && dtype != DH_BF16) || (grad_type != DH_F32 && grad_type != dtype))
+        return set_error(DH_ERR_INVALID, "dh_linear_loss_plan: dtype must be fp32 or bf16, grad_type fp32 or dtype");
+    if (N < 1 || V < 1 || D < 1 || K < 0 || N > MOST_ROWS || V > 0x7FFFFE00 || D > 1 << 20)
+        return set_error(DH_ERR_INVALID, "dh_linear_loss_plan: shape N=%d V=%d D=%d K=%d", N, V, D, K);
+    if (!plan) return set_error(DH_ERR_INVALID, "dh_linear_loss_plan: null pointer");
+    std::fill(plan, plan + 8, 0);
+    if (!is_few(dtype, N, V, 0)) {
+        const Plan p = make_plan(dtype, -1, N, V, D, K, nullptr, 1);
+        plan[0] = side(p.lse);
+        plan[6] = ws_bytes < least_ws(dtype, N, V, D, K, 0) ? 0 : piece_rows(p, N, V, D, ws_bytes);
+    }
+    if (!is_few(dtype, N, V, 1)) {
+        const Plan p = make_plan(dtype, grad_type, N, V, D, K, nullptr, 1);
+        plan[1] = side(p.g);
+        plan[2] = side(p.dh);
+        plan[3] = side(p.dw);
+        plan[4] = p.splits;
+        plan[5] = p.wsplits;
+        plan[7] = ws_bytes < least_ws(dtype, N, V, D, K, 1) ? 0 : piece_rows(p, N, V, D, ws_bytes);
+    }
+    return DH_OK;
+}
+
 size_t dh_linear_xent_workspace(int dtype, int N, int V, int D, int backward) {
     return N < 0 || V < 1 || D < 1 ? 0 : least_ws(dtype, N, V, D, 0, backward);
 }

@@ -86,6 +86,7 @@ _SIGS = {
     "dh_embedding_fwd": (_i, [_i, _i, _i, _i, _f, _vp, _vp, _i, _vp, _i]),
     "dh_embedding_bwd_workspace": (_sz, [_i, _i, _i]),
     "dh_embedding_bwd": (_i, [_i, _i, _i, _i, _f, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _sz]),
+    "dh_linear_loss_plan": (_i, [_i, _i, _i, _i, _i, _i, _sz, ctypes.POINTER(_i)]),
     "dh_linear_xent_workspace": (_sz, [_i, _i, _i, _i, _i]),
     "dh_linear_xent_fwd": (_i, [_i, _i, _i, _i, _f, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _sz]),
     "dh_linear_xent_bwd": (_i, [_i, _i, _i, _i, _f, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i,
@@ -352,6 +353,13 @@ def embedding_bwd(dtype, N, V, D, scale, ids, dY, lddy, dW, lddw, grad_type, acc
     check(load().dh_embedding_bwd(dtype, N, V, D, float(scale), _p(ids), _p(dY), lddy, _p(dW),
                                   lddw, grad_type, int(accumulate), _p(ws), int(ws_bytes)),
           "dh_embedding_bwd")
+
+
+def linear_loss_plan(dtype, grad_type, N, V, D, K, ws_bytes):
+    """Tile sides of the statistics, G, dH and dW, splits of dH and dW, rows of a piece (forward, gradient)."""
+    plan = (_i * 8)()
+    check(load().dh_linear_loss_plan(dtype, grad_type, N, V, D, K, int(ws_bytes), plan), "dh_linear_loss_plan")
+    return tuple(plan)
 
 
 def linear_xent_workspace(dtype, N, V, D, backward):

@@ -383,6 +383,11 @@ int dh_linear_distill_bwd(int dtype, int N, int V, int D, int K, float T, const 
                           const float* d_lse, const float* d_dloss, void* d_dH, int lddh,
                           int acc_dH, void* d_dW, int lddw, int acc_dW, int grad_type, void* d_ws,
                           size_t ws_bytes);
+/* How a loss of these sizes runs (K: 0 for cross entropy; no device needed), 8 values: the side of the tiles
+ * of the logits' statistics, of the gradient's logits, of dH and of dW (0: read row by row, the
+ * form for few rows), the splits of dH and dW, and the table rows of a piece of the forward and of the gradient
+ * in ws_bytes (the whole of V in one piece is fastest; 0: too little, or the form for few rows). */
+int dh_linear_loss_plan(int dtype, int grad_type, int N, int V, int D, int K, size_t ws_bytes, int* plan);
 
 #ifdef __cplusplus
 }
