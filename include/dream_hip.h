@@ -371,9 +371,10 @@ int dh_linear_xent_bwd(int dtype, int N, int V, int D, float scale, const void* 
                        int lddw, int acc_dW, int grad_type, void* d_ws, size_t ws_bytes);
 /* Distillation of the same logits at a temperature T > 0, z = H W^T / T, from a teacher's K best
  * logits a row (top_id, top_logit: N x K, in any order; an entry of logit -inf is none):
- * q = softmax(top_logit / T) over the row's entries, loss[n] = T^2 KL(q || softmax(z)) =
- * T^2 sum_k q_k (log q_k - z_k + lse).  A token that occurs twice in a row counts with the sum of
- * its probabilities.  A row without entries is padding. */
+ * q = softmax(top_logit / T) over the row's entries, loss[n] = T^2 sum_k q_k (log q_k - z_k + lse): T^2 times
+ * KL(q || softmax(z)) where no token occurs twice in a row.  One that does counts with the sum of its
+ * probabilities in the gradient; in the loss each of its entries keeps its own log q_k (which no
+ * gradient sees: the loss is T^2 sum q_k log (Q / q_k) below T^2 KL, Q its token's sum).  A row without entries is padding. */
 size_t dh_linear_distill_workspace(int dtype, int N, int V, int D, int K, int backward);
 int dh_linear_distill_fwd(int dtype, int N, int V, int D, int K, float T, const void* d_H, int ldh,
                           const void* d_W, int ldw, const int* d_top_id, const float* d_top_logit,
