@@ -597,6 +597,49 @@ __global__ void __launch_bounds__(512) teacher_dots(Rows rows, Teacher t, int V,
     base[i] = part;
 }
 
+// The probabilities of a row's tokens, for many entries: q[k] of the first entry of a token is the sum over its
+// entries, of the others -1.  Sums are integers of 2^-62, so they do not go by the order of the atomics (q below
+// 2^-39 is cut there, far below what the products take of it).  A work-group per row; the table's tokens go
+// by in ranges of SUM_RANGE, each a look at all entries.  Looking through the row for each entry instead, as
+// fewer do, is quadratic in K (forward and gradient of D = 256 bf16, us, that / so: 512 x 32000 of 128 entries 179 / 181,
+// 256 215 / 210, 1024 594 / 375, 8192 16755 / 2021; 512 x 131072 of 256 469 / 496, 512 567 / 552, 2048 1838 / 957; 4096 x
+// 32000 of 128 710 / 768, 256 931 / 937, 1024 2837 / 1929).
+constexpr int SUM_RANGE = 4096, SUM_LEAST = 128;
+bool by_sums(int V, int K) { return K > SUM_LEAST && (long long)K * K > 2LL * V; }
+__global__ void __launch_bounds__(1024) teacher_sums(const int* __restrict__ cnt, const int* __restrict__ row,
+                                                     Teacher t, int V, float* __restrict__ q) {
+    __shared__ unsigned long long sum[SUM_RANGE];
+    __shared__ int first[SUM_RANGE];
+    const int i = (int)grid_index();
+    if (cnt && i >= *cnt) return;
+    const size_t at = (size_t)(row ? row[i] : i) * t.K, to = (size_t)i * t.K;
+    float mx, log_sum;
+    teacher_stats(t, at, V, mx, log_sum);
+    auto prob = [&](int k) { return __expf((t.logit[at + k] - mx) * t.inv_t - log_sum); };
+    const bool sound = log_sum - log_sum == 0.f && mx < INFINITY;   // else every entry's q is NaN
+    for (int k = threadIdx.x; k < t.K; k += 1024) q[to + k] = sound ? -1.f : NAN;
+    if (!sound) return;
+    for (long long v0 = 0; v0 < V; v0 += SUM_RANGE) {
+        __syncthreads();   // the range before has been read
+        for (int r = threadIdx.x; r < SUM_RANGE; r += 1024) {
+            sum[r] = 0;
+            first[r] = t.K;
+        }
+        __syncthreads();
+        for (int k = threadIdx.x; k < t.K; k += 1024) {
+            const long long r = t.id[at + k] - v0;
+            if (r < 0 || r >= SUM_RANGE || !entry_counts(t, at + k, V)) continue;
+            atomicAdd(&sum[r], (unsigned long long)(prob(k) * 0x1p62f));
+            atomicMin(&first[r], k);
+        }
+        __syncthreads();
+        for (int k = threadIdx.x; k < t.K; k += 1024) {
+            const long long r = t.id[at + k] - v0;
+            if (r >= 0 && r < SUM_RANGE && first[r] == k) q[to + k] = (float)sum[r] * 0x1p-62f;
+        }
+    }
+}
+
 // ---- products -------------------------------------------------------------------------------------
 // C (M x N) = sum over k of A and B, operands of PA and PB fp16 parts (or both BF).  AK: A is stored
 // [m][k], else [k][m]; BK: B is stored [n][k], else [k][n].  One of M, N and K counts packed rows: its
@@ -1530,8 +1573,9 @@ __global__ void __launch_bounds__(256) lse_join_few(const float2* __restrict__ p
 }
 
 // The entries of G at the teacher's tokens inside a piece, from the fp32 logits: p - q, q
-// summed where a token occurs more than once (each of its entries writes the same value).
-template <int GP>
+// summed where a token occurs more than once: by its first entry (SUMS: teacher_sums has done it), else each of
+// its entries writes the same value.
+template <int GP, bool SUMS>
 __global__ void __launch_bounds__(256) teacher_entries(Rows rows, Teacher t, int V, int v0, int R,
                                                        const float* __restrict__ q,
                                                        const float* __restrict__ z,
@@ -1545,8 +1589,13 @@ __global__ void __launch_bounds__(256) teacher_entries(Rows rows, Teacher t, int
         const int id = t.id[at + k];
         if (id < v0 || id >= v0 + R || !entry_counts(t, at + k, V)) continue;
         float sum = 0.f;
-        for (int j = 0; j < t.K; ++j)
-            if (t.id[at + j] == id) sum += q[from + j];
+        if constexpr (SUMS) {
+            sum = q[from + k];
+            if (sum < 0.f) continue;
+        } else {
+            for (int j = 0; j < t.K; ++j)
+                if (t.id[at + j] == id) sum += q[from + j];
+        }
         uint16_t parts[GP];
         to_parts<GP>(0x1p14f * (__expf(z[from + k] - lse) - sum), parts);
         uint16_t* to = G + (size_t)i * ldg + (id - v0);
@@ -1605,6 +1654,7 @@ struct Few {
     int ldw;
     float c;
     uint32_t* keep;      // the rows that count, as bits, from few_mark; null: they have a target
+    const float* sums;   // of teacher_sums, or null
     float2* part;        // [work-group of few_lse][ldpart]
     int ldpart;
     float* G;
@@ -1872,9 +1922,16 @@ __global__ void __launch_bounds__(256) few_teacher(Few f) {
     const Teacher& t = f.targets.t;
     const int V = f.targets.V;
     const size_t at = (size_t)n * t.K;
+    const float w = (f.dloss ? f.dloss[n] : 1.f) * f.wscale;
+    if (f.sums) {
+        for (int k = threadIdx.x; k < t.K; k += 256) {
+            const float q = f.sums[at + k];
+            if (entry_counts(t, at + k, V) && !(q < 0.f)) f.G[(size_t)t.id[at + k] * FEW + n] -= w * q;
+        }
+        return;
+    }
     float mx, log_sum;
     teacher_stats(t, at, V, mx, log_sum);
-    const float w = (f.dloss ? f.dloss[n] : 1.f) * f.wscale;
     for (int k = threadIdx.x; k < t.K; k += 256) {
         if (!entry_counts(t, at + k, V)) continue;
         const int id = t.id[at + k];
@@ -2170,9 +2227,9 @@ bool is_few(int dtype, int N, int V, int backward) {
 struct FewPlan {
     int Dp, rows, waves, blocks;   // of few_lse and few_g: table rows and waves of a work-group
     int splits, rows_per_split, hslabs, wslabs, wrows, wlanes;
-    size_t G, acc, keep, total;   // the parts of the forward lie at G
+    size_t G, acc, keep, sums, total;   // the parts of the forward lie at G
 };
-FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int backward) {
+FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int K, int backward) {
     FewPlan p{};
     const int C = dtype == DH_F32 ? 4 : 8, CW = grad_type == DH_F32 ? 4 : 8;
     p.Dp = (D + 3) / 4 * 4;
@@ -2200,15 +2257,16 @@ FewPlan few_plan(int dtype, int grad_type, int N, int V, int D, int backward) {
     p.wrows = (V + chunks - 1) / chunks;
     p.acc = up256((size_t)p.blocks * p.rows * FEW * 4);
     p.keep = p.acc + up256((size_t)p.splits * FEW * p.Dp * 4);
-    p.total = p.keep + 256;
+    p.sums = p.keep + 256;
+    p.total = p.sums + (by_sums(V, K) ? up256((size_t)N * K * 4) : 0);
     return p;
 }
 
 // The workspace that serves any alignment of the operands (staged tables take more).
 size_t least_ws(int dtype, int N, int V, int D, int K, int backward) {
     if (is_few(dtype, N, V, backward))   // whichever type the gradients have
-        return std::max(few_plan(dtype, DH_F32, N, V, D, backward).total,
-                        few_plan(dtype, dtype, N, V, D, backward).total);
+        return std::max(few_plan(dtype, DH_F32, N, V, D, K, backward).total,
+                        few_plan(dtype, dtype, N, V, D, K, backward).total);
     size_t need = 0;
     for (int g : {(int)DH_F32, dtype}) {
         const Plan p = make_plan(dtype, backward ? g : -1, N, V, D, K, nullptr, 1);
@@ -2438,6 +2496,10 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     }
     const int scan = h.V < 16 * SCAN ? (h.V + 15) / 16 : SCAN;
     DH_TRY((prepare_rows<T, P>(h, w, a, scan)));
+    if (!h.target && by_sums(h.V, h.teacher.K)) {
+        teacher_sums<<<long_grid(h.N), 1024, 0, stream()>>>(w.rows.cnt, w.rows.row, h.teacher, h.V, w.q);
+        DH_TRY(check_launch(h.op));
+    }
     const int groups = (h.N + PACK - 1) / PACK;
     if (h.N > MANY) {
         scales<GP><<<1, 1024, 0, stream()>>>(w.exps, groups, scan);
@@ -2461,8 +2523,8 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
             DH_TRY((product<true, true, TOK_M, P, P>(
                 h.op, p.g, g, 1,
                 EpiG<GP, false>{h.c, w.rows.lse, nullptr, w.rows.hexp, w.exps.E, v0, G, rows, gplane})));
-            teacher_entries<GP><<<long_grid(h.N), 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, rows,
-                                                           gplane);
+            auto entries = by_sums(h.V, h.teacher.K) ? teacher_entries<GP, true> : teacher_entries<GP, false>;
+            entries<<<long_grid(h.N), 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, rows, gplane);
             DH_TRY(check_launch(h.op));
         }
         const Prod gh{G, staged, rows, p.Dp, gplane, wplane, h.N, h.D, R, 0, w.rows.cnt};
@@ -2516,7 +2578,7 @@ int few_rows(const Head& h, Few& f, const FewPlan& p, void* ws) {
 
 template <typename T>
 int few_forward(const Head& h, float* loss, float* lse, void* ws) {
-    const FewPlan p = few_plan(h.dtype, h.dtype, h.N, h.V, h.D, 0);
+    const FewPlan p = few_plan(h.dtype, h.dtype, h.N, h.V, h.D, 0, 0);
     Few f = few_args(h);
     DH_TRY(few_rows(h, f, p, ws));
     f.part = (float2*)ws;
@@ -2537,7 +2599,7 @@ int few_forward(const Head& h, float* loss, float* lse, void* ws) {
 
 template <typename T, typename OT>
 int few_backward(const Head& h, const Grads& d, void* ws) {
-    const FewPlan p = few_plan(h.dtype, d.type, h.N, h.V, h.D, 1);
+    const FewPlan p = few_plan(h.dtype, d.type, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, 1);
     Few f = few_args(h);
     DH_TRY(few_rows(h, f, p, ws));
     f.G = (float*)ws;
@@ -2556,6 +2618,11 @@ int few_backward(const Head& h, const Grads& d, void* ws) {
     g<<<p.blocks, 64 * p.waves, 0, stream()>>>(f);
     DH_TRY(check_launch(h.op));
     if (!h.target && h.teacher.K > 0) {
+        if (by_sums(h.V, h.teacher.K)) {
+            f.sums = (const float*)((char*)ws + p.sums);
+            teacher_sums<<<long_grid(h.N), 1024, 0, stream()>>>(nullptr, nullptr, h.teacher, h.V, (float*)f.sums);
+            DH_TRY(check_launch(h.op));
+        }
         few_teacher<<<h.N, 256, 0, stream()>>>(f);
         DH_TRY(check_launch(h.op));
     }
