@@ -21,14 +21,16 @@
 // hi hi: the cross products are added first, the accumulators scaled by 2^-11 (exactly), then the
 // third is added (lo lo, at most 2^-22 of the product, is left out).  Three 16-bit products at 16 times the rate of an fp32 one.
 //   fp32 inputs            two parts of all operands
-//   bf16, gradients bf16   one part: H and W fit exactly, G and w_n H_n are rounded to 11 bits, whose
-//                          2^-11 is an eighth of the result's own rounding (to bf16 G would lose as much
-//                          as the result does, and at the targets in one direction); as many products
-//   bf16, gradients fp32   one part of H and W, two of G and w_n H_n: 1, 2 and 3 products
+//   bf16, gradients bf16   one part: H and W fit exactly, G is rounded to 11 bits, whose 2^-11 is an eighth
+//                          of the result's own rounding (to bf16 G would lose as much as the result
+//                          does, and at the targets in one direction); as many products
+//   bf16, gradients fp32   one part of H and W, two of G: 1, 2 and 2 products
+// A row's weight is w_n = wtop 2^k m with wtop the largest weight and m in [1/2, 1): G has m, and 2^k, which
+// is exact, goes to the other operand of dW and to dH's rows, so neither loses rows of small weight.
 // With the operand's largest value scaled below 2^15, the others are taken to 2^-23 (one part: 2^-11) of
 // themselves or 2^-50 (2^-39) of it, whichever is more.  What the scale is common to: a row
 // where k runs along the row (H, and W in the forward), else all of the operand (W in the
-// backward, where its rows are summed over; G, whose entries are p - q; and w_n H_n, the other
+// backward, where its rows are summed over; G, whose entries are m (p - q); and 2^k H_n, the other
 // operand of dW).
 #include <algorithm>
 #include <type_traits>
@@ -185,14 +187,14 @@ struct Rows {
     int* row;          // packed -> row
     int* target;
     int* hexp;
-    float *w, *lse;    // backward only
+    float *w, *lse;    // backward only.  w: w_n, from stage_scaled on its m
+    float* rest;       // and wtop 2^k
 };
 // fp16: the scales of the other operands.
 struct Exps {
     int* e;            // forward: of the piece's table rows
-    int *X, *E;        // backward: of w_n H_n and of the table
-    float* wtop;       // one part: the largest weight.  w_n / wtop H_n is the operand then, which is
-                       // exact where all weights are equal
+    int *X, *E;        // backward: of 2^k H_n and of the table
+    float* wtop;       // the largest weight
     int* group;        // per group of packed rows, the largest scale that w_n H_n asks for,
     float* gtop;       // and its largest weight
     float* wmax;       // per work-group of the scan, the table's largest value
@@ -432,47 +434,45 @@ __global__ void __launch_bounds__(256) stage_table(const T* __restrict__ W, int 
     if (P != BF && lane == 0) exps[r] = e;
 }
 
-// Backward: the scales of the table and of w_n H_n (one part: w_n / wtop H_n), from the scan's results and the
+// Backward: the scales of the table and of 2^k H_n, and the largest weight, from the scan's results and the
 // groups', by a work-group of WAVES waves.
-template <int XP, int WAVES>
+template <int WAVES>
 __device__ inline void find_scales(const Exps& exps, int groups, int scan, int& E, int& X, float& top) {
-    __shared__ float redf[WAVES], redw[WAVES];
-    __shared__ int redi[WAVES];
+    __shared__ float red[3][WAVES];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    float mx = 0.f;
-    for (int g = threadIdx.x; g < scan; g += 64 * WAVES) mx = fmaxf(mx, exps.wmax[g]);
-    mx = wave_reduce(mx, OpMax());
-    X = NO_EXP;
+    float mx = 0.f, x = NO_EXP;   // exponents are exact as floats
     top = 0.f;
-    for (int g = threadIdx.x; g < groups; g += 64 * WAVES) {
-        X = max(X, exps.group[g]);
-        if (XP == 1) top = fmaxf(top, exps.gtop[g]);
+    for (int g = threadIdx.x; g < max(scan, groups); g += 64 * WAVES) {   // all loads before the first wait
+        if (g < scan) mx = fmaxf(mx, exps.wmax[g]);
+        if (g < groups) {
+            x = fmaxf(x, (float)exps.group[g]);
+            top = fmaxf(top, exps.gtop[g]);
+        }
     }
-    for (int m = 1; m < 64; m <<= 1) X = max(X, __shfl_xor(X, m, 64));
-    if (XP == 1) top = wave_reduce(top, OpMax());
+    mx = wave_reduce(mx, OpMax());
+    x = wave_reduce(x, OpMax());
+    top = wave_reduce(top, OpMax());
     if (lane == 0) {
-        redf[w] = mx;
-        redw[w] = top;
-        redi[w] = X;
+        red[0][w] = mx;
+        red[1][w] = x;
+        red[2][w] = top;
     }
     __syncthreads();
-    for (int x = 0; x < WAVES; ++x) {
-        mx = fmaxf(mx, redf[x]);
-        top = fmaxf(top, redw[x]);
-        X = max(X, redi[x]);
+    for (int o = 0; o < WAVES; ++o) {
+        mx = fmaxf(mx, red[0][o]);
+        x = fmaxf(x, red[1][o]);
+        top = fmaxf(top, red[2][o]);
     }
+    X = (int)x;
     E = scale_of(mx);
-    if (XP == 1) {
-        if (!(top > 0.f)) top = 1.f;   // all weights are zero
-        X = X - exponent(top) + 1;     // |w_n / top| < 2^(its exponent - top's + 1)
-    }
+    if (!(top > 0.f)) top = 1.f;   // all weights are zero
+    X = X - exponent(top) + 1;     // |w_n / top| < 2^(its exponent - top's + 1), and so 2^k at most
 }
 // For N above MANY: once, instead of by every work-group of stage_scaled.
-template <int XP>
 __global__ void __launch_bounds__(1024) scales(Exps exps, int groups, int scan) {
     int E, X;
     float top;
-    find_scales<XP, 16>(exps, groups, scan, E, X, top);
+    find_scales<16>(exps, groups, scan, E, X, top);
     if (threadIdx.x != 0) return;
     *exps.E = E;
     *exps.X = X;
@@ -480,9 +480,9 @@ __global__ void __launch_bounds__(1024) scales(Exps exps, int groups, int scan) 
 }
 
 // Backward: rows of the table at its scale; the work-groups behind (first piece) convert the packed rows of
-// w_n H_n at theirs, in XP parts.  Unless the scales are known, each work-group finds them, and the first one
+// 2^k H_n at theirs, and take the weights apart.  Unless the scales are known, each work-group finds them, and the first one
 // writes them down.
-template <typename T, int P, int XP>
+template <typename T, int P>
 __global__ void __launch_bounds__(256) stage_scaled(const T* __restrict__ W, int ldw, int v0, int R,
                                                     int D, uint16_t* __restrict__ dst, int Dp,
                                                     long long plane, Exps exps, int groups, int scan, int known,
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(256) stage_scaled(const T* __restrict__ W, int
         X = *exps.X;
         top = *exps.wtop;
     } else {
-        find_scales<XP, 4>(exps, groups, scan, E, X, top);
+        find_scales<4>(exps, groups, scan, E, X, top);
         if (blockIdx.x == 0 && threadIdx.x == 0) {
             *exps.E = E;
             *exps.X = X;
@@ -512,9 +512,16 @@ __global__ void __launch_bounds__(256) stage_scaled(const T* __restrict__ W, int
     const int i = (blockIdx.x - tables) * 4 + w;
     if (i >= *rows.cnt) return;
     const int h = rows.hexp[i];
-    const float wn = XP == 1 ? rows.w[i] / top : rows.w[i];
-    convert_row<T, XP, false>(H + (size_t)rows.row[i] * ldh, D, Xp + (size_t)i * Dp, Dp, xplane, lane, h,
-                              __builtin_ldexpf(wn, h - X));
+    // A weight of zero (or none: G has the infinity or NaN) takes nothing of H.
+    const float share = rows.w[i] / top;
+    const int k = exponent(share);
+    const bool some = k != NO_EXP;
+    convert_row<T, P, false>(H + (size_t)rows.row[i] * ldh, D, Xp + (size_t)i * Dp, Dp, xplane, lane, h,
+                             some ? __builtin_ldexpf(1.f, k + h - X) : 0.f);
+    if (lane == 0) {
+        rows.w[i] = some ? __builtin_ldexpf(share, -k) : share;
+        rows.rest[i] = some ? __builtin_ldexpf(top, k) : 1.f;
+    }
 }
 
 // ---- teachers ------------------------------------------------------------------------------------
@@ -1249,17 +1256,17 @@ __global__ void __launch_bounds__(S::THREADS) vocab_gemm(Prod g, Epi epi) {
 }
 
 // dH and dW of a piece in one launch: the first `first` work-groups are dH's, splits one after the
-// other.  W in P parts, G and w_n H_n in GP.
+// other.  H and W in P parts, G in GP.
 template <class S, int P, int GP, class EpiH, class EpiW>
 __global__ void __launch_bounds__(S::THREADS) vocab_grads(Prod gh, EpiH eh, int tiles_h, int first, Prod gw,
                                                           EpiW ew, int tiles_w) {
-    __shared__ __attribute__((aligned(16))) uint16_t ring[std::max(ring_of<S, true, GP, P>(), ring_of<S, false, GP, GP>())];
+    __shared__ __attribute__((aligned(16))) uint16_t ring[ring_of<S, true, GP, P>()];
     const int b = blockIdx.x;
     if (b < first)
         gemm_form<S, true, false, TOK_M, GP, P>(ring, gh, eh, b % tiles_h, tiles_h, b / tiles_h);
     else
-        gemm_form<S, false, false, TOK_K, GP, GP>(ring, gw, ew, (b - first) % tiles_w, tiles_w,
-                                                  (b - first) / tiles_w);
+        gemm_form<S, false, false, TOK_K, GP, P>(ring, gw, ew, (b - first) % tiles_w, tiles_w,
+                                                 (b - first) / tiles_w);
 }
 
 // Forward: rows are table rows, columns packed rows.  A lane holds half of the wave's logits of
@@ -1328,14 +1335,13 @@ struct EpiLse {
     }
 };
 
-// Backward: rows are packed rows, columns the piece's table rows.  G = 2^14 (p - q) in GP fp16 parts,
-// without the row's weight, whose range over the rows it need not hold.  Columns past the table's end
-// up to the tile's are zero.
+// Backward: rows are packed rows, columns the piece's table rows.  G = 2^14 m (p - q) in GP fp16
+// parts.  Columns past the table's end up to the tile's are zero.
 template <int GP, bool HARD>
 struct EpiG {
     static constexpr bool LDS = true;
     float c;
-    const float* lse;
+    const float *lse, *w;
     const int *target, *h, *E;
     int v0;
     uint16_t* G;
@@ -1354,6 +1360,7 @@ struct EpiG {
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int row = row0 + reg_row(a, 4 * r4, lane);
                 const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + row);
+                const f32x4 w4 = *reinterpret_cast<const f32x4*>(w + row);
                 const i32x4 h4 = *reinterpret_cast<const i32x4*>(h + row);
                 i32x4 t4;
                 if constexpr (HARD) t4 = *reinterpret_cast<const i32x4*>(target + row);
@@ -1361,6 +1368,7 @@ struct EpiG {
                 for (int e = 0; e < 4; ++e) {
                     const float k = __builtin_ldexpf(c1, h4[e] + table);
                     const float l = GP == 1 ? l4[e] * LOG2E : l4[e];
+                    const float m = 0x1p14f * w4[e];
 #pragma unroll
                     for (int b = 0; b < FN; ++b) {
                         const float x = __builtin_fmaf(k, acc[a][b][4 * r4 + e], -l);
@@ -1368,7 +1376,7 @@ struct EpiG {
                         if constexpr (HARD)
                             if (col + 32 * b == t4[e] - v0) p -= 1.f;
                         uint16_t parts[GP];
-                        to_parts<GP>(col + 32 * b < N ? 0x1p14f * p : 0.f, parts);
+                        to_parts<GP>(col + 32 * b < N ? m * p : 0.f, parts);
 #pragma unroll
                         for (int q = 0; q < GP; ++q) v[q][b][4 * r4 + e] = parts[q];
                     }
@@ -1410,8 +1418,8 @@ struct EpiAcc {
     }
 };
 
-// A gradient's rows and their scales: dH's packed rows go to their places, times w_n 2^(E - 14); dW's
-// stay in order, times 2^(X - 14), and wtop where w_n H_n has one part.
+// A gradient's rows and their scales: dH's packed rows go to their places, times wtop 2^k 2^(E - 14); dW's
+// stay in order, times wtop 2^(X - 14).
 template <typename OT>
 struct Grad {
     OT* C;
@@ -1420,7 +1428,8 @@ struct Grad {
     const float* w;
     int own;               // w is the rows', else one for all
     __device__ int scale() const { return *exp - 14; }
-    __device__ float weight(int i) const { return w ? w[own ? i : 0] : 1.f; }
+    __device__ float common() const { return own ? 1.f : *w; }
+    __device__ float weight(int i, float common) const { return own ? w[i] : common; }
     __device__ OT* at(int i) const { return C + (size_t)(row ? row[i] : i) * ldc; }
     __device__ void put(OT* to, float v) const {
         if constexpr (sizeof(OT) == 4) {
@@ -1441,6 +1450,7 @@ struct EpiOut {
     __device__ void run(const f32x16 (&acc)[FM][FN], int M, int N, int row0, int col0, int lane, int,
                         uint16_t* lds) const {
         const int s = out.scale();
+        const float common = out.common();
         if constexpr (LDS) {
             if (!out.accumulate) {
 #pragma unroll
@@ -1449,7 +1459,7 @@ struct EpiOut {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int row = row0 + reg_row(a, r, lane);
-                        const float w = row < M ? out.weight(row) : 0.f;
+                        const float w = row < M ? out.weight(row, common) : 0.f;
 #pragma unroll
                         for (int b = 0; b < FN; ++b) v[b][r] = rne_bf16(__builtin_ldexpf(acc[a][b][r], s) * w);
                     }
@@ -1475,7 +1485,7 @@ struct EpiOut {
                 const int row = row0 + reg_row(a, r, lane);
                 if (row >= M) continue;
                 OT* to = out.at(row);
-                const float w = out.weight(row);
+                const float w = out.weight(row, common);
 #pragma unroll
                 for (int b = 0; b < FN; ++b) {
                     const int col = col0 + 32 * b + (lane & 31);
@@ -1572,7 +1582,7 @@ __global__ void __launch_bounds__(256) lse_join_few(const float2* __restrict__ p
     out.put(i, m, s);
 }
 
-// The entries of G at the teacher's tokens inside a piece, from the fp32 logits: p - q, q
+// The entries of G at the teacher's tokens inside a piece, from the fp32 logits: m (p - q), q
 // summed where a token occurs more than once: by its first entry (SUMS: teacher_sums has done it), else each of
 // its entries writes the same value.
 template <int GP, bool SUMS>
@@ -1584,7 +1594,7 @@ __global__ void __launch_bounds__(256) teacher_entries(Rows rows, Teacher t, int
     const int i = (int)grid_index();
     if (i >= *rows.cnt) return;
     const size_t at = (size_t)rows.row[i] * t.K, from = (size_t)i * t.K;
-    const float lse = rows.lse[i];
+    const float m = 0x1p14f * rows.w[i], lse = rows.lse[i];
     for (int k = threadIdx.x; k < t.K; k += 256) {
         const int id = t.id[at + k];
         if (id < v0 || id >= v0 + R || !entry_counts(t, at + k, V)) continue;
@@ -1597,7 +1607,7 @@ __global__ void __launch_bounds__(256) teacher_entries(Rows rows, Teacher t, int
                 if (t.id[at + j] == id) sum += q[from + j];
         }
         uint16_t parts[GP];
-        to_parts<GP>(0x1p14f * (__expf(z[from + k] - lse) - sum), parts);
+        to_parts<GP>(m * (__expf(z[from + k] - lse) - sum), parts);
         uint16_t* to = G + (size_t)i * ldg + (id - v0);
 #pragma unroll
         for (int p = 0; p < GP; ++p) to[p * plane] = parts[p];
@@ -1630,7 +1640,7 @@ __global__ void __launch_bounds__(256) finish(Finish<OT> h, Finish<OT> w, int D)
     for (int s = 0; s < f.splits; ++s)
         v += *reinterpret_cast<const f32x4*>(f.acc + s * f.split + (size_t)i * f.lda + c);
     const int e = f.out.scale();
-    const float wi = f.out.weight((int)i);
+    const float wi = f.out.weight((int)i, f.out.common());
     OT* to = f.out.at((int)i) + c;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -2154,12 +2164,12 @@ Choice pick(long long M, long long N, long long K, int kinds, bool split) {
 
 // The workspace: a part whose size the shapes give, and a piece whose size is what is left.
 struct Plan {
-    int parts, gparts;        // of H and W; of G and w_n H_n
+    int parts, gparts;        // of H and W; of G
     int Dp, Nt;               // columns and rows as the workspace holds them
     bool direct;              // the table is read in place
     Kind lse, g, dh, dw;      // the products' tiles
     int splits, wsplits;      // of dH and dW
-    size_t ints, w, lses, base, q, z, state, Hp, Xp, acc, wacc;
+    size_t ints, w, lses, rest, base, q, z, state, Hp, Xp, acc, wacc;
     size_t piece;             // first byte of the piece's buffers
     size_t per_block;         // bytes of a piece per 256 table rows
 };
@@ -2177,7 +2187,7 @@ Plan make_plan(int dtype, int gtype, int N, int V, int D, int K, const void* W, 
     p.lse = pick(V, N, D, kinds_of(p.parts, p.parts), false).kind;
     p.g = pick(N, V, D, kinds_of(p.parts, p.parts), false).kind;
     const Choice dh = pick(N, D, V, kinds_of(p.gparts, p.parts), true),
-                 dw = pick(V, D, N, kinds_of(p.gparts, p.gparts), true);
+                 dw = pick(V, D, N, kinds_of(p.gparts, p.parts), true);
     p.dh = dh.kind;
     p.dw = dw.kind;
     p.splits = dh.splits;
@@ -2191,13 +2201,14 @@ Plan make_plan(int dtype, int gtype, int N, int V, int D, int K, const void* W, 
     p.ints = take(((size_t)4 * p.Nt + 2 * (p.Nt / PACK) + 64 + SCAN + p.Nt / COUNT + 1) * 4);   // cnt and scales, row, target, ...
     p.w = take((size_t)p.Nt * 4);
     p.lses = take((size_t)p.Nt * 4);
+    p.rest = take((size_t)p.Nt * 4);
     p.base = take((size_t)p.Nt * 4);
     p.q = take((size_t)N * K * 4);
     p.z = take((size_t)N * K * 4);
     p.Hp = take((size_t)p.parts * N * p.Dp * 2);
     if (backward) {
         p.acc = take((size_t)p.splits * N * p.Dp * 4);
-        p.Xp = take((size_t)p.gparts * N * p.Dp * 2);
+        p.Xp = take((size_t)p.parts * N * p.Dp * 2);
         p.per_block = (size_t)p.gparts * N * 256 * 2;
         // dW's sums over splits of the rows: a piece's, fp32.
         if (p.wsplits > 1) p.per_block += (size_t)p.wsplits * 256 * p.Dp * 4;
@@ -2329,7 +2340,8 @@ Work lay_out(const Plan& p, void* ws) {
     auto array = [&](int k) { return ints + 64 + (size_t)k * p.Nt; };
     Work w{};
     w.p = p;
-    w.rows = {ints, array(0), array(1), array(2), (float*)(b + p.w), (float*)(b + p.lses)};
+    w.rows = {ints, array(0), array(1), array(2), (float*)(b + p.w), (float*)(b + p.lses),
+              (float*)(b + p.rest)};
     w.flags = array(3);
     const int groups = p.Nt / PACK;
     w.exps = {nullptr, ints + 1, ints + 2, (float*)(ints + 3), array(4), (float*)(array(4) + groups),
@@ -2470,11 +2482,11 @@ int gradients(const char* op, const Plan& p, const Prod* gh, const EpiH& eh, con
         return check_launch(op);
     }
     if (gh) DH_TRY((product<true, false, TOK_M, GP, P>(op, p.dh, *gh, p.splits, eh)));
-    if (gw) DH_TRY((product<false, false, TOK_K, GP, GP>(op, p.dw, *gw, p.wsplits, ew)));
+    if (gw) DH_TRY((product<false, false, TOK_K, GP, P>(op, p.dw, *gw, p.wsplits, ew)));
     return DH_OK;
 }
 
-// P parts of H and W, GP of G and w_n H_n.
+// P parts of H and W, GP of G.
 template <typename T, int P, int GP, typename OT>
 int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     const Plan p = make_plan(h.dtype, d.type, h.N, h.V, h.D, h.target ? 0 : h.teacher.K, h.W, h.ldw);
@@ -2502,15 +2514,15 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
     }
     const int groups = (h.N + PACK - 1) / PACK;
     if (h.N > MANY) {
-        scales<GP><<<1, 1024, 0, stream()>>>(w.exps, groups, scan);
+        scales<<<1, 1024, 0, stream()>>>(w.exps, groups, scan);
         DH_TRY(check_launch(h.op));
     }
-    const Grad<OT> to_dH{(OT*)d.dH, d.lddh, d.acc_dH, w.rows.row, w.exps.E, w.rows.w, 1};
+    const Grad<OT> to_dH{(OT*)d.dH, d.lddh, d.acc_dH, w.rows.row, w.exps.E, w.rows.rest, 1};
     for (int v0 = 0;; v0 += rows) {
         const int R = h.V - v0 < rows ? h.V - v0 : rows;
         const bool last = h.V - v0 <= rows;
         const int tables = (R + 3) / 4;
-        stage_scaled<T, P, GP><<<tables + (v0 == 0 ? (h.N + 3) / 4 : 0), 256, 0, stream()>>>(
+        stage_scaled<T, P><<<tables + (v0 == 0 ? (h.N + 3) / 4 : 0), 256, 0, stream()>>>(
             (const T*)h.W, h.ldw, v0, R, h.D, staged, p.Dp, wplane, w.exps, groups, scan, v0 > 0 || h.N > MANY, tables,
             w.rows, (const T*)h.H, h.ldh, w.Xp, hplane);
         DH_TRY(check_launch(h.op));
@@ -2518,11 +2530,11 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         if (h.target) {
             DH_TRY((product<true, true, TOK_M, P, P>(
                 h.op, p.g, g, 1,
-                EpiG<GP, true>{h.c, w.rows.lse, w.rows.target, w.rows.hexp, w.exps.E, v0, G, rows, gplane})));
+                EpiG<GP, true>{h.c, w.rows.lse, w.rows.w, w.rows.target, w.rows.hexp, w.exps.E, v0, G, rows, gplane})));
         } else {
             DH_TRY((product<true, true, TOK_M, P, P>(
                 h.op, p.g, g, 1,
-                EpiG<GP, false>{h.c, w.rows.lse, nullptr, w.rows.hexp, w.exps.E, v0, G, rows, gplane})));
+                EpiG<GP, false>{h.c, w.rows.lse, w.rows.w, nullptr, w.rows.hexp, w.exps.E, v0, G, rows, gplane})));
             auto entries = by_sums(h.V, h.teacher.K) ? teacher_entries<GP, true> : teacher_entries<GP, false>;
             entries<<<long_grid(h.N), 256, 0, stream()>>>(w.rows, h.teacher, h.V, v0, R, w.q, w.z, G, rows, gplane);
             DH_TRY(check_launch(h.op));
@@ -2531,7 +2543,7 @@ int backward(const Head& h, const Grads& d, void* ws, size_t ws_bytes) {
         const Prod gw{G, w.Xp, rows, p.Dp, gplane, hplane, R, h.D, h.N, 0, w.rows.cnt};
         const Prod *ph = d.dH ? &gh : nullptr, *pw = d.dW ? &gw : nullptr;
         const Grad<OT> to_dW{d.dW ? (OT*)d.dW + (size_t)v0 * d.lddw : nullptr, d.lddw, d.acc_dW, nullptr, w.exps.X,
-                             GP == 1 ? w.exps.wtop : nullptr, 0};
+                             w.exps.wtop, 0};
         // Straight to the gradient, or as sums that the last launch adds.
         const bool direct_h = one && p.splits == 1, direct_w = p.wsplits == 1;
         const EpiAcc sum_h{w.acc, p.Dp, v0 == 0, hplane}, sum_w{wacc, p.Dp, 1, wplane};

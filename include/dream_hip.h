@@ -360,10 +360,10 @@ int dh_linear_xent_fwd(int dtype, int N, int V, int D, float scale, const void* 
                        void* d_ws, size_t ws_bytes);
 /* Its gradient from the forward's lse: G = dloss[n] scale (softmax(z) - onehot(target)),
  * dH = G W, dW = G^T H.  d_dloss (N, fp32) may be NULL: ones.  d_dH or d_dW may be NULL: not
- * computed.  acc_dH / acc_dW add into them.  bf16 gradients: softmax - onehot and the rows of
- * dloss H are taken to 2^-11 of themselves, or 2^-38 (of 1, and of the largest), before the products:
- * an eighth of the result's own rounding.  DH_F32 gradients of bf16 inputs are as exact as those of fp32
- * inputs, for twice the products.
+ * computed.  acc_dH / acc_dW add into them.  bf16 gradients: softmax - onehot, times the mantissa of the
+ * row's weight, is taken to 2^-11 of itself or 2^-38 before the products: an eighth of the result's own
+ * rounding.  DH_F32 gradients of bf16 inputs are as exact as those of fp32 inputs, for five products
+ * where bf16 ones take three.
  * dH must not overlap H, nor dW W. */
 int dh_linear_xent_bwd(int dtype, int N, int V, int D, float scale, const void* d_H, int ldh,
                        const void* d_W, int ldw, const int* d_target, const float* d_lse,

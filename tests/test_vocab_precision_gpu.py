@@ -3,8 +3,8 @@
 Errors of a gradient's value, with S the sum of the sizes of its terms w (p + q) |operand|:
   p               logits to 1e-5 (fp32 sums, operands as they are), so p to 1e-5 of itself; the sum
                   over the terms in fp32: together at most 2e-5 S, what the losses are held to
-  G = p - q, w H  in one fp16 part (bf16 gradients): 2^-11 of themselves each, 2^-10 S together; in two
-                  parts (fp32 gradients): 2^-23, within the 2e-5
+  G = w (p - q)   in one fp16 part (bf16 gradients): 2^-11 of itself; in two parts (fp32 gradients): 2^-23, within
+                  the 2e-5
   bf16 result     one rounding, 2^-8 of the value
 An fp16 part's values lie 2^-24 apart at least, so it is off by 2^-25 beside a largest value of 2^13 (w H; W of
 2^14, G of 2^14): 2^-38 of the largest, in two parts 2^-49.  FLOOR adds that up over the terms.
@@ -48,8 +48,8 @@ def sizes(c, lse, grad):
     return (dH, P.T @ H[k]), [FLOOR[grad] * x + 2.0 ** -126 for x in low]
 
 
-def check(c, grad, accumulate=False, extra=0, part=2.0 ** -10):
-    """All four results to the bounds above; `part` is what one part of G and of w H loses."""
+def check(c, grad, accumulate=False, extra=0, part=2.0 ** -11):
+    """All four results to the bounds above; `part` is what one part of G loses."""
     dH, dW, loss, lse, old = gradients(c, grad, accumulate, extra)
     ref = c.ref()
     close(loss, ref[0], F32_TOL, floor=1.0)
@@ -123,7 +123,7 @@ def test_gradients_keep_rows_of_any_weight(weights, grad):
     dH, dW, _, lse, _ = gradients(c, grad)
     ref = c.ref()
     S, _ = sizes(c, ref[1], grad)
-    tol = F32_TOL + (2.0 ** -8 + 2.0 ** -10 if grad == "bf16" else 0)
+    tol = F32_TOL + (2.0 ** -8 + 2.0 ** -11 if grad == "bf16" else 0)
     rows = np.maximum(S[0].max(1, keepdims=True), 2.0 ** -110)
     assert (np.abs(dH - ref[2]) <= 2 * tol * rows).all()
     close(dW, ref[3], 2 * tol, floor=max(S[1].max(), 2.0 ** -110))
@@ -131,9 +131,13 @@ def test_gradients_keep_rows_of_any_weight(weights, grad):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("k", [-60, 0, 60])
-def test_gradients_of_operands_of_any_scale(k):
+@pytest.mark.parametrize("weights", ["any", "zero"])
+def test_gradients_of_operands_of_any_scale(k, weights):
     """H 2^k and W 2^-k: bf16 has fp32's range."""
     c = Loss(70, 300, 40, "bf16", seed=3)
+    if weights == "zero":
+        c.dloss[:] = 0
+        c.dlb = DB.from_numpy(c.dloss)
     c.Hb, c.H = store(np.ldexp(c.H, k), "bf16")
     c.Wb, c.W = store(np.ldexp(c.W, -k), "bf16")
     for grad in ("f32", "bf16"):
