@@ -235,8 +235,8 @@ struct Targets {
 // flag[n] = 0 where row n has an entry, -1 where it has none: for so many entries that pack_rows
 // had better not look for them again and again (2048 rows x 32: packing 16.0 us alone, 8.3 with the
 // flags, which take 5.1), or for so many of a row that one without entries, which is known only after all,
-// holds its group up (200 x 100 entries x 2000 x 256 bf16, 0.3 of the rows padding, forward and gradient 85 us
-// without and 62 with flags; without padding 59 and 63).  A wave per row.
+// holds its group up (200 x 100 entries x 2000 x 256 bf16, 0.3 of the rows padding, forward and gradient 86 us
+// without and 66 with flags; without padding 64 and 67).  A wave per row.
 __global__ void __launch_bounds__(256) teacher_flags(Teacher t, int N, int V, int* __restrict__ flag) {
     const int lane = threadIdx.x & 63;
     const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(1024) scales(Exps exps, int groups, int scan) 
 
 // Backward: rows of the table at its scale; the work-groups behind (first piece) convert the packed rows of
 // 2^k H_n at theirs, and take the weights apart.  Unless the scales are known, each work-group finds them, and the first one
-// writes them down.
+// writes them down.  HBM-bound: 131072 x 2048 bf16 187 us, 5.7 TB/s (and pack_rows' scan before it 133 us, 4.0 TB/s).
 template <typename T, int P>
 __global__ void __launch_bounds__(256) stage_scaled(const T* __restrict__ W, int ldw, int v0, int R,
                                                     int D, uint16_t* __restrict__ dst, int Dp,
@@ -1242,12 +1242,12 @@ __device__ inline void gemm_form(uint16_t* ring, const Prod& g, const Epi& epi, 
     else gemm_tile<S, AK, BK, TOK, PA, PB>(ring, g, epi, tile, tiles, split);
 }
 
-// The four products.  Bound by the matrix cores under the card's power limit (1.54 to 1.65 GHz).  Measured for
-// 8192 rows x 131072 x 2048 bf16, 4.4 TFLOP each, in ms, PFLOP/s and share of the time that the matrix
-// cores are busy: statistics 3.58 / 1.23 / 76%, G 4.02 / 1.09 / 64% (exponentials, and 16-bit G
-// through LDS), dH 3.26 / 1.35 / 84%, dW 3.84 / 1.14 / 67% (both operands by transposing reads, 32-k
+// The four products.  Bound by the matrix cores, at a clock that falls under them (by the cycles counted at most
+// 1.55 to 1.71 of 2.4 GHz).  Measured for 8192 rows x 131072 x 2048 bf16, 4.4 TFLOP each, in ms, PFLOP/s and share of
+// the cycles that the matrix cores are busy: statistics 3.48 / 1.26 / 76%, G 3.90 / 1.13 / 63% (exponentials, and
+// 16-bit G through LDS), dH 3.28 / 1.34 / 82%, dW 3.76 / 1.17 / 67% (both operands by transposing reads, 32-k
 // stages); a bf16 product of 8192^3 by the vendor's library reaches 1.23 here.  2048 x 32000 x 1024 fp32,
-// 0.134 TFLOP each, in us and TFLOP/s of fp32: 373 / 360, 408 / 329, 346 / 388, 419 / 321; the fp32 matrix
+// 0.134 TFLOP each, in us and TFLOP/s of fp32: 342 / 392, 375 / 358, 329 / 408, 371 / 362; the fp32 matrix
 // cores themselves end at 157.
 template <class S, bool AK, bool BK, int TOK, int PA, int PB, class Epi>
 __global__ void __launch_bounds__(S::THREADS) vocab_gemm(Prod g, Epi epi) {

@@ -13,7 +13,8 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("dtype,grad", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
 @pytest.mark.parametrize("N,V,K", [(40, 50, 200), (3, 50, 200), (40, 4097, 1100), (9, 4097, 1100), (20, 300, 128), (20, 300, 129),
-                                   (17, 13000, 3000), (16, 13000, 300), (40, 8192, 8192)])
+                                   (17, 13000, 3000), (16, 13000, 300), (40, 8192, 8192),
+                                   (11000, 50, 130)])
 def test_many_entries(N, V, K, dtype, grad):
     check(Loss(N, V, 40, dtype, K=K, T=2.0, pad=0.2, seed=K), grad)
 
