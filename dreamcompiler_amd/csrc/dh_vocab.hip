@@ -374,8 +374,8 @@ __global__ void __launch_bounds__(1024) pack_rows(Pack a) {
     int most = NO_EXP;
     float top = 0.f;   // the weight's size, where finite
     if (keep) {
-        const int h = convert_row<T, P, true>(H + (size_t)n * a.ldh, D, a.Hp + (size_t)i * a.Dp, a.Dp,
-                                                  a.plane, lane);
+        const int h = convert_row<T, P, true>(H + (size_t)n * a.ldh, D, a.Hp + (size_t)i * a.Dp, a.Dp, a.plane,
+                                              lane);
         const int target = a.targets.target ? a.targets.target[n] : 0;
         if (a.base) {
             const float d = row_dot(H + (size_t)n * a.ldh, W + (size_t)target * a.ldw, D, lane);
@@ -1427,8 +1427,10 @@ struct Grad {
     const int *row, *exp;
     const float* w;
     int own;               // w is the rows', else one for all
-    __device__ int scale() const { return *exp - 14; }
-    __device__ float common() const { return own ? 1.f : *w; }
+    // wtop in two: its power of two goes with the scale, so that a sum of large H and a small weight stay
+    // within fp32 between the two steps.
+    __device__ int scale() const { return *exp - 14 + (own ? 0 : __builtin_amdgcn_frexp_expf(*w)); }
+    __device__ float common() const { return own ? 1.f : __builtin_amdgcn_frexp_mantf(*w); }
     __device__ float weight(int i, float common) const { return own ? w[i] : common; }
     __device__ OT* at(int i) const { return C + (size_t)(row ? row[i] : i) * ldc; }
     __device__ void put(OT* to, float v) const {

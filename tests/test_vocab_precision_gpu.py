@@ -157,3 +157,24 @@ def test_products_whose_low_parts_all_add_up(N, V, D):
     c.Wb, c.W = store(np.ldexp(one, r.integers(-3, 1, (V, 1)) * np.ones((1, D), int) - int(np.log2(D)) + 4), "f32")
     assert 5 < (c.H @ c.W.T).max() < 25
     check(c, "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,grad", [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("k,weight", [(120, -110), (-60, 60)])
+def test_large_operands_of_small_weights(k, weight, dtype, grad):
+    """w H is within fp32 where H's sum over the rows is not."""
+    c = Loss(400, 60, 40, dtype, seed=3)
+    c.Hb, c.H = store(np.ldexp(np.abs(c.H), k), dtype)
+    c.Wb, c.W = store(np.ldexp(c.W, -k), dtype)
+    c.ids = ints(np.full(c.N, 3))
+    c.q[:] = 0
+    c.q[:, 3] = 1
+    c.dloss = np.ldexp(c.dloss, weight).astype(np.float32)
+    c.dlb = DB.from_numpy(c.dloss)
+    dH, dW, *_ = gradients(c, grad)
+    ref = c.ref()
+    S, low = sizes(c, ref[1], grad)
+    tol = F32_TOL + (2.0 ** -8 + 2.0 ** -11 if grad == "bf16" else 0)
+    assert np.isfinite(dW).all() and (np.abs(dW - ref[3]) <= 2 * tol * S[1] + low[1]).all()
+    assert np.isfinite(dH).all() and (np.abs(dH - ref[2]) <= 2 * tol * S[0] + low[0]).all()
