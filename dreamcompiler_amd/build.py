@@ -33,6 +33,9 @@ HIP_SOURCES = [
     "dh_f64.hip",
     "dh_embedding.hip",
     "dh_vocab.hip",
+    "dh_qk_norm.hip",
+    "dh_kv_cache.hip",
+    "dh_paged_attention.hip",
 ]
 RT_SOURCES = ["dream_rt.cpp"]
 

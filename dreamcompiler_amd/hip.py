@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(PKG, "lib", "libdream_hip.so")
 
 DH_OK, DH_ERR_NO_DEVICE, DH_ERR_INVALID, DH_ERR_OOM, DH_ERR_HIP, DH_ERR_UNSUPPORTED = range(6)
 F32, BF16, F64 = 0, 1, 2
+I8, F8 = 3, 4    # values of a key-value cache
 _DT = {np.dtype(np.float32): F32, np.dtype(np.uint16): BF16, np.dtype(np.float64): F64}
 
 _vp = ctypes.c_void_p
@@ -96,6 +97,16 @@ _SIGS = {
                                    _vp, _sz]),
     "dh_linear_distill_bwd": (_i, [_i, _i, _i, _i, _i, _f, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp,
                                    _vp, _i, _i, _vp, _i, _i, _i, _vp, _sz]),
+    "dh_rope_table": (_i, [_i, _i, _d, _vp]),
+    "dh_qk_norm_rope_fwd": (_i, [_i] * 8 + [_f, _vp, _vp, _i] + [_vp] * 10),
+    "dh_qk_norm_rope_bwd_workspace": (_sz, [_i]),
+    "dh_qk_norm_rope_bwd": (_i, [_i] * 8 + [_f, _vp, _vp, _i] + [_vp] * 6 + [_i] + [_vp] * 4
+                            + [_i] + [_vp] * 6 + [_i, _vp, _sz]),
+    "dh_kv_cache_write": (_i, [_i] * 6 + [_vp] * 6 + [_i, _i, _vp, _i] + [_vp] * 4),
+    "dh_kv_cache_read": (_i, [_i] * 6 + [_vp] * 6 + [_i, _i, _vp, _i] + [_vp] * 4),
+    "dh_paged_attention_workspace": (_sz, [_i] * 6),
+    "dh_paged_attention": (_i, [_i] * 6 + [_f, _i, _vp, _vp, _vp] + [_i] * 3 + [_vp, _i]
+                           + [_vp] * 8 + [_sz]),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -397,6 +408,71 @@ def linear_distill_bwd(dtype, N, V, D, K, T, H, ldh, W, ldw, top_id, top_logit, 
                                        _p(top_id), _p(top_logit), _p(lse), _p(dloss), _p(dH), lddh,
                                        int(acc_dH), _p(dW), lddw, int(acc_dW), grad_type, _p(ws),
                                        int(ws_bytes)), "dh_linear_distill_bwd")
+
+
+# Norm and rotation of queries and keys, a paged key-value cache and attention over it
+# (include/dream_hip.h).  Strides are tuples in elements: (sequence, token, head) for the norm,
+# (token, head) for the cache, (sequence, head) for the attention.
+def _strides(v):
+    return None if v is None else (_ll * len(v))(*[int(x) for x in v])
+
+
+def rope_table(P, R, base, table):
+    check(load().dh_rope_table(P, R, float(base), _p(table)), "dh_rope_table")
+
+
+def qk_norm_rope_fwd(dtype, B, S, Hq, Hk, D, R, pairs, eps, pos, table, P, Q, q_strides, K,
+                     k_strides, gq, gk, Qo, qo_strides, Ko, ko_strides):
+    check(load().dh_qk_norm_rope_fwd(dtype, B, S, Hq, Hk, D, R, int(pairs), float(eps), _p(pos),
+                                     _p(table), P, _p(Q), _strides(q_strides), _p(K),
+                                     _strides(k_strides), _p(gq), _p(gk), _p(Qo),
+                                     _strides(qo_strides), _p(Ko), _strides(ko_strides)),
+          "dh_qk_norm_rope_fwd")
+
+
+def qk_norm_rope_bwd_workspace(D):
+    return load().dh_qk_norm_rope_bwd_workspace(D)
+
+
+def qk_norm_rope_bwd(dtype, B, S, Hq, Hk, D, R, pairs, eps, pos, table, P, Q, q_strides, K,
+                     k_strides, gq, gk, dout_type, dQo, dqo_strides, dKo, dko_strides, grad_type,
+                     dQ, dq_strides, dK, dk_strides, dgq, dgk, accumulate, ws, ws_bytes):
+    check(load().dh_qk_norm_rope_bwd(dtype, B, S, Hq, Hk, D, R, int(pairs), float(eps), _p(pos),
+                                     _p(table), P, _p(Q), _strides(q_strides), _p(K),
+                                     _strides(k_strides), _p(gq), _p(gk), dout_type, _p(dQo),
+                                     _strides(dqo_strides), _p(dKo), _strides(dko_strides),
+                                     grad_type, _p(dQ), _strides(dq_strides), _p(dK),
+                                     _strides(dk_strides), _p(dgq), _p(dgk), int(accumulate),
+                                     _p(ws), int(ws_bytes)), "dh_qk_norm_rope_bwd")
+
+
+def kv_cache_write(dtype, cache_type, B, N, Hk, D, K, k_strides, V, v_strides, first, len_, pages,
+                   page, table, ld_table, Kc, Vc, Ks=None, Vs=None):
+    check(load().dh_kv_cache_write(dtype, cache_type, B, N, Hk, D, _p(K), _strides(k_strides),
+                                   _p(V), _strides(v_strides), _p(first), _p(len_), pages, page,
+                                   _p(table), ld_table, _p(Kc), _p(Vc), _p(Ks), _p(Vs)),
+          "dh_kv_cache_write")
+
+
+def kv_cache_read(dtype, cache_type, B, N, Hk, D, K, k_strides, V, v_strides, first, len_, pages,
+                  page, table, ld_table, Kc, Vc, Ks=None, Vs=None):
+    check(load().dh_kv_cache_read(dtype, cache_type, B, N, Hk, D, _p(K), _strides(k_strides),
+                                  _p(V), _strides(v_strides), _p(first), _p(len_), pages, page,
+                                  _p(table), ld_table, _p(Kc), _p(Vc), _p(Ks), _p(Vs)),
+          "dh_kv_cache_read")
+
+
+def paged_attention_workspace(cache_type, B, Hq, Hk, D, max_len):
+    return load().dh_paged_attention_workspace(cache_type, B, Hq, Hk, D, max_len)
+
+
+def paged_attention(dtype, cache_type, B, Hq, Hk, D, scale, window, Q, q_strides, len_, max_len,
+                    pages, page, table, ld_table, Kc, Vc, Ks, Vs, O, o_strides, lse, ws, ws_bytes):
+    check(load().dh_paged_attention(dtype, cache_type, B, Hq, Hk, D, float(scale), int(window),
+                                    _p(Q), _strides(q_strides), _p(len_), max_len, pages, page,
+                                    _p(table), ld_table, _p(Kc), _p(Vc), _p(Ks), _p(Vs), _p(O),
+                                    _strides(o_strides), _p(lse), _p(ws), int(ws_bytes)),
+          "dh_paged_attention")
 
 
 class Timer:

@@ -39,6 +39,9 @@ enum {
 };
 
 enum { DH_F32 = 0, DH_BF16 = 1, DH_F64 = 2 };
+/* Values of a key-value cache only: 8-bit integers -127 .. 127, and e4m3 floats (1.4.3, largest
+ * 448, no infinities). */
+enum { DH_I8 = 3, DH_F8 = 4 };
 
 /* ---- device / init --------------------------------------------------------
  * Replaces initBackend() (runtime/backend/gpu.inc:313-361): lazy, idempotent, logs
@@ -389,6 +392,83 @@ int dh_linear_distill_bwd(int dtype, int N, int V, int D, int K, float T, const 
  * form for few rows), the splits of dH and dW, and the table rows of a piece of the forward and of the gradient
  * in ws_bytes (the whole of V in one piece is fastest; 0: too little, or the form for few rows). */
 int dh_linear_loss_plan(int dtype, int grad_type, int N, int V, int D, int K, size_t ws_bytes, int* plan);
+
+/* ---- around a decoder's attention: norm and rotation of queries and keys, a paged cache ----
+ * Additions to the reference, next to flash attention.  dtype DH_F32 or DH_BF16 for queries, keys,
+ * values and outputs.  Every sum, norm and softmax statistic is held in fp32 and results are rounded
+ * once; no floating-point atomics, so reruns are bit-identical.  No call here allocates: all can be
+ * captured.  Workspaces are the caller's, as for the vocabulary above: calls that may overlap in time
+ * need their own.
+ *
+ * cos and sin of the angles p base^(-2 i / R), i < R / 2, for positions p < P: P rows of R floats, the
+ * R / 2 cosines first (angles in fp64).  The calls below take any table of this form. */
+int dh_rope_table(int P, int R, double base, float* d_table);
+/* For every token and head of queries Q (Hq heads) and keys K (Hk heads), x being its D values:
+ *   y = x (mean x^2 + eps)^(-1/2) g,   out = y with its first R values turned by the token's position:
+ *   out[i] = y[i] cos - y[j] sin,  out[j] = y[j] cos + y[i] sin   for pairs (i, j = i + R / 2), or
+ *   with pairs != 0 (2 i, 2 i + 1);  the values past R stay y.
+ * B sequences of S tokens; d_pos (B x S) is each token's row of the table, NULL: 0 .. S - 1 in every
+ * sequence.  A position outside 0 .. P - 1 is padding: a zero row, no gradient.  R = 0 turns nothing
+ * (d_table may be NULL; d_pos, if given, still marks padding).  Weights gq, gk: D floats, NULL: ones.
+ * Strides: three of each tensor, in elements, of sequence, token and head (a row's D values lie side by
+ * side); inputs may repeat rows (stride 0), outputs must have theirs apart.  An output may be its input
+ * (same pointer, strides and type), no other overlap.  D up to 1024, R even and up to D, eps > 0,
+ * B S up to 2^31 - 2^20; Hq or Hk of 0 leaves that side out. */
+int dh_qk_norm_rope_fwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, int pairs, float eps,
+                        const int* d_pos, const float* d_table, int P, const void* d_Q,
+                        const long long* q_strides, const void* d_K, const long long* k_strides,
+                        const float* d_gq, const float* d_gk, void* d_Qo,
+                        const long long* qo_strides, void* d_Ko, const long long* ko_strides);
+/* Its gradient from the forward's inputs: with dy = dout turned back and r as above,
+ *   dgq, dgk (+)= sum of dy x r over tokens and heads,   dx = r (dy g - x r mean(dy g x r)).
+ * dQo, dKo are of dout_type, dQ, dK of grad_type: the inputs' type or DH_F32 (what dh_flash_bwd leaves).
+ * dgq, dgk are fp32 (either may be NULL); accumulate adds into them.  dQ may be dQo or Q as above. */
+size_t dh_qk_norm_rope_bwd_workspace(int D);
+int dh_qk_norm_rope_bwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, int pairs, float eps,
+                        const int* d_pos, const float* d_table, int P, const void* d_Q,
+                        const long long* q_strides, const void* d_K, const long long* k_strides,
+                        const float* d_gq, const float* d_gk, int dout_type, const void* d_dQo,
+                        const long long* dqo_strides, const void* d_dKo, const long long* dko_strides,
+                        int grad_type, void* d_dQ, const long long* dq_strides, void* d_dK,
+                        const long long* dk_strides, float* d_dgq, float* d_dgk, int accumulate,
+                        void* d_ws, size_t ws_bytes);
+/* A paged key-value cache: d_Kc and d_Vc are pages x Hk x page x D values of cache_type each (16-byte
+ * aligned): the inputs' dtype, DH_I8 or DH_F8.  8-bit types have a scale for every row of D, d_Ks and
+ * d_Vs, pages x Hk x page floats (ignored otherwise): s = max |x| / 127 or / 448 as an fp32 quotient,
+ * and the value nearest to x / s, ties to even, stands for value * s.  A row with an infinity or NaN
+ * reads back as NaN.  Token t of sequence b is in page d_table[b ld_table + t / page].  A table entry
+ * outside 0 .. pages - 1, or past the table's row, holds nothing: such tokens are not written, read as
+ * zero and are not attended.  page is a power of two from 16 to 4096, D a multiple of 16 up to 256
+ * (callers zero-pad others), B and Hk up to 65535.  Offsets are 64-bit.
+ *
+ * Writes N new tokens: rows d_first[b] .. d_first[b + 1] - 1 of K and V (strides of token and head) are the
+ * last tokens of sequence b, which holds d_len[b] of them after the call.  d_first (B + 1 values, rising)
+ * may be NULL: one each, N = B.  Rows before d_first[0] or from d_first[B] on are of no sequence.  A page
+ * that is written must be of one sequence only (the same place written twice holds either, or pieces of both). */
+int dh_kv_cache_write(int dtype, int cache_type, int B, int N, int Hk, int D, const void* d_K,
+                      const long long* k_strides, const void* d_V, const long long* v_strides,
+                      const int* d_first, const int* d_len, int pages, int page, const int* d_table,
+                      int ld_table, void* d_Kc, void* d_Vc, float* d_Ks, float* d_Vs);
+/* Reads tokens back into rows of K and V, addressed as above: rows of no sequence are left as they were. */
+int dh_kv_cache_read(int dtype, int cache_type, int B, int N, int Hk, int D, void* d_K,
+                     const long long* k_strides, void* d_V, const long long* v_strides,
+                     const int* d_first, const int* d_len, int pages, int page, const int* d_table,
+                     int ld_table, const void* d_Kc, const void* d_Vc, const float* d_Ks,
+                     const float* d_Vs);
+/* Attention of one new token of each sequence (its key and value already in the cache) over its
+ * d_len[b] tokens, the last `window` of them if window > 0:
+ *   O = softmax(scale q K^T) V,   lse = log sum exp(scale q k) (B x Hq, natural log, fp32; may be NULL).
+ * Hq is a multiple of Hk: query head h reads cache head h / (Hq / Hk).  Strides of Q and O: sequence,
+ * head.  max_len bounds the lengths (at most ld_table page; a longer sequence is cut off there): the
+ * work is split over it.  A sequence without tokens, or whose scores are all -infinity, has O = 0,
+ * lse = -infinity.  scale finite and > 0.  What a page holds past a sequence's end does not matter, NaN included. */
+size_t dh_paged_attention_workspace(int cache_type, int B, int Hq, int Hk, int D, int max_len);
+int dh_paged_attention(int dtype, int cache_type, int B, int Hq, int Hk, int D, float scale,
+                       int window, const void* d_Q, const long long* q_strides, const int* d_len,
+                       int max_len, int pages, int page, const int* d_table, int ld_table,
+                       const void* d_Kc, const void* d_Vc, const float* d_Ks, const float* d_Vs,
+                       void* d_O, const long long* o_strides, float* d_lse, void* d_ws,
+                       size_t ws_bytes);
 
 #ifdef __cplusplus
 }
