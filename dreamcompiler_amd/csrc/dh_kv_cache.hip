@@ -27,6 +27,8 @@ int check_paged(const char* op, int dtype, int cache_type, int B, int Hk, int D,
         return set_error(DH_ERR_INVALID, "%s: pages=%d, ld_table=%d", op, pages, ld);
     if (!table || !Kc || !Vc || (scaled && (!Ks || !Vs))) return set_error(DH_ERR_INVALID, "%s: null pointer", op);
     if (((uintptr_t)Kc | (uintptr_t)Vc) & 15) return set_error(DH_ERR_INVALID, "%s: cache not 16-byte aligned", op);
+    if (scaled && (((uintptr_t)Ks | (uintptr_t)Vs) & 15))
+        return set_error(DH_ERR_INVALID, "%s: scales not 16-byte aligned", op);
     int shift = 0;
     while ((1 << shift) < page) ++shift;
     c = Paged{pages, shift, Hk, D, table, ld, (void*)Kc, (void*)Vc, (float*)Ks, (float*)Vs};

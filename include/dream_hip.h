@@ -433,7 +433,7 @@ int dh_qk_norm_rope_bwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, i
                         const long long* dk_strides, float* d_dgq, float* d_dgk, int accumulate,
                         void* d_ws, size_t ws_bytes);
 /* A paged key-value cache: d_Kc and d_Vc are pages x Hk x page x D values of cache_type each (16-byte
- * aligned): the inputs' dtype, DH_I8 or DH_F8.  8-bit types have a scale for every row of D, d_Ks and
+ * aligned, scales too): the inputs' dtype, DH_I8 or DH_F8.  8-bit types have a scale for every row of D, d_Ks and
  * d_Vs, pages x Hk x page floats (ignored otherwise): s = max |x| / 127 or / 448 as an fp32 quotient,
  * and the value nearest to x / s, ties to even, stands for value * s.  A row with an infinity or NaN
  * reads back as NaN.  Token t of sequence b is in page d_table[b ld_table + t / page].  A table entry
@@ -459,7 +459,7 @@ int dh_kv_cache_read(int dtype, int cache_type, int B, int N, int Hk, int D, voi
  * d_len[b] tokens, the last `window` of them if window > 0:
  *   O = softmax(scale q K^T) V,   lse = log sum exp(scale q k) (B x Hq, natural log, fp32; may be NULL).
  * Hq is a multiple of Hk: query head h reads cache head h / (Hq / Hk).  Strides of Q and O: sequence,
- * head.  max_len bounds the lengths (at most ld_table page; a longer sequence is cut off there): the
+ * head.  max_len bounds the lengths (at most ld_table page, and 2^31 - 2^20; a longer sequence is cut off there): the
  * work is split over it.  A sequence without tokens, or whose scores are all -infinity, has O = 0,
  * lse = -infinity.  scale finite and > 0.  What a page holds past a sequence's end does not matter, NaN included. */
 size_t dh_paged_attention_workspace(int cache_type, int B, int Hq, int Hk, int D, int max_len);
