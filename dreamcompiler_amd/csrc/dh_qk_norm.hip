@@ -178,21 +178,259 @@ __global__ void __launch_bounds__(256) qk_bwd(Shape s, int gridq, Rows<const T> 
     }
 }
 
-// dg (+)= the sum of its partials, in order.
-__global__ void __launch_bounds__(256) qk_join(const float* __restrict__ part, int D, int gridq, int grid,
-                                               float* __restrict__ dgq, float* __restrict__ dgk, int acc) {
-    __shared__ float red[4][64];
+// ---- rows in pieces ------------------------------------------------------------------------------
+// Where rows begin with whole pieces of V values (16 or 8 bytes) and the values that turn together lie
+// in whole pieces too, a row is L lanes of a piece each, and a wave takes 64 / L heads of a token at
+// once: their rows usually lie side by side, and the token's cosines and sines are read once for all
+// heads.  HEADS heads make a unit: all of a token's where there are many tokens.
+template <typename T, int V>
+__device__ inline void load_piece(const T* p, float (&v)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V), aligned(V * sizeof(T) < 16 ? V * sizeof(T) : 16)));
+    const vec x = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = up(x[e]);
+}
+template <typename T, int V>
+__device__ inline void store_piece(T* p, const float (&v)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V), aligned(V * sizeof(T) < 16 ? V * sizeof(T) : 16)));
+    vec x;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = down<T>(v[e]);
+    *reinterpret_cast<vec*>(p) = x;
+}
+
+// The sum over each L lanes, in all of them.
+template <int L>
+__device__ inline float group_sum(float v) {
+    if (L > 1) v += dpp_quad_xor1(v);
+    if (L > 2) v += dpp_quad_xor2(v);
+    if (L > 4) v += dpp_half_mirror(v);
+    if (L > 8) v += dpp_row_mirror(v);
+    float lo, hi;
+    if (L > 16) {
+        halves16(v, lo, hi);
+        v = lo + hi;
+    }
+    if (L > 32) {
+        halves32(v, lo, hi);
+        v = lo + hi;
+    }
+    return v;
+}
+
+// What a lane's piece turns with: y -> y c + partner sn, the partners in another lane's piece (halves) or
+// in this one (pairs).
+template <int V>
+struct Turn {
+    float c[V], sn[V];
+    int from;   // the lane that has the partners
+    bool turns;
+    __device__ void find(const Shape& s, int piece) {
+        const int half = s.R / (2 * V), lane = threadIdx.x & 63;
+        turns = piece * V < s.R;
+        from = !turns || s.pairs ? lane : piece < half ? lane + half : lane - half;
+    }
+    __device__ void load(const Shape& s, const float* __restrict__ row, int piece) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) c[e] = 1.f, sn[e] = 0.f;
+        if (!turns) return;
+        const int half = s.R >> 1;
+        if (s.pairs) {
+            typedef float vec __attribute__((ext_vector_type(V / 2), aligned(4)));
+            const vec a = *reinterpret_cast<const vec*>(row + piece * (V / 2));
+            const vec b = *reinterpret_cast<const vec*>(row + half + piece * (V / 2));
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                c[e] = a[e / 2];
+                sn[e] = e & 1 ? b[e / 2] : -b[e / 2];
+            }
+        } else {
+            const bool second = piece * V >= half;
+            const int i = piece * V - (second ? half : 0);
+            typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
+            const vec a = *reinterpret_cast<const vec*>(row + i), b = *reinterpret_cast<const vec*>(row + half + i);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                c[e] = a[e];
+                sn[e] = second ? b[e] : -b[e];
+            }
+        }
+    }
+    // y turned; by the angle's negative with back = -1.
+    __device__ void apply(const Shape& s, float (&y)[V], float back) const {
+        float other[V];
+        if (s.pairs) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) other[e] = y[e ^ 1];
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) other[e] = __shfl(y[e], from);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = y[e] * c[e] + other[e] * (sn[e] * back);
+    }
+};
+
+struct Units {
+    int heads, per;   // heads of a unit, units of a token
+    long long n;
+};
+
+template <typename T, int V, int L>
+__global__ void __launch_bounds__(256) qk_fwd_pieces(Shape s, Units u, Rows<const T> q, Rows<const T> k,
+                                                     const float* __restrict__ gq, const float* __restrict__ gk,
+                                                     Rows<T> qo, Rows<T> ko) {
+    constexpr int G = 64 / L, AHEAD = 4;
+    const int lane = threadIdx.x & 63, piece = lane & (L - 1), sub = lane / L;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = s.H[0] + s.H[1];
+    const bool in = piece * V < s.D;
+    float wq[V], wk[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        wq[e] = gq && in ? gq[piece * V + e] : 1.f;
+        wk[e] = gk && in ? gk[piece * V + e] : 1.f;
+    }
+    Turn<V> turn;
+    turn.find(s, piece);
+    for (long long i = 4LL * blockIdx.x + wave; i < u.n; i += 4LL * gridDim.x) {
+        const long long n = i / u.per;
+        const int h0 = (int)(i - n * u.per) * u.heads, h1 = min(h0 + u.heads, heads);
+        const int b = (int)(n / s.S), t = (int)(n - (long long)b * s.S);
+        const int p = position(s, b, t);
+        turn.load(s, s.table + (long long)max(p, 0) * s.R, piece);
+        for (int h = h0 + sub; h - sub < h1; h += AHEAD * G) {
+            float x[AHEAD][V];
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int hh = h + a * G;
+                const bool key = hh >= s.H[0];
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[a][e] = 0.f;
+                if (hh < h1 && in)
+                    load_piece<T, V>((key ? k.at(b, t, hh - s.H[0]) : q.at(b, t, hh)) + piece * V, x[a]);
+            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int hh = h + a * G;
+                const bool key = hh >= s.H[0];
+                if (hh - sub >= h1) break;
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum += x[a][e] * x[a][e];
+                const float inv = 1.f / sqrtf(group_sum<L>(sum) / s.D + s.eps);
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[a][e] *= inv * (key ? wk[e] : wq[e]);
+                turn.apply(s, x[a], 1.f);
+                if (p < 0)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[a][e] = 0.f;
+                if (hh < h1 && in)
+                    store_piece<T, V>((key ? ko.at(b, t, hh - s.H[0]) : qo.at(b, t, hh)) + piece * V, x[a]);
+            }
+        }
+    }
+}
+
+// The gradient: a work-group leaves its sums of dgq and dgk in rows blockIdx.x and gridDim.x + blockIdx.x of part.
+template <typename T, typename GT, typename OT, int V, int L>
+__global__ void __launch_bounds__(256) qk_bwd_pieces(Shape s, Units u, Rows<const T> q, Rows<const T> k,
+                                                     const float* __restrict__ gq, const float* __restrict__ gk,
+                                                     Rows<const GT> dqo, Rows<const GT> dko, Rows<OT> dq, Rows<OT> dk,
+                                                     float* __restrict__ part) {
+    constexpr int G = 64 / L, AHEAD = 2;
+    __shared__ float red[4 * G][2][L * V];
+    const int lane = threadIdx.x & 63, piece = lane & (L - 1), sub = lane / L;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = s.H[0] + s.H[1];
+    const bool in = piece * V < s.D;
+    float wq[V], wk[V], aq[V] = {}, ak[V] = {};
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        wq[e] = gq && in ? gq[piece * V + e] : 1.f;
+        wk[e] = gk && in ? gk[piece * V + e] : 1.f;
+    }
+    Turn<V> turn;
+    turn.find(s, piece);
+    for (long long i = 4LL * blockIdx.x + wave; i < u.n; i += 4LL * gridDim.x) {
+        const long long n = i / u.per;
+        const int h0 = (int)(i - n * u.per) * u.heads, h1 = min(h0 + u.heads, heads);
+        const int b = (int)(n / s.S), t = (int)(n - (long long)b * s.S);
+        const int p = position(s, b, t);
+        turn.load(s, s.table + (long long)max(p, 0) * s.R, piece);
+        for (int h = h0 + sub; h - sub < h1; h += AHEAD * G) {
+            float x[AHEAD][V], d[AHEAD][V];
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int hh = h + a * G;
+                const bool key = hh >= s.H[0];
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[a][e] = d[a][e] = 0.f;
+                if (hh < h1 && in && p >= 0) {
+                    load_piece<T, V>((key ? k.at(b, t, hh - s.H[0]) : q.at(b, t, hh)) + piece * V, x[a]);
+                    load_piece<GT, V>((key ? dko.at(b, t, hh - s.H[0]) : dqo.at(b, t, hh)) + piece * V, d[a]);
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int hh = h + a * G;
+                const bool key = hh >= s.H[0];
+                if (hh - sub >= h1) break;
+                float sum = 0.f, dot = 0.f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum += x[a][e] * x[a][e];
+                const float inv = 1.f / sqrtf(group_sum<L>(sum) / s.D + s.eps);
+                turn.apply(s, d[a], -1.f);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[a][e] *= inv;
+                    const float w = d[a][e] * x[a][e];
+                    aq[e] += key ? 0.f : w;
+                    ak[e] += key ? w : 0.f;
+                    d[a][e] *= key ? wk[e] : wq[e];
+                    dot += d[a][e] * x[a][e];
+                }
+                const float mean = group_sum<L>(dot) / s.D;
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[a][e] = inv * (d[a][e] - x[a][e] * mean);
+                if (hh < h1 && in)
+                    store_piece<OT, V>((key ? dk.at(b, t, hh - s.H[0]) : dq.at(b, t, hh)) + piece * V, d[a]);
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        red[wave * G + sub][0][piece * V + e] = aq[e];
+        red[wave * G + sub][1][piece * V + e] = ak[e];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * s.D; i += 256) {
+        const int side = i >= s.D, e = side ? i - s.D : i;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4 * G; ++j) sum += red[j][side][e];
+        part[((long long)side * gridDim.x + blockIdx.x) * s.D + e] = sum;
+    }
+}
+
+// dg (+)= the sum of its partials: 16 waves take every 16th, in order.
+__global__ void __launch_bounds__(1024) qk_join(const float* __restrict__ part, int D, int gridq, int grid,
+                                                float* __restrict__ dgq, float* __restrict__ dgk, int acc) {
+    __shared__ float red[16][64];
     const bool key = blockIdx.y;
     float* out = key ? dgk : dgq;
     if (!out) return;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
     float sum = 0.f;
-    if (e < D)
-        for (int i = (key ? gridq : 0) + w; i < (key ? grid : gridq); i += 4) sum += part[(long long)i * D + e];
+    if (e < D) {
+        const int end = key ? grid : gridq;
+#pragma unroll 8
+        for (int i = (key ? gridq : 0) + w; i < end; i += 16) sum += part[(long long)i * D + e];
+    }
     red[w][lane] = sum;
     __syncthreads();
     if (w > 0 || e >= D) return;
-    sum = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += red[i][lane];
     out[e] = acc ? out[e] + sum : sum;
 }
 
@@ -250,6 +488,54 @@ Rows<T> rows_of(const void* p, const long long* st) {
     return {(T*)p, st[0], st[1], st[2]};
 }
 
+// Values of a piece for rows of these tensors: 8 or 4 where every row begins with whole pieces of up to
+// 16 bytes (`size`: of the smallest type) and pieces turn together, else 1: the form for any rows.
+struct Piece {
+    int V;
+    const Shape& s;
+    Piece(const Shape& s, int size) : V(16 / size), s(s) {
+        while (V > 1 && !fits()) V = V == 8 ? 4 : 1;
+    }
+    bool fits() const {
+        return s.D % V == 0 && s.D <= 64 * V && s.R % V == 0 && (s.pairs || s.R % (2 * V) == 0);
+    }
+    void rows(int H, const void* p, const long long* st, int size) {
+        const int n[3] = {s.B, s.S, H};
+        long long bits = 0;
+        for (int i = 0; i < 3; ++i) bits |= n[i] > 1 ? st[i] : 0;
+        while (V > 1 && H > 0 && (bits % V != 0 || (uintptr_t)p % (V * size < 16 ? V * size : 16) != 0 || !fits()))
+            V = V == 8 ? 4 : 1;
+    }
+    int lanes() const {
+        int L = 4;   // a row of 32 bf16
+        while (L * V < s.D) L *= 2;
+        return L;
+    }
+};
+// Heads of a unit: all of a token's where that gives each of the GPU's 8192 waves a unit, else as few as
+// the wave takes at once.
+Units units_of(const Shape& s, int at_once) {
+    const long long n = (long long)s.B * s.S;
+    const int heads = s.H[0] + s.H[1];
+    int per = (heads + at_once - 1) / at_once;
+    int each = (int)(n >= 8192 ? per : (n * per + 8191) / 8192);
+    if (each < 1) each = 1;
+    const int unit = each * at_once;
+    per = (heads + unit - 1) / unit;
+    return Units{unit, per, n * per};
+}
+
+template <typename T, int V, int L>
+int launch_fwd_pieces(const Shape& s, const void* Q, const long long* sq, const void* K, const long long* sk,
+                      const float* gq, const float* gk, void* Qo, const long long* sqo, void* Ko,
+                      const long long* sko) {
+    const Units u = units_of(s, 64 / L);
+    const long long groups = (u.n + 3) / 4, most = 1 << 20;
+    qk_fwd_pieces<T, V, L><<<(unsigned)(groups < most ? groups : most), 256, 0, stream()>>>(
+        s, u, rows_of<const T>(Q, sq), rows_of<const T>(K, sk), gq, gk, rows_of<T>(Qo, sqo), rows_of<T>(Ko, sko));
+    return check_launch("dh_qk_norm_rope_fwd");
+}
+
 template <typename T, int J>
 int launch_fwd(const Shape& s, const void* Q, const long long* sq, const void* K, const long long* sk, const float* gq,
                const float* gk, void* Qo, const long long* sqo, void* Ko, const long long* sko) {
@@ -273,6 +559,23 @@ void bwd_groups(const Shape& s, int& gridq, int& gridk) {
     gridk = s.H[1] ? groups(s.H[1]) : 0;
 }
 
+template <typename T, typename GT, typename OT, int V, int L>
+int launch_bwd_pieces(const Shape& s, const void* Q, const long long* sq, const void* K, const long long* sk,
+                      const float* gq, const float* gk, const void* dQo, const long long* sdqo, const void* dKo,
+                      const long long* sdko, void* dQ, const long long* sdq, void* dK, const long long* sdk,
+                      float* dgq, float* dgk, int acc, float* part) {
+    const Units u = units_of(s, 64 / L);
+    const long long groups = (u.n + 3) / 4, most = QK_GROUPS / 2;
+    const int grid = (int)(groups < most ? groups : most);
+    qk_bwd_pieces<T, GT, OT, V, L><<<grid, 256, 0, stream()>>>(
+        s, u, rows_of<const T>(Q, sq), rows_of<const T>(K, sk), gq, gk, rows_of<const GT>(dQo, sdqo),
+        rows_of<const GT>(dKo, sdko), rows_of<OT>(dQ, sdq), rows_of<OT>(dK, sdk), part);
+    DH_TRY(check_launch("dh_qk_norm_rope_bwd"));
+    if (!dgq && !dgk) return DH_OK;
+    qk_join<<<dim3((s.D + 63) / 64, 2), 1024, 0, stream()>>>(part, s.D, grid, 2 * grid, dgq, dgk, acc);
+    return check_launch("dh_qk_norm_rope_bwd");
+}
+
 template <typename T, typename GT, typename OT, int J>
 int launch_bwd(const Shape& s, const void* Q, const long long* sq, const void* K, const long long* sk, const float* gq,
                const float* gk, const void* dQo, const long long* sdqo, const void* dKo, const long long* sdko,
@@ -285,7 +588,7 @@ int launch_bwd(const Shape& s, const void* Q, const long long* sq, const void* K
         rows_of<const GT>(dKo, sdko), rows_of<OT>(dQ, sdq), rows_of<OT>(dK, sdk), part);
     DH_TRY(check_launch("dh_qk_norm_rope_bwd"));
     if (!dgq && !dgk) return DH_OK;
-    qk_join<<<dim3((s.D + 63) / 64, 2), 256, 0, stream()>>>(part, s.D, gridq, gridq + gridk, dgq, dgk, acc);
+    qk_join<<<dim3((s.D + 63) / 64, 2), 1024, 0, stream()>>>(part, s.D, gridq, gridq + gridk, dgq, dgk, acc);
     return check_launch("dh_qk_norm_rope_bwd");
 }
 
@@ -334,6 +637,18 @@ int dh_qk_norm_rope_fwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, i
     if (Hq == 0) sq = sqo = none;
     if (Hk == 0) sk = sko = none;
     const bool small = D <= 256;
+    const int size = dtype == DH_F32 ? 4 : 2;
+    Piece p(s, size);
+    p.rows(Hq, Q, sq, size), p.rows(Hk, K, sk, size), p.rows(Hq, Qo, sqo, size), p.rows(Hk, Ko, sko, size);
+    if (p.V > 1) {
+        const int L = p.lanes();
+#define DH_QK(T, V)                                                                                \
+    (L == 4 ? launch_fwd_pieces<T, V, 4> : L == 8 ? launch_fwd_pieces<T, V, 8> : L == 16 ? launch_fwd_pieces<T, V, 16>                   \
+     : L == 32 ? launch_fwd_pieces<T, V, 32> : launch_fwd_pieces<T, V, 64>)
+        auto pieces = dtype == DH_F32 ? DH_QK(float, 4) : p.V == 8 ? DH_QK(uint16_t, 8) : DH_QK(uint16_t, 4);
+#undef DH_QK
+        return pieces(s, Q, sq, K, sk, gq, gk, Qo, sqo, Ko, sko);
+    }
     auto run = dtype == DH_F32 ? small ? launch_fwd<float, 4> : launch_fwd<float, 16>
                                : small ? launch_fwd<uint16_t, 4> : launch_fwd<uint16_t, 16>;
     return run(s, Q, sq, K, sk, gq, gk, Qo, sqo, Ko, sko);
@@ -378,12 +693,30 @@ int dh_qk_norm_rope_bwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, i
     if (Hk == 0) sk = sdko = sdk = none;
     if (!any || Hq + Hk == 0) {   // no row: sums of nothing
         if (accumulate || (!dgq && !dgk)) return DH_OK;
-        qk_join<<<dim3((D + 63) / 64, 2), 256, 0, stream()>>>((float*)ws, D, 0, 0, dgq, dgk, 0);
+        qk_join<<<dim3((D + 63) / 64, 2), 1024, 0, stream()>>>((float*)ws, D, 0, 0, dgq, dgk, 0);
         return check_launch(op);
     }
     const bool small = D <= 256;
-#define DH_QK(T, GT, OT) (small ? launch_bwd<T, GT, OT, 4> : launch_bwd<T, GT, OT, 16>)
     const bool gw = dout_type == DH_F32, ow = grad_type == DH_F32;
+    const int size = dtype == DH_F32 ? 4 : 2, gsize = gw ? 4 : 2, osize = ow ? 4 : 2;
+    Piece p(s, size);
+    p.rows(Hq, Q, sq, size), p.rows(Hk, K, sk, size), p.rows(Hq, dQo, sdqo, gsize), p.rows(Hk, dKo, sdko, gsize);
+    p.rows(Hq, dQ, sdq, osize), p.rows(Hk, dK, sdk, osize);
+    if (p.V > 1) {
+        const int L = p.lanes();
+#define DH_QL(T, GT, OT, V)                                                                                \
+    (L == 4 ? launch_bwd_pieces<T, GT, OT, V, 4> : L == 8 ? launch_bwd_pieces<T, GT, OT, V, 8> : L == 16 ? launch_bwd_pieces<T, GT, OT, V, 16>           \
+     : L == 32 ? launch_bwd_pieces<T, GT, OT, V, 32> : launch_bwd_pieces<T, GT, OT, V, 64>)
+#define DH_QK(GT, OT) (p.V == 8 ? DH_QL(uint16_t, GT, OT, 8) : DH_QL(uint16_t, GT, OT, 4))
+        auto pieces = dtype == DH_F32 ? DH_QL(float, float, float, 4)
+                      : gw ? ow ? DH_QK(float, float) : DH_QK(float, uint16_t)
+                           : ow ? DH_QK(uint16_t, float) : DH_QK(uint16_t, uint16_t);
+#undef DH_QK
+#undef DH_QL
+        return pieces(s, Q, sq, K, sk, gq, gk, dQo, sdqo, dKo, sdko, dQ, sdq, dK, sdk, dgq, dgk, accumulate,
+                      (float*)ws);
+    }
+#define DH_QK(T, GT, OT) (small ? launch_bwd<T, GT, OT, 4> : launch_bwd<T, GT, OT, 16>)
     auto run = dtype == DH_F32 ? DH_QK(float, float, float)
                : gw ? ow ? DH_QK(uint16_t, float, float) : DH_QK(uint16_t, float, uint16_t)
                     : ow ? DH_QK(uint16_t, uint16_t, float) : DH_QK(uint16_t, uint16_t, uint16_t);
