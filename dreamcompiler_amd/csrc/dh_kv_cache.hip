@@ -93,19 +93,22 @@ struct Strides {
 
 // The sequence that row n is of, and its token's position there: the rows of sequence b are its last
 // first[b + 1] - first[b] tokens (first NULL: one each); t = -1 if it has fewer.  False for a row of
-// no sequence.
+// no sequence.  A wave looks at 64 beginnings at once: two loads for up to 4096 sequences.
 __device__ inline bool place(const int* __restrict__ first, const int* __restrict__ len, int B, int n, int& b,
                              int& t) {
     long long behind = 1;
     b = n;
     if (first) {
-        int lo = 0, hi = B;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (first[mid] <= n) lo = mid;
-            else hi = mid;
+        const int lane = threadIdx.x & 63;
+        int lo = 0, count = B;   // the last one at or before n is among lo .. lo + count - 1, or none
+        while (count > 1) {
+            const int step = (count + 63) >> 6, at = lo + lane * step;
+            const uint64_t before = __ballot(lane * step < count && first[min(at, B)] <= n);
+            const int k = max(__popcll(before), 1) - 1;
+            lo += k * step;
+            count = min(step, count - k * step);
         }
-        b = lo;
+        b = __builtin_amdgcn_readfirstlane(lo);
         behind = (long long)first[b + 1] - n;
         if (first[b] > n || behind <= 0) return false;
     }
@@ -114,7 +117,7 @@ __device__ inline bool place(const int* __restrict__ first, const int* __restric
     return true;
 }
 
-// A wave per row of one token, head and side.
+// ---- any rows: a wave each ---------------------------------------------------------------------
 template <typename T, typename CT>
 __global__ void __launch_bounds__(256) cache_write(Paged c, int B, int N, const int* __restrict__ first,
                                                    const int* __restrict__ len, const T* __restrict__ K, Strides sk,
@@ -185,22 +188,279 @@ __global__ void __launch_bounds__(256) cache_read(Paged c, int B, int N, const i
     }
 }
 
+// ---- rows that begin with 16 bytes ---------------------------------------------------------------
+// A row is L lanes of V values, 16 bytes of the model's type; a wave takes 64 / L of a token's 2 Hk rows (keys
+// of all heads, then values) at once, `rows` of them in all: a token's whole where there are many tokens.
+struct Units {
+    int rows, per;   // of a unit, units of a token
+    long long n;
+};
+
+template <typename T> struct Piece;
+template <> struct Piece<float> { static constexpr int V = 4; };
+template <> struct Piece<uint16_t> { static constexpr int V = 8; };
+
+template <typename T, int V>
+__device__ inline void load_piece(const T* p, float (&v)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    const vec x = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = paged_up(x[e]);
+}
+template <typename T, int V>
+__device__ inline void store_piece(T* p, const float (&v)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec x;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = down<T>(v[e]);
+    *reinterpret_cast<vec*>(p) = x;
+}
+
+// The largest of L lanes' bits, in all of them.
+template <int L>
+__device__ inline uint32_t group_max(uint32_t v) {
+    auto step = [](uint32_t a, float b) { return max(a, __builtin_bit_cast(uint32_t, b)); };
+    auto f = [](uint32_t a) { return __builtin_bit_cast(float, a); };
+    if (L > 1) v = step(v, dpp_quad_xor1(f(v)));
+    if (L > 2) v = step(v, dpp_quad_xor2(f(v)));
+    if (L > 4) v = step(v, dpp_half_mirror(f(v)));
+    if (L > 8) v = step(v, dpp_row_mirror(f(v)));
+    float lo, hi;
+    if (L > 16) {
+        halves16(f(v), lo, hi);
+        v = step(__builtin_bit_cast(uint32_t, lo), hi);
+    }
+    if (L > 32) {
+        halves32(f(v), lo, hi);
+        v = step(__builtin_bit_cast(uint32_t, lo), hi);
+    }
+    return v;
+}
+
+// Codes of four values x / s.  A quotient's neighbours 2^-22 of it below and above x (1 / s) have the exact one
+// between them: where both round to one code, that is its; else (3 of 10^5 values) the wave takes the
+// exact quotient's.
+template <typename CT> __device__ inline uint32_t codes_of(const float (&y)[4]);
+template <> __device__ inline uint32_t codes_of<int8_t>(const float (&y)[4]) {
+    uint32_t c[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)   // 1.5 2^23 leaves the rounded integer in the last bits
+        c[e] = __builtin_bit_cast(uint32_t, fminf(fmaxf(y[e], -127.f), 127.f) + 12582912.f);
+    const uint32_t a = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), b = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
+    return a | b << 16;
+}
+template <> __device__ inline uint32_t codes_of<uint8_t>(const float (&y)[4]) {
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = fminf(fmaxf(y[e], -448.f), 448.f);
+    const int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true);
+}
+template <typename CT, int V>
+__device__ inline void codes(const float (&x)[V], float s, float rs, uint32_t (&out)[V / 4]) {
+    bool unsure = false;
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        float lo[4], hi[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float y = x[4 * i + e] * rs;
+            lo[e] = y * (1.f - 0x1p-22f);
+            hi[e] = y * (1.f + 0x1p-22f);
+        }
+        out[i] = codes_of<CT>(lo);
+        unsure |= out[i] != codes_of<CT>(hi);
+    }
+    if (!__any(unsure)) return;
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = quotient(x[4 * i + e], s);
+        out[i] = codes_of<CT>(y);
+    }
+}
+
+template <typename T, typename CT, int L>
+__global__ void __launch_bounds__(256) cache_write_pieces(Paged c, Units u, int B, const int* __restrict__ first,
+                                                          const int* __restrict__ len, const T* __restrict__ K,
+                                                          Strides sk, const T* __restrict__ V, Strides sv) {
+    constexpr int P = Piece<T>::V, G = 64 / L, AHEAD = 4;
+    constexpr bool scaled = sizeof(CT) == 1;
+    const int lane = threadIdx.x & 63, piece = lane & (L - 1), sub = lane / L;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool in = piece * P < c.D;
+    for (long long i = 4LL * blockIdx.x + wave; i < u.n; i += 4LL * gridDim.x) {
+        const int n = (int)(i / u.per), r0 = (int)(i - (long long)n * u.per) * u.rows, r1 = min(r0 + u.rows, 2 * c.Hk);
+        int id = -1, at = 0;
+        for (int r = r0; r < r1; r += AHEAD * G) {
+            float x[AHEAD][P];
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int k = r + a * G + sub, h = k < c.Hk ? k : k - c.Hk;
+#pragma unroll
+                for (int e = 0; e < P; ++e) x[a][e] = 0.f;
+                if (k < r1 && in)
+                    load_piece<T, P>((k < c.Hk ? K + n * sk.token + h * sk.head : V + n * sv.token + h * sv.head) + piece * P,
+                                     x[a]);
+            }
+            if (r == r0) {   // the rows are on their way meanwhile
+                int b, t;
+                if (!place(first, len, B, n, b, t)) break;
+                id = c.page_of(b, t);
+                at = t & ((1 << c.shift) - 1);
+            }
+            if (id < 0) break;
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int k = r + a * G + sub, h = k < c.Hk ? k : k - c.Hk;
+                if (r + a * G >= r1) break;
+                const long long row = c.row(id, h, at);
+                CT* o = (CT*)(k < c.Hk ? c.K : c.V) + row * c.D + piece * P;
+                if constexpr (!scaled) {
+                    if (k < r1 && in) store_piece<CT, P>(o, x[a]);
+                } else {
+                    uint32_t most = 0, out[P / 4];
+#pragma unroll
+                    for (int e = 0; e < P; ++e) most = max(most, __builtin_bit_cast(uint32_t, x[a][e]) & 0x7FFFFFFFu);
+                    most = group_max<L>(most);
+                    const float s = most >= 0x7F800000u ? __builtin_nanf("")
+                                                        : __builtin_bit_cast(float, most) / Code<CT>::top;
+                    if (k < r1 && piece == 0) (k < c.Hk ? c.Ks : c.Vs)[row] = s;
+                    const float f = s < 0x1p-40f ? 0x1p64f : 1.f, sf = s > 0.f ? s * f : 1.f;
+#pragma unroll
+                    for (int e = 0; e < P; ++e) x[a][e] = s > 0.f ? x[a][e] * f : 0.f;
+                    codes<CT, P>(x[a], sf, 1.f / sf, out);
+                    if (k < r1 && in) {
+                        if constexpr (P == 8) *reinterpret_cast<u32x2*>(o) = u32x2{out[0], out[1]};
+                        else *reinterpret_cast<uint32_t*>(o) = out[0];
+                    }
+                }
+            }
+        }
+    }
+}
+
+// V values of a cache's type.
+template <typename CT, int V>
+__device__ inline void load_codes(const CT* p, float (&v)[V]) {
+    if constexpr (sizeof(CT) > 1) {
+        load_piece<CT, V>(p, v);
+    } else {
+        uint32_t w[V / 4];
+        if constexpr (V == 8) {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+            w[0] = x[0], w[1] = x[1];
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            if constexpr (__is_same(CT, int8_t)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * i + e] = (float)(int8_t)(w[i] >> (8 * e));
+            } else {
+                v[4 * i] = __builtin_amdgcn_cvt_f32_fp8(w[i], 0), v[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(w[i], 1);
+                v[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(w[i], 2), v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(w[i], 3);
+            }
+        }
+    }
+}
+
+template <typename T, typename CT, int L>
+__global__ void __launch_bounds__(256) cache_read_pieces(Paged c, Units u, int B, const int* __restrict__ first,
+                                                         const int* __restrict__ len, T* __restrict__ K, Strides sk,
+                                                         T* __restrict__ V, Strides sv) {
+    constexpr int P = Piece<T>::V, G = 64 / L, AHEAD = 4;
+    constexpr bool scaled = sizeof(CT) == 1;
+    const int lane = threadIdx.x & 63, piece = lane & (L - 1), sub = lane / L;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool in = piece * P < c.D;
+    for (long long i = 4LL * blockIdx.x + wave; i < u.n; i += 4LL * gridDim.x) {
+        const int n = (int)(i / u.per), r0 = (int)(i - (long long)n * u.per) * u.rows, r1 = min(r0 + u.rows, 2 * c.Hk);
+        int b, t;
+        if (!place(first, len, B, n, b, t)) continue;
+        const int id = c.page_of(b, t), at = t & ((1 << c.shift) - 1);
+        for (int r = r0; r < r1; r += AHEAD * G) {
+            float x[AHEAD][P], s[AHEAD];
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int k = r + a * G + sub, h = k < c.Hk ? k : k - c.Hk;
+                s[a] = 1.f;
+#pragma unroll
+                for (int e = 0; e < P; ++e) x[a][e] = 0.f;
+                if (k < r1 && in && id >= 0) {
+                    const long long row = c.row(id, h, at);
+                    if constexpr (scaled) s[a] = (k < c.Hk ? c.Ks : c.Vs)[row];
+                    load_codes<CT, P>((const CT*)(k < c.Hk ? c.K : c.V) + row * c.D + piece * P, x[a]);
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int k = r + a * G + sub, h = k < c.Hk ? k : k - c.Hk;
+                if (k >= r1 || !in) continue;
+                if constexpr (scaled)
+#pragma unroll
+                    for (int e = 0; e < P; ++e) x[a][e] *= s[a];
+                store_piece<T, P>((k < c.Hk ? K + n * sk.token + h * sk.head : V + n * sv.token + h * sv.head) + piece * P,
+                                  x[a]);
+            }
+        }
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
 int groups_of(long long rows) {
     const long long groups = (rows + 3) / 4, most = num_cus() * 32LL;
     return (int)(groups < most ? groups : most);
 }
 
+// Rows of a unit: all of a token's where that gives each of the GPU's 8192 waves a unit, else as few
+// as the wave takes at once.
+Units units_of(int N, int rows, int at_once) {
+    int per = (rows + at_once - 1) / at_once, each = (int)(N >= 8192 ? per : ((long long)N * per + 8191) / 8192);
+    if (each < 1) each = 1;
+    per = (per + each - 1) / each;
+    return Units{each * at_once, per, (long long)N * per};
+}
+bool whole_pieces(const void* p, Strides st, int N, int Hk, int size) {
+    const long long bits = (N > 1 ? st.token : 0) | (Hk > 1 ? st.head : 0);
+    return ((uintptr_t)p & 15) == 0 && bits * size % 16 == 0;
+}
+int piece_groups(const Units& u) {
+    const long long groups = (u.n + 3) / 4;
+    return (int)(groups < 1 << 20 ? groups : 1 << 20);
+}
+
 template <typename T, typename CT>
 int launch_write(const Paged& c, int B, int N, const int* first, const int* len, const void* K, Strides sk,
                  const void* V, Strides sv) {
-    cache_write<T, CT><<<groups_of(2LL * N * c.Hk), 256, 0, stream()>>>(c, B, N, first, len, (const T*)K, sk,
-                                                                        (const T*)V, sv);
+    if (whole_pieces(K, sk, N, c.Hk, sizeof(T)) && whole_pieces(V, sv, N, c.Hk, sizeof(T))) {
+        const int lanes = c.D / Piece<T>::V, L = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
+        const Units u = units_of(N, 2 * c.Hk, 64 / L);
+        auto run = L == 4 ? cache_write_pieces<T, CT, 4> : L == 8 ? cache_write_pieces<T, CT, 8>
+                   : L == 16 ? cache_write_pieces<T, CT, 16> : L == 32 ? cache_write_pieces<T, CT, 32>
+                                                                       : cache_write_pieces<T, CT, 64>;
+        run<<<piece_groups(u), 256, 0, stream()>>>(c, u, B, first, len, (const T*)K, sk, (const T*)V, sv);
+    } else {
+        cache_write<T, CT><<<groups_of(2LL * N * c.Hk), 256, 0, stream()>>>(c, B, N, first, len, (const T*)K, sk,
+                                                                            (const T*)V, sv);
+    }
     return check_launch("dh_kv_cache_write");
 }
 template <typename T, typename CT>
 int launch_read(const Paged& c, int B, int N, const int* first, const int* len, void* K, Strides sk, void* V,
                 Strides sv) {
-    cache_read<T, CT><<<groups_of(2LL * N * c.Hk), 256, 0, stream()>>>(c, B, N, first, len, (T*)K, sk, (T*)V, sv);
+    if (whole_pieces(K, sk, N, c.Hk, sizeof(T)) && whole_pieces(V, sv, N, c.Hk, sizeof(T))) {
+        const int lanes = c.D / Piece<T>::V, L = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
+        const Units u = units_of(N, 2 * c.Hk, 64 / L);
+        auto run = L == 4 ? cache_read_pieces<T, CT, 4> : L == 8 ? cache_read_pieces<T, CT, 8>
+                   : L == 16 ? cache_read_pieces<T, CT, 16> : L == 32 ? cache_read_pieces<T, CT, 32>
+                                                                      : cache_read_pieces<T, CT, 64>;
+        run<<<piece_groups(u), 256, 0, stream()>>>(c, u, B, first, len, (T*)K, sk, (T*)V, sv);
+    } else {
+        cache_read<T, CT><<<groups_of(2LL * N * c.Hk), 256, 0, stream()>>>(c, B, N, first, len, (T*)K, sk, (T*)V, sv);
+    }
     return check_launch("dh_kv_cache_read");
 }
 
