@@ -4,6 +4,7 @@ The product path: every call goes to the HIP library.  There is no CPU fallback;
 if the library is missing or no GPU is usable the calls raise.
 """
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -190,6 +191,10 @@ class DeviceBuffer:
         assert out.nbytes <= self.nbytes
         check(load().dh_memcpy_d2h(out.ctypes.data, self.ptr, out.nbytes), "dh_memcpy_d2h")
         return out
+
+    @property
+    def _as_parameter_(self):   # as ctypes takes it
+        return self.ptr
 
     def fill_zero(self):
         check(load().dh_memset(self.ptr, 0, self.nbytes), "dh_memset")
@@ -413,21 +418,23 @@ def linear_distill_bwd(dtype, N, V, D, K, T, H, ldh, W, ldw, top_id, top_logit, 
 # Norm and rotation of queries and keys, a paged key-value cache and attention over it
 # (include/dream_hip.h).  Strides are tuples in elements: (sequence, token, head) for the norm,
 # (token, head) for the cache, (sequence, head) for the attention.
+# Buffers and addresses go to ctypes as they are and arrays of strides are made once: a step of a
+# decoder is a few microseconds of calls.
+@functools.lru_cache(maxsize=4096)
 def _strides(v):
-    return None if v is None else (_ll * len(v))(*[int(x) for x in v])
+    return None if v is None else (_ll * len(v))(*map(int, v))
 
 
 def rope_table(P, R, base, table):
-    check(load().dh_rope_table(P, R, float(base), _p(table)), "dh_rope_table")
+    check(load().dh_rope_table(P, R, base, table), "dh_rope_table")
 
 
 def qk_norm_rope_fwd(dtype, B, S, Hq, Hk, D, R, pairs, eps, pos, table, P, Q, q_strides, K,
                      k_strides, gq, gk, Qo, qo_strides, Ko, ko_strides):
-    check(load().dh_qk_norm_rope_fwd(dtype, B, S, Hq, Hk, D, R, int(pairs), float(eps), _p(pos),
-                                     _p(table), P, _p(Q), _strides(q_strides), _p(K),
-                                     _strides(k_strides), _p(gq), _p(gk), _p(Qo),
-                                     _strides(qo_strides), _p(Ko), _strides(ko_strides)),
-          "dh_qk_norm_rope_fwd")
+    check(load().dh_qk_norm_rope_fwd(dtype, B, S, Hq, Hk, D, R, pairs, eps, pos, table, P, Q,
+                                     _strides(q_strides), K, _strides(k_strides), gq, gk, Qo,
+                                     _strides(qo_strides), Ko, _strides(ko_strides)),
+                                     "dh_qk_norm_rope_fwd")
 
 
 def qk_norm_rope_bwd_workspace(D):
@@ -437,29 +444,26 @@ def qk_norm_rope_bwd_workspace(D):
 def qk_norm_rope_bwd(dtype, B, S, Hq, Hk, D, R, pairs, eps, pos, table, P, Q, q_strides, K,
                      k_strides, gq, gk, dout_type, dQo, dqo_strides, dKo, dko_strides, grad_type,
                      dQ, dq_strides, dK, dk_strides, dgq, dgk, accumulate, ws, ws_bytes):
-    check(load().dh_qk_norm_rope_bwd(dtype, B, S, Hq, Hk, D, R, int(pairs), float(eps), _p(pos),
-                                     _p(table), P, _p(Q), _strides(q_strides), _p(K),
-                                     _strides(k_strides), _p(gq), _p(gk), dout_type, _p(dQo),
-                                     _strides(dqo_strides), _p(dKo), _strides(dko_strides),
-                                     grad_type, _p(dQ), _strides(dq_strides), _p(dK),
-                                     _strides(dk_strides), _p(dgq), _p(dgk), int(accumulate),
-                                     _p(ws), int(ws_bytes)), "dh_qk_norm_rope_bwd")
+    check(load().dh_qk_norm_rope_bwd(dtype, B, S, Hq, Hk, D, R, pairs, eps, pos, table, P, Q,
+                                     _strides(q_strides), K, _strides(k_strides), gq, gk,
+                                     dout_type, dQo, _strides(dqo_strides), dKo,
+                                     _strides(dko_strides), grad_type, dQ, _strides(dq_strides),
+                                     dK, _strides(dk_strides), dgq, dgk, accumulate, ws, ws_bytes),
+                                     "dh_qk_norm_rope_bwd")
 
 
 def kv_cache_write(dtype, cache_type, B, N, Hk, D, K, k_strides, V, v_strides, first, len_, pages,
                    page, table, ld_table, Kc, Vc, Ks=None, Vs=None):
-    check(load().dh_kv_cache_write(dtype, cache_type, B, N, Hk, D, _p(K), _strides(k_strides),
-                                   _p(V), _strides(v_strides), _p(first), _p(len_), pages, page,
-                                   _p(table), ld_table, _p(Kc), _p(Vc), _p(Ks), _p(Vs)),
-          "dh_kv_cache_write")
+    check(load().dh_kv_cache_write(dtype, cache_type, B, N, Hk, D, K, _strides(k_strides), V,
+                                   _strides(v_strides), first, len_, pages, page, table, ld_table,
+                                   Kc, Vc, Ks, Vs), "dh_kv_cache_write")
 
 
 def kv_cache_read(dtype, cache_type, B, N, Hk, D, K, k_strides, V, v_strides, first, len_, pages,
                   page, table, ld_table, Kc, Vc, Ks=None, Vs=None):
-    check(load().dh_kv_cache_read(dtype, cache_type, B, N, Hk, D, _p(K), _strides(k_strides),
-                                  _p(V), _strides(v_strides), _p(first), _p(len_), pages, page,
-                                  _p(table), ld_table, _p(Kc), _p(Vc), _p(Ks), _p(Vs)),
-          "dh_kv_cache_read")
+    check(load().dh_kv_cache_read(dtype, cache_type, B, N, Hk, D, K, _strides(k_strides), V,
+                                  _strides(v_strides), first, len_, pages, page, table, ld_table,
+                                  Kc, Vc, Ks, Vs), "dh_kv_cache_read")
 
 
 def paged_attention_workspace(cache_type, B, Hq, Hk, D, max_len):
@@ -468,11 +472,10 @@ def paged_attention_workspace(cache_type, B, Hq, Hk, D, max_len):
 
 def paged_attention(dtype, cache_type, B, Hq, Hk, D, scale, window, Q, q_strides, len_, max_len,
                     pages, page, table, ld_table, Kc, Vc, Ks, Vs, O, o_strides, lse, ws, ws_bytes):
-    check(load().dh_paged_attention(dtype, cache_type, B, Hq, Hk, D, float(scale), int(window),
-                                    _p(Q), _strides(q_strides), _p(len_), max_len, pages, page,
-                                    _p(table), ld_table, _p(Kc), _p(Vc), _p(Ks), _p(Vs), _p(O),
-                                    _strides(o_strides), _p(lse), _p(ws), int(ws_bytes)),
-          "dh_paged_attention")
+    check(load().dh_paged_attention(dtype, cache_type, B, Hq, Hk, D, scale, window, Q,
+                                    _strides(q_strides), len_, max_len, pages, page, table,
+                                    ld_table, Kc, Vc, Ks, Vs, O, _strides(o_strides), lse, ws,
+                                    ws_bytes), "dh_paged_attention")
 
 
 class Timer:
