@@ -38,7 +38,7 @@ struct Rows {
 struct Shape {
     int B, S, H[2], D, R, P;
     bool pairs;
-    float eps;
+    float eps, by_d;   // 1 / D
     const int* pos;
     const float* table;
 };
@@ -49,132 +49,145 @@ __device__ inline int position(const Shape& s, int b, int t) {
     return (s.pos || s.R > 0) && (unsigned)p >= (unsigned)s.P ? -1 : p;
 }
 
-// What value e of a row turns with: its partner, cosine and sine (signed so that the forward
-// is y[e] c + y[partner] s).  Values past R turn with nothing.
-__device__ inline int turn(const Shape& s, const float* __restrict__ row, int e, float& c, float& sn) {
-    c = 1.f, sn = 0.f;
-    if (e >= s.R) return e;
-    const int half = s.R >> 1;
-    const int i = s.pairs ? e >> 1 : e < half ? e : e - half;
-    const bool second = s.pairs ? e & 1 : e >= half;
-    c = row[i];
-    sn = second ? row[half + i] : -row[half + i];
-    if (s.pairs) return e ^ 1;
-    return second ? e - half : e + half;
+// Units of work for waves: blocks of heads of a token, those of queries first; a unit is `each` of them.
+struct Units {
+    int nq, n, each;      // blocks of queries, of all
+    FastDiv per, S;       // units of a token, tokens of a sequence
+    uint32_t units;
+};
+
+// 1 / sqrt(mean + eps) to 2^-22: the sum's own rounding is up to 2^-20.
+__device__ inline float norm_of(float sum, const Shape& s) {
+    return __builtin_amdgcn_rsqf(fmaf(sum, s.by_d, s.eps));
 }
 
-// A wave per row, 64 values at a time: any D, strides and alignment.
-template <typename T, int J>
-__global__ void __launch_bounds__(256) qk_fwd(Shape s, Rows<const T> q, Rows<const T> k,
-                                              const float* __restrict__ gq, const float* __restrict__ gk,
-                                              Rows<T> qo, Rows<T> ko) {
-    const int lane = threadIdx.x & 63, heads = s.H[0] + s.H[1];
-    const long long rows = (long long)s.B * s.S * heads, waves = (long long)gridDim.x * 4;
-    for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += waves) {
-        const long long n = r / heads;
-        int h = (int)(r - n * heads);
-        const int b = (int)(n / s.S), t = (int)(n - (long long)b * s.S);
-        const bool key = h >= s.H[0];
-        if (key) h -= s.H[0];
-        const T* x = key ? k.at(b, t, h) : q.at(b, t, h);
-        T* o = key ? ko.at(b, t, h) : qo.at(b, t, h);
-        const float* g = key ? gk : gq;
-        const int p = position(s, b, t);
-        if (p < 0) {
-            for (int e = lane; e < s.D; e += 64) o[e] = down<T>(0.f);
-            continue;
-        }
-        const float* row = s.table + (long long)p * s.R;
-        float v[J], sum = 0.f;
+// ---- any rows ------------------------------------------------------------------------------------
+// A wave per row, J values a lane, 64 apart: any D, strides and alignment.  What value e = 64 j + lane turns
+// with: its partner's place, cosine and sine (signed so that the forward is y[e] c + y[partner] sn).
+template <int J>
+struct TurnAny {
+    float c[J], sn[J];
+    int other[J];
+    __device__ void load(const Shape& s, const float* __restrict__ row) {
+        const int lane = threadIdx.x & 63, half = s.R >> 1;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int e = 64 * j + lane;
-            v[j] = e < s.D ? up(x[e]) : 0.f;
-            sum += v[j] * v[j];
+            c[j] = 1.f, sn[j] = 0.f, other[j] = min(e, s.D - 1);
+            if (e >= s.R) continue;
+            const int i = s.pairs ? e >> 1 : e < half ? e : e - half;
+            const bool second = s.pairs ? e & 1 : e >= half;
+            c[j] = row[i];
+            sn[j] = second ? row[half + i] : -row[half + i];
+            other[j] = s.pairs ? e ^ 1 : second ? e - half : e + half;
         }
-        const float inv = 1.f / sqrtf(wave_reduce(sum, OpSum()) / s.D + s.eps);
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int e = 64 * j + lane;
-            if (e >= s.D) continue;
-            float c, sn;
-            const int other = turn(s, row, e, c, sn);
-            const float y = v[j] * inv * (g ? g[e] : 1.f);
-            v[j] = other == e ? y : y * c + up(x[other]) * inv * (g ? g[other] : 1.f) * sn;
-        }
-        wave_fence();   // o may be x
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-            if (64 * j + lane < s.D) o[64 * j + lane] = down<T>(v[j]);
     }
-}
-
-// The gradient: work-groups [0, gridq) take rows of queries, the others of keys; each leaves its sum
-// of dg in part (one row of D a work-group).
-template <typename T, typename GT, typename OT, int J>
-__global__ void __launch_bounds__(256) qk_bwd(Shape s, int gridq, Rows<const T> q, Rows<const T> k,
-                                              const float* __restrict__ gq, const float* __restrict__ gk,
-                                              Rows<const GT> dqo, Rows<const GT> dko, Rows<OT> dq,
-                                              Rows<OT> dk, float* __restrict__ part) {
-    __shared__ float red[3][64 * J];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const bool key = (int)blockIdx.x >= gridq;
-    const int H = s.H[key], group = key ? blockIdx.x - gridq : blockIdx.x;
-    const long long rows = (long long)s.B * s.S * H, waves = 4LL * (key ? gridDim.x - gridq : gridq);
-    const float* g = key ? gk : gq;
-    float acc[J] = {};
-    for (long long r = 4LL * group + w; r < rows; r += waves) {
-        const long long n = r / H;
-        const int h = (int)(r - n * H);
-        const int b = (int)(n / s.S), t = (int)(n - (long long)b * s.S);
-        const T* x = key ? k.at(b, t, h) : q.at(b, t, h);
-        const GT* d = key ? dko.at(b, t, h) : dqo.at(b, t, h);
-        OT* o = key ? dk.at(b, t, h) : dq.at(b, t, h);
-        const int p = position(s, b, t);
-        if (p < 0) {
-            for (int e = lane; e < s.D; e += 64) o[e] = down<OT>(0.f);
-            continue;
-        }
-        const float* row = s.table + (long long)p * s.R;
-        float v[J], dy[J], sum = 0.f, dot = 0.f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int e = 64 * j + lane;
-            v[j] = e < s.D ? up(x[e]) : 0.f;
-            dy[j] = 0.f;
-            if (e < s.D) {
-                float c, sn;
-                const int other = turn(s, row, e, c, sn);
-                dy[j] = up(d[e]);
-                if (other != e) dy[j] = dy[j] * c - up(d[other]) * sn;
-            }
-            sum += v[j] * v[j];
-        }
-        const float inv = 1.f / sqrtf(wave_reduce(sum, OpSum()) / s.D + s.eps);
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int e = 64 * j + lane;
-            v[j] *= inv;
-            acc[j] += dy[j] * v[j];
-            dy[j] *= g && e < s.D ? g[e] : 1.f;
-            dot += dy[j] * v[j];
-        }
-        const float mean = wave_reduce(dot, OpSum()) / s.D;
-        wave_fence();   // o may be x or d
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-            if (64 * j + lane < s.D) o[64 * j + lane] = down<OT>(inv * (dy[j] - v[j] * mean));
-    }
-    if (w > 0)
-#pragma unroll
-        for (int j = 0; j < J; ++j) red[w - 1][64 * j + lane] = acc[j];
-    __syncthreads();
-    if (w > 0) return;
+};
+template <int J>
+__device__ inline void load_any(const float* __restrict__ g, int D, const int* other, float (&w)[J], float (&wo)[J]) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-        const int e = 64 * j + lane;
-        for (int i = 0; i < 3; ++i) acc[j] += red[i][e];
-        if (e < s.D) part[(long long)blockIdx.x * s.D + e] = acc[j];
+        w[j] = g && 64 * j + lane < D ? g[64 * j + lane] : 1.f;
+        wo[j] = g ? g[other[j]] : 1.f;
+    }
+}
+
+template <typename T, int J>
+__global__ void __launch_bounds__(256) qk_fwd(Shape s, Units u, Rows<const T> q, Rows<const T> k,
+                                              const float* __restrict__ gq, const float* __restrict__ gk,
+                                              Rows<T> qo, Rows<T> ko) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TurnAny<J> turn;
+    for (uint32_t i = 4 * blockIdx.x + wave; i < u.units; i += 4 * gridDim.x) {
+        const uint32_t n = fdiv(i, u.per);
+        const int b = fdiv(n, u.S), t = n - b * s.S, h0 = (i - n * u.per.d) * u.each, h1 = min(h0 + u.each, u.n);
+        const int p = position(s, b, t);
+        turn.load(s, s.table + (long long)max(p, 0) * s.R);
+        for (int h = h0; h < h1; ++h) {
+            const bool key = h >= s.H[0];
+            const T* x = key ? k.at(b, t, h - s.H[0]) : q.at(b, t, h);
+            T* o = key ? ko.at(b, t, h - s.H[0]) : qo.at(b, t, h);
+            float w[J], wo[J], v[J], vo[J], sum = 0.f;
+            load_any<J>(key ? gk : gq, s.D, turn.other, w, wo);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int e = 64 * j + lane;
+                v[j] = vo[j] = 0.f;
+                if (p >= 0 && e < s.D) v[j] = up(x[e]), vo[j] = up(x[turn.other[j]]);
+                sum += v[j] * v[j];
+            }
+            const float inv = norm_of(wave_reduce(sum, OpSum()), s);
+            wave_fence();   // o may be x
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int e = 64 * j + lane;
+                const float y = e < s.R ? v[j] * inv * w[j] * turn.c[j] + vo[j] * inv * wo[j] * turn.sn[j] : v[j] * inv * w[j];
+                if (e < s.D) o[e] = down<T>(y);
+            }
+        }
+    }
+}
+
+// The gradient: a work-group leaves its sums of dgq and dgk in rows blockIdx.x and gridDim.x + blockIdx.x of part.
+template <typename T, typename GT, typename OT, int J>
+__global__ void __launch_bounds__(256) qk_bwd(Shape s, Units u, Rows<const T> q, Rows<const T> k,
+                                              const float* __restrict__ gq, const float* __restrict__ gk,
+                                              Rows<const GT> dqo, Rows<const GT> dko, Rows<OT> dq, Rows<OT> dk,
+                                              float* __restrict__ part) {
+    __shared__ float red[4][64 * J];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float acc[2][J] = {};
+    TurnAny<J> turn;
+    for (uint32_t i = 4 * blockIdx.x + wave; i < u.units; i += 4 * gridDim.x) {
+        const uint32_t n = fdiv(i, u.per);
+        const int b = fdiv(n, u.S), t = n - b * s.S, h0 = (i - n * u.per.d) * u.each, h1 = min(h0 + u.each, u.n);
+        const int p = position(s, b, t);
+        turn.load(s, s.table + (long long)max(p, 0) * s.R);
+        for (int h = h0; h < h1; ++h) {
+            const bool key = h >= s.H[0];
+            const T* x = key ? k.at(b, t, h - s.H[0]) : q.at(b, t, h);
+            const GT* d = key ? dko.at(b, t, h - s.H[0]) : dqo.at(b, t, h);
+            OT* o = key ? dk.at(b, t, h - s.H[0]) : dq.at(b, t, h);
+            const float* g = key ? gk : gq;
+            float v[J], dy[J], sum = 0.f, dot = 0.f;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int e = 64 * j + lane;
+                v[j] = dy[j] = 0.f;
+                if (p >= 0 && e < s.D) {
+                    v[j] = up(x[e]);
+                    dy[j] = up(d[e]);
+                    if (e < s.R) dy[j] = dy[j] * turn.c[j] - up(d[turn.other[j]]) * turn.sn[j];
+                }
+                sum += v[j] * v[j];
+            }
+            const float inv = norm_of(wave_reduce(sum, OpSum()), s);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int e = 64 * j + lane;
+                v[j] *= inv;
+                const float term = dy[j] * v[j];
+                acc[0][j] += key ? 0.f : term;
+                acc[1][j] += key ? term : 0.f;
+                dy[j] *= g && e < s.D ? g[e] : 1.f;
+                dot += dy[j] * v[j];
+            }
+            const float mean = wave_reduce(dot, OpSum()) * s.by_d;
+            wave_fence();   // o may be x or d
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                if (64 * j + lane < s.D) o[64 * j + lane] = down<OT>(inv * (dy[j] - v[j] * mean));
+        }
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        if (side) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < J; ++j) red[wave][64 * j + lane] = acc[side][j];
+        __syncthreads();
+        for (int e = threadIdx.x; e < s.D; e += 256)
+            part[((long long)side * gridDim.x + blockIdx.x) * s.D + e] = red[0][e] + red[1][e] + red[2][e] + red[3][e];
     }
 }
 
@@ -271,129 +284,157 @@ struct Turn {
     }
 };
 
-struct Units {
-    int heads, per;   // heads of a unit, units of a token
-    long long n;
+// Rows of a lane in flight: more of them leave room for fewer waves.
+template <int V> constexpr int ahead() { return 8 / V; }
+
+template <int V>
+__device__ inline void load_weights(const float* __restrict__ g, int piece, bool in, float (&w)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = 1.f;
+    typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
+    if (!g || !in) return;
+    const vec x = *reinterpret_cast<const vec*>(g + piece * V);
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = x[e];
+}
+
+// A wave's tokens at once: where a token has fewer heads than the wave has places for rows, the places of a
+// power of two `heads` of each side belong to a token, and a unit is as many tokens as that leaves.
+struct Many {
+    int heads, tokens;
+    long long n;   // tokens of the call
 };
 
-template <typename T, int V, int L>
-__global__ void __launch_bounds__(256) qk_fwd_pieces(Shape s, Units u, Rows<const T> q, Rows<const T> k,
+template <typename T, int V, int L, bool MANY>
+__global__ void __launch_bounds__(256) qk_fwd_pieces(Shape s, Units u, Many m, Rows<const T> q, Rows<const T> k,
                                                      const float* __restrict__ gq, const float* __restrict__ gk,
                                                      Rows<T> qo, Rows<T> ko) {
-    constexpr int G = 64 / L, AHEAD = 4;
+    constexpr int G = 64 / L, AHEAD = MANY ? 1 : ahead<V>();
     const int lane = threadIdx.x & 63, piece = lane & (L - 1), sub = lane / L;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = s.H[0] + s.H[1];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool in = piece * V < s.D;
     float wq[V], wk[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        wq[e] = gq && in ? gq[piece * V + e] : 1.f;
-        wk[e] = gk && in ? gk[piece * V + e] : 1.f;
-    }
+    load_weights<V>(gq, piece, in, wq);
+    load_weights<V>(gk, piece, in, wk);
     Turn<V> turn;
     turn.find(s, piece);
-    for (long long i = 4LL * blockIdx.x + wave; i < u.n; i += 4LL * gridDim.x) {
-        const long long n = i / u.per;
-        const int h0 = (int)(i - n * u.per) * u.heads, h1 = min(h0 + u.heads, heads);
-        const int b = (int)(n / s.S), t = (int)(n - (long long)b * s.S);
+    auto block = [&](const Rows<const T>& x, const Rows<T>& o, const float (&w)[V], int H, int b, int t, int h0, bool there) {
+        const int hs = MANY ? 0 : sub;   // the lane's head is h0 + hs; h0 is one for the wave unless MANY
+        const T* xp = x.at(b, t, h0) + (hs * x.s2 + piece * V);
+        T* op = o.at(b, t, h0) + (hs * o.s2 + piece * V);
+        float v[AHEAD][V];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[a][e] = 0.f;
+            if (h0 + a * G + hs < H && in && there) load_piece<T, V>(xp + a * G * x.s2, v[a]);
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (!MANY && h0 + a * G >= H) break;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum += v[a][e] * v[a][e];
+            const float inv = norm_of(group_sum<L>(sum), s);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[a][e] *= inv * w[e];
+            turn.apply(s, v[a], 1.f);
+            if (h0 + a * G + hs < H && in) store_piece<T, V>(op + a * G * o.s2, v[a]);
+        }
+    };
+    for (uint32_t i = 4 * blockIdx.x + wave; i < u.units; i += 4 * gridDim.x) {
+        if constexpr (MANY) {   // one lane's token is not another's
+            const uint32_t n = i * m.tokens + sub / m.heads;
+            const bool any = n < m.n;
+            const int b = any ? fdiv(n, u.S) : 0, t = any ? n - b * s.S : 0, p = any ? position(s, b, t) : -1;
+            turn.load(s, s.table + (long long)max(p, 0) * s.R, piece);
+            const int h = sub & (m.heads - 1);
+            if (s.H[0] > 0) block(q, qo, wq, any ? s.H[0] : 0, b, t, h, p >= 0);
+            if (s.H[1] > 0) block(k, ko, wk, any ? s.H[1] : 0, b, t, h, p >= 0);
+            continue;
+        }
+        const uint32_t n = fdiv(i, u.per);
+        const int b = fdiv(n, u.S), t = n - b * s.S, j0 = (i - n * u.per.d) * u.each, j1 = min(j0 + u.each, u.n);
         const int p = position(s, b, t);
         turn.load(s, s.table + (long long)max(p, 0) * s.R, piece);
-        for (int h = h0 + sub; h - sub < h1; h += AHEAD * G) {
-            float x[AHEAD][V];
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int hh = h + a * G;
-                const bool key = hh >= s.H[0];
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[a][e] = 0.f;
-                if (hh < h1 && in)
-                    load_piece<T, V>((key ? k.at(b, t, hh - s.H[0]) : q.at(b, t, hh)) + piece * V, x[a]);
-            }
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int hh = h + a * G;
-                const bool key = hh >= s.H[0];
-                if (hh - sub >= h1) break;
-                float sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < V; ++e) sum += x[a][e] * x[a][e];
-                const float inv = 1.f / sqrtf(group_sum<L>(sum) / s.D + s.eps);
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[a][e] *= inv * (key ? wk[e] : wq[e]);
-                turn.apply(s, x[a], 1.f);
-                if (p < 0)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[a][e] = 0.f;
-                if (hh < h1 && in)
-                    store_piece<T, V>((key ? ko.at(b, t, hh - s.H[0]) : qo.at(b, t, hh)) + piece * V, x[a]);
-            }
+        for (int j = j0; j < j1; ++j) {
+            if (j < u.nq) block(q, qo, wq, s.H[0], b, t, j * AHEAD * G, p >= 0);
+            else block(k, ko, wk, s.H[1], b, t, (j - u.nq) * AHEAD * G, p >= 0);
         }
     }
 }
 
 // The gradient: a work-group leaves its sums of dgq and dgk in rows blockIdx.x and gridDim.x + blockIdx.x of part.
-template <typename T, typename GT, typename OT, int V, int L>
-__global__ void __launch_bounds__(256) qk_bwd_pieces(Shape s, Units u, Rows<const T> q, Rows<const T> k,
+template <typename T, typename GT, typename OT, int V, int L, bool MANY>
+__global__ void __launch_bounds__(256) qk_bwd_pieces(Shape s, Units u, Many m, Rows<const T> q, Rows<const T> k,
                                                      const float* __restrict__ gq, const float* __restrict__ gk,
                                                      Rows<const GT> dqo, Rows<const GT> dko, Rows<OT> dq, Rows<OT> dk,
                                                      float* __restrict__ part) {
-    constexpr int G = 64 / L, AHEAD = 2;
+    constexpr int G = 64 / L, AHEAD = MANY ? 1 : ahead<V>();
     __shared__ float red[4 * G][2][L * V];
     const int lane = threadIdx.x & 63, piece = lane & (L - 1), sub = lane / L;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = s.H[0] + s.H[1];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool in = piece * V < s.D;
     float wq[V], wk[V], aq[V] = {}, ak[V] = {};
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        wq[e] = gq && in ? gq[piece * V + e] : 1.f;
-        wk[e] = gk && in ? gk[piece * V + e] : 1.f;
-    }
+    load_weights<V>(gq, piece, in, wq);
+    load_weights<V>(gk, piece, in, wk);
     Turn<V> turn;
     turn.find(s, piece);
-    for (long long i = 4LL * blockIdx.x + wave; i < u.n; i += 4LL * gridDim.x) {
-        const long long n = i / u.per;
-        const int h0 = (int)(i - n * u.per) * u.heads, h1 = min(h0 + u.heads, heads);
-        const int b = (int)(n / s.S), t = (int)(n - (long long)b * s.S);
+    auto block = [&](const Rows<const T>& x, const Rows<const GT>& dy, const Rows<OT>& o, const float (&w)[V],
+                     float (&acc)[V], int H, int b, int t, int h0, bool there) {
+        const int hs = MANY ? 0 : sub;
+        const T* xp = x.at(b, t, h0) + (hs * x.s2 + piece * V);
+        const GT* dp = dy.at(b, t, h0) + (hs * dy.s2 + piece * V);
+        OT* op = o.at(b, t, h0) + (hs * o.s2 + piece * V);
+        float v[AHEAD][V], d[AHEAD][V];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[a][e] = d[a][e] = 0.f;
+            if (h0 + a * G + hs < H && in && there) {
+                load_piece<T, V>(xp + a * G * x.s2, v[a]);
+                load_piece<GT, V>(dp + a * G * dy.s2, d[a]);
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (!MANY && h0 + a * G >= H) break;
+            float sum = 0.f, dot = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum += v[a][e] * v[a][e];
+            const float inv = norm_of(group_sum<L>(sum), s);
+            turn.apply(s, d[a], -1.f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[a][e] *= inv;
+                acc[e] += d[a][e] * v[a][e];
+                d[a][e] *= w[e];
+                dot += d[a][e] * v[a][e];
+            }
+            const float mean = group_sum<L>(dot) * s.by_d;
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[a][e] = inv * (d[a][e] - v[a][e] * mean);
+            if (h0 + a * G + hs < H && in) store_piece<OT, V>(op + a * G * o.s2, d[a]);
+        }
+    };
+    for (uint32_t i = 4 * blockIdx.x + wave; i < u.units; i += 4 * gridDim.x) {
+        if constexpr (MANY) {   // one lane's token is not another's
+            const uint32_t n = i * m.tokens + sub / m.heads;
+            const bool any = n < m.n;
+            const int b = any ? fdiv(n, u.S) : 0, t = any ? n - b * s.S : 0, p = any ? position(s, b, t) : -1;
+            turn.load(s, s.table + (long long)max(p, 0) * s.R, piece);
+            const int h = sub & (m.heads - 1);
+            if (s.H[0] > 0) block(q, dqo, dq, wq, aq, any ? s.H[0] : 0, b, t, h, p >= 0);
+            if (s.H[1] > 0) block(k, dko, dk, wk, ak, any ? s.H[1] : 0, b, t, h, p >= 0);
+            continue;
+        }
+        const uint32_t n = fdiv(i, u.per);
+        const int b = fdiv(n, u.S), t = n - b * s.S, j0 = (i - n * u.per.d) * u.each, j1 = min(j0 + u.each, u.n);
         const int p = position(s, b, t);
         turn.load(s, s.table + (long long)max(p, 0) * s.R, piece);
-        for (int h = h0 + sub; h - sub < h1; h += AHEAD * G) {
-            float x[AHEAD][V], d[AHEAD][V];
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int hh = h + a * G;
-                const bool key = hh >= s.H[0];
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[a][e] = d[a][e] = 0.f;
-                if (hh < h1 && in && p >= 0) {
-                    load_piece<T, V>((key ? k.at(b, t, hh - s.H[0]) : q.at(b, t, hh)) + piece * V, x[a]);
-                    load_piece<GT, V>((key ? dko.at(b, t, hh - s.H[0]) : dqo.at(b, t, hh)) + piece * V, d[a]);
-                }
-            }
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int hh = h + a * G;
-                const bool key = hh >= s.H[0];
-                if (hh - sub >= h1) break;
-                float sum = 0.f, dot = 0.f;
-#pragma unroll
-                for (int e = 0; e < V; ++e) sum += x[a][e] * x[a][e];
-                const float inv = 1.f / sqrtf(group_sum<L>(sum) / s.D + s.eps);
-                turn.apply(s, d[a], -1.f);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    x[a][e] *= inv;
-                    const float w = d[a][e] * x[a][e];
-                    aq[e] += key ? 0.f : w;
-                    ak[e] += key ? w : 0.f;
-                    d[a][e] *= key ? wk[e] : wq[e];
-                    dot += d[a][e] * x[a][e];
-                }
-                const float mean = group_sum<L>(dot) / s.D;
-#pragma unroll
-                for (int e = 0; e < V; ++e) d[a][e] = inv * (d[a][e] - x[a][e] * mean);
-                if (hh < h1 && in)
-                    store_piece<OT, V>((key ? dk.at(b, t, hh - s.H[0]) : dq.at(b, t, hh)) + piece * V, d[a]);
-            }
+        for (int j = j0; j < j1; ++j) {
+            if (j < u.nq) block(q, dqo, dq, wq, aq, s.H[0], b, t, j * AHEAD * G, p >= 0);
+            else block(k, dko, dk, wk, ak, s.H[1], b, t, (j - u.nq) * AHEAD * G, p >= 0);
         }
     }
 #pragma unroll
@@ -411,26 +452,25 @@ __global__ void __launch_bounds__(256) qk_bwd_pieces(Shape s, Units u, Rows<cons
     }
 }
 
-// dg (+)= the sum of its partials: 16 waves take every 16th, in order.
-__global__ void __launch_bounds__(1024) qk_join(const float* __restrict__ part, int D, int gridq, int grid,
+// dg (+)= the sum of its n partials a side: a work-group per 16 columns, 64 partials at a time, in order.
+__global__ void __launch_bounds__(1024) qk_join(const float* __restrict__ part, int D, int n,
                                                 float* __restrict__ dgq, float* __restrict__ dgk, int acc) {
-    __shared__ float red[16][64];
-    const bool key = blockIdx.y;
-    float* out = key ? dgk : dgq;
+    __shared__ float red[64][17];
+    const int side = blockIdx.y, col = threadIdx.x & 15, r = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
+    float* out = side ? dgk : dgq;
     if (!out) return;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
     float sum = 0.f;
     if (e < D) {
-        const int end = key ? grid : gridq;
+        const float* p = part + (long long)side * n * D + e;
 #pragma unroll 8
-        for (int i = (key ? gridq : 0) + w; i < end; i += 16) sum += part[(long long)i * D + e];
+        for (int i = r; i < n; i += 64) sum += p[(long long)i * D];
     }
-    red[w][lane] = sum;
+    red[r][col] = sum;
     __syncthreads();
-    if (w > 0 || e >= D) return;
+    if (r > 0 || e >= D) return;
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += red[i][lane];
+    for (int i = 0; i < 64; ++i) sum += red[i][col];
     out[e] = acc ? out[e] + sum : sum;
 }
 
@@ -476,10 +516,11 @@ int check_qk(const char* op, int dtype, int B, int S, int Hq, int Hk, int D, int
         (long long)B * S > 0x7FF00000)
         return set_error(DH_ERR_INVALID, "%s: shape B=%d S=%d Hq=%d Hk=%d D=%d", op, B, S, Hq, Hk, D);
     if (R < 0 || R > D || (R & 1)) return set_error(DH_ERR_INVALID, "%s: R=%d must be even and at most D", op, R);
-    if (!(eps > 0.f) || !(eps - eps == 0.f)) return set_error(DH_ERR_INVALID, "%s: eps must be finite and > 0", op);
+    if (!(eps >= 1.17549435e-38f) || !(eps - eps == 0.f))
+        return set_error(DH_ERR_INVALID, "%s: eps must be finite and at least 2^-126", op);
     if ((R > 0 && !table) || ((R > 0 || pos) && P < 1) || (R > 0 && !pos && S > P))
         return set_error(DH_ERR_INVALID, "%s: no table of %d positions (P=%d)", op, pos ? 1 : S, P);
-    s = Shape{B, S, {Hq, Hk}, D, R, P, pairs != 0, eps, pos, (const float*)table};
+    s = Shape{B, S, {Hq, Hk}, D, R, P, pairs != 0, eps, 1.f / D, pos, (const float*)table};
     return DH_OK;
 }
 
@@ -512,84 +553,119 @@ struct Piece {
         return L;
     }
 };
-// Heads of a unit: all of a token's where that gives each of the GPU's 8192 waves a unit, else as few as
-// the wave takes at once.
-Units units_of(const Shape& s, int at_once) {
+// Blocks of a unit: all of a token's where that gives each of the GPU's 8192 waves a unit, else down to one.
+// Units and tokens stay below 2^31, as FastDiv needs: there are at most 2^31 - 2^20 tokens.
+Units units_of(const Shape& s, int heads) {
     const long long n = (long long)s.B * s.S;
-    const int heads = s.H[0] + s.H[1];
-    int per = (heads + at_once - 1) / at_once;
-    int each = (int)(n >= 8192 ? per : (n * per + 8191) / 8192);
-    if (each < 1) each = 1;
-    const int unit = each * at_once;
-    per = (heads + unit - 1) / unit;
-    return Units{unit, per, n * per};
+    const int nq = (s.H[0] + heads - 1) / heads, nk = (s.H[1] + heads - 1) / heads, blocks = nq + nk;
+    int each = (int)(n >= 8192 ? blocks : (n * blocks + 8191) / 8192);
+    const int per = (blocks + each - 1) / each;
+    return Units{nq, blocks, each, make_fastdiv(per), make_fastdiv(s.S), (uint32_t)(n * per)};
 }
+
+// Places for `heads` heads of a side where a wave has twice as many or more, and their tokens; else 0.
+Many many_of(const Shape& s, int places) {
+    int heads = 1;
+    while (heads < s.H[0] || heads < s.H[1]) heads *= 2;
+    return Many{2 * heads <= places ? heads : 0, 2 * heads <= places ? places / heads : 0, (long long)s.B * s.S};
+}
+unsigned groups_of(uint32_t units, uint32_t most) {
+    const uint32_t groups = (units + 3) / 4;
+    return groups < most ? groups : most;
+}
+// Work-groups of the gradient: enough to fill the GPU, few enough that their partials are a small part
+// of the work.
+constexpr int QK_GROUPS = 1024, FWD_GROUPS = 1 << 20;
+
+struct Call {
+    const void *Q, *K, *dQo, *dKo;
+    const long long *sq, *sk, *sdqo, *sdko;
+    const float *gq, *gk;
+    void *Qo, *Ko;   // dQ, dK of the gradient
+    const long long *sqo, *sko;
+    float *dgq, *dgk, *part;
+    int acc;
+};
 
 template <typename T, int V, int L>
-int launch_fwd_pieces(const Shape& s, const void* Q, const long long* sq, const void* K, const long long* sk,
-                      const float* gq, const float* gk, void* Qo, const long long* sqo, void* Ko,
-                      const long long* sko) {
-    const Units u = units_of(s, 64 / L);
-    const long long groups = (u.n + 3) / 4, most = 1 << 20;
-    qk_fwd_pieces<T, V, L><<<(unsigned)(groups < most ? groups : most), 256, 0, stream()>>>(
-        s, u, rows_of<const T>(Q, sq), rows_of<const T>(K, sk), gq, gk, rows_of<T>(Qo, sqo), rows_of<T>(Ko, sko));
+int launch_fwd_pieces(const Shape& s, const Call& c) {
+    Units u = units_of(s, ahead<V>() * 64 / L);
+    const Many m = many_of(s, 64 / L);
+    auto run = qk_fwd_pieces<T, V, L, false>;
+    if constexpr (L < 64)
+        if (m.heads) u.units = (uint32_t)((m.n + m.tokens - 1) / m.tokens), run = qk_fwd_pieces<T, V, L, true>;
+    run<<<groups_of(u.units, FWD_GROUPS), 256, 0, stream()>>>(s, u, m, rows_of<const T>(c.Q, c.sq), rows_of<const T>(c.K, c.sk),
+                                                              c.gq, c.gk, rows_of<T>(c.Qo, c.sqo), rows_of<T>(c.Ko, c.sko));
     return check_launch("dh_qk_norm_rope_fwd");
 }
-
 template <typename T, int J>
-int launch_fwd(const Shape& s, const void* Q, const long long* sq, const void* K, const long long* sk, const float* gq,
-               const float* gk, void* Qo, const long long* sqo, void* Ko, const long long* sko) {
-    const long long rows = (long long)s.B * s.S * (s.H[0] + s.H[1]), most = num_cus() * 32LL;
-    const long long groups = (rows + 3) / 4;
-    qk_fwd<T, J><<<(unsigned)(groups < most ? groups : most), 256, 0, stream()>>>(
-        s, rows_of<const T>(Q, sq), rows_of<const T>(K, sk), gq, gk, rows_of<T>(Qo, sqo), rows_of<T>(Ko, sko));
+int launch_fwd(const Shape& s, const Call& c) {
+    const Units u = units_of(s, 1);
+    qk_fwd<T, J><<<groups_of(u.units, FWD_GROUPS), 256, 0, stream()>>>(s, u, rows_of<const T>(c.Q, c.sq),
+                                                                       rows_of<const T>(c.K, c.sk), c.gq, c.gk,
+                                                                       rows_of<T>(c.Qo, c.sqo), rows_of<T>(c.Ko, c.sko));
     return check_launch("dh_qk_norm_rope_fwd");
 }
 
-// Work-groups of the gradient for queries and keys: enough to fill the GPU, few enough that their
-// partials are a small part of the work.
-constexpr int QK_GROUPS = 2048;
-void bwd_groups(const Shape& s, int& gridq, int& gridk) {
-    const long long n = (long long)s.B * s.S;
-    auto groups = [&](int H) {
-        const long long g = (n * H + 3) / 4, most = (long long)QK_GROUPS * H / (s.H[0] + s.H[1]) + 1;
-        return (int)(g < most ? g : most);
-    };
-    gridq = s.H[0] ? groups(s.H[0]) : 0;
-    gridk = s.H[1] ? groups(s.H[1]) : 0;
+int join(const Shape& s, const Call& c, int n) {
+    DH_TRY(check_launch("dh_qk_norm_rope_bwd"));
+    if (!c.dgq && !c.dgk) return DH_OK;
+    qk_join<<<dim3((s.D + 15) / 16, 2), 1024, 0, stream()>>>(c.part, s.D, n, c.dgq, c.dgk, c.acc);
+    return check_launch("dh_qk_norm_rope_bwd");
 }
-
 template <typename T, typename GT, typename OT, int V, int L>
-int launch_bwd_pieces(const Shape& s, const void* Q, const long long* sq, const void* K, const long long* sk,
-                      const float* gq, const float* gk, const void* dQo, const long long* sdqo, const void* dKo,
-                      const long long* sdko, void* dQ, const long long* sdq, void* dK, const long long* sdk,
-                      float* dgq, float* dgk, int acc, float* part) {
-    const Units u = units_of(s, 64 / L);
-    const long long groups = (u.n + 3) / 4, most = QK_GROUPS / 2;
-    const int grid = (int)(groups < most ? groups : most);
-    qk_bwd_pieces<T, GT, OT, V, L><<<grid, 256, 0, stream()>>>(
-        s, u, rows_of<const T>(Q, sq), rows_of<const T>(K, sk), gq, gk, rows_of<const GT>(dQo, sdqo),
-        rows_of<const GT>(dKo, sdko), rows_of<OT>(dQ, sdq), rows_of<OT>(dK, sdk), part);
-    DH_TRY(check_launch("dh_qk_norm_rope_bwd"));
-    if (!dgq && !dgk) return DH_OK;
-    qk_join<<<dim3((s.D + 63) / 64, 2), 1024, 0, stream()>>>(part, s.D, grid, 2 * grid, dgq, dgk, acc);
-    return check_launch("dh_qk_norm_rope_bwd");
+int launch_bwd_pieces(const Shape& s, const Call& c) {
+    Units u = units_of(s, ahead<V>() * 64 / L);
+    const Many m = many_of(s, 64 / L);
+    auto run = qk_bwd_pieces<T, GT, OT, V, L, false>;
+    if constexpr (L < 64)
+        if (m.heads) u.units = (uint32_t)((m.n + m.tokens - 1) / m.tokens), run = qk_bwd_pieces<T, GT, OT, V, L, true>;
+    const unsigned grid = groups_of(u.units, QK_GROUPS);
+    run<<<grid, 256, 0, stream()>>>(s, u, m, rows_of<const T>(c.Q, c.sq), rows_of<const T>(c.K, c.sk), c.gq, c.gk,
+                                    rows_of<const GT>(c.dQo, c.sdqo), rows_of<const GT>(c.dKo, c.sdko),
+                                    rows_of<OT>(c.Qo, c.sqo), rows_of<OT>(c.Ko, c.sko), c.part);
+    return join(s, c, grid);
+}
+template <typename T, typename GT, typename OT, int J>
+int launch_bwd(const Shape& s, const Call& c) {
+    const Units u = units_of(s, 1);
+    const unsigned grid = groups_of(u.units, QK_GROUPS);
+    qk_bwd<T, GT, OT, J><<<grid, 256, 0, stream()>>>(s, u, rows_of<const T>(c.Q, c.sq), rows_of<const T>(c.K, c.sk), c.gq, c.gk,
+                                                     rows_of<const GT>(c.dQo, c.sdqo), rows_of<const GT>(c.dKo, c.sdko),
+                                                     rows_of<OT>(c.Qo, c.sqo), rows_of<OT>(c.Ko, c.sko), c.part);
+    return join(s, c, grid);
 }
 
-template <typename T, typename GT, typename OT, int J>
-int launch_bwd(const Shape& s, const void* Q, const long long* sq, const void* K, const long long* sk, const float* gq,
-               const float* gk, const void* dQo, const long long* sdqo, const void* dKo, const long long* sdko,
-               void* dQ, const long long* sdq, void* dK, const long long* sdk, float* dgq, float* dgk, int acc,
-               float* part) {
-    int gridq, gridk;
-    bwd_groups(s, gridq, gridk);
-    qk_bwd<T, GT, OT, J><<<gridq + gridk, 256, 0, stream()>>>(
-        s, gridq, rows_of<const T>(Q, sq), rows_of<const T>(K, sk), gq, gk, rows_of<const GT>(dQo, sdqo),
-        rows_of<const GT>(dKo, sdko), rows_of<OT>(dQ, sdq), rows_of<OT>(dK, sdk), part);
-    DH_TRY(check_launch("dh_qk_norm_rope_bwd"));
-    if (!dgq && !dgk) return DH_OK;
-    qk_join<<<dim3((s.D + 63) / 64, 2), 1024, 0, stream()>>>(part, s.D, gridq, gridq + gridk, dgq, dgk, acc);
-    return check_launch("dh_qk_norm_rope_bwd");
+template <typename T, int V>
+int fwd_by_lanes(int L, const Shape& s, const Call& c) {
+    return L == 4    ? launch_fwd_pieces<T, V, 4>(s, c)
+           : L == 8  ? launch_fwd_pieces<T, V, 8>(s, c)
+           : L == 16 ? launch_fwd_pieces<T, V, 16>(s, c)
+           : L == 32 ? launch_fwd_pieces<T, V, 32>(s, c)
+                     : launch_fwd_pieces<T, V, 64>(s, c);
+}
+// D <= 256 fits four values a lane.
+template <typename T>
+int fwd_of(const Piece& p, const Shape& s, const Call& c) {
+    if (p.V == 1) return s.D <= 256 ? launch_fwd<T, 4>(s, c) : launch_fwd<T, 16>(s, c);
+    if constexpr (sizeof(T) == 2)
+        if (p.V == 8) return fwd_by_lanes<T, 8>(p.lanes(), s, c);
+    return fwd_by_lanes<T, 4>(p.lanes(), s, c);
+}
+template <typename T, typename GT, typename OT, int V>
+int bwd_by_lanes(int L, const Shape& s, const Call& c) {
+    return L == 4    ? launch_bwd_pieces<T, GT, OT, V, 4>(s, c)
+           : L == 8  ? launch_bwd_pieces<T, GT, OT, V, 8>(s, c)
+           : L == 16 ? launch_bwd_pieces<T, GT, OT, V, 16>(s, c)
+           : L == 32 ? launch_bwd_pieces<T, GT, OT, V, 32>(s, c)
+                     : launch_bwd_pieces<T, GT, OT, V, 64>(s, c);
+}
+template <typename T, typename GT, typename OT>
+int bwd_of(const Piece& p, const Shape& s, const Call& c) {
+    if (p.V == 1) return s.D <= 256 ? launch_bwd<T, GT, OT, 4>(s, c) : launch_bwd<T, GT, OT, 16>(s, c);
+    if constexpr (sizeof(T) == 2)
+        if (p.V == 8) return bwd_by_lanes<T, GT, OT, 8>(p.lanes(), s, c);
+    return bwd_by_lanes<T, GT, OT, 4>(p.lanes(), s, c);
 }
 
 }  // namespace
@@ -636,26 +712,15 @@ int dh_qk_norm_rope_fwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, i
     if (!any || Hq + Hk == 0) return DH_OK;
     if (Hq == 0) sq = sqo = none;
     if (Hk == 0) sk = sko = none;
-    const bool small = D <= 256;
     const int size = dtype == DH_F32 ? 4 : 2;
     Piece p(s, size);
     p.rows(Hq, Q, sq, size), p.rows(Hk, K, sk, size), p.rows(Hq, Qo, sqo, size), p.rows(Hk, Ko, sko, size);
-    if (p.V > 1) {
-        const int L = p.lanes();
-#define DH_QK(T, V)                                                                                \
-    (L == 4 ? launch_fwd_pieces<T, V, 4> : L == 8 ? launch_fwd_pieces<T, V, 8> : L == 16 ? launch_fwd_pieces<T, V, 16>                   \
-     : L == 32 ? launch_fwd_pieces<T, V, 32> : launch_fwd_pieces<T, V, 64>)
-        auto pieces = dtype == DH_F32 ? DH_QK(float, 4) : p.V == 8 ? DH_QK(uint16_t, 8) : DH_QK(uint16_t, 4);
-#undef DH_QK
-        return pieces(s, Q, sq, K, sk, gq, gk, Qo, sqo, Ko, sko);
-    }
-    auto run = dtype == DH_F32 ? small ? launch_fwd<float, 4> : launch_fwd<float, 16>
-                               : small ? launch_fwd<uint16_t, 4> : launch_fwd<uint16_t, 16>;
-    return run(s, Q, sq, K, sk, gq, gk, Qo, sqo, Ko, sko);
+    const Call c{Q, K, nullptr, nullptr, sq, sk, none, none, gq, gk, Qo, Ko, sqo, sko, nullptr, nullptr, nullptr, 0};
+    return dtype == DH_F32 ? fwd_of<float>(p, s, c) : fwd_of<uint16_t>(p, s, c);
 }
 
 size_t dh_qk_norm_rope_bwd_workspace(int D) {
-    return D < 1 || D > QK_MOST_D ? 0 : (size_t)(QK_GROUPS + 2) * D * 4;
+    return D < 1 || D > QK_MOST_D ? 0 : (size_t)2 * QK_GROUPS * D * 4;
 }
 
 int dh_qk_norm_rope_bwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, int pairs, float eps, const int* pos,
@@ -693,35 +758,18 @@ int dh_qk_norm_rope_bwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, i
     if (Hk == 0) sk = sdko = sdk = none;
     if (!any || Hq + Hk == 0) {   // no row: sums of nothing
         if (accumulate || (!dgq && !dgk)) return DH_OK;
-        qk_join<<<dim3((D + 63) / 64, 2), 1024, 0, stream()>>>((float*)ws, D, 0, 0, dgq, dgk, 0);
+        qk_join<<<dim3((D + 15) / 16, 2), 1024, 0, stream()>>>((float*)ws, D, 0, dgq, dgk, 0);
         return check_launch(op);
     }
-    const bool small = D <= 256;
     const bool gw = dout_type == DH_F32, ow = grad_type == DH_F32;
     const int size = dtype == DH_F32 ? 4 : 2, gsize = gw ? 4 : 2, osize = ow ? 4 : 2;
     Piece p(s, size);
     p.rows(Hq, Q, sq, size), p.rows(Hk, K, sk, size), p.rows(Hq, dQo, sdqo, gsize), p.rows(Hk, dKo, sdko, gsize);
     p.rows(Hq, dQ, sdq, osize), p.rows(Hk, dK, sdk, osize);
-    if (p.V > 1) {
-        const int L = p.lanes();
-#define DH_QL(T, GT, OT, V)                                                                                \
-    (L == 4 ? launch_bwd_pieces<T, GT, OT, V, 4> : L == 8 ? launch_bwd_pieces<T, GT, OT, V, 8> : L == 16 ? launch_bwd_pieces<T, GT, OT, V, 16>           \
-     : L == 32 ? launch_bwd_pieces<T, GT, OT, V, 32> : launch_bwd_pieces<T, GT, OT, V, 64>)
-#define DH_QK(GT, OT) (p.V == 8 ? DH_QL(uint16_t, GT, OT, 8) : DH_QL(uint16_t, GT, OT, 4))
-        auto pieces = dtype == DH_F32 ? DH_QL(float, float, float, 4)
-                      : gw ? ow ? DH_QK(float, float) : DH_QK(float, uint16_t)
-                           : ow ? DH_QK(uint16_t, float) : DH_QK(uint16_t, uint16_t);
-#undef DH_QK
-#undef DH_QL
-        return pieces(s, Q, sq, K, sk, gq, gk, dQo, sdqo, dKo, sdko, dQ, sdq, dK, sdk, dgq, dgk, accumulate,
-                      (float*)ws);
-    }
-#define DH_QK(T, GT, OT) (small ? launch_bwd<T, GT, OT, 4> : launch_bwd<T, GT, OT, 16>)
-    auto run = dtype == DH_F32 ? DH_QK(float, float, float)
-               : gw ? ow ? DH_QK(uint16_t, float, float) : DH_QK(uint16_t, float, uint16_t)
-                    : ow ? DH_QK(uint16_t, uint16_t, float) : DH_QK(uint16_t, uint16_t, uint16_t);
-#undef DH_QK
-    return run(s, Q, sq, K, sk, gq, gk, dQo, sdqo, dKo, sdko, dQ, sdq, dK, sdk, dgq, dgk, accumulate, (float*)ws);
+    const Call c{Q, K, dQo, dKo, sq, sk, sdqo, sdko, gq, gk, dQ, dK, sdq, sdk, dgq, dgk, (float*)ws, accumulate};
+    if (dtype == DH_F32) return bwd_of<float, float, float>(p, s, c);
+    if (gw) return ow ? bwd_of<uint16_t, float, float>(p, s, c) : bwd_of<uint16_t, float, uint16_t>(p, s, c);
+    return ow ? bwd_of<uint16_t, uint16_t, float>(p, s, c) : bwd_of<uint16_t, uint16_t, uint16_t>(p, s, c);
 }
 
 }  // extern "C"

@@ -412,7 +412,7 @@ int dh_rope_table(int P, int R, double base, float* d_table);
  * (d_table may be NULL; d_pos, if given, still marks padding).  Weights gq, gk: D floats, NULL: ones.
  * Strides: three of each tensor, in elements, of sequence, token and head (a row's D values lie side by
  * side); inputs may repeat rows (stride 0), outputs must have theirs apart.  An output may be its input
- * (same pointer, strides and type), no other overlap.  D up to 1024, R even and up to D, eps > 0,
+ * (same pointer, strides and type), no other overlap.  D up to 1024, R even and up to D, eps >= 2^-126,
  * B S up to 2^31 - 2^20; Hq or Hk of 0 leaves that side out. */
 int dh_qk_norm_rope_fwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, int pairs, float eps,
                         const int* d_pos, const float* d_table, int P, const void* d_Q,
