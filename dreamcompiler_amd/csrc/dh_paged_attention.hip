@@ -20,8 +20,9 @@ struct Strides {
     long long seq, head;
 };
 struct Work {
-    int B, Hq, G, groups, window, max_len, chunk, splits;
+    int B, Hq, G, window, max_len, chunk, splits;
     float scale;
+    FastDiv by_groups, by_heads;   // groups of 16 RT query heads of a cache head, cache heads
     const int* len;
     float* part;    // splits x B x Hq rows of D: a chunk's o before its division
     float2* stat;   // as many: its m (in units of log 2) and sum
@@ -115,52 +116,79 @@ struct Form {
     static constexpr int column(int seg) { return (wide ? 64 : 128) * seg; }
 };
 
-template <typename T, typename CT, int DP, bool FULL, int RT>
-__global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __restrict__ Q, Strides sq,
+// What a lane loads of a tile.
+template <typename F, int DP>
+struct Tile {
+    u32x4 kr[F::SUBS][F::KSTEPS];
+    uint32_t vr[F::SUBS][4][DP / 64 * (16 / F::E)];
+    f32x4 ks[F::SUBS], vs[F::SUBS];   // scales of tokens 4 g .. 4 g + 3 of each 16
+    bool there[F::SUBS], whole;       // whether there is a page, and whether all tokens count
+};
+
+template <typename T, typename CT, int DP, bool FULL, int RT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const T* __restrict__ Q, Strides sq,
                                                    T* __restrict__ O, Strides so, float* __restrict__ lse) {
     typedef Form<T, CT, DP> F;
     constexpr int SUBS = F::SUBS, KSTEPS = F::KSTEPS, E = F::E, LD = DP + 4;
     constexpr bool wide = F::wide, narrow = F::narrow;
     __shared__ float ol[4][16][LD];
-    __shared__ float2 ml[4][16 * RT];
+    __shared__ float2 ml[WAVES][16 * RT];
     const int D = FULL ? DP : c.D;
     const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int split = blockIdx.x, b = blockIdx.z;
-    const int hk = blockIdx.y / w.groups, first = (blockIdx.y - hk * w.groups) * 16 * RT;   // head of the group
-    int from, to, start;
+    // Chunks of a sequence are spread over the XCDs (work-group i runs on XCD i % 8), and so are a
+    // chunk's sequences: long sequences have more chunks than short ones.  128 sequences of 1024 to 8192 tokens
+    // e4m3: 318 us with chunk j of each on XCD j.
+    const int split = blockIdx.y;
+    uint32_t at = blockIdx.x + split % gridDim.x;
+    if (at >= gridDim.x) at -= gridDim.x;
+    const int pair = fdiv(at, w.by_groups), b = fdiv(pair, w.by_heads), hk = pair - b * c.Hk;
+    const int first = (at - pair * w.by_groups.d) * 16 * RT;   // head of the group
+
+    // Queries, lengths and pages are on their way together: with no window, the chunk's pages do not hang on the
+    // length.  (Loads under a condition would wait for each other: 4 us of a call.)
+    typedef T qvec __attribute__((ext_vector_type(wide ? 4 : 8), aligned(sizeof(T))));
+    constexpr int QN = wide ? 4 : 8, QI = DP / (4 * QN);
+    qvec qr[RT][QI];
+    auto q_column = [&](int i) {   // piece of QN values: of 16-byte piece i (fp32, bf16), or a half of piece i / 2
+        return narrow ? 16 * (4 * (i / 2) + g) + 8 * (i % 2) : QN * (4 * i + g);
+    };
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const T* q = Q + b * sq.seq + (long long)(hk * w.G + min(first + 16 * rt + l, w.G - 1)) * sq.head;
+#pragma unroll
+        for (int i = 0; i < QI; ++i)
+            qr[rt][i] = *reinterpret_cast<const qvec*>(q + (FULL || q_column(i) < D ? q_column(i) : 0));
+    }
+    int from, to, start = 0;
+    if (w.window > 0) w.span(b, from, to, start);
+    const int c0 = start + split * w.chunk, page0 = c0 >> c.shift;
+    // Two pages a lane (at most 2048 tokens of at least 16 a page).
+    int ids[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ids[i] = c.table[(long long)b * c.ld + min(page0 + 64 * i + lane, c.ld - 1)];
     w.span(b, from, to, start);
     const int n_chunks = w.chunks(to, start);
     if (split >= max(n_chunks, 1)) return;
-    const int c0 = start + split * w.chunk, c1 = min(c0 + w.chunk, to);
-
-    // The chunk's pages, one a lane (at most 1024 tokens of at least 16 a page).
-    const int page0 = c0 >> c.shift;
-    int ids = -1;
-    if (c0 < c1 && page0 + lane <= (c1 - 1) >> c.shift) ids = c.page_of(b, (page0 + lane) << c.shift);
+    const int c1 = min(c0 + w.chunk, to);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (page0 + 64 * i + lane >= c.ld || (unsigned)ids[i] >= (unsigned)c.pages) ids[i] = -1;
 
     // Queries: the values of d that the lane has of a key.
     u32x4 qf[RT][F::QP][wide ? 1 : DP / 32];
     float qw[RT][wide ? DP / 4 : 1];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int h = first + 16 * rt + l;
-        const T* q = Q + b * sq.seq + (long long)(hk * w.G + min(h, w.G - 1)) * sq.head;
-        constexpr int N = wide ? 4 : 8;
+        const bool head = first + 16 * rt + l < w.G;
 #pragma unroll
-        for (int i = 0; i < DP / (4 * N); ++i) {
-            // piece of N values: of 16-byte piece i (fp32, bf16), or a half of piece i / 2
-            const int d = narrow ? 16 * (4 * (i / 2) + g) + 8 * (i % 2) : N * (4 * i + g);
-            float x[N] = {};
-            if (h < w.G && d < D) {
-                typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-                const vec v = *reinterpret_cast<const vec*>(q + d);
+        for (int i = 0; i < QI; ++i) {
+            float x[QN];
 #pragma unroll
-                for (int e = 0; e < N; ++e) x[e] = paged_up(v[e]);
-            }
+            for (int e = 0; e < QN; ++e) x[e] = head && (FULL || q_column(i) < D) ? paged_up(qr[rt][i][e]) : 0.f;
             if constexpr (wide) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) qw[rt][N * i + e] = x[e];
+                for (int e = 0; e < QN; ++e) qw[rt][QN * i + e] = x[e];
             } else {
                 u32x4 parts[F::QP];
                 split8<F::QP>(x, parts);
@@ -189,30 +217,31 @@ __global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __r
         v_off[s] = 4 * g * row_bytes + (FULL || col < D ? col : 0) * (int)sizeof(CT);
     }
 
-    for (int base = c0 + F::TILE * wave; base < c1; base += 4 * F::TILE) {
-        u32x4 kr[SUBS][KSTEPS];
-        uint32_t vr[SUBS][4][DP / 16 * sizeof(CT) / 4];
-        f32x4 ks[SUBS], vs[SUBS];
-        bool there[SUBS], whole = base >= from && base + F::TILE <= to;
+    Tile<F, DP> x;
+    auto load = [&](Tile<F, DP>& x, int base) {
+        x.whole = base >= from && base + F::TILE <= to;
 #pragma unroll
         for (int s = 0; s < SUBS; ++s) {
             const int t = base + 16 * s;
             int id = -1;
-            if (t < c1) id = __builtin_amdgcn_readlane(ids, (t >> c.shift) - page0);
-            there[s] = id >= 0;
-            whole = whole && there[s];
-            const long long row = there[s] ? c.row(id, hk, t & ((1 << c.shift) - 1)) : 0;
+            if (t < c1) {
+                const int i = (t >> c.shift) - page0;
+                id = __builtin_amdgcn_readlane(i < 64 ? ids[0] : ids[1], i & 63);
+            }
+            x.there[s] = id >= 0;
+            x.whole = x.whole && x.there[s];
+            const long long row = x.there[s] ? c.row(id, hk, t & ((1 << c.shift) - 1)) : 0;
             const char* kp = (const char*)c.K + row * row_bytes;
             const char* vp = (const char*)c.V + row * row_bytes;
 #pragma unroll
             for (int i = 0; i < KSTEPS; ++i) {
                 uint32_t at = k_off + 64 * i;
                 if (!FULL && E * (4 * i + g) >= D) at = l * row_bytes;
-                kr[s][i] = *reinterpret_cast<const u32x4*>(kp + at);
+                x.kr[s][i] = *reinterpret_cast<const u32x4*>(kp + at);
             }
             if constexpr (narrow) {
-                ks[s] = *reinterpret_cast<const f32x4*>(c.Ks + row + 4 * g);
-                vs[s] = *reinterpret_cast<const f32x4*>(c.Vs + row + 4 * g);
+                x.ks[s] = *reinterpret_cast<const f32x4*>(c.Ks + row + 4 * g);
+                x.vs[s] = *reinterpret_cast<const f32x4*>(c.Vs + row + 4 * g);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -222,21 +251,22 @@ __global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __r
                     constexpr int bytes = sizeof(CT);
                     const char* p = vp + (v_off[sg] + i * row_bytes);
                     if (F::width(sg) * bytes == 16) {
-                        const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+                        const u32x4 y = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) vr[s][i][at + e] = x[e];
+                        for (int e = 0; e < 4; ++e) x.vr[s][i][at + e] = y[e];
                         at += 4;
                     } else if (F::width(sg) * bytes == 8) {
-                        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-                        vr[s][i][at] = x[0], vr[s][i][at + 1] = x[1];
+                        const u32x2 y = *reinterpret_cast<const u32x2*>(p);
+                        x.vr[s][i][at] = y[0], x.vr[s][i][at + 1] = y[1];
                         at += 2;
                     } else {
-                        vr[s][i][at++] = *reinterpret_cast<const uint32_t*>(p);
+                        x.vr[s][i][at++] = *reinterpret_cast<const uint32_t*>(p);
                     }
                 }
             }
         }
-
+    };
+    auto compute = [&](Tile<F, DP>& x, int base) {
         // Scores, in units of log 2.
         float z[RT][SUBS][4];
 #pragma unroll
@@ -246,18 +276,18 @@ __global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __r
             for (int rt = 0; rt < RT; ++rt) acc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < KSTEPS; ++i) {
-                u32x4 x = kr[s][i];
-                if (!FULL && E * (4 * i + g) >= D) x = u32x4{0, 0, 0, 0};
+                u32x4 y = x.kr[s][i];
+                if (!FULL && E * (4 * i + g) >= D) y = u32x4{0, 0, 0, 0};
                 if constexpr (wide) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
-                            acc[rt] = mfma(__builtin_bit_cast(float, (uint32_t)x[e]), qw[rt][4 * i + e], acc[rt]);
+                            acc[rt] = mfma(__builtin_bit_cast(float, (uint32_t)y[e]), qw[rt][4 * i + e], acc[rt]);
                 } else if constexpr (narrow) {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const u32x2 a = words_bf16<CT>(x[2 * half]), bb = words_bf16<CT>(x[2 * half + 1]);
+                        const u32x2 a = words_bf16<CT>(y[2 * half]), bb = words_bf16<CT>(y[2 * half + 1]);
                         const u32x4 k = {a[0], a[1], bb[0], bb[1]};
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
@@ -266,7 +296,7 @@ __global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __r
                     }
                 } else {
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) acc[rt] = mfma(x, qf[rt][0][i], acc[rt]);
+                    for (int rt = 0; rt < RT; ++rt) acc[rt] = mfma(y, qf[rt][0][i], acc[rt]);
                 }
             }
 #pragma unroll
@@ -274,22 +304,22 @@ __global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __r
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float f = unit;
-                    if constexpr (narrow) f *= ks[s][r];
+                    if constexpr (narrow) f *= x.ks[s][r];
                     z[rt][s][r] = acc[rt][r] * f;
                 }
         }
-        if (!whole) {   // tokens that do not count: no score, no value, whatever lies there
+        if (!x.whole) {   // tokens that do not count: no score, no value, whatever lies there
 #pragma unroll
             for (int s = 0; s < SUBS; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int t = base + 16 * s + 4 * g + r;
-                    const bool in = there[s] && t >= from && t < to;
+                    const bool in = x.there[s] && t >= from && t < to;
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) z[rt][s][r] = in ? z[rt][s][r] : -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < (int)(DP / 16 * sizeof(CT) / 4); ++e) vr[s][r][e] = in ? vr[s][r][e] : 0;
-                    if constexpr (narrow) vs[s][r] = in ? vs[s][r] : 0.f;
+                    for (int e = 0; e < (int)(DP / 16 * sizeof(CT) / 4); ++e) x.vr[s][r][e] = in ? x.vr[s][r][e] : 0;
+                    if constexpr (narrow) x.vs[s][r] = in ? x.vs[s][r] : 0.f;
                 }
         }
 
@@ -321,10 +351,10 @@ __global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __r
             for (int s = 0; s < SUBS; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float x = __builtin_amdgcn_exp2f(z[rt][s][r] - off);
-                    sum[rt] += x;
-                    if constexpr (narrow) x *= vs[s][r];
-                    p[4 * s + r] = x;
+                    float y = __builtin_amdgcn_exp2f(z[rt][s][r] - off);
+                    sum[rt] += y;
+                    if constexpr (narrow) y *= x.vs[s][r];
+                    p[4 * s + r] = y;
                 }
             if constexpr (wide) {
 #pragma unroll
@@ -342,22 +372,22 @@ __global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __r
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
-                        o[rt][j] = mfma(__builtin_bit_cast(float, vr[0][r][j]), pw[rt][r], o[rt][j]);
+                        o[rt][j] = mfma(__builtin_bit_cast(float, x.vr[0][r][j]), pw[rt][r], o[rt][j]);
         } else {
 #pragma unroll
             for (int jj = 0; jj < DP / 32; ++jj) {   // two columns: a word of bf16
-                uint32_t x[8];
+                uint32_t y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if constexpr (narrow) x[i] = words_bf16<CT>(vr[i / 4][i % 4][jj / 2])[jj % 2];
-                    else x[i] = vr[i / 4][i % 4][jj];
+                    if constexpr (narrow) y[i] = words_bf16<CT>(x.vr[i / 4][i % 4][jj / 2])[jj % 2];
+                    else y[i] = x.vr[i / 4][i % 4][jj];
                 }
 #pragma unroll
                 for (int odd = 0; odd < 2; ++odd) {
                     u32x4 a;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        a[i] = odd ? pack_hi16(x[2 * i], x[2 * i + 1]) : pack_lo16(x[2 * i], x[2 * i + 1]);
+                        a[i] = odd ? pack_hi16(y[2 * i], y[2 * i + 1]) : pack_lo16(y[2 * i], y[2 * i + 1]);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -366,9 +396,14 @@ __global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __r
                 }
             }
         }
+    };
+    for (int base = c0 + F::TILE * wave; base < c1; base += WAVES * F::TILE) {
+        load(x, base);
+        compute(x, base);
     }
 
-    // The waves' sums meet: o[..][j][r] is column W (4 g + r) + j of its segment.
+    // The waves' sums meet, four waves at a time: o[..][j][r] is column W (4 g + r) + j of its segment.
+    constexpr int PER = 16 * DP / 4 > 64 * WAVES ? 16 * DP / 4 / (64 * WAVES) : 1;   // pieces of 4 columns a thread
     const bool last = n_chunks <= 1;
     const long long heads = (long long)w.B * w.Hq;
 #pragma unroll
@@ -379,118 +414,202 @@ __global__ void __launch_bounds__(256) paged_chunk(Paged c, Work w, const T* __r
         halves32(s, lo, hi);
         s = lo + hi;
         if (g == 0) ml[wave][16 * rt + l] = float2{m[rt], s};
-        if (rt > 0) __syncthreads();
-        int j = 0;
+        f32x4 v[PER];
+        float top[PER], total[PER];
 #pragma unroll
-        for (int sg = 0; sg < F::SEGS; ++sg) {
+        for (int round = 0; round < WAVES / 4; ++round) {
+            if (rt + round > 0) __syncthreads();
+            if (wave / 4 == round) {
+                int j = 0;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+                for (int sg = 0; sg < F::SEGS; ++sg) {
 #pragma unroll
-                for (int e = 0; e < F::width(sg); e += 4) {
-                    const f32x4 x = {o[rt][j + e][r], o[rt][j + e + 1][r], o[rt][j + e + 2][r], o[rt][j + e + 3][r]};
-                    *reinterpret_cast<f32x4*>(&ol[wave][l][F::column(sg) + F::width(sg) * (4 * g + r) + e]) = x;
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int e = 0; e < F::width(sg); e += 4) {
+                            const f32x4 x = {o[rt][j + e][r], o[rt][j + e + 1][r], o[rt][j + e + 2][r], o[rt][j + e + 3][r]};
+                            *reinterpret_cast<f32x4*>(&ol[wave % 4][l][F::column(sg) + F::width(sg) * (4 * g + r) + e]) = x;
+                        }
+                    j += F::width(sg);
                 }
-            j += F::width(sg);
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * DP / 4; i += 256) {
-            const int hl = i / (DP / 4), d = 4 * (i % (DP / 4)), h = first + 16 * rt + hl;
-            if (h >= w.G || d >= D) continue;
-            float top = -INFINITY, total = 0.f;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) top = fmaxf(top, ml[x][16 * rt + hl].x);
-            const float off = top == -INFINITY ? 0.f : top;
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const float2 st = ml[x][16 * rt + hl];
-                const float f = __builtin_amdgcn_exp2f(st.x - off);
-                total += st.y * f;
-                v += *reinterpret_cast<const f32x4*>(&ol[x][hl][d]) * f;
             }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int at = threadIdx.x + 64 * WAVES * i, hl = at / (DP / 4) % 16, d = 4 * (at % (DP / 4));
+                if (round == 0) {
+                    top[i] = -INFINITY, total[i] = 0.f, v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int x = 0; x < WAVES; ++x) top[i] = fmaxf(top[i], ml[x][16 * rt + hl].x);
+                }
+                const float off = top[i] == -INFINITY ? 0.f : top[i];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float2 st = ml[4 * round + x][16 * rt + hl];
+                    const float f = __builtin_amdgcn_exp2f(st.x - off);
+                    total[i] += st.y * f;
+                    v[i] += *reinterpret_cast<const f32x4*>(&ol[x][hl][d]) * f;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int at = threadIdx.x + 64 * WAVES * i, hl = at / (DP / 4), d = 4 * (at % (DP / 4)), h = first + 16 * rt + hl;
+            if (hl >= 16 || h >= w.G || d >= D) continue;
             const int hq = hk * w.G + h;
             if (last) {
-                const float f = total == 0.f ? 0.f : 1.f / total;
+                const float f = total[i] == 0.f ? 0.f : 1.f / total[i];
                 T* out = O + b * so.seq + (long long)hq * so.head + d;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) out[e] = down<T>(v[e] * f);
-                if (lse && d == 0) lse[(long long)b * w.Hq + hq] = total == 0.f ? -INFINITY : top * LN2 + logf(total);
+                for (int e = 0; e < 4; ++e) out[e] = down<T>(v[i][e] * f);
+                if (lse && d == 0) lse[(long long)b * w.Hq + hq] = total[i] == 0.f ? -INFINITY : top[i] * LN2 + logf(total[i]);
             } else {
-                const long long at = split * heads + (long long)b * w.Hq + hq;
-                *reinterpret_cast<f32x4*>(w.part + at * D + d) = v;
-                if (d == 0) w.stat[at] = float2{top, total};
+                const long long to_ = split * heads + (long long)b * w.Hq + hq;
+                *reinterpret_cast<f32x4*>(w.part + to_ * D + d) = v[i];
+                if (d == 0) w.stat[to_] = float2{top[i], total[i]};
             }
         }
     }
 }
 
 // ---- the chunks of a sequence -------------------------------------------------------------------
-// A work-group per head: its waves take every fourth chunk, in order, and meet in LDS.
-template <typename T>
-__global__ void __launch_bounds__(256) paged_join(Work w, int D, T* __restrict__ O, Strides so,
-                                                  float* __restrict__ lse) {
-    __shared__ float red[4][PAGED_MOST_D];
-    __shared__ float2 stats[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.x, b = blockIdx.y;
+// WAVES waves join a head's chunks (four heads a work-group of single waves): L lanes hold a row of D, so
+// that 64 / L rows a wave and four times that are in flight, in a fixed order.
+template <typename T, int L, int WAVES>
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) paged_join(Work w, int D, T* __restrict__ O, Strides so,
+                                                                           float* __restrict__ lse) {
+    constexpr int ROWS = 64 / L, STEP = ROWS * WAVES, AHEAD = 4;
+    __shared__ f32x4 red[WAVES == 1 ? 1 : WAVES][L];
+    __shared__ float reds[WAVES == 1 ? 1 : WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = 4 * (lane & (L - 1)), b = blockIdx.y;
+    const int h = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
     int from, to, start;
     w.span(b, from, to, start);
     const int n = w.chunks(to, start);
-    if (n <= 1) return;   // its one chunk wrote the result
+    if (n <= 1 || h >= w.Hq) return;   // its one chunk wrote the result
     const long long step = (long long)w.B * w.Hq, at = (long long)b * w.Hq + h;
+    const int i0 = (WAVES == 1 ? 0 : wave * ROWS) + lane / L;
+    f32x4 x[AHEAD];
+    float2 st[AHEAD];
+    auto load = [&](int i) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            x[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+            st[a] = float2{-INFINITY, 0.f};
+            if (i + a * STEP < n) {
+                st[a] = w.stat[(i + a * STEP) * step + at];
+                if (d < D) x[a] = *reinterpret_cast<const f32x4*>(w.part + ((i + a * STEP) * step + at) * D + d);
+            }
+        }
+    };
+    load(i0);
     float m = -INFINITY, sum = 0.f;
     for (int i = lane; i < n; i += 64) m = fmaxf(m, w.stat[i * step + at].x);
     m = wave_reduce(m, OpMax());
     const float off = m == -INFINITY ? 0.f : m;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = wave; i < n; i += 4) {
-        const float2 s = w.stat[i * step + at];
-        const float f = __builtin_amdgcn_exp2f(s.x - off);
-        sum += s.y * f;
-        if (4 * lane < D) o += *reinterpret_cast<const f32x4*>(w.part + (i * step + at) * D + 4 * lane) * f;
+    for (int i = i0;;) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const float f = __builtin_amdgcn_exp2f(st[a].x - off);
+            sum += st[a].y * f;
+            o += x[a] * f;
+        }
+        i += AHEAD * STEP;
+        if (i - i0 >= n) break;
+        load(i);
     }
-    *reinterpret_cast<f32x4*>(&red[wave][4 * lane]) = o;
-    if (lane == 0) stats[wave] = float2{m, sum};
-    __syncthreads();
-    sum = stats[0].y + stats[1].y + stats[2].y + stats[3].y;
-    const int d = threadIdx.x;
-    if (d < D) {
-        const float x = red[0][d] + red[1][d] + red[2][d] + red[3][d];
-        O[b * so.seq + h * so.head + d] = down<T>(sum == 0.f ? 0.f : x / sum);
+#pragma unroll
+    for (int x = L; x < 64; x *= 2) {
+        sum += __shfl_xor(sum, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
     }
-    if (lse && d == 0) lse[at] = sum == 0.f ? -INFINITY : m * LN2 + logf(sum);
+    if constexpr (WAVES > 1) {
+        if (lane < L) red[wave][lane] = o;
+        if (lane == 0) reds[wave] = sum;
+        __syncthreads();
+        if (wave > 0) return;
+        sum = 0.f, o = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < WAVES; ++x) {
+            sum += reds[x];
+            o += red[x][lane & (L - 1)];
+        }
+    }
+    if (lane < L && d < D) {
+        const float f = sum == 0.f ? 0.f : 1.f / sum;
+        T* out = O + b * so.seq + (long long)h * so.head + d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = down<T>(o[e] * f);
+    }
+    if (lse && lane == 0) lse[at] = sum == 0.f ? -INFINITY : m * LN2 + logf(sum);
 }
 
 // ---- host --------------------------------------------------------------------------------------
-// Work-groups of all sequences at their longest: several for every place on the GPU, so that what is left
-// when the short sequences are done evens out.
-constexpr int WORK_GROUPS = 2048;
-constexpr int LEAST = 128, MOST = 1024;   // tokens of a chunk: a tile for each wave, a page for each lane
+// How the work is split.  A chunk is a multiple of LEAST tokens (a tile for each of four waves) and at most
+// MOST (the pages that a work-group's lanes hold) or CHUNK_BYTES of keys and values; a sequence has as many as make about
+// WORK_GROUPS of all sequences at their longest.  Larger ones leave a tail of busy work-groups while others are
+// done, smaller ones wait more often for their first loads (64 sequences up to 8192 bf16, chunks of 256 /
+// 512 / 1024 / 2048 tokens: 288 / 234 / 230 / 236 us; 128 of e4m3: 364 / 271 / 257 / 251).
+// Joining costs a launch: what one work-group reads in the same time stays whole, FEW tokens, or ONE where there
+// are sequences enough for half the CUs (16 x 8 heads x 1024 tokens bf16: 13.8 us whole, 14.7 split; 4 x 8: 12.7, 9.0).
+constexpr int LEAST = 128, MOST = 2048, CHUNK_BYTES = 512 << 10, WORK_GROUPS = 1024;
+constexpr int FEW = 512, ONE = 1088, MANY = 128;
 
-// Tokens of a chunk and the most chunks of a sequence.
-void plan(int B, int Hk, int max_len, int window, int& chunk, int& splits) {
+struct Plan {
+    int chunk, splits;
+};
+int whole_tokens(long long pairs) { return pairs >= MANY ? ONE : FEW; }
+int most_tokens(int D, int size) {
+    const int n = CHUNK_BYTES / (2 * D * size) / LEAST * LEAST;
+    return n > MOST ? MOST : n;   // D size <= 1024
+}
+Plan plan(long long pairs, int D, int size, int max_len, int window) {
     // a window that begins inside a tile sees up to 31 tokens before it
     const long long seen = window > 0 && window < max_len - 31 ? window + 31LL : max_len;
-    const long long want = ((long long)B * Hk * seen + WORK_GROUPS - 1) / WORK_GROUPS;
-    chunk = (int)(want > MOST ? MOST : want < LEAST ? LEAST : (want + LEAST - 1) / LEAST * LEAST);
-    splits = seen > chunk ? (int)((seen + chunk - 1) / chunk) : 1;
+    if (seen <= whole_tokens(pairs)) return {(ONE + LEAST - 1) / LEAST * LEAST, 1};
+    const int most = most_tokens(D, size);
+    long long n = WORK_GROUPS / pairs;   // chunks of the longest sequence
+    if (n < (seen + most - 1) / most) n = (seen + most - 1) / most;
+    if (n > (seen + LEAST - 1) / LEAST) n = (seen + LEAST - 1) / LEAST;
+    const int chunk = (int)(((seen + n - 1) / n + LEAST - 1) / LEAST * LEAST);
+    return {chunk, (int)((seen + chunk - 1) / chunk)};
 }
 // At least as many for every window.
-long long most_splits(int B, int Hk, int max_len) {
-    const long long a = ((long long)max_len + LEAST - 1) / LEAST, b = WORK_GROUPS / ((long long)B * Hk) + 1,
-                    c = ((long long)max_len + MOST - 1) / MOST;
+long long most_splits(long long pairs, int D, int size, int max_len) {
+    if (max_len <= whole_tokens(pairs)) return 1;
+    const int most = most_tokens(D, size);
+    const long long a = ((long long)max_len + LEAST - 1) / LEAST, b = WORK_GROUPS / pairs,
+                    c = ((long long)max_len + most - 1) / most;
     return a < b ? a : b > c ? b : c;
 }
+int size_of(int cache_type) { return cache_type == DH_F32 ? 4 : cache_type == DH_BF16 ? 2 : 1; }
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// A wave for what it has in flight at once (8 chunks of D = 128), four or sixteen for more.
+template <typename T, int L>
+int join(const Work& w, int D, void* O, Strides so, float* lse) {
+    const int once = 4 * 64 / L;
+    if (w.splits <= once) paged_join<T, L, 1><<<dim3((w.Hq + 3) / 4, w.B), 256, 0, stream()>>>(w, D, (T*)O, so, lse);
+    else if (w.splits <= 4 * once) paged_join<T, L, 4><<<dim3(w.Hq, w.B), 256, 0, stream()>>>(w, D, (T*)O, so, lse);
+    else paged_join<T, L, 16><<<dim3(w.Hq, w.B), 1024, 0, stream()>>>(w, D, (T*)O, so, lse);
+    return check_launch("dh_paged_attention");
+}
 
 template <typename T, typename CT, int DP, bool FULL, int RT>
 int launch_form(const Paged& c, Work w, const void* Q, Strides sq, void* O, Strides so, float* lse) {
-    w.groups = (w.G + 16 * RT - 1) / (16 * RT);
-    paged_chunk<T, CT, DP, FULL, RT><<<dim3(w.splits, c.Hk * w.groups, w.B), 256, 0, stream()>>>(
-        c, w, (const T*)Q, sq, (T*)O, so, lse);
+    const int groups = (w.G + 16 * RT - 1) / (16 * RT);
+    w.by_groups = make_fastdiv(groups);
+    const dim3 grid(w.B * c.Hk * groups, w.splits);
+    // Eight waves where they have two tiles each, or where there are few work-groups.
+    if (w.chunk >= 512 || (long long)grid.x * grid.y <= 512)
+        paged_chunk<T, CT, DP, FULL, RT, 8><<<grid, 512, 0, stream()>>>(c, w, (const T*)Q, sq, (T*)O, so, lse);
+    else
+        paged_chunk<T, CT, DP, FULL, RT, 4><<<grid, 256, 0, stream()>>>(c, w, (const T*)Q, sq, (T*)O, so, lse);
     DH_TRY(check_launch("dh_paged_attention"));
     if (w.splits == 1) return DH_OK;
-    paged_join<T><<<dim3(w.Hq, w.B), 256, 0, stream()>>>(w, c.D, (T*)O, so, lse);
-    return check_launch("dh_paged_attention");
+    return c.D <= 64 ? join<T, 16>(w, c.D, O, so, lse) : c.D <= 128 ? join<T, 32>(w, c.D, O, so, lse)
+                                                                    : join<T, 64>(w, c.D, O, so, lse);
 }
 
 template <typename T, typename CT>
@@ -512,8 +631,8 @@ using namespace dh;
 extern "C" {
 
 size_t dh_paged_attention_workspace(int cache_type, int B, int Hq, int Hk, int D, int max_len) {
-    if (B < 1 || Hq < 1 || Hk < 1 || D < 1 || max_len < 1) return 0;
-    const long long splits = most_splits(B, Hk, max_len);
+    if (B < 1 || Hq < 1 || Hk < 1 || D < 1 || D > PAGED_MOST_D || max_len < 1) return 0;
+    const long long splits = most_splits((long long)B * Hk, D, size_of(cache_type), max_len);
     if (splits == 1) return 0;
     const size_t rows = (size_t)splits * B * Hq;
     return up256(rows * D * 4) + rows * 8;
@@ -527,9 +646,10 @@ int dh_paged_attention(int dtype, int cache_type, int B, int Hq, int Hk, int D, 
     Paged c;
     DH_TRY(check_paged(op, dtype, cache_type, B, Hk, D, pages, page, table, ld_table, Kc, Vc, Ks, Vs, c));
     if (Hq < 1 || Hq > 65535 || Hq % Hk) return set_error(DH_ERR_INVALID, "%s: Hq=%d of Hk=%d", op, Hq, Hk);
+    if ((long long)B * Hq > 1 << 22) return set_error(DH_ERR_INVALID, "%s: shape B=%d Hq=%d", op, B, Hq);
     if (!(scale > 0.f) || !(scale - scale == 0.f))
         return set_error(DH_ERR_INVALID, "%s: scale must be finite and > 0", op);
-    if (window < 0 || max_len < 0 || max_len > 0x7FF00000 || (long long)max_len > (long long)ld_table * page)
+    if (window < 0 || max_len < 0 || max_len > 1 << 25 || (long long)max_len > (long long)ld_table * page)
         return set_error(DH_ERR_INVALID, "%s: window=%d, max_len=%d (the table has %lld)", op, window, max_len,
                          (long long)ld_table * page);
     DH_TRY(check_strides(op, "Q", sq, B, Hq, D, false));
@@ -541,8 +661,9 @@ int dh_paged_attention(int dtype, int cache_type, int B, int Hq, int Hk, int D, 
         return set_error(DH_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", op, ws_bytes, need);
     DH_TRY(ensure_init());
     if (B == 0) return DH_OK;
-    Work w{B, Hq, Hq / Hk, 1, window, max_len, 0, 0, scale, len, nullptr, nullptr};
-    plan(B, Hk, max_len, window, w.chunk, w.splits);
+    Work w{B, Hq, Hq / Hk, window, max_len, 0, 0, scale, {}, make_fastdiv(Hk), len, nullptr, nullptr};
+    const Plan p = plan((long long)B * Hk, D, size_of(cache_type), max_len, window);
+    w.chunk = p.chunk, w.splits = p.splits;
     w.part = (float*)ws;
     w.stat = (float2*)((char*)ws + up256((size_t)w.splits * B * Hq * D * 4));
     auto run = dtype == DH_F32 ? cache_type == DH_F32 ? launch<float, float>

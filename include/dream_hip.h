@@ -458,8 +458,8 @@ int dh_kv_cache_read(int dtype, int cache_type, int B, int N, int Hk, int D, voi
 /* Attention of one new token of each sequence (its key and value already in the cache) over its
  * d_len[b] tokens, the last `window` of them if window > 0:
  *   O = softmax(scale q K^T) V,   lse = log sum exp(scale q k) (B x Hq, natural log, fp32; may be NULL).
- * Hq is a multiple of Hk: query head h reads cache head h / (Hq / Hk).  Strides of Q and O: sequence,
- * head.  max_len bounds the lengths (at most ld_table page, and 2^31 - 2^20; a longer sequence is cut off there): the
+ * Hq is a multiple of Hk, B Hq at most 2^22: query head h reads cache head h / (Hq / Hk).  Strides of Q and O: sequence,
+ * head.  max_len bounds the lengths (at most ld_table page, and 2^25; a longer sequence is cut off there): the
  * work is split over it.  A sequence without tokens, or whose scores are all -infinity, has O = 0,
  * lse = -infinity.  scale finite and > 0.  What a page holds past a sequence's end does not matter, NaN included. */
 size_t dh_paged_attention_workspace(int cache_type, int B, int Hq, int Hk, int D, int max_len);
