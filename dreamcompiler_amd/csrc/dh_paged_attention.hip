@@ -131,7 +131,14 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
     typedef Form<T, CT, DP> F;
     constexpr int SUBS = F::SUBS, KSTEPS = F::KSTEPS, E = F::E, LD = DP + 4;
     constexpr bool wide = F::wide, narrow = F::narrow;
-    __shared__ float ol[4][16][LD];
+    // Queries that would take too many registers wait in LDS, where the waves' sums meet afterwards.
+    constexpr int Q_WORDS = wide ? RT * DP / 4 : RT * F::QP * DP / 8;
+    constexpr bool Q_LDS = Q_WORDS > 32 || (!wide && Q_WORDS > 16);
+    __shared__ union {
+        float o[4][16][LD];
+        u32x4 q[Q_LDS ? Q_WORDS / 4 : 1][64];
+    } shared;
+    auto& ol = shared.o;
     __shared__ float2 ml[WAVES][16 * RT];
     const int D = FULL ? DP : c.D;
     const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
@@ -175,9 +182,8 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
     for (int i = 0; i < 2; ++i)
         if (page0 + 64 * i + lane >= c.ld || (unsigned)ids[i] >= (unsigned)c.pages) ids[i] = -1;
 
-    // Queries: the values of d that the lane has of a key.
-    u32x4 qf[RT][F::QP][wide ? 1 : DP / 32];
-    float qw[RT][wide ? DP / 4 : 1];
+    // Queries: the values of d that the lane has of a key, as words of operands.
+    u32x4 qf[Q_LDS ? 1 : Q_WORDS / 4];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const bool head = first + 16 * rt + l < w.G;
@@ -186,17 +192,22 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
             float x[QN];
 #pragma unroll
             for (int e = 0; e < QN; ++e) x[e] = head && (FULL || q_column(i) < D) ? paged_up(qr[rt][i][e]) : 0.f;
+            u32x4 parts[F::QP];
             if constexpr (wide) {
 #pragma unroll
-                for (int e = 0; e < QN; ++e) qw[rt][QN * i + e] = x[e];
+                for (int e = 0; e < QN; ++e) parts[0][e] = __builtin_bit_cast(uint32_t, x[e]);
             } else {
-                u32x4 parts[F::QP];
                 split8<F::QP>(x, parts);
+            }
 #pragma unroll
-                for (int p = 0; p < F::QP; ++p) qf[rt][p][i] = parts[p];
+            for (int p = 0; p < F::QP; ++p) {
+                const int at = (rt * QI + i) * F::QP + p;
+                if constexpr (!Q_LDS) qf[at] = parts[p];
+                else if (wave == 0) shared.q[at][lane] = parts[p];
             }
         }
     }
+    if constexpr (Q_LDS) __syncthreads();
 
     f32x4 o[RT][DP / 16];
     float m[RT], sum[RT];
@@ -268,46 +279,61 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
     };
     auto compute = [&](Tile<F, DP>& x, int base) {
         // Scores, in units of log 2.
-        float z[RT][SUBS][4];
+        uint32_t q_lane = lane;
+        if constexpr (Q_LDS) asm volatile("" : "+v"(q_lane));   // read for each tile, not kept
+        auto query = [&](int rt, int i, int p) {
+            const int at = (rt * QI + i) * F::QP + p;
+            if constexpr (Q_LDS) return shared.q[at][q_lane];
+            else return qf[at];
+        };
+        f32x4 acc[RT][SUBS];
 #pragma unroll
-        for (int s = 0; s < SUBS; ++s) {
-            f32x4 acc[RT];
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) acc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < SUBS; ++s) acc[rt][s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < KSTEPS; ++i) {
-                u32x4 y = x.kr[s][i];
-                if (!FULL && E * (4 * i + g) >= D) y = u32x4{0, 0, 0, 0};
-                if constexpr (wide) {
+        for (int i = 0; i < QI; ++i) {
+            u32x4 k[SUBS];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            acc[rt] = mfma(__builtin_bit_cast(float, (uint32_t)y[e]), qw[rt][4 * i + e], acc[rt]);
-                } else if constexpr (narrow) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const u32x2 a = words_bf16<CT>(y[2 * half]), bb = words_bf16<CT>(y[2 * half + 1]);
-                        const u32x4 k = {a[0], a[1], bb[0], bb[1]};
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                            for (int p = 0; p < F::QP; ++p) acc[rt] = mfma(k, qf[rt][p][2 * i + half], acc[rt]);
-                    }
+            for (int s = 0; s < SUBS; ++s) {
+                if constexpr (narrow) {
+                    const u32x4 y = x.kr[s][i / 2];
+                    const u32x2 a = words_bf16<CT>(y[2 * (i % 2)]), c = words_bf16<CT>(y[2 * (i % 2) + 1]);
+                    k[s] = u32x4{a[0], a[1], c[0], c[1]};
                 } else {
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) acc[rt] = mfma(y, qf[rt][0][i], acc[rt]);
+                    k[s] = x.kr[s][i];
                 }
+                if (!FULL && q_column(i) >= D) k[s] = u32x4{0, 0, 0, 0};
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
+                for (int p = 0; p < F::QP; ++p) {
+                    const u32x4 qq = query(rt, i, p);
+#pragma unroll
+                    for (int s = 0; s < SUBS; ++s) {
+                        if constexpr (wide) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                acc[rt][s] = mfma(__builtin_bit_cast(float, (uint32_t)k[s][e]),
+                                                  __builtin_bit_cast(float, (uint32_t)qq[e]), acc[rt][s]);
+                        } else {
+                            acc[rt][s] = mfma(k[s], qq, acc[rt][s]);
+                        }
+                    }
+                }
+        }
+        float z[RT][SUBS][4];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s)
+#pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float f = unit;
                     if constexpr (narrow) f *= x.ks[s][r];
-                    z[rt][s][r] = acc[rt][r] * f;
+                    z[rt][s][r] = acc[rt][s][r] * f;
                 }
-        }
         if (!x.whole) {   // tokens that do not count: no score, no value, whatever lies there
 #pragma unroll
             for (int s = 0; s < SUBS; ++s)
@@ -418,7 +444,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
         float top[PER], total[PER];
 #pragma unroll
         for (int round = 0; round < WAVES / 4; ++round) {
-            if (rt + round > 0) __syncthreads();
+            if (rt + round > 0 || Q_LDS) __syncthreads();
             if (wave / 4 == round) {
                 int j = 0;
 #pragma unroll
@@ -601,8 +627,10 @@ int launch_form(const Paged& c, Work w, const void* Q, Strides sq, void* O, Stri
     const int groups = (w.G + 16 * RT - 1) / (16 * RT);
     w.by_groups = make_fastdiv(groups);
     const dim3 grid(w.B * c.Hk * groups, w.splits);
-    // Eight waves where they have two tiles each, or where there are few work-groups.
-    if (w.chunk >= 512 || (long long)grid.x * grid.y <= 512)
+    // Eight waves where they have two tiles each and the registers leave room for two such work-groups on a
+    // CU, or where there are few work-groups.
+    constexpr bool small = DP <= 128 && RT == 1;
+    if ((small && w.chunk >= 512) || (long long)grid.x * grid.y <= 512)
         paged_chunk<T, CT, DP, FULL, RT, 8><<<grid, 512, 0, stream()>>>(c, w, (const T*)Q, sq, (T*)O, so, lse);
     else
         paged_chunk<T, CT, DP, FULL, RT, 4><<<grid, 256, 0, stream()>>>(c, w, (const T*)Q, sq, (T*)O, so, lse);
