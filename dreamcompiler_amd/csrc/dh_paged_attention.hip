@@ -102,25 +102,49 @@ __device__ inline void split8(const float (&x)[8], u32x4 (&out)[P]) {
 //
 // Precision: fp32 caches take the fp32 matrix instructions.  Else a fp32 query is three parts of bf16 (24
 // bits) and a weight two (16 bits; a bf16 result has 8) or, where the model is fp32, three.
+//
+// DP is D itself for the usual head sizes (FULL), else the next multiple of 64, whose columns past D are
+// clamped and zeroed.
 template <typename T, typename CT, int DP>
 struct Form {
     static constexpr bool wide = sizeof(CT) == 4, narrow = sizeof(CT) == 1;
+    static constexpr int SIZE = sizeof(CT);
     static constexpr int SUBS = wide ? 1 : 2, TILE = 16 * SUBS;   // 16 tokens each
-    static constexpr int E = 16 / sizeof(CT);                     // values of 16 bytes
-    static constexpr int KSTEPS = DP / (4 * E);                   // 16-byte pieces of a lane's part of a key
+    static constexpr int E = 16 / SIZE;                           // values of 16 bytes
+    static constexpr int KSTEPS = (DP + 4 * E - 1) / (4 * E);     // 16-byte pieces of a lane's part of a key
     static constexpr int QP = wide ? 1 : sizeof(T) == 4 ? 3 : 1, PP = sizeof(T) == 4 ? 3 : 2;
-    // Columns of a lane: W = 8 in 128 of them or 4 in 64.
-    static constexpr int W0 = wide || DP % 128 ? 4 : 8;
-    static constexpr int SEGS = wide ? DP / 64 : (DP + 64) / 128;
-    static constexpr int width(int seg) { return wide || 128 * seg + 64 == DP ? 4 : 8; }
-    static constexpr int column(int seg) { return (wide ? 64 : 128) * seg; }
+    static constexpr int QN = wide ? 4 : 8, QI = narrow ? 2 * KSTEPS : KSTEPS;        // the same of a query, by operands
+    // Values of a row, in segments of 16 W columns: W = 8 (4 in fp32: 16 bytes) as often as it goes, then 4, 2, 1.
+    static constexpr int width_at(int column) {
+        const int left = (DP - column) / 16;
+        return left >= 8 && !wide ? 8 : left >= 4 ? 4 : left >= 2 ? 2 : 1;
+    }
+    static constexpr int column(int seg) {
+        int c = 0;
+        for (int i = 0; i < seg; ++i) c += 16 * width_at(c);
+        return c;
+    }
+    static constexpr int width(int seg) { return width_at(column(seg)); }
+    static constexpr int segments() {
+        int n = 0;
+        while (column(n) < DP) ++n;
+        return n;
+    }
+    static constexpr int SEGS = segments();
+    static constexpr int words(int seg) { return (width(seg) * SIZE + 3) / 4; }   // registers of a token's part
+    static constexpr int word(int seg) {
+        int n = 0;
+        for (int i = 0; i < seg; ++i) n += words(i);
+        return n;
+    }
+    static constexpr int WORDS = word(SEGS);
 };
 
 // What a lane loads of a tile.
-template <typename F, int DP>
+template <typename F>
 struct Tile {
     u32x4 kr[F::SUBS][F::KSTEPS];
-    uint32_t vr[F::SUBS][4][DP / 64 * (16 / F::E)];
+    uint32_t vr[F::SUBS][4][F::WORDS];
     f32x4 ks[F::SUBS], vs[F::SUBS];   // scales of tokens 4 g .. 4 g + 3 of each 16
     bool there[F::SUBS], whole;       // whether there is a page, and whether all tokens count
 };
@@ -132,7 +156,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
     constexpr int SUBS = F::SUBS, KSTEPS = F::KSTEPS, E = F::E, LD = DP + 4;
     constexpr bool wide = F::wide, narrow = F::narrow;
     // Queries that would take too many registers wait in LDS, where the waves' sums meet afterwards.
-    constexpr int Q_WORDS = wide ? RT * DP / 4 : RT * F::QP * DP / 8;
+    constexpr int QN = F::QN, QI = F::QI, Q_WORDS = RT * F::QP * QI * 4;
     constexpr bool Q_LDS = Q_WORDS > 32 || (!wide && Q_WORDS > 16);
     __shared__ union {
         float o[4][16][LD];
@@ -155,8 +179,8 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
     // Queries, lengths and pages are on their way together: with no window, the chunk's pages do not hang on the
     // length.  (Loads under a condition would wait for each other: 4 us of a call.)
     typedef T qvec __attribute__((ext_vector_type(wide ? 4 : 8), aligned(sizeof(T))));
-    constexpr int QN = wide ? 4 : 8, QI = DP / (4 * QN);
     qvec qr[RT][QI];
+    auto ends = [](int column) { return FULL && column <= DP; };   // all lanes' pieces up to there are columns
     auto q_column = [&](int i) {   // piece of QN values: of 16-byte piece i (fp32, bf16), or a half of piece i / 2
         return narrow ? 16 * (4 * (i / 2) + g) + 8 * (i % 2) : QN * (4 * i + g);
     };
@@ -165,7 +189,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
         const T* q = Q + b * sq.seq + (long long)(hk * w.G + min(first + 16 * rt + l, w.G - 1)) * sq.head;
 #pragma unroll
         for (int i = 0; i < QI; ++i)
-            qr[rt][i] = *reinterpret_cast<const qvec*>(q + (FULL || q_column(i) < D ? q_column(i) : 0));
+            qr[rt][i] = *reinterpret_cast<const qvec*>(q + (q_column(i) < D ? q_column(i) : 0));
     }
     int from, to, start = 0;
     if (w.window > 0) w.span(b, from, to, start);
@@ -191,7 +215,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
         for (int i = 0; i < QI; ++i) {
             float x[QN];
 #pragma unroll
-            for (int e = 0; e < QN; ++e) x[e] = head && (FULL || q_column(i) < D) ? paged_up(qr[rt][i][e]) : 0.f;
+            for (int e = 0; e < QN; ++e) x[e] = head && q_column(i) < D ? paged_up(qr[rt][i][e]) : 0.f;
             u32x4 parts[F::QP];
             if constexpr (wide) {
 #pragma unroll
@@ -228,8 +252,8 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
         v_off[s] = 4 * g * row_bytes + (FULL || col < D ? col : 0) * (int)sizeof(CT);
     }
 
-    Tile<F, DP> x;
-    auto load = [&](Tile<F, DP>& x, int base) {
+    Tile<F> x;
+    auto load = [&](Tile<F>& x, int base) {
         x.whole = base >= from && base + F::TILE <= to;
 #pragma unroll
         for (int s = 0; s < SUBS; ++s) {
@@ -247,7 +271,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
 #pragma unroll
             for (int i = 0; i < KSTEPS; ++i) {
                 uint32_t at = k_off + 64 * i;
-                if (!FULL && E * (4 * i + g) >= D) at = l * row_bytes;
+                if (!ends(4 * E * (i + 1)) && E * (4 * i + g) >= D) at = l * row_bytes;
                 x.kr[s][i] = *reinterpret_cast<const u32x4*>(kp + at);
             }
             if constexpr (narrow) {
@@ -255,29 +279,30 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
                 x.vs[s] = *reinterpret_cast<const f32x4*>(c.Vs + row + 4 * g);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                int at = 0;
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int sg = 0; sg < F::SEGS; ++sg) {
-                    constexpr int bytes = sizeof(CT);
                     const char* p = vp + (v_off[sg] + i * row_bytes);
-                    if (F::width(sg) * bytes == 16) {
+                    uint32_t* to_ = x.vr[s][i] + F::word(sg);
+                    const int bytes = F::width(sg) * F::SIZE;
+                    if (bytes == 16) {
                         const u32x4 y = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x.vr[s][i][at + e] = y[e];
-                        at += 4;
-                    } else if (F::width(sg) * bytes == 8) {
+                        for (int e = 0; e < 4; ++e) to_[e] = y[e];
+                    } else if (bytes == 8) {
                         const u32x2 y = *reinterpret_cast<const u32x2*>(p);
-                        x.vr[s][i][at] = y[0], x.vr[s][i][at + 1] = y[1];
-                        at += 2;
+                        to_[0] = y[0], to_[1] = y[1];
+                    } else if (bytes == 4) {
+                        *to_ = *reinterpret_cast<const uint32_t*>(p);
+                    } else if (bytes == 2) {
+                        *to_ = *reinterpret_cast<const uint16_t*>(p);
                     } else {
-                        x.vr[s][i][at++] = *reinterpret_cast<const uint32_t*>(p);
+                        *to_ = *reinterpret_cast<const uint8_t*>(p);
                     }
                 }
-            }
         }
     };
-    auto compute = [&](Tile<F, DP>& x, int base) {
+    auto compute = [&](Tile<F>& x, int base) {
         // Scores, in units of log 2.
         uint32_t q_lane = lane;
         if constexpr (Q_LDS) asm volatile("" : "+v"(q_lane));   // read for each tile, not kept
@@ -303,7 +328,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
                 } else {
                     k[s] = x.kr[s][i];
                 }
-                if (!FULL && q_column(i) >= D) k[s] = u32x4{0, 0, 0, 0};
+                if (!ends(narrow ? 64 * (i / 2 + 1) : 4 * QN * (i + 1)) && q_column(i) >= D) k[s] = u32x4{0, 0, 0, 0};
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -344,7 +369,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) z[rt][s][r] = in ? z[rt][s][r] : -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < (int)(DP / 16 * sizeof(CT) / 4); ++e) x.vr[s][r][e] = in ? x.vr[s][r][e] : 0;
+                    for (int e = 0; e < F::WORDS; ++e) x.vr[s][r][e] = in ? x.vr[s][r][e] : 0;
                     if constexpr (narrow) x.vs[s][r] = in ? x.vs[s][r] : 0.f;
                 }
         }
@@ -391,34 +416,38 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
         }
 
         // o += weights x values
-        if constexpr (wide) {
 #pragma unroll
-            for (int j = 0; j < DP / 16; ++j)
+        for (int sg = 0; sg < F::SEGS; ++sg) {
+            const int j0 = F::column(sg) / 16, W = F::width(sg), w0 = F::word(sg);
+            if constexpr (wide) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
+                for (int j = 0; j < W; ++j)
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-                        o[rt][j] = mfma(__builtin_bit_cast(float, x.vr[0][r][j]), pw[rt][r], o[rt][j]);
-        } else {
+                    for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int jj = 0; jj < DP / 32; ++jj) {   // two columns: a word of bf16
-                uint32_t y[8];
+                        for (int rt = 0; rt < RT; ++rt)
+                            o[rt][j0 + j] = mfma(__builtin_bit_cast(float, x.vr[0][r][w0 + j]), pw[rt][r], o[rt][j0 + j]);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if constexpr (narrow) y[i] = words_bf16<CT>(x.vr[i / 4][i % 4][jj / 2])[jj % 2];
-                    else y[i] = x.vr[i / 4][i % 4][jj];
-                }
+                for (int jj = 0; jj < (W + 1) / 2; ++jj) {   // two columns: a word of bf16
+                    uint32_t y[8];
 #pragma unroll
-                for (int odd = 0; odd < 2; ++odd) {
-                    u32x4 a;
+                    for (int i = 0; i < 8; ++i) {
+                        if constexpr (narrow) y[i] = words_bf16<CT>(x.vr[i / 4][i % 4][w0 + jj / 2])[jj % 2];
+                        else y[i] = x.vr[i / 4][i % 4][w0 + jj];
+                    }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        a[i] = odd ? pack_hi16(y[2 * i], y[2 * i + 1]) : pack_lo16(y[2 * i], y[2 * i + 1]);
+                    for (int odd = 0; odd < (W > 1 ? 2 : 1); ++odd) {
+                        u32x4 a;
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
+                        for (int i = 0; i < 4; ++i)
+                            a[i] = odd ? pack_hi16(y[2 * i], y[2 * i + 1]) : pack_lo16(y[2 * i], y[2 * i + 1]);
 #pragma unroll
-                        for (int p = 0; p < F::PP; ++p)
-                            o[rt][2 * jj + odd] = mfma(a, pf[rt][p], o[rt][2 * jj + odd]);
+                        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                            for (int p = 0; p < F::PP; ++p)
+                                o[rt][j0 + 2 * jj + odd] = mfma(a, pf[rt][p], o[rt][j0 + 2 * jj + odd]);
+                    }
                 }
             }
         }
@@ -429,7 +458,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
     }
 
     // The waves' sums meet, four waves at a time: o[..][j][r] is column W (4 g + r) + j of its segment.
-    constexpr int PER = 16 * DP / 4 > 64 * WAVES ? 16 * DP / 4 / (64 * WAVES) : 1;   // pieces of 4 columns a thread
+    constexpr int PER = (16 * DP / 4 + 64 * WAVES - 1) / (64 * WAVES);   // pieces of 4 columns a thread
     const bool last = n_chunks <= 1;
     const long long heads = (long long)w.B * w.Hq;
 #pragma unroll
@@ -446,23 +475,28 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
         for (int round = 0; round < WAVES / 4; ++round) {
             if (rt + round > 0 || Q_LDS) __syncthreads();
             if (wave / 4 == round) {
-                int j = 0;
 #pragma unroll
                 for (int sg = 0; sg < F::SEGS; ++sg) {
+                    const int j0 = F::column(sg) / 16, W = F::width(sg);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+                    for (int r = 0; r < 4; ++r) {
+                        float* to_ = &ol[wave % 4][l][F::column(sg) + W * (4 * g + r)];
+                        if (W >= 4) {
 #pragma unroll
-                        for (int e = 0; e < F::width(sg); e += 4) {
-                            const f32x4 x = {o[rt][j + e][r], o[rt][j + e + 1][r], o[rt][j + e + 2][r], o[rt][j + e + 3][r]};
-                            *reinterpret_cast<f32x4*>(&ol[wave % 4][l][F::column(sg) + F::width(sg) * (4 * g + r) + e]) = x;
+                            for (int e = 0; e < W; e += 4)
+                                *reinterpret_cast<f32x4*>(to_ + e) = f32x4{o[rt][j0 + e][r], o[rt][j0 + e + 1][r],
+                                                                           o[rt][j0 + e + 2][r], o[rt][j0 + e + 3][r]};
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < W; ++e) to_[e] = o[rt][j0 + e][r];
                         }
-                    j += F::width(sg);
+                    }
                 }
             }
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                const int at = threadIdx.x + 64 * WAVES * i, hl = at / (DP / 4) % 16, d = 4 * (at % (DP / 4));
+                const int at = threadIdx.x + 64 * WAVES * i, hl = min(at / (DP / 4), 15), d = 4 * (at % (DP / 4));
                 if (round == 0) {
                     top[i] = -INFINITY, total[i] = 0.f, v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -642,13 +676,21 @@ int launch_form(const Paged& c, Work w, const void* Q, Strides sq, void* O, Stri
 
 template <typename T, typename CT>
 int launch(const Paged& c, const Work& w, const void* Q, Strides sq, void* O, Strides so, float* lse) {
-    const bool two = w.G > 16;
-#define DH_FORM(DP) (c.D == DP ? launch_form<T, CT, DP, true, 1> : launch_form<T, CT, DP, false, 1>)
-    auto run = c.D <= 64 ? DH_FORM(64) : c.D <= 128 ? DH_FORM(128) : c.D <= 192 ? DH_FORM(192) : DH_FORM(256);
-    if (two && c.D == 64) run = launch_form<T, CT, 64, true, 2>;
-    if (two && c.D == 128) run = launch_form<T, CT, 128, true, 2>;
+    // Up to 32 query heads of a cache head read it once.
+    auto run = [&](auto one, auto two) { return w.G > 16 ? two(c, w, Q, sq, O, so, lse) : one(c, w, Q, sq, O, so, lse); };
+#define DH_FORM(DP, FULL) run(launch_form<T, CT, DP, FULL, 1>, launch_form<T, CT, DP, FULL, 2>)
+    switch (c.D) {
+        case 32: return DH_FORM(32, true);
+        case 64: return DH_FORM(64, true);
+        case 80: return DH_FORM(80, true);
+        case 96: return DH_FORM(96, true);
+        case 128: return DH_FORM(128, true);
+        case 192: return DH_FORM(192, true);
+        case 256: return DH_FORM(256, true);
+    }
+    return c.D < 64 ? DH_FORM(64, false) : c.D < 128 ? DH_FORM(128, false) : c.D < 192 ? DH_FORM(192, false)
+                                                                                       : DH_FORM(256, false);
 #undef DH_FORM
-    return run(c, w, Q, sq, O, so, lse);
 }
 
 }  // namespace
