@@ -189,16 +189,99 @@ __global__ void __launch_bounds__(256) cache_read(Paged c, int B, int N, const i
 }
 
 // ---- rows that begin with 16 bytes ---------------------------------------------------------------
-// A row is L lanes of V values, 16 bytes of the model's type; a wave takes 64 / L of a token's 2 Hk rows (keys
-// of all heads, then values) at once, `rows` of them in all: a token's whole where there are many tokens.
+// A row is L lanes of P values, 16 bytes of the model's type, so a wave has 64 / L heads at once, AHEAD times, keys and
+// values.  A wave takes `tokens` rows of K and V, the four waves of a work-group in turn (what lies side by side is
+// then read at the same time): its lanes find a token's place each, so that the waits for beginnings, lengths and pages
+// are those of one token.  Where there are few tokens it takes one of the blocks of heads of one.  Where there are fewer heads than half of the wave's places (MANY), a power of two `heads` of those
+// places belong to a token and the wave has several tokens at once.  (Places found by a work-group of 16 tokens
+// for its four waves, with a barrier, cost 2 to 10% more.)
+constexpr int MOST_TOKENS = 64;
 struct Units {
-    int rows, per;   // of a unit, units of a token
-    long long n;
+    int tokens, heads, blocks, each;   // log2 of a token's places (MANY), blocks of heads of a token, and of those a wave's
+    FastDiv per;                       // waves of the same tokens
+    uint32_t units;
 };
+// Rows of a wave: row t is base + (t / side) step + t % side, side = 1 << shift of them side by side.
+struct Rows {
+    int base, shift, side, step;
+    __device__ int at(int t) const { return base + (t >> shift) * step + (t & (side - 1)); }
+};
+__device__ inline Rows rows_of(const Units& u, uint32_t group, int shift) {
+    const int turns = u.per.d == 1 ? 4 : 1, side = 1 << shift, turn = group & (turns - 1);
+    return Rows{(int)(group - turn) * u.tokens + turn * side, shift, side, turns * side};
+}
 
+// The lane's row, of `lane` as t: page and place in it, page -1 for one that holds nothing and -2 for a row of no
+// sequence.
+__device__ inline int2 find_place(const Paged& c, int B, int N, const int* __restrict__ first,
+                                  const int* __restrict__ len, const Rows& rows, int tokens) {
+    const int lane = threadIdx.x & 63, n = rows.at(lane);
+    const bool any = lane < tokens && n < N;
+    int b = n;
+    long long behind = 1;
+    if (first) {
+        b = 0;
+        if (B <= 64) {   // all beginnings at once, then each token against them
+            const int v = first[min(lane, B - 1)];
+            for (int i = 0; i < tokens; ++i) {
+                const int k = max(__popcll(__ballot(lane < B && v <= rows.at(i))), 1) - 1;
+                b = lane == i ? k : b;
+            }
+        } else {
+            int hi = B;
+            while (hi - b > 1) {
+                const int mid = (b + hi) >> 1;
+                if (first[mid] <= n) b = mid;
+                else hi = mid;
+            }
+        }
+        behind = any && first[b] <= n ? (long long)first[b + 1] - n : 0;
+    }
+    int2 at = {-2, 0};
+    if (any && behind > 0) {
+        const long long t = len[b] - behind;
+        at = int2{t < 0 ? -1 : c.page_of(b, (int)t), (int)t & ((1 << c.shift) - 1)};
+    }
+    return at;
+}
+__device__ inline int2 lane_of(int2 at, int i) {   // i the same in all lanes
+    return int2{__builtin_amdgcn_readlane(at.x, i), __builtin_amdgcn_readlane(at.y, i)};
+}
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// 16 bytes of a row: its values, and the bits of the largest |x| (their order is that of the values, NaN above
+// infinity).
 template <typename T> struct Piece;
-template <> struct Piece<float> { static constexpr int V = 4; };
-template <> struct Piece<uint16_t> { static constexpr int V = 8; };
+template <> struct Piece<float> {
+    static constexpr int V = 4;
+    __device__ static void values(const u32x4& w, float (&v)[V]) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = __builtin_bit_cast(float, (uint32_t)w[e]);
+    }
+    __device__ static uint32_t most(const u32x4& w) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max(m, w[e] & 0x7FFFFFFFu);
+        return m;
+    }
+};
+template <> struct Piece<uint16_t> {
+    static constexpr int V = 8;
+    __device__ static void values(const u32x4& w, float (&v)[V]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[2 * e] = __builtin_bit_cast(float, w[e] << 16);
+            v[2 * e + 1] = __builtin_bit_cast(float, w[e] & 0xFFFF0000u);
+        }
+    }
+    __device__ static uint32_t most(const u32x4& w) {
+        u16x2 m = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[e] & 0x7FFF7FFFu));
+        return (uint32_t)max(m[0], m[1]) << 16;
+    }
+};
 
 template <typename T, int V>
 __device__ inline void load_piece(const T* p, float (&v)[V]) {
@@ -237,111 +320,141 @@ __device__ inline uint32_t group_max(uint32_t v) {
     return v;
 }
 
-// Codes of four values x / s.  A quotient's neighbours 2^-22 of it below and above x (1 / s) have the exact one
-// between them: where both round to one code, that is its; else (3 of 10^5 values) the wave takes the
-// exact quotient's.
+// The scale of a row whose largest |x| is m: the correctly rounded m / top, by one step from the product with
+// the rounded 1 / top (Markstein, "Computation of elementary functions on the IBM RISC System/6000", 1990).
+template <typename CT>
+__device__ inline float scale_of(float m) {
+    constexpr float top = Code<CT>::top, by = 1.f / top;
+    const float s = m * by;
+    return fmaf(fmaf(-s, top, m), by, s);
+}
+
+// Codes of four values y, rounded.
 template <typename CT> __device__ inline uint32_t codes_of(const float (&y)[4]);
 template <> __device__ inline uint32_t codes_of<int8_t>(const float (&y)[4]) {
     uint32_t c[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)   // 1.5 2^23 leaves the rounded integer in the last bits
-        c[e] = __builtin_bit_cast(uint32_t, fminf(fmaxf(y[e], -127.f), 127.f) + 12582912.f);
+        c[e] = __builtin_bit_cast(uint32_t, y[e] + 12582912.f);
     const uint32_t a = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), b = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
     return a | b << 16;
 }
 template <> __device__ inline uint32_t codes_of<uint8_t>(const float (&y)[4]) {
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = fminf(fmaxf(y[e], -448.f), 448.f);
-    const int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true);
+    const int a = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], a, true);
 }
+// Scale and codes of a row from the bits of its largest |x|.  x times the reciprocal of s, less and more by 2^-21 of it, has
+// the exact quotient (which the product is to 2^-22) between: where both round to one code, that is its.  Else (6 of
+// 10^5 values), and for scales below 2^-40, whose remainders could underflow, the wave
+// takes the exact quotient's.
 template <typename CT, int V>
-__device__ inline void codes(const float (&x)[V], float s, float rs, uint32_t (&out)[V / 4]) {
-    bool unsure = false;
+__device__ inline float quantise(const float (&x)[V], uint32_t most, uint32_t (&out)[V / 4]) {
+    const float m = __builtin_bit_cast(float, most);
+    float s = scale_of<CT>(m);
+    const bool plain = s >= 0x1p-40f && most < 0x7F800000u;
+    const float rs = plain ? __builtin_amdgcn_rcpf(s) : 0.f, below = rs * (1.f - 0x1p-21f), above = rs * (1.f + 0x1p-21f);
+    bool unsure = !plain && most > 0;   // zeros round to zeros
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) {
         float lo[4], hi[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float y = x[4 * i + e] * rs;
-            lo[e] = y * (1.f - 0x1p-22f);
-            hi[e] = y * (1.f + 0x1p-22f);
-        }
+        for (int e = 0; e < 4; ++e) lo[e] = x[4 * i + e] * below, hi[e] = x[4 * i + e] * above;
         out[i] = codes_of<CT>(lo);
         unsure |= out[i] != codes_of<CT>(hi);
     }
-    if (!__any(unsure)) return;
+    if (!__any(unsure)) return s;
+    s = most >= 0x7F800000u ? __builtin_nanf("") : m / Code<CT>::top;
+    const float f = s < 0x1p-40f ? 0x1p64f : 1.f;   // both up by 2^64
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) {
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = quotient(x[4 * i + e], s);
+        for (int e = 0; e < 4; ++e)
+            y[e] = s > 0.f ? fminf(fmaxf(quotient(x[4 * i + e] * f, s * f), -Code<CT>::top), Code<CT>::top) : 0.f;
         out[i] = codes_of<CT>(y);
     }
+    return s;
 }
 
-template <typename T, typename CT, int L>
-__global__ void __launch_bounds__(256) cache_write_pieces(Paged c, Units u, int B, const int* __restrict__ first,
+template <typename T, typename CT, int L, bool MANY>
+__global__ void __launch_bounds__(256) cache_write_pieces(Paged c, Units u, int B, int N, const int* __restrict__ first,
                                                           const int* __restrict__ len, const T* __restrict__ K,
                                                           Strides sk, const T* __restrict__ V, Strides sv) {
-    constexpr int P = Piece<T>::V, G = 64 / L, AHEAD = 4;
+    constexpr int P = Piece<T>::V, G = 64 / L, AHEAD = 1;
     constexpr bool scaled = sizeof(CT) == 1;
     const int lane = threadIdx.x & 63, piece = lane & (L - 1), sub = lane / L;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool in = piece * P < c.D;
-    for (long long i = 4LL * blockIdx.x + wave; i < u.n; i += 4LL * gridDim.x) {
-        const int n = (int)(i / u.per), r0 = (int)(i - (long long)n * u.per) * u.rows, r1 = min(r0 + u.rows, 2 * c.Hk);
-        int id = -1, at = 0;
-        for (int r = r0; r < r1; r += AHEAD * G) {
-            float x[AHEAD][P];
+    const uint32_t unit = 4 * blockIdx.x + wave;
+    if (unit >= u.units) return;
+    const uint32_t group = fdiv(unit, u.per);
+    const Rows rows = rows_of(u, group, MANY ? __builtin_ctz(G) - u.heads : 0);
+    const int j0 = (unit - group * u.per.d) * u.each, j1 = min(j0 + u.each, u.blocks);   // blocks of heads
+    u32x4 x[2 * AHEAD];
+    // Head h0 of the wave (the lane's own where MANY) of token i.  Lanes without one read another's row.
+    auto load = [&](int i, int h0) {
+        const int h = min(MANY ? h0 : h0 + sub, c.Hk - 1), e = in ? piece * P : 0;
+        const long long n = min(rows.at(min(i, u.tokens - 1)), N - 1);
+        const T* kp = K + n * sk.token + h * sk.head + e;
+        const T* vp = V + n * sv.token + h * sv.head + e;
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int k = r + a * G + sub, h = k < c.Hk ? k : k - c.Hk;
+        for (int a = 0; a < AHEAD; ++a) {
+            const int more = min(a * G, c.Hk - 1 - h);
+            x[2 * a] = *reinterpret_cast<const u32x4*>(kp + more * sk.head);
+            x[2 * a + 1] = *reinterpret_cast<const u32x4*>(vp + more * sv.head);
+        }
+    };
+    auto store = [&](int2 at, int h0, bool any) {
+        const int h = MANY ? h0 : h0 + sub;
+        const long long row0 = c.row(at.x, h, at.y);
 #pragma unroll
-                for (int e = 0; e < P; ++e) x[a][e] = 0.f;
-                if (k < r1 && in)
-                    load_piece<T, P>((k < c.Hk ? K + n * sk.token + h * sk.head : V + n * sv.token + h * sv.head) + piece * P,
-                                     x[a]);
-            }
-            if (r == r0) {   // the rows are on their way meanwhile
-                int b, t;
-                if (!place(first, len, B, n, b, t)) break;
-                id = c.page_of(b, t);
-                at = t & ((1 << c.shift) - 1);
-            }
-            if (id < 0) break;
+        for (int a = 0; a < AHEAD; ++a) {
+            if (!MANY && h0 + a * G >= c.Hk) break;
+            const bool there = any && h + a * G < c.Hk && at.x >= 0;
+            const long long row = row0 + ((long long)(a * G) << c.shift);
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int k = r + a * G + sub, h = k < c.Hk ? k : k - c.Hk;
-                if (r + a * G >= r1) break;
-                const long long row = c.row(id, h, at);
-                CT* o = (CT*)(k < c.Hk ? c.K : c.V) + row * c.D + piece * P;
+            for (int side = 0; side < 2; ++side) {
+                const u32x4 w = x[2 * a + side];
+                CT* o = (CT*)(side ? c.V : c.K) + row * c.D + piece * P;
                 if constexpr (!scaled) {
-                    if (k < r1 && in) store_piece<CT, P>(o, x[a]);
+                    if (there && in) *reinterpret_cast<u32x4*>(o) = w;
                 } else {
-                    uint32_t most = 0, out[P / 4];
-#pragma unroll
-                    for (int e = 0; e < P; ++e) most = max(most, __builtin_bit_cast(uint32_t, x[a][e]) & 0x7FFFFFFFu);
-                    most = group_max<L>(most);
-                    const float s = most >= 0x7F800000u ? __builtin_nanf("")
-                                                        : __builtin_bit_cast(float, most) / Code<CT>::top;
-                    if (k < r1 && piece == 0) (k < c.Hk ? c.Ks : c.Vs)[row] = s;
-                    const float f = s < 0x1p-40f ? 0x1p64f : 1.f, sf = s > 0.f ? s * f : 1.f;
-#pragma unroll
-                    for (int e = 0; e < P; ++e) x[a][e] = s > 0.f ? x[a][e] * f : 0.f;
-                    codes<CT, P>(x[a], sf, 1.f / sf, out);
-                    if (k < r1 && in) {
+                    uint32_t out[P / 4];
+                    float v[P];
+                    Piece<T>::values(w, v);
+                    const float s = quantise<CT, P>(v, group_max<L>(Piece<T>::most(w)), out);
+                    if (there && piece == 0) (side ? c.Vs : c.Ks)[row] = s;
+                    if (there && in) {
                         if constexpr (P == 8) *reinterpret_cast<u32x2*>(o) = u32x2{out[0], out[1]};
                         else *reinterpret_cast<uint32_t*>(o) = out[0];
                     }
                 }
             }
         }
+    };
+    if constexpr (MANY) {
+        const int h = sub & ((1 << u.heads) - 1);
+        int i = sub >> u.heads;
+        load(i, h);   // on their way while the places are found
+        const int2 places = find_place(c, B, N, first, len, rows, u.tokens);
+        for (int i0 = 0; i0 < u.tokens; i0 += rows.side) {
+            const int2 at = {__shfl(places.x, min(i, 63)), __shfl(places.y, min(i, 63))};
+            store(at, h, i < u.tokens);
+            i += rows.side;
+            load(i, h);
+        }
+    } else {
+        load(0, j0 * AHEAD * G);
+        const int2 places = find_place(c, B, N, first, len, rows, u.tokens);
+        for (int i = 0, j = j0; i < u.tokens && rows.at(i) < N;) {
+            store(lane_of(places, i), j * AHEAD * G, true);
+            if (++j == j1) j = j0, ++i;
+            if (i < u.tokens) load(i, j * AHEAD * G);
+        }
     }
 }
 
-// V values of a cache's type.
+// P values of a cache's type.
 template <typename CT, int V>
 __device__ inline void load_codes(const CT* p, float (&v)[V]) {
     if constexpr (sizeof(CT) > 1) {
@@ -367,44 +480,73 @@ __device__ inline void load_codes(const CT* p, float (&v)[V]) {
     }
 }
 
-template <typename T, typename CT, int L>
-__global__ void __launch_bounds__(256) cache_read_pieces(Paged c, Units u, int B, const int* __restrict__ first,
+template <typename T, typename CT, int L, bool MANY>
+__global__ void __launch_bounds__(256) cache_read_pieces(Paged c, Units u, int B, int N, const int* __restrict__ first,
                                                          const int* __restrict__ len, T* __restrict__ K, Strides sk,
                                                          T* __restrict__ V, Strides sv) {
-    constexpr int P = Piece<T>::V, G = 64 / L, AHEAD = 4;
+    constexpr int P = Piece<T>::V, G = 64 / L, AHEAD = 2;
     constexpr bool scaled = sizeof(CT) == 1;
     const int lane = threadIdx.x & 63, piece = lane & (L - 1), sub = lane / L;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool in = piece * P < c.D;
-    for (long long i = 4LL * blockIdx.x + wave; i < u.n; i += 4LL * gridDim.x) {
-        const int n = (int)(i / u.per), r0 = (int)(i - (long long)n * u.per) * u.rows, r1 = min(r0 + u.rows, 2 * c.Hk);
-        int b, t;
-        if (!place(first, len, B, n, b, t)) continue;
-        const int id = c.page_of(b, t), at = t & ((1 << c.shift) - 1);
-        for (int r = r0; r < r1; r += AHEAD * G) {
-            float x[AHEAD][P], s[AHEAD];
+    const uint32_t unit = 4 * blockIdx.x + wave;
+    if (unit >= u.units) return;
+    const uint32_t group = fdiv(unit, u.per);
+    const Rows rows = rows_of(u, group, MANY ? __builtin_ctz(G) - u.heads : 0);
+    const int j0 = (unit - group * u.per.d) * u.each, j1 = min(j0 + u.each, u.blocks);   // blocks of heads
+    const int2 places = find_place(c, B, N, first, len, rows, u.tokens);
+    // AHEAD heads of the lane, G apart (MANY: head h0 of AHEAD tokens, side by side).
+    auto move = [&](const int2 (&at)[AHEAD], int i, int h0) {
+        float x[AHEAD][2][P], s[AHEAD][2];
+        const int h = MANY ? h0 : h0 + sub, e = in ? piece * P : 0;
+        const long long row0 = MANY ? 0 : c.row(max(at[0].x, 0), min(h, c.Hk - 1), at[0].y);
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int k = r + a * G + sub, h = k < c.Hk ? k : k - c.Hk;
-                s[a] = 1.f;
+        for (int a = 0; a < AHEAD; ++a) {   // lanes without a row read another's
+            const long long row = MANY ? c.row(max(at[a].x, 0), min(h, c.Hk - 1), at[a].y)
+                                       : row0 + ((long long)min(a * G, max(c.Hk - 1 - h, 0)) << c.shift);
 #pragma unroll
-                for (int e = 0; e < P; ++e) x[a][e] = 0.f;
-                if (k < r1 && in && id >= 0) {
-                    const long long row = c.row(id, h, at);
-                    if constexpr (scaled) s[a] = (k < c.Hk ? c.Ks : c.Vs)[row];
-                    load_codes<CT, P>((const CT*)(k < c.Hk ? c.K : c.V) + row * c.D + piece * P, x[a]);
-                }
+            for (int side = 0; side < 2; ++side) {
+                s[a][side] = 1.f;
+                if constexpr (scaled) s[a][side] = (side ? c.Vs : c.Ks)[row];
+                load_codes<CT, P>((const CT*)(side ? c.V : c.K) + row * c.D + e, x[a][side]);
             }
+        }
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int k = r + a * G + sub, h = k < c.Hk ? k : k - c.Hk;
-                if (k >= r1 || !in) continue;
+        for (int a = 0; a < AHEAD; ++a) {
+            const long long n = rows.at(MANY ? i + a * rows.side : i);
+            const int ha = h + (MANY ? 0 : a * G);
+            const bool there = in && at[a].x >= -1 && ha < c.Hk;
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
                 if constexpr (scaled)
 #pragma unroll
-                    for (int e = 0; e < P; ++e) x[a][e] *= s[a];
-                store_piece<T, P>((k < c.Hk ? K + n * sk.token + h * sk.head : V + n * sv.token + h * sv.head) + piece * P,
-                                  x[a]);
+                    for (int e = 0; e < P; ++e) x[a][side][e] *= s[a][side];
+                if (at[a].x < 0)
+#pragma unroll
+                    for (int e = 0; e < P; ++e) x[a][side][e] = 0.f;
+                if (there)
+                    store_piece<T, P>((side ? V + n * sv.token + ha * sv.head : K + n * sk.token + ha * sk.head) + piece * P,
+                                      x[a][side]);
             }
+        }
+    };
+    int2 at[AHEAD];
+    if constexpr (MANY) {
+        const int h = sub & ((1 << u.heads) - 1);
+        for (int i = sub >> u.heads; i - sub / u.heads < u.tokens; i += AHEAD * rows.side) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int t = i + a * rows.side;
+                at[a] = int2{__shfl(places.x, min(t, 63)), __shfl(places.y, min(t, 63))};
+                if (t >= u.tokens) at[a].x = -2;
+            }
+            move(at, i, h);
+        }
+    } else {
+        for (int i = 0; i < u.tokens && rows.at(i) < N; ++i) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) at[a] = lane_of(places, i);
+            for (int j = j0; j < j1; ++j) move(at, i, j * AHEAD * G);
         }
     }
 }
@@ -415,33 +557,52 @@ int groups_of(long long rows) {
     return (int)(groups < most ? groups : most);
 }
 
-// Rows of a unit: all of a token's where that gives each of the GPU's 8192 waves a unit, else as few
-// as the wave takes at once.
-Units units_of(int N, int rows, int at_once) {
-    int per = (rows + at_once - 1) / at_once, each = (int)(N >= 8192 ? per : ((long long)N * per + 8191) / 8192);
-    if (each < 1) each = 1;
-    per = (per + each - 1) / each;
-    return Units{each * at_once, per, (long long)N * per};
+// `places`: rows of a side that a wave has at once, `ahead`: how often.  Tokens of a wave: as many as leave each of
+// 24576 waves some (three times what the GPU holds, for the tail's sake); blocks of heads, where there are fewer tokens, likewise.
+Units units_of(int N, int Hk, int places, int ahead, bool& many) {
+    int shift = 0, tokens = N / 24576;
+    while (1 << shift < Hk) ++shift;
+    many = 2 << shift <= places;
+    const int side = many ? places >> shift : 1;
+    tokens = (tokens + side - 1) / side * side;
+    tokens = tokens < side ? side : tokens > MOST_TOKENS ? MOST_TOKENS : tokens;
+    const int blocks = many ? 1 : (Hk + places * ahead - 1) / (places * ahead);
+    long long groups = ((long long)N + tokens - 1) / tokens;
+    int each = (int)((groups * blocks + 24575) / 24576);
+    if (each > blocks) each = blocks;
+    const int per = (blocks + each - 1) / each;
+    if (per == 1) groups = (groups + 3) / 4 * 4;   // four waves in turn
+    return Units{tokens, shift, blocks, each, make_fastdiv(per), (uint32_t)groups * per};
 }
 bool whole_pieces(const void* p, Strides st, int N, int Hk, int size) {
     const long long bits = (N > 1 ? st.token : 0) | (Hk > 1 ? st.head : 0);
     return ((uintptr_t)p & 15) == 0 && bits * size % 16 == 0;
 }
-int piece_groups(const Units& u) {
-    const long long groups = (u.n + 3) / 4;
-    return (int)(groups < 1 << 20 ? groups : 1 << 20);
+template <typename T, typename CT>
+auto by_lanes_write(int L, bool many) {
+    return L == 4    ? many ? cache_write_pieces<T, CT, 4, true> : cache_write_pieces<T, CT, 4, false>
+           : L == 8  ? many ? cache_write_pieces<T, CT, 8, true> : cache_write_pieces<T, CT, 8, false>
+           : L == 16 ? many ? cache_write_pieces<T, CT, 16, true> : cache_write_pieces<T, CT, 16, false>
+           : L == 32 ? many ? cache_write_pieces<T, CT, 32, true> : cache_write_pieces<T, CT, 32, false>
+                     : cache_write_pieces<T, CT, 64, false>;
 }
-
+template <typename T, typename CT>
+auto by_lanes_read(int L, bool many) {
+    return L == 4    ? many ? cache_read_pieces<T, CT, 4, true> : cache_read_pieces<T, CT, 4, false>
+           : L == 8  ? many ? cache_read_pieces<T, CT, 8, true> : cache_read_pieces<T, CT, 8, false>
+           : L == 16 ? many ? cache_read_pieces<T, CT, 16, true> : cache_read_pieces<T, CT, 16, false>
+           : L == 32 ? many ? cache_read_pieces<T, CT, 32, true> : cache_read_pieces<T, CT, 32, false>
+                     : cache_read_pieces<T, CT, 64, false>;
+}
 template <typename T, typename CT>
 int launch_write(const Paged& c, int B, int N, const int* first, const int* len, const void* K, Strides sk,
                  const void* V, Strides sv) {
     if (whole_pieces(K, sk, N, c.Hk, sizeof(T)) && whole_pieces(V, sv, N, c.Hk, sizeof(T))) {
         const int lanes = c.D / Piece<T>::V, L = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
-        const Units u = units_of(N, 2 * c.Hk, 64 / L);
-        auto run = L == 4 ? cache_write_pieces<T, CT, 4> : L == 8 ? cache_write_pieces<T, CT, 8>
-                   : L == 16 ? cache_write_pieces<T, CT, 16> : L == 32 ? cache_write_pieces<T, CT, 32>
-                                                                       : cache_write_pieces<T, CT, 64>;
-        run<<<piece_groups(u), 256, 0, stream()>>>(c, u, B, first, len, (const T*)K, sk, (const T*)V, sv);
+        bool many;
+        const Units u = units_of(N, c.Hk, 64 / L, 1, many);
+        auto run = by_lanes_write<T, CT>(L, many);
+        run<<<(u.units + 3) / 4, 256, 0, stream()>>>(c, u, B, N, first, len, (const T*)K, sk, (const T*)V, sv);
     } else {
         cache_write<T, CT><<<groups_of(2LL * N * c.Hk), 256, 0, stream()>>>(c, B, N, first, len, (const T*)K, sk,
                                                                             (const T*)V, sv);
@@ -453,11 +614,10 @@ int launch_read(const Paged& c, int B, int N, const int* first, const int* len, 
                 Strides sv) {
     if (whole_pieces(K, sk, N, c.Hk, sizeof(T)) && whole_pieces(V, sv, N, c.Hk, sizeof(T))) {
         const int lanes = c.D / Piece<T>::V, L = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
-        const Units u = units_of(N, 2 * c.Hk, 64 / L);
-        auto run = L == 4 ? cache_read_pieces<T, CT, 4> : L == 8 ? cache_read_pieces<T, CT, 8>
-                   : L == 16 ? cache_read_pieces<T, CT, 16> : L == 32 ? cache_read_pieces<T, CT, 32>
-                                                                      : cache_read_pieces<T, CT, 64>;
-        run<<<piece_groups(u), 256, 0, stream()>>>(c, u, B, first, len, (T*)K, sk, (T*)V, sv);
+        bool many;
+        const Units u = units_of(N, c.Hk, 64 / L, 2, many);
+        auto run = by_lanes_read<T, CT>(L, many);
+        run<<<(u.units + 3) / 4, 256, 0, stream()>>>(c, u, B, N, first, len, (T*)K, sk, (T*)V, sv);
     } else {
         cache_read<T, CT><<<groups_of(2LL * N * c.Hk), 256, 0, stream()>>>(c, B, N, first, len, (T*)K, sk, (T*)V, sv);
     }
@@ -466,7 +626,7 @@ int launch_read(const Paged& c, int B, int N, const int* first, const int* len, 
 
 int check_tokens(const char* op, int B, int N, int Hk, int D, const int* first, const int* len, const void* K,
                  const long long* sk, const void* V, const long long* sv, bool out) {
-    if (N < 0 || N > 0x7FF00000 || (!first && N != B))
+    if (N < 0 || N > 1 << 29 || (!first && N != B))
         return set_error(DH_ERR_INVALID, "%s: N=%d tokens of B=%d sequences", op, N, B);
     DH_TRY(check_strides(op, "K", sk, N, Hk, D, out));
     DH_TRY(check_strides(op, "V", sv, N, Hk, D, out));

@@ -439,7 +439,7 @@ int dh_qk_norm_rope_bwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, i
  * reads back as NaN.  Token t of sequence b is in page d_table[b ld_table + t / page].  A table entry
  * outside 0 .. pages - 1, or past the table's row, holds nothing: such tokens are not written, read as
  * zero and are not attended.  page is a power of two from 16 to 4096, D a multiple of 16 up to 256
- * (callers zero-pad others), B and Hk up to 65535.  Offsets are 64-bit.
+ * (callers zero-pad others), B and Hk up to 65535, N up to 2^29.  Offsets are 64-bit.
  *
  * Writes N new tokens: rows d_first[b] .. d_first[b + 1] - 1 of K and V (strides of token and head) are the
  * last tokens of sequence b, which holds d_len[b] of them after the call.  d_first (B + 1 values, rising)
