@@ -615,6 +615,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) paged_join(Work
 // are sequences enough for half the CUs (16 x 8 heads x 1024 tokens bf16: 13.8 us whole, 14.7 split; 4 x 8: 12.7, 9.0).
 constexpr int LEAST = 128, MOST = 2048, CHUNK_BYTES = 512 << 10, WORK_GROUPS = 1024;
 constexpr int FEW = 512, ONE = 1088, MANY = 128;
+constexpr int MOST_SPLITS = 65535;   // of a launch; at most 2^25 tokens in chunks of MOST are fewer
 
 struct Plan {
     int chunk, splits;
@@ -632,6 +633,7 @@ Plan plan(long long pairs, int D, int size, int max_len, int window) {
     long long n = WORK_GROUPS / pairs;   // chunks of the longest sequence
     if (n < (seen + most - 1) / most) n = (seen + most - 1) / most;
     if (n > (seen + LEAST - 1) / LEAST) n = (seen + LEAST - 1) / LEAST;
+    if (n > MOST_SPLITS) n = MOST_SPLITS;
     const int chunk = (int)(((seen + n - 1) / n + LEAST - 1) / LEAST * LEAST);
     return {chunk, (int)((seen + chunk - 1) / chunk)};
 }
@@ -640,9 +642,15 @@ long long most_splits(long long pairs, int D, int size, int max_len) {
     if (max_len <= whole_tokens(pairs)) return 1;
     const int most = most_tokens(D, size);
     const long long a = ((long long)max_len + LEAST - 1) / LEAST, b = WORK_GROUPS / pairs,
-                    c = ((long long)max_len + most - 1) / most;
-    return a < b ? a : b > c ? b : c;
+                    c = ((long long)max_len + most - 1) / most, n = a < b ? a : b > c ? b : c;
+    return n < MOST_SPLITS ? n : MOST_SPLITS;
 }
+// Waves of a work-group: eight where they have two tiles each and the registers leave room for two such
+// work-groups on a CU, or where there are few work-groups (33 x 12 sequences fp32: 37 us with eight, 45 with four).
+int waves_of(int D, int row_tiles, int chunk, long long groups) {
+    return (D <= 128 && row_tiles == 1 && chunk >= 512) || groups <= 512 ? 8 : 4;
+}
+int row_tiles_of(int G) { return G > 16 ? 2 : 1; }
 int size_of(int cache_type) { return cache_type == DH_F32 ? 4 : cache_type == DH_BF16 ? 2 : 1; }
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -661,10 +669,7 @@ int launch_form(const Paged& c, Work w, const void* Q, Strides sq, void* O, Stri
     const int groups = (w.G + 16 * RT - 1) / (16 * RT);
     w.by_groups = make_fastdiv(groups);
     const dim3 grid(w.B * c.Hk * groups, w.splits);
-    // Eight waves where they have two tiles each and the registers leave room for two such work-groups on a
-    // CU, or where there are few work-groups.
-    constexpr bool small = DP <= 128 && RT == 1;
-    if ((small && w.chunk >= 512) || (long long)grid.x * grid.y <= 512)
+    if (waves_of(c.D, RT, w.chunk, (long long)grid.x * grid.y) == 8)
         paged_chunk<T, CT, DP, FULL, RT, 8><<<grid, 512, 0, stream()>>>(c, w, (const T*)Q, sq, (T*)O, so, lse);
     else
         paged_chunk<T, CT, DP, FULL, RT, 4><<<grid, 256, 0, stream()>>>(c, w, (const T*)Q, sq, (T*)O, so, lse);
@@ -677,7 +682,7 @@ int launch_form(const Paged& c, Work w, const void* Q, Strides sq, void* O, Stri
 template <typename T, typename CT>
 int launch(const Paged& c, const Work& w, const void* Q, Strides sq, void* O, Strides so, float* lse) {
     // Up to 32 query heads of a cache head read it once.
-    auto run = [&](auto one, auto two) { return w.G > 16 ? two(c, w, Q, sq, O, so, lse) : one(c, w, Q, sq, O, so, lse); };
+    auto run = [&](auto one, auto two) { return row_tiles_of(w.G) == 2 ? two(c, w, Q, sq, O, so, lse) : one(c, w, Q, sq, O, so, lse); };
 #define DH_FORM(DP, FULL) run(launch_form<T, CT, DP, FULL, 1>, launch_form<T, CT, DP, FULL, 2>)
     switch (c.D) {
         case 32: return DH_FORM(32, true);
@@ -706,6 +711,18 @@ size_t dh_paged_attention_workspace(int cache_type, int B, int Hq, int Hk, int D
     if (splits == 1) return 0;
     const size_t rows = (size_t)splits * B * Hq;
     return up256(rows * D * 4) + rows * 8;
+}
+
+int dh_paged_attention_plan(int cache_type, int B, int Hq, int Hk, int D, int max_len, int window, int* plan_out) {
+    if (!plan_out) return set_error(DH_ERR_INVALID, "dh_paged_attention_plan: null pointer");
+    if (B < 1 || Hk < 1 || Hq < 1 || Hq % Hk || D < 1 || D > PAGED_MOST_D || max_len < 0 || max_len > 1 << 25 || window < 0)
+        return set_error(DH_ERR_INVALID, "dh_paged_attention_plan: shape B=%d Hq=%d Hk=%d D=%d max_len=%d window=%d", B,
+                         Hq, Hk, D, max_len, window);
+    const Plan p = plan((long long)B * Hk, D, size_of(cache_type), max_len, window);
+    const int rt = row_tiles_of(Hq / Hk), groups = (Hq / Hk + 16 * rt - 1) / (16 * rt);
+    plan_out[0] = p.chunk, plan_out[1] = p.splits;
+    plan_out[2] = waves_of(D, rt, p.chunk, (long long)B * Hk * groups * p.splits), plan_out[3] = groups;
+    return DH_OK;
 }
 
 int dh_paged_attention(int dtype, int cache_type, int B, int Hq, int Hk, int D, float scale, int window,

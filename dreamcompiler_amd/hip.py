@@ -106,6 +106,7 @@ _SIGS = {
     "dh_kv_cache_write": (_i, [_i] * 6 + [_vp] * 6 + [_i, _i, _vp, _i] + [_vp] * 4),
     "dh_kv_cache_read": (_i, [_i] * 6 + [_vp] * 6 + [_i, _i, _vp, _i] + [_vp] * 4),
     "dh_paged_attention_workspace": (_sz, [_i] * 6),
+    "dh_paged_attention_plan": (_i, [_i] * 7 + [ctypes.POINTER(_i)]),
     "dh_paged_attention": (_i, [_i] * 6 + [_f, _i, _vp, _vp, _vp] + [_i] * 3 + [_vp, _i]
                            + [_vp] * 8 + [_sz]),
 }
@@ -468,6 +469,14 @@ def kv_cache_read(dtype, cache_type, B, N, Hk, D, K, k_strides, V, v_strides, fi
 
 def paged_attention_workspace(cache_type, B, Hq, Hk, D, max_len):
     return load().dh_paged_attention_workspace(cache_type, B, Hq, Hk, D, max_len)
+
+
+def paged_attention_plan(cache_type, B, Hq, Hk, D, max_len, window):
+    """Tokens of a chunk, most chunks of a sequence, waves of a work-group, work-groups of a chunk."""
+    plan = (_i * 4)()
+    check(load().dh_paged_attention_plan(cache_type, B, Hq, Hk, D, max_len, window, plan),
+          "dh_paged_attention_plan")
+    return tuple(plan)
 
 
 def paged_attention(dtype, cache_type, B, Hq, Hk, D, scale, window, Q, q_strides, len_, max_len,

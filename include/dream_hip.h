@@ -469,6 +469,11 @@ int dh_paged_attention(int dtype, int cache_type, int B, int Hq, int Hk, int D, 
                        const void* d_Kc, const void* d_Vc, const float* d_Ks, const float* d_Vs,
                        void* d_O, const long long* o_strides, float* d_lse, void* d_ws,
                        size_t ws_bytes);
+/* How a call of these sizes runs (no device needed), 4 values: the tokens of a chunk, the most chunks of a sequence (one
+ * needs no workspace and no second launch), the waves of a work-group, and the work-groups of a chunk and cache head,
+ * each of which reads it (1 up to 32 query heads). */
+int dh_paged_attention_plan(int cache_type, int B, int Hq, int Hk, int D, int max_len, int window,
+                            int* plan);
 
 #ifdef __cplusplus
 }

@@ -66,7 +66,7 @@ def test_qk_shapes(f):
     for R in (-2, 3, 10):
         with raises("R="):
             f(R=R)
-    for eps in (0.0, -1.0, NAN, INF):
+    for eps in (0.0, -1.0, 1e-39, NAN, INF):
         with raises("eps"):
             f(eps=eps)
     for bad in (dict(table=None), dict(n=0), dict(pos=None, n=2), dict(R=0, n=0)):
@@ -136,14 +136,14 @@ def test_cache_shapes(f):
     for bad in (dict(pages=0), dict(ld=0), dict(pages=2 ** 31 - 1, page=4096, D=256, Hk=64)):
         with raises("pages="):
             f(**bad)
-    for n in ("Kc", "Vc"):
+    for n in ("Kc", "Vc", "Ks", "Vs"):
         with raises("aligned"):
             f(**{n: ODD})
 
 
 @pytest.mark.parametrize("f", [write, read])
 def test_cache_rows(f):
-    for bad in (dict(N=-1), dict(N=2 ** 31 - 1), dict(first=None)):
+    for bad in (dict(N=-1), dict(N=2 ** 29 + 1), dict(N=2 ** 31 - 1), dict(first=None)):
         with raises("tokens"):
             f(**bad)
     for n in ("sk", "sv"):
@@ -165,7 +165,9 @@ def test_attention_arguments():
     for s in (0.0, -1.0, NAN, INF):
         with raises("scale"):
             attend(scale=s)
-    for bad in (dict(window=-1), dict(max_len=-1), dict(max_len=33)):
+    with raises("shape"):
+        attend(B=65535, Hq=128, sq=(128 * 32, 32), so=(128 * 32, 32))
+    for bad in (dict(window=-1), dict(max_len=-1), dict(max_len=33), dict(ld=2 ** 22, max_len=2 ** 25 + 1)):
         with raises("max_len"):
             attend(**bad)
     for n in ("sq", "so"):
@@ -184,3 +186,25 @@ def test_attention_arguments():
         attend(B=1, ld=8192, max_len=131072, ws=ODD)
     assert hip.paged_attention_workspace(3, 1, 4, 2, 32, 16) == 0
     assert hip.paged_attention_workspace(3, 0, 4, 2, 32, 1000) == 0
+
+
+def test_plans_fit_their_workspaces():
+    """For lengths, windows and shapes of all sizes: the chunks cover what is seen, a work-group's lanes hold a
+    chunk's pages, the launch holds the chunks, and the query's workspace has room for the partial results of every window."""
+    for ct in (0, 1, 3, 4):
+        for B, Hq, Hk, D in ((1, 1, 1, 16), (1, 32, 8, 128), (3, 12, 3, 80), (16, 16, 8, 256), (64, 64, 8, 128), (500, 40, 2, 64),
+                             (4096, 8, 8, 32), (65535, 64, 1, 256)):
+            for max_len in (0, 1, 31, 128, 512, 513, 1088, 1089, 2047, 5000, 40000, 131072, 2 ** 20, 2 ** 25):
+                room = hip.paged_attention_workspace(ct, B, Hq, Hk, D, max_len)
+                for window in (0, 1, 97, 512, 1000, 1057, 1058, 3000, 33333, 2 ** 31 - 1):
+                    chunk, splits, waves, groups = hip.paged_attention_plan(ct, B, Hq, Hk, D, max_len, window)
+                    seen = min(max_len, window + 31) if window else max_len
+                    assert chunk % 128 == 0 and 128 <= chunk <= 2048 and 1 <= splits <= 65535
+                    assert chunk * splits >= seen and waves in (4, 8)
+                    assert groups == (-(-(Hq // Hk) // 32) if Hq // Hk > 16 else 1)
+                    need = splits * B * Hq * (D + 2) * 4 if splits > 1 else 0
+                    assert need <= room, (ct, B, Hq, Hk, D, max_len, window)
+    for bad in (dict(B=0), dict(Hq=3), dict(D=300), dict(max_len=-1), dict(window=-1), dict(max_len=2 ** 25 + 1)):
+        a = {**dict(cache_type=3, B=2, Hq=4, Hk=2, D=32, max_len=100, window=0), **bad}
+        with raises("shape"):
+            hip.paged_attention_plan(**a)

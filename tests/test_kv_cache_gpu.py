@@ -183,6 +183,59 @@ def test_many_tokens(dtype, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("Hk,D", [(1, 16), (2, 80), (3, 32), (5, 256)])
+def test_many_sequences(Hk, D, dtype, kind):
+    """More sequences than lanes, empty ones among them, beside few heads (several tokens a wave) and many."""
+    lens = [(7 * b) % 23 for b in range(150)]
+    run(dtype, kind, lens, [n if b % 3 else n // 2 for b, n in enumerate(lens)], Hk, D, 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("Hk,D,T", [(1, 32, 60000), (2, 64, 52001), (9, 16, 51000)])
+def test_long(Hk, D, T, dtype, kind):
+    """Several tokens a wave, by turns of four waves; all of a sequence written, and read back."""
+    r = np.random.default_rng(4)
+    page = 64
+    c = Cache(kind, [T], Hk, D, page).upload()
+    K, V = (Strided(r.standard_normal((T, Hk, D)), dtype) for _ in "KV")
+    first = ints([0, T])
+    hip.kv_cache_write(TYPE[dtype], TYPE[kind], 1, T, Hk, D, K, K.strides, V, V.strides, first, c.lbuf, *c.args())
+    out = [Strided(np.zeros((T, Hk, D)), dtype) for _ in "KV"]
+    hip.kv_cache_read(TYPE[dtype], TYPE[kind], 1, T, Hk, D, out[0], out[0].strides, out[1], out[1].strides, first, c.lbuf,
+                      *c.args())
+    raw, scale = c.download()
+    t = np.arange(T)
+    at = (c.table[0, t // page], slice(None), t % page)
+    for n, x, o in (("K", K, out[0]), ("V", V, out[1])):
+        if kind in TOP:
+            codes, s = quantised(x.value, kind)
+            assert np.array_equal(decode(raw[n][at], kind), codes) and np.array_equal(scale[n][at], s)
+        else:
+            codes, s = x.value, None
+            assert np.array_equal(raw[n][at].view(np.uint8), rounded(x.value, kind)[0].view(np.uint8))
+        assert np.array_equal(o.get(), read_back(codes, s, kind, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [[5, 3, 9, 9], [-7, 4, 2, 12], [0, 2 ** 31 - 1, 3, 6], [0, 0, 0, 0], [9, 9, 9, 9]])
+def test_beginnings_that_do_not_rise(first):
+    """What no caller means: nothing is read or written out of place, and rows of no sequence stay."""
+    Hk, D, N = 2, 32, 8
+    c = Cache("bf16", [20, 20, 20], Hk, D, 16).upload()
+    K = Strided(np.ones((N, Hk, D)), "bf16")
+    hip.kv_cache_write(hip.BF16, hip.BF16, 3, N, Hk, D, K, K.strides, K, K.strides, ints(first), c.lbuf, *c.args())
+    out = Strided(np.full((N, Hk, D), 7.0), "bf16")
+    hip.kv_cache_read(hip.BF16, hip.BF16, 3, N, Hk, D, out, out.strides, out, out.strides, ints(first), c.lbuf, *c.args())
+    got, raw = out.get(), c.download()[0]["K"]
+    assert (np.isnan(got) | (got == 0) | (got == 1) | (got == 7)).all()
+    assert ((raw == 0x7FC0) | (raw == 0x3F80)).all()
+    if first in ([0, 0, 0, 0], [9, 9, 9, 9]):
+        assert (got == 7).all() and (raw == 0x7FC0).all()
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """Places whose offsets pass 2^32 values and 2^32 rows' bytes."""
     Hk, D, page, pages = 8, 256, 4096, 700          # 5.9e9 values

@@ -97,9 +97,36 @@ def test_lengths(dtype, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("D", [32, 128, 192])
+def test_long_chunks_of_many_sequences(D, dtype, kind):
+    """Sequences enough for whole chunks: up to 2048 tokens, of more pages than lanes, by eight waves; and ones that
+    are not split at all."""
+    Hk = 1
+    lens = [4100, 3000, 17, 0] + [1 + b % 40 for b in range(508)]
+    chunk, splits, _, _ = hip.paged_attention_plan(TYPE[kind], len(lens), 2, Hk, D, 4112, 0)
+    assert splits >= 2 and (D > 32 or chunk > 1024)
+    Case(dtype, kind, lens, 2, Hk, D, 16).run().check()
+    lens = [1088, 1087, 1025, 1024, 1000] + [3] * 123
+    assert hip.paged_attention_plan(TYPE[kind], 128, 2, Hk, D, 1088, 0)[1] == 1
+    Case(dtype, kind, lens, 2, Hk, D, 16).run().check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("D,T", [(32, 5000), (48, 9000), (96, 5000), (112, 9000), (160, 2500), (208, 1500), (256, 9000)])
+def test_joins(D, T, dtype, kind):
+    """Chunks for one, four and sixteen waves, of every length of a row."""
+    Case(dtype, kind, [T, T // 2, 600, 5], 3, 1, D, 32).run().check()
+    Case(dtype, kind, [T // 3, 129], 34, 2, D, 16, window=700).run().check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("window", [1, 2, 16, 31, 100, 257, 1000, 2 ** 31 - 1])
 def test_windows(window, dtype, kind):
     Case(dtype, kind, [0, 1, 100, 258, 999, 1300], 6, 2, 64, 16, window=window).run().check()
+    if window <= 257:
+        Case(dtype, kind, [6001, 3000, 2], 4, 1, 128, 16, window=window).run().check()
 
 
 @pytest.mark.gpu

@@ -8,8 +8,8 @@ Tolerances (u = 2^-24, ub = 2^-8: the largest relative error of one rounding to 
            of the row's largest y.  Then one rounding to the output's type.
  dx        x r to 16 u, dy g to 5 u, their mean over D: 25 u of the terms' mean size: under 64 u of
            r (max |dy g| + max |x r| mean |dy g x r|); one rounding to its type.
- dg        each term to 24 u; a chain of additions is at most the rows of a wave (of rows / 8192, here 1), 3 for
-           the waves, and a quarter of 2050 work-groups: under (64 + min(rows, 520)) u of the terms' sizes.
+ dg        each term to 24 u; a chain of additions is at most the rows of a lane (of 4096 waves), the 64 rows that
+           meet in a work-group, 16 of 1024 work-groups, and 64: under (64 + min(rows, 520)) u of the terms' sizes.
 """
 import numpy as np
 import pytest
@@ -112,8 +112,43 @@ def test_sides_that_are_left_out(dtype):
 def test_sizes_of_values():
     """Rows far below eps, far above 1, and of zeros."""
     for scale in (0.0, 1e-30, 1e-3, 1e15):
-        run(1, 6, 3, 2, 64, 32, False, "f32", scale=scale)
-        run(1, 6, 3, 2, 64, 32, True, "bf16", scale=scale)
+        for D in (64, 50):
+            run(1, 6, 3, 2, D, 32, False, "f32", scale=scale)
+            run(1, 6, 3, 2, D, 32, True, "bf16", scale=scale)
+    run(1, 6, 3, 2, 64, 32, False, "f32", scale=0.0, eps=2.0 ** -126)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_broken_rows_stay_alone(dtype):
+    """A NaN or an infinity in a row, or in padding, reaches no other row; padding is zero whatever it holds."""
+    r = np.random.default_rng(2)
+    B, S, Hq, Hk = 1, 9, 4, 2
+    for D, R in ((64, 64), (32, 32), (50, 10)):
+        x = [r.standard_normal((B, S, H, D)) for H in (Hq, Hk)]
+        clean = [y.copy() for y in x]
+        x[0][0, 2, 1, 3], x[0][0, 4, :, :], x[1][0, 5, 0, 0] = np.nan, np.inf, -np.inf
+        where = np.arange(S)
+        where[4] = -1
+        table = floats(rope_table(S, R))
+        got = []
+        for v in (x, clean):
+            X = [Strided(y, dtype) for y in v]
+            out, dX = ([Strided(0 * y, dtype) for y in clean] for _ in range(2))
+            dg = [DB(4 * D) for _ in range(2)]
+            a = (TYPE[dtype], B, S, Hq, Hk, D, R, False, EPS, ints(where), table, S, X[0], X[0].strides, X[1], X[1].strides,
+                 None, None)
+            hip.qk_norm_rope_fwd(*a, out[0], out[0].strides, out[1], out[1].strides)
+            dY = [Strided(y, dtype) for y in clean]
+            size = hip.qk_norm_rope_bwd_workspace(D)
+            hip.qk_norm_rope_bwd(*a, TYPE[dtype], dY[0], dY[0].strides, dY[1], dY[1].strides, TYPE[dtype], dX[0], dX[0].strides,
+                                 dX[1], dX[1].strides, *dg, False, DB(size), size)
+            got.append([y.get() for y in out + dX])
+        for i, (a, b) in enumerate(zip(*got)):
+            bad = np.zeros(a.shape[:3], bool)
+            bad[0, (2, 5)[i % 2], (1, 0)[i % 2]] = True
+            assert np.isnan(a[bad]).any() and np.array_equal(a[~bad], b[~bad])
+            assert (a[0, 4] == 0).all()
 
 
 @pytest.mark.gpu
@@ -123,6 +158,15 @@ def test_many_rows_and_reruns():
     b = run(2, 1500, 7, 3, 64, 64, False, "bf16", "f32", "bf16")
     assert all(np.array_equal(x, y) for x, y in zip(a, b))
     run(1, 3001, 5, 1, 48, 20, True, "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("S,Hq,Hk,D,R", [(9001, 6, 2, 64, 64), (9001, 1, 1, 32, 16), (700, 40, 8, 32, 32), (9001, 3, 1, 30, 10),
+                                         (2500, 1, 2, 128, 128)])
+def test_units(S, Hq, Hk, D, R, dtype):
+    """Whole tokens to a wave and parts of one, several tokens at once, waves that take several units; padded ends."""
+    run(1, S, Hq, Hk, D, R, False, dtype, pos="any")
 
 
 @pytest.mark.gpu
