@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) paged_join(Work
 // 512 / 1024 / 2048 tokens: 288 / 234 / 230 / 236 us; 128 of e4m3: 364 / 271 / 257 / 251).
 // Joining costs a launch: what one work-group reads in the same time stays whole, FEW tokens, or ONE where there
 // are sequences enough for half the CUs (16 x 8 heads x 1024 tokens bf16: 13.8 us whole, 14.7 split; 4 x 8: 12.7, 9.0).
-constexpr int LEAST = 128, MOST = 2048, CHUNK_BYTES = 512 << 10, WORK_GROUPS = 1024;
+constexpr int LEAST = 128, MOST = 2048, CHUNK_BYTES = 512 << 10, WORK_GROUPS = 768;
 constexpr int FEW = 512, ONE = 1088, MANY = 128;
 constexpr int MOST_SPLITS = 65535;   // of a launch; at most 2^25 tokens in chunks of MOST are fewer
 
