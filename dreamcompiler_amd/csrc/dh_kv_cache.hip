@@ -189,12 +189,13 @@ __global__ void __launch_bounds__(256) cache_read(Paged c, int B, int N, const i
 }
 
 // ---- rows that begin with 16 bytes ---------------------------------------------------------------
-// A row is L lanes of P values, 16 bytes of the model's type, so a wave has 64 / L heads at once, AHEAD times, keys and
-// values.  A wave takes `tokens` rows of K and V, the four waves of a work-group in turn (what lies side by side is
-// then read at the same time): its lanes find a token's place each, so that the waits for beginnings, lengths and pages
-// are those of one token.  Where there are few tokens it takes one of the blocks of heads of one.  Where there are fewer heads than half of the wave's places (MANY), a power of two `heads` of those
-// places belong to a token and the wave has several tokens at once.  (Places found by a work-group of 16 tokens
-// for its four waves, with a barrier, cost 2 to 10% more.)
+// A row is L lanes of P values, 16 bytes of the model's type, so a wave has 64 / L heads at once, keys and values (the
+// read twice that).  A wave takes `tokens` rows of K and V, the four waves of a work-group in turn (what lies side by
+// side is then read at the same time): its lanes find a token's place each, so that the waits for beginnings, lengths
+// and pages are those of one token.  Where there are few tokens it takes one of the blocks of heads of one.  Where there
+// are fewer heads than half of the wave's places (MANY), a power of two `heads` of those places belong to a token and the
+// wave has several tokens at once.  (Places found by a work-group of 16 tokens for its four waves, with a barrier,
+// cost 2 to 10% more.)
 constexpr int MOST_TOKENS = 64;
 struct Units {
     int tokens, heads, blocks, each;   // log2 of a token's places (MANY), blocks of heads of a token, and of those a wave's
@@ -406,7 +407,7 @@ template <typename T, typename CT, int L, bool MANY>
 __global__ void __launch_bounds__(256) cache_write_pieces(Paged c, Units u, int B, int N, const int* __restrict__ first,
                                                           const int* __restrict__ len, const T* __restrict__ K,
                                                           Strides sk, const T* __restrict__ V, Strides sv) {
-    constexpr int P = Piece<T>::V, G = 64 / L, AHEAD = 1;
+    constexpr int P = Piece<T>::V, G = 64 / L;
     constexpr bool scaled = sizeof(CT) == 1;
     const int lane = threadIdx.x & 63, piece = lane & (L - 1), sub = lane / L;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -416,44 +417,33 @@ __global__ void __launch_bounds__(256) cache_write_pieces(Paged c, Units u, int 
     const uint32_t group = fdiv(unit, u.per);
     const Rows rows = rows_of(u, group, MANY ? __builtin_ctz(G) - u.heads : 0);
     const int j0 = (unit - group * u.per.d) * u.each, j1 = min(j0 + u.each, u.blocks);   // blocks of heads
-    u32x4 x[2 * AHEAD];
+    u32x4 x[2];
     // Head h0 of the wave (the lane's own where MANY) of token i.  Lanes without one read another's row.
     auto load = [&](int i, int h0) {
         const int h = min(MANY ? h0 : h0 + sub, c.Hk - 1), e = in ? piece * P : 0;
         const long long n = min(rows.at(min(i, u.tokens - 1)), N - 1);
-        const T* kp = K + n * sk.token + h * sk.head + e;
-        const T* vp = V + n * sv.token + h * sv.head + e;
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            const int more = min(a * G, c.Hk - 1 - h);
-            x[2 * a] = *reinterpret_cast<const u32x4*>(kp + more * sk.head);
-            x[2 * a + 1] = *reinterpret_cast<const u32x4*>(vp + more * sv.head);
-        }
+        x[0] = *reinterpret_cast<const u32x4*>(K + n * sk.token + h * sk.head + e);
+        x[1] = *reinterpret_cast<const u32x4*>(V + n * sv.token + h * sv.head + e);
     };
     auto store = [&](int2 at, int h0, bool any) {
         const int h = MANY ? h0 : h0 + sub;
-        const long long row0 = c.row(at.x, h, at.y);
+        const bool there = any && h < c.Hk && at.x >= 0;
+        const long long row = c.row(at.x, h, at.y);
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            if (!MANY && h0 + a * G >= c.Hk) break;
-            const bool there = any && h + a * G < c.Hk && at.x >= 0;
-            const long long row = row0 + ((long long)(a * G) << c.shift);
-#pragma unroll
-            for (int side = 0; side < 2; ++side) {
-                const u32x4 w = x[2 * a + side];
-                CT* o = (CT*)(side ? c.V : c.K) + row * c.D + piece * P;
-                if constexpr (!scaled) {
-                    if (there && in) *reinterpret_cast<u32x4*>(o) = w;
-                } else {
-                    uint32_t out[P / 4];
-                    float v[P];
-                    Piece<T>::values(w, v);
-                    const float s = quantise<CT, P>(v, group_max<L>(Piece<T>::most(w)), out);
-                    if (there && piece == 0) (side ? c.Vs : c.Ks)[row] = s;
-                    if (there && in) {
-                        if constexpr (P == 8) *reinterpret_cast<u32x2*>(o) = u32x2{out[0], out[1]};
-                        else *reinterpret_cast<uint32_t*>(o) = out[0];
-                    }
+        for (int side = 0; side < 2; ++side) {
+            const u32x4 w = x[side];
+            CT* o = (CT*)(side ? c.V : c.K) + row * c.D + piece * P;
+            if constexpr (!scaled) {
+                if (there && in) *reinterpret_cast<u32x4*>(o) = w;
+            } else {
+                uint32_t out[P / 4];
+                float v[P];
+                Piece<T>::values(w, v);
+                const float s = quantise<CT, P>(v, group_max<L>(Piece<T>::most(w)), out);
+                if (there && piece == 0) (side ? c.Vs : c.Ks)[row] = s;
+                if (there && in) {
+                    if constexpr (P == 8) *reinterpret_cast<u32x2*>(o) = u32x2{out[0], out[1]};
+                    else *reinterpret_cast<uint32_t*>(o) = out[0];
                 }
             }
         }
@@ -470,12 +460,12 @@ __global__ void __launch_bounds__(256) cache_write_pieces(Paged c, Units u, int 
             load(i, h);
         }
     } else {
-        load(0, j0 * AHEAD * G);
+        load(0, j0 * G);
         const int2 places = find_place(c, B, N, first, len, rows, u.tokens);
         for (int i = 0, j = j0; i < u.tokens && rows.at(i) < N;) {
-            store(lane_of(places, i), j * AHEAD * G, true);
+            store(lane_of(places, i), j * G, true);
             if (++j == j1) j = j0, ++i;
-            if (i < u.tokens) load(i, j * AHEAD * G);
+            if (i < u.tokens) load(i, j * G);
         }
     }
 }

@@ -60,12 +60,6 @@ template <> __device__ inline u32x2 words_bf16<uint8_t>(uint32_t w) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true))};
 }
 
-// N words at any element's alignment.
-template <int N> struct Words;
-template <> struct Words<1> { typedef uint32_t type; };
-template <> struct Words<2> { typedef u32x2 type; };
-template <> struct Words<4> { typedef u32x4 type; };
-
 // x (8 values) in P parts of bf16 that add up to it: 8 bits each.
 template <int P>
 __device__ inline void split8(const float (&x)[8], u32x4 (&out)[P]) {

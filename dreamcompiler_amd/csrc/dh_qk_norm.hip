@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256) qk_fwd(Shape s, Units u, Rows<const T> q,
             for (int j = 0; j < J; ++j) {
                 const int e = 64 * j + lane;
                 const float y = e < s.R ? v[j] * inv * w[j] * turn.c[j] + vo[j] * inv * wo[j] * turn.sn[j] : v[j] * inv * w[j];
-                if (e < s.D) o[e] = down<T>(y);
+                if (e < s.D) o[e] = down<T>(p >= 0 ? y : 0.f);   // whatever the table and the weights hold
             }
         }
     }
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(256) qk_bwd(Shape s, Units u, Rows<const T> q,
             wave_fence();   // o may be x or d
 #pragma unroll
             for (int j = 0; j < J; ++j)
-                if (64 * j + lane < s.D) o[64 * j + lane] = down<OT>(inv * (dy[j] - v[j] * mean));
+                if (64 * j + lane < s.D) o[64 * j + lane] = down<OT>(p >= 0 ? inv * (dy[j] - v[j] * mean) : 0.f);
         }
     }
 #pragma unroll
@@ -339,6 +339,8 @@ __global__ void __launch_bounds__(256) qk_fwd_pieces(Shape s, Units u, Many m, R
 #pragma unroll
             for (int e = 0; e < V; ++e) v[a][e] *= inv * w[e];
             turn.apply(s, v[a], 1.f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[a][e] = there ? v[a][e] : 0.f;   // whatever the table and the weights hold
             if (h0 + a * G + hs < H && in) store_piece<T, V>(op + a * G * o.s2, v[a]);
         }
     };
@@ -407,13 +409,14 @@ __global__ void __launch_bounds__(256) qk_bwd_pieces(Shape s, Units u, Many m, R
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 v[a][e] *= inv;
+                d[a][e] = there ? d[a][e] : 0.f;
                 acc[e] += d[a][e] * v[a][e];
                 d[a][e] *= w[e];
                 dot += d[a][e] * v[a][e];
             }
             const float mean = group_sum<L>(dot) * s.by_d;
 #pragma unroll
-            for (int e = 0; e < V; ++e) d[a][e] = inv * (d[a][e] - v[a][e] * mean);
+            for (int e = 0; e < V; ++e) d[a][e] = there ? inv * (d[a][e] - v[a][e] * mean) : 0.f;
             if (h0 + a * G + hs < H && in) store_piece<OT, V>(op + a * G * o.s2, d[a]);
         }
     };
@@ -748,6 +751,8 @@ int dh_qk_norm_rope_bwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, i
     const bool any = (long long)B * S > 0;
     if (any && ((Hq > 0 && (!Q || !dQo || !dQ)) || (Hk > 0 && (!K || !dKo || !dK))))
         return set_error(DH_ERR_INVALID, "%s: null pointer", op);
+    if (dgq && dgk && dgq < dgk + D && dgk < dgq + D)
+        return set_error(DH_ERR_INVALID, "%s: dgq and dgk must not overlap", op);
     const size_t need = dh_qk_norm_rope_bwd_workspace(D);
     if (!ws) return set_error(DH_ERR_INVALID, "%s: null pointer", op);
     if ((uintptr_t)ws & 15) return set_error(DH_ERR_INVALID, "%s: workspace not 16-byte aligned", op);

@@ -422,7 +422,8 @@ int dh_qk_norm_rope_fwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, i
 /* Its gradient from the forward's inputs: with dy = dout turned back and r as above,
  *   dgq, dgk (+)= sum of dy x r over tokens and heads,   dx = r (dy g - x r mean(dy g x r)).
  * dQo, dKo are of dout_type, dQ, dK of grad_type: the inputs' type or DH_F32 (what dh_flash_bwd leaves).
- * dgq, dgk are fp32 (either may be NULL); accumulate adds into them.  dQ may be dQo or Q as above. */
+ * dgq, dgk are fp32 (either may be NULL) and must not overlap: weights that both sides share have the sum of two.
+ * accumulate adds into them.  dQ may be dQo or Q as above. */
 size_t dh_qk_norm_rope_bwd_workspace(int D);
 int dh_qk_norm_rope_bwd(int dtype, int B, int S, int Hq, int Hk, int D, int R, int pairs, float eps,
                         const int* d_pos, const float* d_table, int P, const void* d_Q,
@@ -449,7 +450,8 @@ int dh_kv_cache_write(int dtype, int cache_type, int B, int N, int Hk, int D, co
                       const long long* k_strides, const void* d_V, const long long* v_strides,
                       const int* d_first, const int* d_len, int pages, int page, const int* d_table,
                       int ld_table, void* d_Kc, void* d_Vc, float* d_Ks, float* d_Vs);
-/* Reads tokens back into rows of K and V, addressed as above: rows of no sequence are left as they were. */
+/* Reads tokens back into rows of K and V, addressed as above: rows of no sequence are left as they were.  K and V
+ * must not overlap each other or the cache. */
 int dh_kv_cache_read(int dtype, int cache_type, int B, int N, int Hk, int D, void* d_K,
                      const long long* k_strides, void* d_V, const long long* v_strides,
                      const int* d_first, const int* d_len, int pages, int page, const int* d_table,
@@ -461,7 +463,7 @@ int dh_kv_cache_read(int dtype, int cache_type, int B, int N, int Hk, int D, voi
  * Hq is a multiple of Hk, B Hq at most 2^22: query head h reads cache head h / (Hq / Hk).  Strides of Q and O: sequence,
  * head.  max_len bounds the lengths (at most ld_table page, and 2^25; a longer sequence is cut off there): the
  * work is split over it.  A sequence without tokens, or whose scores are all -infinity, has O = 0,
- * lse = -infinity.  scale finite and > 0.  What a page holds past a sequence's end does not matter, NaN included. */
+ * lse = -infinity.  scale finite and > 0.  O and lse overlap nothing else.  What a page holds past a sequence's end does not matter, NaN included. */
 size_t dh_paged_attention_workspace(int cache_type, int B, int Hq, int Hk, int D, int max_len);
 int dh_paged_attention(int dtype, int cache_type, int B, int Hq, int Hk, int D, float scale,
                        int window, const void* d_Q, const long long* q_strides, const int* d_len,

@@ -20,9 +20,9 @@ def qk_fwd(dt=0, B=2, S=3, Hq=4, Hk=2, D=8, R=8, eps=1e-6, pos=P, table=P, n=9, 
 
 def qk_bwd(dt=0, B=2, S=3, Hq=4, Hk=2, D=8, R=8, eps=1e-6, pos=P, table=P, n=9, Q=P, K=P, dQo=P, dKo=P, dQ=P, dK=P,
            sq=(96, 32, 8), sk=(48, 16, 8), sdqo=(96, 32, 8), sdko=(48, 16, 8), sdq=(96, 32, 8), sdk=(48, 16, 8), dout=0, gt=0,
-           ws=P, size=BIG):
+           dgq=None, dgk=None, ws=P, size=BIG):
     hip.qk_norm_rope_bwd(dt, B, S, Hq, Hk, D, R, False, eps, pos, table, n, Q, sq, K, sk, None, None, dout, dQo, sdqo, dKo,
-                         sdko, gt, dQ, sdq, dK, sdk, None, None, False, ws, size)
+                         sdko, gt, dQ, sdq, dK, sdk, dgq, dgk, False, ws, size)
 
 
 def write(dt=0, ct=3, B=2, N=5, Hk=2, D=32, K=P, sk=(64, 32), V=P, sv=(64, 32), first=P, len_=P, pages=4, page=16, table=P,
@@ -112,6 +112,12 @@ def test_qk_gradient_types_and_workspace():
             qk_bwd(size=need - 1, **a)
         with raises("aligned"):
             qk_bwd(ws=ODD, **a)
+
+
+def test_weights_gradients_apart():
+    for d in (0, 4, 28, -28):
+        with raises("overlap"):
+            qk_bwd(dgq=P, dgk=P + d)
 
 
 def test_tables():

@@ -152,6 +152,38 @@ def test_broken_rows_stay_alone(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("Hq,Hk,D,R", [(6, 2, 64, 64), (20, 9, 128, 64), (3, 1, 50, 50), (2, 2, 300, 300)])
+def test_padding_is_zero_whatever_the_rest_holds(Hq, Hk, D, R, dtype):
+    """NaN in padding's rows, NaN and infinities in the table's first row and in the weights."""
+    r = np.random.default_rng(3)
+    B, S = 2, 5
+    where = np.array([[-1, 1, 2, 9, -7], [3, -1, 9, 1, 2]])
+    pad = (where < 0) | (where >= 4)
+    table = rope_table(4, R)
+    table[0, ::2], table[0, 1::2] = np.nan, np.inf
+    x = [r.standard_normal((B, S, H, D)) for H in (Hq, Hk, Hq, Hk)]
+    for v in x:
+        v[pad] = np.nan
+    Q, K, dQo, dKo = [Strided(v, dtype, (0, 1, 2), 0) for v in x]
+    out = [Strided(np.full((B, S, H, D), 7.0), dtype, (0, 2, 1), 0) for H in (Hq, Hk, Hq, Hk)]
+    for g in (np.inf, np.nan, 1.0):
+        gb = [floats(np.full(D, g, np.float32)) for _ in range(2)]
+        dg = [floats(np.zeros(D, np.float32)) for _ in range(2)]
+        a = (TYPE[dtype], B, S, Hq, Hk, D, R, False, EPS, ints(where), floats(table), 4, Q, Q.strides, K, K.strides, *gb)
+        hip.qk_norm_rope_fwd(*a, out[0], out[0].strides, out[1], out[1].strides)
+        size = hip.qk_norm_rope_bwd_workspace(D)
+        ws = DB(size)
+        hip.qk_norm_rope_bwd(*a, TYPE[dtype], dQo, dQo.strides, dKo, dKo.strides, TYPE[dtype], out[2], out[2].strides, out[3],
+                             out[3].strides, *dg, False, ws, size)
+        for o in out:
+            assert (o.get()[pad] == 0).all()
+            assert g != 1.0 or np.isfinite(o.get()).all()
+        for d in dg:   # the weights have no part in it
+            assert np.isfinite(d.numpy()).all()
+
+
+@pytest.mark.gpu
 def test_many_rows_and_reruns():
     """More rows than waves: each wave takes several.  Reruns are equal bit for bit."""
     a = run(2, 1500, 7, 3, 64, 64, False, "bf16", "f32", "bf16")
