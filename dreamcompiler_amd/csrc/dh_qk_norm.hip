@@ -66,118 +66,147 @@ __device__ inline float norm_of(float sum, const Shape& s) {
 // with: its partner's place, cosine and sine (signed so that the forward is y[e] c + y[partner] sn).
 template <int J>
 struct TurnAny {
+    uint32_t R, half, other[J];
+    bool pairs;
     float c[J], sn[J];
-    int other[J];
-    __device__ void load(const Shape& s, const float* __restrict__ row) {
-        const int lane = threadIdx.x & 63, half = s.R >> 1;
+    __device__ explicit TurnAny(const Shape& s) : R(s.R), half(s.R >> 1), pairs(s.pairs) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int e = 64 * j + lane;
-            c[j] = 1.f, sn[j] = 0.f, other[j] = min(e, s.D - 1);
-            if (e >= s.R) continue;
-            const int i = s.pairs ? e >> 1 : e < half ? e : e - half;
-            const bool second = s.pairs ? e & 1 : e >= half;
-            c[j] = row[i];
-            sn[j] = second ? row[half + i] : -row[half + i];
-            other[j] = s.pairs ? e ^ 1 : second ? e - half : e + half;
+            const uint32_t e = 64 * j + (threadIdx.x & 63);
+            other[j] = e >= R ? min(e, (uint32_t)s.D - 1) : pairs ? e ^ 1 : e < half ? e + half : e - half;
+        }
+    }
+    __device__ void load(const float* __restrict__ row) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const uint32_t e = 64 * j + (threadIdx.x & 63), i = pairs ? e >> 1 : e < half ? e : e - half;
+            const bool second = pairs ? e & 1 : e >= half;
+            c[j] = 1.f, sn[j] = 0.f;
+            if (e < R) c[j] = row[i], sn[j] = second ? row[half + i] : -row[half + i];
         }
     }
 };
+// The lane's weights, and its partners'.
 template <int J>
-__device__ inline void load_any(const float* __restrict__ g, int D, const int* other, float (&w)[J], float (&wo)[J]) {
-    const int lane = threadIdx.x & 63;
+struct WeightsAny {
+    float w[J], wo[J];
+    __device__ WeightsAny(const float* __restrict__ g, const Shape& s, const TurnAny<J>& turn) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-        w[j] = g && 64 * j + lane < D ? g[64 * j + lane] : 1.f;
-        wo[j] = g ? g[other[j]] : 1.f;
+        for (int j = 0; j < J; ++j) {
+            w[j] = g ? g[(uint32_t)min(64 * j + (int)(threadIdx.x & 63), s.D - 1)] : 1.f;
+            wo[j] = g ? g[turn.other[j]] : 1.f;
+        }
     }
-}
+};
 
-template <typename T, int J>
+// A rows of a wave are in flight: one at a time took 2 to 3 times as long (6592 tokens of 40 heads of 100 bf16 with
+// R = 100 in halves, forward and gradient: 300 us with one, 145 with four, 101 with eight; of 6 heads: 54, 28, 31).
+template <typename T, int J, int A>
 __global__ void __launch_bounds__(256) qk_fwd(Shape s, Units u, Rows<const T> q, Rows<const T> k,
                                               const float* __restrict__ gq, const float* __restrict__ gk,
                                               Rows<T> qo, Rows<T> ko) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    TurnAny<J> turn;
+    TurnAny<J> turn(s);
+    const WeightsAny<J> wq(gq, s, turn), wk(gk, s, turn);
+    auto block = [&](const Rows<const T>& x, const Rows<T>& o, const WeightsAny<J>& w, int H, int b, int t, int h0, bool there) {
+        float v[A][J], vo[A][J];
+#pragma unroll
+        for (int a = 0; a < A; ++a) {   // without a condition each, so that they are on their way together
+            const T* p = x.at(b, t, min(h0 + a, H - 1));
+#pragma unroll
+            for (int j = 0; j < J; ++j) v[a][j] = up(p[(uint32_t)min(64 * j + lane, s.D - 1)]), vo[a][j] = up(p[turn.other[j]]);
+        }
+        wave_fence();   // o may be x
+#pragma unroll
+        for (int a = 0; a < A; ++a) {
+            if (h0 + a >= H) break;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < J; ++j) sum += 64 * j + lane < s.D ? v[a][j] * v[a][j] : 0.f;
+            const float inv = norm_of(wave_reduce(sum, OpSum()), s);
+            T* p = o.at(b, t, h0 + a);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int e = 64 * j + lane;
+                float y = v[a][j] * inv * w.w[j];
+                if (e < s.R) y = y * turn.c[j] + vo[a][j] * inv * w.wo[j] * turn.sn[j];
+                if (e < s.D) p[e] = down<T>(there ? y : 0.f);   // padding: whatever the rest holds
+            }
+        }
+    };
     for (uint32_t i = 4 * blockIdx.x + wave; i < u.units; i += 4 * gridDim.x) {
         const uint32_t n = fdiv(i, u.per);
-        const int b = fdiv(n, u.S), t = n - b * s.S, h0 = (i - n * u.per.d) * u.each, h1 = min(h0 + u.each, u.n);
+        const int b = fdiv(n, u.S), t = n - b * s.S, j0 = (i - n * u.per.d) * u.each, j1 = min(j0 + u.each, u.n);
         const int p = position(s, b, t);
-        turn.load(s, s.table + (long long)max(p, 0) * s.R);
-        for (int h = h0; h < h1; ++h) {
-            const bool key = h >= s.H[0];
-            const T* x = key ? k.at(b, t, h - s.H[0]) : q.at(b, t, h);
-            T* o = key ? ko.at(b, t, h - s.H[0]) : qo.at(b, t, h);
-            float w[J], wo[J], v[J], vo[J], sum = 0.f;
-            load_any<J>(key ? gk : gq, s.D, turn.other, w, wo);
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int e = 64 * j + lane;
-                v[j] = vo[j] = 0.f;
-                if (p >= 0 && e < s.D) v[j] = up(x[e]), vo[j] = up(x[turn.other[j]]);
-                sum += v[j] * v[j];
-            }
-            const float inv = norm_of(wave_reduce(sum, OpSum()), s);
-            wave_fence();   // o may be x
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int e = 64 * j + lane;
-                const float y = e < s.R ? v[j] * inv * w[j] * turn.c[j] + vo[j] * inv * wo[j] * turn.sn[j] : v[j] * inv * w[j];
-                if (e < s.D) o[e] = down<T>(p >= 0 ? y : 0.f);   // whatever the table and the weights hold
-            }
+        turn.load(s.table + (long long)max(p, 0) * s.R);
+        for (int j = j0; j < j1; ++j) {
+            if (j < u.nq) block(q, qo, wq, s.H[0], b, t, j * A, p >= 0);
+            else block(k, ko, wk, s.H[1], b, t, (j - u.nq) * A, p >= 0);
         }
     }
 }
 
 // The gradient: a work-group leaves its sums of dgq and dgk in rows blockIdx.x and gridDim.x + blockIdx.x of part.
-template <typename T, typename GT, typename OT, int J>
+template <typename T, typename GT, typename OT, int J, int A>
 __global__ void __launch_bounds__(256) qk_bwd(Shape s, Units u, Rows<const T> q, Rows<const T> k,
                                               const float* __restrict__ gq, const float* __restrict__ gk,
                                               Rows<const GT> dqo, Rows<const GT> dko, Rows<OT> dq, Rows<OT> dk,
                                               float* __restrict__ part) {
     __shared__ float red[4][64 * J];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TurnAny<J> turn(s);
+    const WeightsAny<J> wq(gq, s, turn), wk(gk, s, turn);
     float acc[2][J] = {};
-    TurnAny<J> turn;
-    for (uint32_t i = 4 * blockIdx.x + wave; i < u.units; i += 4 * gridDim.x) {
-        const uint32_t n = fdiv(i, u.per);
-        const int b = fdiv(n, u.S), t = n - b * s.S, h0 = (i - n * u.per.d) * u.each, h1 = min(h0 + u.each, u.n);
-        const int p = position(s, b, t);
-        turn.load(s, s.table + (long long)max(p, 0) * s.R);
-        for (int h = h0; h < h1; ++h) {
-            const bool key = h >= s.H[0];
-            const T* x = key ? k.at(b, t, h - s.H[0]) : q.at(b, t, h);
-            const GT* d = key ? dko.at(b, t, h - s.H[0]) : dqo.at(b, t, h);
-            OT* o = key ? dk.at(b, t, h - s.H[0]) : dq.at(b, t, h);
-            const float* g = key ? gk : gq;
-            float v[J], dy[J], sum = 0.f, dot = 0.f;
+    auto block = [&](const Rows<const T>& x, const Rows<const GT>& d, const Rows<OT>& o, const WeightsAny<J>& w,
+                     float (&acc)[J], int H, int b, int t, int h0, bool there) {
+        float v[A][J], dy[A][J], other[A][J];
+#pragma unroll
+        for (int a = 0; a < A; ++a) {
+            const int h = min(h0 + a, H - 1);
+            const T* p = x.at(b, t, h);
+            const GT* r = d.at(b, t, h);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                const int e = 64 * j + lane;
-                v[j] = dy[j] = 0.f;
-                if (p >= 0 && e < s.D) {
-                    v[j] = up(x[e]);
-                    dy[j] = up(d[e]);
-                    if (e < s.R) dy[j] = dy[j] * turn.c[j] - up(d[turn.other[j]]) * turn.sn[j];
-                }
-                sum += v[j] * v[j];
+                const uint32_t e = min(64 * j + lane, s.D - 1);
+                v[a][j] = up(p[e]), dy[a][j] = up(r[e]), other[a][j] = up(r[turn.other[j]]);
+            }
+        }
+        wave_fence();   // o may be x or d
+#pragma unroll
+        for (int a = 0; a < A; ++a) {
+            if (h0 + a >= H) break;
+            float sum = 0.f, dot = 0.f;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const bool in = there && 64 * j + lane < s.D;   // a row of padding: whatever the rest holds
+                v[a][j] = in ? v[a][j] : 0.f;
+                if (64 * j + lane < s.R) dy[a][j] = dy[a][j] * turn.c[j] - other[a][j] * turn.sn[j];
+                dy[a][j] = in ? dy[a][j] : 0.f;
+                sum += v[a][j] * v[a][j];
             }
             const float inv = norm_of(wave_reduce(sum, OpSum()), s);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                const int e = 64 * j + lane;
-                v[j] *= inv;
-                const float term = dy[j] * v[j];
-                acc[0][j] += key ? 0.f : term;
-                acc[1][j] += key ? term : 0.f;
-                dy[j] *= g && e < s.D ? g[e] : 1.f;
-                dot += dy[j] * v[j];
+                v[a][j] *= inv;
+                acc[j] += dy[a][j] * v[a][j];
+                dy[a][j] *= 64 * j + lane < s.D ? w.w[j] : 0.f;
+                dot += dy[a][j] * v[a][j];
             }
             const float mean = wave_reduce(dot, OpSum()) * s.by_d;
-            wave_fence();   // o may be x or d
+            OT* p = o.at(b, t, h0 + a);
 #pragma unroll
             for (int j = 0; j < J; ++j)
-                if (64 * j + lane < s.D) o[64 * j + lane] = down<OT>(p >= 0 ? inv * (dy[j] - v[j] * mean) : 0.f);
+                if (64 * j + lane < s.D) p[64 * j + lane] = down<OT>(there ? inv * (dy[a][j] - v[a][j] * mean) : 0.f);
+        }
+    };
+    for (uint32_t i = 4 * blockIdx.x + wave; i < u.units; i += 4 * gridDim.x) {
+        const uint32_t n = fdiv(i, u.per);
+        const int b = fdiv(n, u.S), t = n - b * s.S, j0 = (i - n * u.per.d) * u.each, j1 = min(j0 + u.each, u.n);
+        const int p = position(s, b, t);
+        turn.load(s.table + (long long)max(p, 0) * s.R);
+        for (int j = j0; j < j1; ++j) {
+            if (j < u.nq) block(q, dqo, dq, wq, acc[0], s.H[0], b, t, j * A, p >= 0);
+            else block(k, dko, dk, wk, acc[1], s.H[1], b, t, (j - u.nq) * A, p >= 0);
         }
     }
 #pragma unroll
@@ -601,10 +630,10 @@ int launch_fwd_pieces(const Shape& s, const Call& c) {
                                                               c.gq, c.gk, rows_of<T>(c.Qo, c.sqo), rows_of<T>(c.Ko, c.sko));
     return check_launch("dh_qk_norm_rope_fwd");
 }
-template <typename T, int J>
+template <typename T, int J, int A>
 int launch_fwd(const Shape& s, const Call& c) {
-    const Units u = units_of(s, 1);
-    qk_fwd<T, J><<<groups_of(u.units, FWD_GROUPS), 256, 0, stream()>>>(s, u, rows_of<const T>(c.Q, c.sq),
+    const Units u = units_of(s, A);
+    qk_fwd<T, J, A><<<groups_of(u.units, FWD_GROUPS), 256, 0, stream()>>>(s, u, rows_of<const T>(c.Q, c.sq),
                                                                        rows_of<const T>(c.K, c.sk), c.gq, c.gk,
                                                                        rows_of<T>(c.Qo, c.sqo), rows_of<T>(c.Ko, c.sko));
     return check_launch("dh_qk_norm_rope_fwd");
@@ -629,11 +658,11 @@ int launch_bwd_pieces(const Shape& s, const Call& c) {
                                     rows_of<OT>(c.Qo, c.sqo), rows_of<OT>(c.Ko, c.sko), c.part);
     return join(s, c, grid);
 }
-template <typename T, typename GT, typename OT, int J>
+template <typename T, typename GT, typename OT, int J, int A>
 int launch_bwd(const Shape& s, const Call& c) {
-    const Units u = units_of(s, 1);
+    const Units u = units_of(s, A);
     const unsigned grid = groups_of(u.units, QK_GROUPS);
-    qk_bwd<T, GT, OT, J><<<grid, 256, 0, stream()>>>(s, u, rows_of<const T>(c.Q, c.sq), rows_of<const T>(c.K, c.sk), c.gq, c.gk,
+    qk_bwd<T, GT, OT, J, A><<<grid, 256, 0, stream()>>>(s, u, rows_of<const T>(c.Q, c.sq), rows_of<const T>(c.K, c.sk), c.gq, c.gk,
                                                      rows_of<const GT>(c.dQo, c.sdqo), rows_of<const GT>(c.dKo, c.sdko),
                                                      rows_of<OT>(c.Qo, c.sqo), rows_of<OT>(c.Ko, c.sko), c.part);
     return join(s, c, grid);
@@ -647,10 +676,14 @@ int fwd_by_lanes(int L, const Shape& s, const Call& c) {
            : L == 32 ? launch_fwd_pieces<T, V, 32>(s, c)
                      : launch_fwd_pieces<T, V, 64>(s, c);
 }
-// D <= 256 fits four values a lane.
+bool few_heads(const Shape& s) { return s.H[0] <= 4 && s.H[1] <= 4; }
 template <typename T>
 int fwd_of(const Piece& p, const Shape& s, const Call& c) {
-    if (p.V == 1) return s.D <= 256 ? launch_fwd<T, 4>(s, c) : launch_fwd<T, 16>(s, c);
+    if (p.V == 1)
+        return s.D > 512   ? launch_fwd<T, 16, 2>(s, c)
+               : s.D > 256 ? launch_fwd<T, 8, 4>(s, c)
+               : s.D > 128 ? launch_fwd<T, 4, 4>(s, c)
+               : few_heads(s) ? launch_fwd<T, 2, 4>(s, c) : launch_fwd<T, 2, 8>(s, c);
     if constexpr (sizeof(T) == 2)
         if (p.V == 8) return fwd_by_lanes<T, 8>(p.lanes(), s, c);
     return fwd_by_lanes<T, 4>(p.lanes(), s, c);
@@ -665,7 +698,11 @@ int bwd_by_lanes(int L, const Shape& s, const Call& c) {
 }
 template <typename T, typename GT, typename OT>
 int bwd_of(const Piece& p, const Shape& s, const Call& c) {
-    if (p.V == 1) return s.D <= 256 ? launch_bwd<T, GT, OT, 4>(s, c) : launch_bwd<T, GT, OT, 16>(s, c);
+    if (p.V == 1)
+        return s.D > 512   ? launch_bwd<T, GT, OT, 16, 1>(s, c)
+               : s.D > 256 ? launch_bwd<T, GT, OT, 8, 4>(s, c)
+               : s.D > 128 ? launch_bwd<T, GT, OT, 4, 4>(s, c)
+               : few_heads(s) ? launch_bwd<T, GT, OT, 2, 4>(s, c) : launch_bwd<T, GT, OT, 2, 8>(s, c);
     if constexpr (sizeof(T) == 2)
         if (p.V == 8) return bwd_by_lanes<T, GT, OT, 8>(p.lanes(), s, c);
     return bwd_by_lanes<T, GT, OT, 4>(p.lanes(), s, c);

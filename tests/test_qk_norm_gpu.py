@@ -8,7 +8,7 @@ Tolerances (u = 2^-24, ub = 2^-8: the largest relative error of one rounding to 
            of the row's largest y.  Then one rounding to the output's type.
  dx        x r to 16 u, dy g to 5 u, their mean over D: 25 u of the terms' mean size: under 64 u of
            r (max |dy g| + max |x r| mean |dy g x r|); one rounding to its type.
- dg        each term to 24 u; a chain of additions is at most the rows of a lane (of 4096 waves), the 64 rows that
+ dg        each term to 24 u of the products it is made of; a chain of additions is at most the rows of a lane (of 4096 waves), the 64 rows that
            meet in a work-group, 16 of 1024 work-groups, and 64: under (64 + min(rows, 520)) u of the terms' sizes.
 """
 import numpy as np
@@ -199,6 +199,15 @@ def test_many_rows_and_reruns():
 def test_units(S, Hq, Hk, D, R, dtype):
     """Whole tokens to a wave and parts of one, several tokens at once, waves that take several units; padded ends."""
     run(1, S, Hq, Hk, D, R, False, dtype, pos="any")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,pairs", [("f32", False), ("bf16", False), ("bf16", True)])
+@pytest.mark.parametrize("shape", [(1, 9, 40, 9, 100, 50), (2, 3, 4, 1, 100, 100), (1, 7, 5, 9, 250, 250), (1, 5, 3, 7, 301, 50),
+                                   (1, 4, 2, 5, 511, 510), (1, 5, 3, 2, 1001, 50), (1, 3, 5, 1, 1023, 1022)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_rows_in_no_whole_pieces(shape, dtype, pairs):
+    run(*shape, pairs, dtype, grad="f32", pos="any", pad=1, seed=7)
 
 
 @pytest.mark.gpu
