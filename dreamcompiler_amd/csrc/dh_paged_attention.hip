@@ -5,6 +5,11 @@
 // over the tokens t of the sequence (its last `window` ones).  One pass over keys and values with the
 // running maximum m and sum; a sequence's tokens are split into chunks, whose o, m and sum meet in a
 // second launch.  Bound by HBM: each key and value is read once.
+//
+// Measured, D = 128 and 8 cache heads, where a copy of 1 GiB moves 5.14 TB/s: 64 sequences of 1024 to 8192 tokens bf16 with
+// 32 query heads 227 us (5.4 TB/s), 128 of e4m3 with 64 query heads 248 (5.1), one of 131072 bf16 102 (5.3), 33 of up to 2047
+// fp32 (D = 64, 12 heads, the last 1000 tokens) 36 (4.7).  One of 512 tokens and 16 heads: 8.1, a launch that waits for
+// length, pages and two tiles a wave, on 16 CUs: a CU takes about 22 bytes a clock from memory, whatever it asks for.
 #include "dh_paged.hpp"
 
 namespace dh {
@@ -80,8 +85,8 @@ __device__ inline void split8(const float (&x)[8], u32x4 (&out)[P]) {
 }
 
 // ---- a chunk -----------------------------------------------------------------------------------
-// A work-group of 4 waves takes a chunk of a sequence's tokens for 16 RT query heads of one cache head;
-// its waves take every fourth tile of TILE tokens, each with its own maximum, sum and o, which
+// A work-group of 4 or 8 waves takes a chunk of a sequence's tokens for 16 RT query heads of one cache head;
+// its waves take the tiles of TILE tokens in turn, each with its own maximum, sum and o, which
 // meet in LDS.  Keys and values go from memory into registers, with no LDS between, as both products
 // take them as they lie:
 //   scores  keys x queries: lane l holds 16 bytes of key l % 16 (an A operand; the order of d inside a
@@ -602,7 +607,8 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) paged_join(Work
 // ---- host --------------------------------------------------------------------------------------
 // How the work is split.  A chunk is a multiple of LEAST tokens (a tile for each of four waves) and at most
 // MOST (the pages that a work-group's lanes hold) or CHUNK_BYTES of keys and values; a sequence has as many as make about
-// WORK_GROUPS of all sequences at their longest.  Larger ones leave a tail of busy work-groups while others are
+// WORK_GROUPS of all sequences at their longest: three a CU (two or four: up to 13% slower with few long sequences,
+// the same with many).  Larger chunks leave a tail of busy work-groups while others are
 // done, smaller ones wait more often for their first loads (64 sequences up to 8192 bf16, chunks of 256 /
 // 512 / 1024 / 2048 tokens: 288 / 234 / 230 / 236 us; 128 of e4m3: 364 / 271 / 257 / 251).
 // Joining costs a launch: what one work-group reads in the same time stays whole, FEW tokens, or ONE where there

@@ -110,9 +110,9 @@ def norm_rope(x, g, pos, table, R, pairs, eps, dout=None):
     dx = r * (dyg - xr * (dyg * xr).mean(-1, keepdims=True))
     size = r * (np.abs(dyg).max(-1, keepdims=True)
                 + np.abs(xr).max(-1, keepdims=True) * np.abs(dyg * xr).mean(-1, keepdims=True))
-    # A turned value is a sum of two products, each rounded relative to itself, that may cancel: with one row
-    # of 1023 values, a sum of 0.0023 of products that add up to 0.79 was off by 1.4e-8: 0.3 u of the products, 100 u of the sum.  So the bound of
-    # a term of dg counts both products' sizes: the larger of |a| |c| + |b| |s| taken with either sign.
+    # A turned value is a sum of two products, each rounded relative to itself, that may cancel: in a row of 1023
+    # values, a difference of 0.0023 of products that add up to 0.79 was off by 1.4e-8: 0.3 u of the products, 100 u of
+    # the difference.  So the bound of a term of dg counts both products: |a| |c| + |b| |s|, the larger of both signs.
     both = np.maximum(turn(np.abs(dout), np.abs(cos), -np.abs(sin), R, pairs),
                       turn(np.abs(dout), np.abs(cos), np.abs(sin), R, pairs))
     terms = np.where(keep, both * np.abs(xr), 0.0).sum((0, 1, 2))

@@ -8,7 +8,8 @@ Tolerances (u = 2^-24, ub = 2^-8: the largest relative error of one rounding to 
            of the row's largest y.  Then one rounding to the output's type.
  dx        x r to 16 u, dy g to 5 u, their mean over D: 25 u of the terms' mean size: under 64 u of
            r (max |dy g| + max |x r| mean |dy g x r|); one rounding to its type.
- dg        each term to 24 u of the products it is made of; a chain of additions is at most the rows of a lane (of 4096 waves), the 64 rows that
+ dg        each term to 24 u of the products it is made of; a
+           chain of additions is at most the rows of a lane (of 4096 waves), the 64 rows that
            meet in a work-group, 16 of 1024 work-groups, and 64: under (64 + min(rows, 520)) u of the terms' sizes.
 """
 import numpy as np
