@@ -156,6 +156,27 @@ def test_pages_that_hold_nothing(dtype, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,kind", KINDS)
+def test_shared_pages(dtype, kind):
+    """A prefix that sequences share, and a page that one sequence has twice."""
+    x = Case(dtype, kind, [700, 150, 64], 6, 2, 64, 16)
+    for b in (1, 2):
+        x.c.table[b, :4] = x.c.table[0, :4]
+    x.c.table[1, 6] = x.c.table[1, 5]
+    x.c.upload()
+    for v in x.value:
+        v[1][:64], v[2][:64] = v[0][:64], v[0][:64]
+        v[1][96:112] = v[1][80:96]
+    x.run().check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind", KINDS)
+def test_many_short_sequences(dtype, kind):
+    Case(dtype, kind, [(5 * b) % 19 for b in range(3000)], 2, 1, 16, 16).run().check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("pad,order", [(0, (1, 0)), (3, (0, 1)), (8, (1, 0)), (1, (1, 0))])
 def test_strides(pad, order, dtype, kind):
     Case(dtype, kind, [50, 7, 290], 6, 3, 80, 16, order=order, pad=pad).run().check()
