@@ -8,8 +8,8 @@
 // that they do not hang on how a division rounds.  A row with an infinity or a NaN gets a NaN as its
 // scale, and reads back as NaN.
 //
-// Bound by HBM: 32768 tokens of 8 heads of 128 bf16 into e4m3 take 58 us (3.5 TB/s; a fifth less with no tie to
-// decide), 80896 of them back 93 (5.4 TB/s); a copy of 1 GiB moves 5.14.  Few tokens are bound by the
+// Bound by HBM: 32768 tokens of 8 heads of 128 bf16 into e4m3 and 80896 of them back take 149 us in turn, 4.7 TB/s, where
+// a copy of 1 GiB moves 5.14; each by itself 49 and 104.  Few tokens are bound by the
 // waits for beginnings, a length, a page and a row after each other: 64 sequences' next token 4.7 us, read back 4.1.
 #include "dh_paged.hpp"
 
@@ -359,7 +359,7 @@ template <> __device__ inline float value_of<uint8_t>(uint32_t w, int e) {
 // the exact quotient (which the product is to 2^-22) between: where both round to one code, that is its.  Else the
 // border t between the two codes decides: the sign of x - t s, which fma gives exactly, and the even code where it is
 // zero.  bf16 rows often have such ties (one row of seven has some), so this path is made short: 32768 x 16 rows of
-// 128 bf16 to e4m3 take 43 us without it, 66 with the exact quotient of every value in it.  Scales below 2^-40,
+// 128 bf16 to e4m3 take 43 us without it, 49 with it, 66 with the exact quotient of every value instead.  Scales below 2^-40,
 // where remainders could underflow, and rows that are not finite take the exact quotient.
 template <typename CT, int V>
 __device__ inline float quantise(const float (&x)[V], uint32_t most, uint32_t (&out)[V / 4]) {
@@ -368,29 +368,22 @@ __device__ inline float quantise(const float (&x)[V], uint32_t most, uint32_t (&
     const bool plain = (s >= 0x1p-40f && most < 0x7F800000u) || most == 0;   // zeros round to zeros
     const float rs = plain && most > 0 ? __builtin_amdgcn_rcpf(s) : 0.f;
     const float below = rs * (1.f - 0x1p-21f), above = rs * (1.f + 0x1p-21f);
-    bool unsure = false;
-    uint32_t up[V / 4];
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) {
         float lo[4], hi[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) lo[e] = x[4 * i + e] * below, hi[e] = x[4 * i + e] * above;
         out[i] = codes_of<CT>(lo);
-        up[i] = codes_of<CT>(hi);
-        unsure |= out[i] != up[i];
-    }
-    if (__any(unsure)) {
+        const uint32_t up = codes_of<CT>(hi);
+        if (!__any(out[i] != up)) continue;
+        uint32_t pick = 0;   // bytes of up
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) {
-            uint32_t pick = 0;   // bytes of up
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float t = 0.5f * (value_of<CT>(out[i], e) + value_of<CT>(up[i], e));
-                const float r = fmaf(-fabsf(t), s, fabsf(x[4 * i + e]));
-                if (r > 0.f || (r == 0.f && (out[i] >> (8 * e) & 1))) pick |= 0xFFu << (8 * e);
-            }
-            out[i] = (out[i] & ~pick) | (up[i] & pick);
+        for (int e = 0; e < 4; ++e) {
+            const float t = 0.5f * (value_of<CT>(out[i], e) + value_of<CT>(up, e));
+            const float r = fmaf(-fabsf(t), s, fabsf(x[4 * i + e]));
+            if (r > 0.f || (r == 0.f && (out[i] >> (8 * e) & 1))) pick |= 0xFFu << (8 * e);
         }
+        out[i] = (out[i] & ~pick) | (up & pick);
     }
     if (!__any(!plain)) return s;
     const float exact = most >= 0x7F800000u ? __builtin_nanf("") : m / Code<CT>::top;
