@@ -646,9 +646,11 @@ long long most_splits(long long pairs, int D, int size, int max_len) {
     return n < MOST_SPLITS ? n : MOST_SPLITS;
 }
 // Waves of a work-group: eight where they have two tiles each and the registers leave room for two such
-// work-groups on a CU, or where there are few work-groups (33 x 12 sequences fp32: 37 us with eight, 45 with four).
+// work-groups on a CU (33 x 12 sequences fp32: 37 us with eight, 45 with four), or where there is at most one for each CU
+// (5 x 8 of up to 3024 tokens, D = 192, in 480 work-groups: 22.7 with eight, 18.9 with four).  Two tiles of query
+// rows have twice the sums to join: four (the same with 160 heads: 29.9 with eight, 22.1 with four; 1 x 8: 15.9, 13.7).
 int waves_of(int D, int row_tiles, int chunk, long long groups) {
-    return (D <= 128 && row_tiles == 1 && chunk >= 512) || groups <= 512 ? 8 : 4;
+    return row_tiles == 1 && ((D <= 128 && chunk >= 512) || groups <= 256) ? 8 : 4;
 }
 int row_tiles_of(int G) { return G > 16 ? 2 : 1; }
 int size_of(int cache_type) { return cache_type == DH_F32 ? 4 : cache_type == DH_BF16 ? 2 : 1; }
@@ -669,10 +671,11 @@ int launch_form(const Paged& c, Work w, const void* Q, Strides sq, void* O, Stri
     const int groups = (w.G + 16 * RT - 1) / (16 * RT);
     w.by_groups = make_fastdiv(groups);
     const dim3 grid(w.B * c.Hk * groups, w.splits);
-    if (waves_of(c.D, RT, w.chunk, (long long)grid.x * grid.y) == 8)
-        paged_chunk<T, CT, DP, FULL, RT, 8><<<grid, 512, 0, stream()>>>(c, w, (const T*)Q, sq, (T*)O, so, lse);
-    else
-        paged_chunk<T, CT, DP, FULL, RT, 4><<<grid, 256, 0, stream()>>>(c, w, (const T*)Q, sq, (T*)O, so, lse);
+    const int waves = waves_of(c.D, RT, w.chunk, (long long)grid.x * grid.y);
+    auto run = paged_chunk<T, CT, DP, FULL, RT, 4>;
+    if constexpr (RT == 1)
+        if (waves == 8) run = paged_chunk<T, CT, DP, FULL, RT, 8>;
+    run<<<grid, 64 * waves, 0, stream()>>>(c, w, (const T*)Q, sq, (T*)O, so, lse);
     DH_TRY(check_launch("dh_paged_attention"));
     if (w.splits == 1) return DH_OK;
     return c.D <= 64 ? join<T, 16>(w, c.D, O, so, lse) : c.D <= 128 ? join<T, 32>(w, c.D, O, so, lse)
