@@ -11,6 +11,7 @@
 // Bound by HBM: 32768 tokens of 8 heads of 128 bf16 into e4m3 and 80896 of them back take 149 us in turn, 4.7 TB/s, where
 // a copy of 1 GiB moves 5.14; each by itself 49 and 104.  Few tokens are bound by the
 // waits for beginnings, a length, a page and a row after each other: 64 sequences' next token 4.7 us, read back 4.1.
+#include "dh_kv_split.hpp"
 #include "dh_paged.hpp"
 
 namespace dh {
@@ -197,14 +198,10 @@ __global__ void __launch_bounds__(256) cache_read(Paged c, int B, int N, const i
 // read twice that).  A wave takes `tokens` rows of K and V, the four waves of a work-group in turn (what lies side by
 // side is then read at the same time): its lanes find a token's place each, so that the waits for beginnings, lengths
 // and pages are those of one token.  Where there are few tokens it takes one of the blocks of heads of one.  Where there
-// are fewer heads than half of the wave's places (MANY), a power of two `heads` of those places belong to a token and the
-// wave has several tokens at once.  (Places found by a work-group of 16 tokens for its four waves, with a barrier,
-// cost 2 to 10% more.)
-constexpr int MOST_TOKENS = 64;
-struct Units {
-    int tokens, heads, blocks, each;   // log2 of a token's places (MANY), blocks of heads of a token, and of those a wave's
-    FastDiv per;                       // waves of the same tokens
-    uint32_t units;
+// are few heads (MANY) the wave has several tokens at once.  (Places found by a work-group of 16 tokens for its four
+// waves, with a barrier, cost 2 to 10% more.)
+struct Units : Split {
+    FastDiv by_per;
 };
 // Rows of a wave: row t is base + (t / side) step + t % side, side = 1 << shift of them side by side.
 struct Rows {
@@ -212,7 +209,7 @@ struct Rows {
     __device__ int at(int t) const { return base + (t >> shift) * step + (t & (side - 1)); }
 };
 __device__ inline Rows rows_of(const Units& u, uint32_t group, int shift) {
-    const int turns = u.per.d == 1 ? 4 : 1, side = 1 << shift, turn = group & (turns - 1);
+    const int turns = u.per == 1 ? 4 : 1, side = 1 << shift, turn = group & (turns - 1);
     return Rows{(int)(group - turn) * u.tokens + turn * side, shift, side, turns * side};
 }
 
@@ -411,9 +408,9 @@ __global__ void __launch_bounds__(256) cache_write_pieces(Paged c, Units u, int 
     const bool in = piece * P < c.D;
     const uint32_t unit = 4 * blockIdx.x + wave;
     if (unit >= u.units) return;
-    const uint32_t group = fdiv(unit, u.per);
-    const Rows rows = rows_of(u, group, MANY ? __builtin_ctz(G) - u.heads : 0);
-    const int j0 = (unit - group * u.per.d) * u.each, j1 = min(j0 + u.each, u.blocks);   // blocks of heads
+    const uint32_t group = fdiv(unit, u.by_per);
+    const Rows rows = rows_of(u, group, MANY ? __builtin_ctz(G) - u.log_heads : 0);
+    const int j0 = (unit - group * u.per) * u.each, j1 = min(j0 + u.each, u.blocks);   // blocks of heads
     u32x4 x[2];
     // Head h0 of the wave (the lane's own where MANY) of token i.  Lanes without one read another's row.
     auto load = [&](int i, int h0) {
@@ -446,8 +443,8 @@ __global__ void __launch_bounds__(256) cache_write_pieces(Paged c, Units u, int 
         }
     };
     if constexpr (MANY) {
-        const int h = sub & ((1 << u.heads) - 1);
-        int i = sub >> u.heads;
+        const int h = sub & ((1 << u.log_heads) - 1);
+        int i = first_token(sub, u.log_heads);
         load(i, h);   // on their way while the places are found
         const int2 places = find_place(c, B, N, first, len, rows, u.tokens);
         for (int i0 = 0; i0 < u.tokens; i0 += rows.side) {
@@ -504,9 +501,9 @@ __global__ void __launch_bounds__(256) cache_read_pieces(Paged c, Units u, int B
     const bool in = piece * P < c.D;
     const uint32_t unit = 4 * blockIdx.x + wave;
     if (unit >= u.units) return;
-    const uint32_t group = fdiv(unit, u.per);
-    const Rows rows = rows_of(u, group, MANY ? __builtin_ctz(G) - u.heads : 0);
-    const int j0 = (unit - group * u.per.d) * u.each, j1 = min(j0 + u.each, u.blocks);   // blocks of heads
+    const uint32_t group = fdiv(unit, u.by_per);
+    const Rows rows = rows_of(u, group, MANY ? __builtin_ctz(G) - u.log_heads : 0);
+    const int j0 = (unit - group * u.per) * u.each, j1 = min(j0 + u.each, u.blocks);   // blocks of heads
     const int2 places = find_place(c, B, N, first, len, rows, u.tokens);
     // AHEAD heads of the lane, G apart (MANY: head h0 of AHEAD tokens, side by side).
     auto move = [&](const int2 (&at)[AHEAD], int i, int h0) {
@@ -545,8 +542,8 @@ __global__ void __launch_bounds__(256) cache_read_pieces(Paged c, Units u, int B
     };
     int2 at[AHEAD];
     if constexpr (MANY) {
-        const int h = sub & ((1 << u.heads) - 1);
-        for (int i = sub >> u.heads; i - sub / u.heads < u.tokens; i += AHEAD * rows.side) {
+        const int h = sub & ((1 << u.log_heads) - 1), rounds = rounds_of(u.tokens, rows.side, AHEAD);
+        for (int k = 0, i = first_token(sub, u.log_heads); k < rounds; ++k, i += AHEAD * rows.side) {
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) {
                 const int t = i + a * rows.side;
@@ -570,23 +567,9 @@ int groups_of(long long rows) {
     return (int)(groups < most ? groups : most);
 }
 
-// `places`: rows of a side that a wave has at once, `ahead`: how often.  Tokens of a wave: as many as leave each of
-// 24576 waves some (three times what the GPU holds, for the tail's sake); blocks of heads, where there are fewer tokens, likewise.
-Units units_of(int N, int Hk, int places, int ahead, bool& many) {
-    int shift = 0, tokens = N / 24576;
-    while (1 << shift < Hk) ++shift;
-    many = 2 << shift <= places;
-    const int side = many ? places >> shift : 1;
-    tokens = (tokens + side - 1) / side * side;
-    tokens = tokens < side ? side : tokens > MOST_TOKENS ? MOST_TOKENS : tokens;
-    const int blocks = many ? 1 : (Hk + places * ahead - 1) / (places * ahead);
-    long long groups = ((long long)N + tokens - 1) / tokens;
-    int each = (int)((groups * blocks + 24575) / 24576);
-    if (each > blocks) each = blocks;
-    const int per = (blocks + each - 1) / each;
-    each = (blocks + per - 1) / per;   // as many for each
-    if (per == 1) groups = (groups + 3) / 4 * 4;   // four waves in turn
-    return Units{tokens, shift, blocks, each, make_fastdiv(per), (uint32_t)groups * per};
+Units units_of(int N, int Hk, int places, int ahead) {
+    const Split s = split_tokens(N, Hk, places, ahead);
+    return Units{s, make_fastdiv(s.per)};
 }
 bool whole_pieces(const void* p, Strides st, int N, int Hk, int size) {
     const long long bits = (N > 1 ? st.token : 0) | (Hk > 1 ? st.head : 0);
@@ -613,9 +596,8 @@ int launch_write(const Paged& c, int B, int N, const int* first, const int* len,
                  const void* V, Strides sv) {
     if (whole_pieces(K, sk, N, c.Hk, sizeof(T)) && whole_pieces(V, sv, N, c.Hk, sizeof(T))) {
         const int lanes = c.D / Piece<T>::V, L = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
-        bool many;
-        const Units u = units_of(N, c.Hk, 64 / L, 1, many);
-        auto run = by_lanes_write<T, CT>(L, many);
+        const Units u = units_of(N, c.Hk, 64 / L, 1);
+        auto run = by_lanes_write<T, CT>(L, u.many);
         run<<<(u.units + 3) / 4, 256, 0, stream()>>>(c, u, B, N, first, len, (const T*)K, sk, (const T*)V, sv);
     } else {
         cache_write<T, CT><<<groups_of(2LL * N * c.Hk), 256, 0, stream()>>>(c, B, N, first, len, (const T*)K, sk,
@@ -628,9 +610,8 @@ int launch_read(const Paged& c, int B, int N, const int* first, const int* len, 
                 Strides sv) {
     if (whole_pieces(K, sk, N, c.Hk, sizeof(T)) && whole_pieces(V, sv, N, c.Hk, sizeof(T))) {
         const int lanes = c.D / Piece<T>::V, L = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
-        bool many;
-        const Units u = units_of(N, c.Hk, 64 / L, 2, many);
-        auto run = by_lanes_read<T, CT>(L, many);
+        const Units u = units_of(N, c.Hk, 64 / L, 2);
+        auto run = by_lanes_read<T, CT>(L, u.many);
         run<<<(u.units + 3) / 4, 256, 0, stream()>>>(c, u, B, N, first, len, (T*)K, sk, (T*)V, sv);
     } else {
         cache_read<T, CT><<<groups_of(2LL * N * c.Hk), 256, 0, stream()>>>(c, B, N, first, len, (T*)K, sk, (T*)V, sv);
