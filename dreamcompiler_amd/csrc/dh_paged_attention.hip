@@ -517,11 +517,12 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
             if (hl >= 16 || h >= w.G || d >= D) continue;
             const int hq = hk * w.G + h;
             if (last) {
-                const float f = total[i] == 0.f ? 0.f : 1.f / total[i];
+                const bool none = total[i] == 0.f;   // no score: whatever the values hold
+                const float f = 1.f / total[i];
                 T* out = O + b * so.seq + (long long)hq * so.head + d;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) out[e] = down<T>(v[i][e] * f);
-                if (lse && d == 0) lse[(long long)b * w.Hq + hq] = total[i] == 0.f ? -INFINITY : top[i] * LN2 + logf(total[i]);
+                for (int e = 0; e < 4; ++e) out[e] = down<T>(none ? 0.f : v[i][e] * f);
+                if (lse && d == 0) lse[(long long)b * w.Hq + hq] = none ? -INFINITY : top[i] * LN2 + logf(total[i]);
             } else {
                 const long long to_ = split * heads + (long long)b * w.Hq + hq;
                 *reinterpret_cast<f32x4*>(w.part + to_ * D + d) = v[i];
@@ -595,13 +596,14 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) paged_join(Work
             o += red[x][lane & (L - 1)];
         }
     }
+    const bool none = sum == 0.f;   // no score: whatever the values hold
     if (lane < L && d < D) {
-        const float f = sum == 0.f ? 0.f : 1.f / sum;
+        const float f = 1.f / sum;
         T* out = O + b * so.seq + (long long)h * so.head + d;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = down<T>(o[e] * f);
+        for (int e = 0; e < 4; ++e) out[e] = down<T>(none ? 0.f : o[e] * f);
     }
-    if (lse && lane == 0) lse[at] = sum == 0.f ? -INFINITY : m * LN2 + logf(sum);
+    if (lse && lane == 0) lse[at] = none ? -INFINITY : m * LN2 + logf(sum);
 }
 
 // ---- host --------------------------------------------------------------------------------------

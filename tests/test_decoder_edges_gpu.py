@@ -1,0 +1,43 @@
+"""The operators around a decoder's attention where their sizes, addresses and values are at an edge.  Tolerances are
+those of the operators' own tests."""
+import numpy as np
+import pytest
+
+from _decoder import U, UB, attention, within
+from test_paged_attention_gpu import Case
+
+SAME = [("f32", "f32"), ("bf16", "bf16")]
+
+
+# ------------------------------------------------------------------------------ attention
+
+def near(x, b, heads=slice(None)):
+    """Sequence b's results for these heads, by the bounds of the attention's own tests."""
+    o, lse, A = (y[heads] for y in attention(x.Q.value[b], x.value[0][b], x.value[1][b], x.scale))
+    dz = (2 * x.D ** 0.5 + 8) * U * A
+    bf16 = x.dtype == "bf16"
+    tol = ((2 * dz + 64 * U + (2.0 ** -16 if bf16 else 0)) * np.abs(x.value[1][b]).max())[:, None]
+    within(x.O.get()[b][heads], o, tol + (UB * (np.abs(o) + tol) if bf16 else 0))
+    within(x.lse.numpy()[b][heads], lse, dz + 64 * U + 2 * U * np.abs(lse))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind", SAME)
+@pytest.mark.parametrize("Hq,Hk,D", [(4, 2, 64), (20, 1, 128), (3, 1, 48)])
+def test_no_score_but_values_that_are_not_finite(Hq, Hk, D, dtype, kind):
+    """Sequences whose scores are all -infinity are empty rows, whatever their values hold: of one chunk, of a few
+    that one wave joins, and of many."""
+    def away(q, K, V):
+        q[:] = np.abs(q) + 0.1
+        for b, (k, v) in enumerate(zip(K, V)):
+            if b % 2 == 0:
+                k[:] = -np.inf
+                v[::3], v[1::3] = np.inf, np.nan
+
+    for T in (40, 2000, 20000):
+        x = Case(dtype, kind, [T, 33, T // 2, 1], Hq, Hk, D, 16, change=away).run()
+        got, L = x.O.get(), x.lse.numpy()
+        for b in (0, 2):
+            assert (got[b] == 0).all() and (L[b] == -np.inf).all()
+        for b in (1, 3):
+            near(x, b)
