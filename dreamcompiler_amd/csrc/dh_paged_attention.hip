@@ -65,8 +65,9 @@ template <> __device__ inline u32x2 words_bf16<uint8_t>(uint32_t w) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true))};
 }
 
-// x (8 values) in P parts of bf16 that add up to it: 8 bits each.
-template <int P>
+// x (8 values) in P parts of bf16 that add up to it: 8 bits each.  An infinity, where x may be one (INF), is its first
+// part alone: what is left of it would be NaN.
+template <int P, bool INF = false>
 __device__ inline void split8(const float (&x)[8], u32x4 (&out)[P]) {
     float r[8];
 #pragma unroll
@@ -78,8 +79,9 @@ __device__ inline void split8(const float (&x)[8], u32x4 (&out)[P]) {
             const uint32_t w = pk_bf16(r[2 * e], r[2 * e + 1]);
             out[q][e] = w;
             if (q + 1 < P) {
-                r[2 * e] -= __builtin_bit_cast(float, w << 16);
-                r[2 * e + 1] -= __builtin_bit_cast(float, w & 0xFFFF0000u);
+                const float lo = __builtin_bit_cast(float, w << 16), hi = __builtin_bit_cast(float, w & 0xFFFF0000u);
+                r[2 * e] = INF && fabsf(lo) == INFINITY ? 0.f : r[2 * e] - lo;
+                r[2 * e + 1] = INF && fabsf(hi) == INFINITY ? 0.f : r[2 * e + 1] - hi;
             }
         }
 }
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk(Paged c, Work w, const
 #pragma unroll
                 for (int e = 0; e < QN; ++e) parts[0][e] = __builtin_bit_cast(uint32_t, x[e]);
             } else {
-                split8<F::QP>(x, parts);
+                split8<F::QP, true>(x, parts);
             }
 #pragma unroll
             for (int p = 0; p < F::QP; ++p) {

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from _decoder import U, UB, attention, within
-from test_paged_attention_gpu import Case
+from test_paged_attention_gpu import KINDS, Case
 
 SAME = [("f32", "f32"), ("bf16", "bf16")]
 
@@ -41,3 +41,24 @@ def test_no_score_but_values_that_are_not_finite(Hq, Hk, D, dtype, kind):
             assert (got[b] == 0).all() and (L[b] == -np.inf).all()
         for b in (1, 3):
             near(x, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind", KINDS)
+def test_queries_at_infinity(dtype, kind):
+    """Keys above zero and a query of -infinity: no score; where one value of it is +infinity beside: NaN.  The other heads
+    and sequences stay as they are."""
+    def far(q, K, V):
+        for k in K:
+            k[:] = np.abs(k) + 0.5
+        q[0, 1, 5] = -np.inf
+        q[2, :] = -np.inf
+        q[0, 2, 3], q[0, 2, 9] = -np.inf, np.inf
+
+    x = Case(dtype, kind, [70, 40, 1500], 4, 2, 64, 16, change=far).run()
+    got, L = x.O.get(), x.lse.numpy()
+    for b, h in ((0, 1), (2, slice(None))):
+        assert (got[b, h] == 0).all() and (L[b, h] == -np.inf).all()
+    assert np.isnan(got[0, 2]).all() and np.isnan(L[0, 2])
+    for b, heads in ((0, [0, 3]), (1, [0, 1, 2, 3])):
+        near(x, b, heads)
