@@ -748,7 +748,9 @@ int dh_paged_attention(int dtype, int cache_type, int B, int Hq, int Hk, int D, 
                          (long long)ld_table * page);
     DH_TRY(check_strides(op, "Q", sq, B, Hq, D, false));
     DH_TRY(check_strides(op, "O", so, B, Hq, D, true));
-    const size_t need = dh_paged_attention_workspace(cache_type, B, Hq, Hk, D, max_len);
+    const Plan p = B > 0 ? plan((long long)B * Hk, D, size_of(cache_type), max_len, window) : Plan{LEAST, 1};
+    // One chunk (a short window) leaves nothing to join, whatever the longest sequence.
+    const size_t need = p.splits > 1 ? dh_paged_attention_workspace(cache_type, B, Hq, Hk, D, max_len) : 0;
     if (B > 0 && (!Q || !len || !O || (need > 0 && !ws))) return set_error(DH_ERR_INVALID, "%s: null pointer", op);
     if (need > 0 && ((uintptr_t)ws & 15)) return set_error(DH_ERR_INVALID, "%s: workspace not 16-byte aligned", op);
     if (ws_bytes < need)
@@ -756,7 +758,6 @@ int dh_paged_attention(int dtype, int cache_type, int B, int Hq, int Hk, int D, 
     DH_TRY(ensure_init());
     if (B == 0) return DH_OK;
     Work w{B, Hq, Hq / Hk, window, max_len, 0, 0, scale, {}, make_fastdiv(Hk), len, nullptr, nullptr};
-    const Plan p = plan((long long)B * Hk, D, size_of(cache_type), max_len, window);
     w.chunk = p.chunk, w.splits = p.splits;
     w.part = (float*)ws;
     w.stat = (float2*)((char*)ws + up256((size_t)w.splits * B * Hq * D * 4));

@@ -3,7 +3,8 @@ those of the operators' own tests."""
 import numpy as np
 import pytest
 
-from _decoder import U, UB, attention, within
+from _decoder import TYPE, U, UB, attention, within
+from dreamcompiler_amd import hip
 from test_paged_attention_gpu import KINDS, Case
 
 SAME = [("f32", "f32"), ("bf16", "bf16")]
@@ -62,3 +63,17 @@ def test_queries_at_infinity(dtype, kind):
     assert np.isnan(got[0, 2]).all() and np.isnan(L[0, 2])
     for b, heads in ((0, [0, 3]), (1, [0, 1, 2, 3])):
         near(x, b, heads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kind", KINDS)
+def test_one_chunk_needs_no_workspace(dtype, kind):
+    """A window that is not split, over sequences that would be."""
+    x = Case(dtype, kind, [3000, 5, 2999], 4, 2, 64, 16, window=300)
+    assert hip.paged_attention_plan(TYPE[kind], 3, 4, 2, 64, x.max_len, 300)[1] == 1 and x.size > 0
+    x.run().check()
+    want = x.values()
+    x.wipe()
+    x.ws, x.size = None, 0
+    x.run().check()
+    assert all(np.array_equal(a, b) for a, b in zip(x.values(), want))
