@@ -615,16 +615,24 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) paged_join(Work
 // the same with many).  Larger chunks leave a tail of busy work-groups while others are
 // done, smaller ones wait more often for their first loads (64 sequences up to 8192 bf16, chunks of 256 /
 // 512 / 1024 / 2048 tokens: 288 / 234 / 230 / 236 us; 128 of e4m3: 364 / 271 / 257 / 251).
-// Joining costs a launch: what one work-group reads in the same time stays whole, FEW tokens, or ONE where there
-// are sequences enough for half the CUs (16 x 8 heads x 1024 tokens bf16: 13.8 us whole, 14.7 split; 4 x 8: 12.7, 9.0).
+// Joining costs a launch: what one work-group reads in the same time stays whole, FEW_BYTES of keys and values, at most
+// ONE tokens.  One sequence on 1 to 32 heads, whole and split: 256 KB are 8.6 and 9.4 us in fp32 of D = 64, 9.5 and
+// 10.6 of D = 128, 8.8 and 10.0 in bf16 of D = 64; 512 KB 14.5 and 10.2 in fp32 of D = 128, 13.9 and 11.0 in bf16 of
+// D = 256; 1 MB (512 tokens in fp32 of D = 256) 29.8 and 15.0.  Where there are pairs of sequence and head for half the CUs
+// (MANY), up to ONE tokens, 1024 and some that follow, whatever their bytes: 16 x 8 heads x 1088 tokens bf16 of D = 128
+// 14.0 us whole, 14.9 split, e4m3 11.2 and 12.5 (bytes would tell better there too: bf16 of D = 256 24.9 and 21.4, fp32
+// of D = 64 17.8 and 14.2, of D = 256 61 and 42).
 constexpr int LEAST = 128, MOST = 2048, CHUNK_BYTES = 512 << 10, WORK_GROUPS = 768;
-constexpr int FEW = 512, ONE = 1088, MANY = 128;
+constexpr int FEW_BYTES = 256 << 10, ONE = 1088, MANY = 128;
 constexpr int MOST_SPLITS = 65535;   // of a launch; at most 2^25 tokens in chunks of MOST are fewer
 
 struct Plan {
     int chunk, splits;
 };
-int whole_tokens(long long pairs) { return pairs >= MANY ? ONE : FEW; }
+int whole_tokens(long long pairs, int D, int size) {
+    const int n = FEW_BYTES / (2 * D * size);
+    return pairs >= MANY || n > ONE ? ONE : n;
+}
 int most_tokens(int D, int size) {
     const int n = CHUNK_BYTES / (2 * D * size) / LEAST * LEAST;
     return n > MOST ? MOST : n;   // D size <= 1024
@@ -632,7 +640,7 @@ int most_tokens(int D, int size) {
 Plan plan(long long pairs, int D, int size, int max_len, int window) {
     // a window that begins inside a tile sees up to 31 tokens before it
     const long long seen = window > 0 && window < max_len - 31 ? window + 31LL : max_len;
-    if (seen <= whole_tokens(pairs)) return {(ONE + LEAST - 1) / LEAST * LEAST, 1};
+    if (seen <= whole_tokens(pairs, D, size)) return {(ONE + LEAST - 1) / LEAST * LEAST, 1};
     const int most = most_tokens(D, size);
     long long n = WORK_GROUPS / pairs;   // chunks of the longest sequence
     if (n < (seen + most - 1) / most) n = (seen + most - 1) / most;
@@ -643,7 +651,7 @@ Plan plan(long long pairs, int D, int size, int max_len, int window) {
 }
 // At least as many for every window.
 long long most_splits(long long pairs, int D, int size, int max_len) {
-    if (max_len <= whole_tokens(pairs)) return 1;
+    if (max_len <= whole_tokens(pairs, D, size)) return 1;
     const int most = most_tokens(D, size);
     const long long a = ((long long)max_len + LEAST - 1) / LEAST, b = WORK_GROUPS / pairs,
                     c = ((long long)max_len + most - 1) / most, n = a < b ? a : b > c ? b : c;
