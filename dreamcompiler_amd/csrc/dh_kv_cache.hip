@@ -8,8 +8,9 @@
 // that they do not hang on how a division rounds.  A row with an infinity or a NaN gets a NaN as its
 // scale, and reads back as NaN.
 //
-// Bound by HBM: 32768 tokens of 8 heads of 128 bf16 into e4m3 and 80896 of them back take 149 us in turn, 4.7 TB/s, where
-// a copy of 1 GiB moves 5.14; each by itself 49 and 104.  Few tokens are bound by the
+// Bound by HBM: 32512 tokens of 8 heads of 128 bf16 into e4m3 and 80896 of them back take 149 us in turn, 4.7 TB/s, where
+// a copy of 1 GiB moves 5.14 (a trace of both: 55 and 93); each by itself 51 and 104, to and from int8 47 and 104, in bf16
+// 53 and 129, in fp32 107 and 252, at the copy's rate 39 and 98, 52 and 129, 104 and 258.  Few tokens are bound by the
 // waits for beginnings, a length, a page and a row after each other: 64 sequences' next token 4.7 us, read back 4.1.
 #include "dh_kv_split.hpp"
 #include "dh_paged.hpp"
@@ -355,8 +356,8 @@ template <> __device__ inline float value_of<uint8_t>(uint32_t w, int e) {
 // Scale and codes of a row from the bits of its largest |x|.  x times the reciprocal of s, less and more by 2^-21 of it, has
 // the exact quotient (which the product is to 2^-22) between: where both round to one code, that is its.  Else the
 // border t between the two codes decides: the sign of x - t s, which fma gives exactly, and the even code where it is
-// zero.  bf16 rows often have such ties (one row of seven has some), so this path is made short: 32768 x 16 rows of
-// 128 bf16 to e4m3 take 43 us without it, 49 with it, 66 with the exact quotient of every value instead.  Scales below 2^-40,
+// zero.  bf16 rows often have such ties (one row of seven has some), so this path is made short: 32512 x 16 rows of
+// 128 bf16 to e4m3 take 43 us without it, 50 with it, 66 with the exact quotient of every value instead.  Scales below 2^-40,
 // where remainders could underflow, and rows that are not finite take the exact quotient.
 template <typename CT, int V>
 __device__ inline float quantise(const float (&x)[V], uint32_t most, uint32_t (&out)[V / 4]) {

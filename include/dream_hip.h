@@ -396,7 +396,8 @@ int dh_linear_loss_plan(int dtype, int grad_type, int N, int V, int D, int K, si
 /* ---- around a decoder's attention: norm and rotation of queries and keys, a paged cache ----
  * Additions to the reference, next to flash attention.  dtype DH_F32 or DH_BF16 for queries, keys,
  * values and outputs.  Every sum, norm and softmax statistic is held in fp32 and results are rounded
- * once; no floating-point atomics, so reruns are bit-identical.  No call here allocates: all can be
+ * once; where the model is bf16, the attention's weights go into their products with 16 bits.  No
+ * floating-point atomics, so reruns are bit-identical.  No call here allocates: all can be
  * captured.  Workspaces are the caller's, as for the vocabulary above: calls that may overlap in time
  * need their own.
  *
@@ -461,9 +462,14 @@ int dh_kv_cache_read(int dtype, int cache_type, int B, int N, int Hk, int D, voi
  * d_len[b] tokens, the last `window` of them if window > 0:
  *   O = softmax(scale q K^T) V,   lse = log sum exp(scale q k) (B x Hq, natural log, fp32; may be NULL).
  * Hq is a multiple of Hk, B Hq at most 2^22: query head h reads cache head h / (Hq / Hk).  Strides of Q and O: sequence,
- * head.  max_len bounds the lengths (at most ld_table page, and 2^25; a longer sequence is cut off there): the
- * work is split over it.  A sequence without tokens, or whose scores are all -infinity, has O = 0,
- * lse = -infinity.  scale finite and > 0.  O and lse overlap nothing else.  What a page holds past a sequence's end does not matter, NaN included. */
+ * head.  max_len bounds the lengths (at most ld_table page, and 2^25; a longer sequence is cut off there).  The
+ * work is split by max_len, not by the lengths themselves: give the longest where it is known.  A bound far above it
+ * leaves fewer and larger chunks than the length would have (one sequence of 2048 bf16 tokens, 32 on 8 heads of 128:
+ * 10 us, 17 under a bound of 131072; 64 of 8192 under 32768: 226 and 241).  The workspace's size is for any window; a call whose
+ * plan has one chunk needs none.  A sequence without tokens, or whose scores are all -infinity, has O = 0,
+ * lse = -infinity.  scale finite and > 0.  O and lse overlap nothing else.  What a page holds past a sequence's end does not
+ * matter, NaN included.  Weights, up to 2^8, are summed with the values before the division: max |v| times 2^8 times the
+ * number of tokens has to stay below fp32's largest.  8-bit rows whose largest |x| is below 2^-100 lose bits. */
 size_t dh_paged_attention_workspace(int cache_type, int B, int Hq, int Hk, int D, int max_len);
 int dh_paged_attention(int dtype, int cache_type, int B, int Hq, int Hk, int D, float scale,
                        int window, const void* d_Q, const long long* q_strides, const int* d_len,
